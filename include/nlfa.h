@@ -316,6 +316,63 @@ int nlfa_fwd_cached_positions(const void* q, const void* k_cache, const void* v_
                               int L, int D, float scale, int causal, int window, int sinks, int dtype, int path,
                               void* scratch, size_t scratch_bytes, void* stream);
 
+/* The head of a language model with its loss, without the logits: for x [n, d], the weight w [V, d] and n targets,
+ *   l = x w^T,  loss_i = log sum_v exp(l_iv) - l_i,target(i),
+ * averaged or summed over the rows whose target is not `ignore_index`, or one per row (zero where ignored).  Stands where
+ * nanolab's `lm_head` and `F.cross_entropy` stand (nanolab/model.py:364-453).  Every extent may be of any size; x and w
+ * are contiguous, of x_dtype and w_dtype; `dtype` is what the products run in (the autocast type, say): 16-bit types on
+ * the tensor cores, NLFA_DTYPE_F32 on the tensor cores as sums of three bf16 parts.  Sums are float32, and so is `loss`.
+ * Targets are int32 or int64 (target_bytes 4 or 8).  A target outside [0, V) that is not ignore_index gives a NaN loss and
+ * NaN gradients.  Rows that are ignored cost nothing and reach nothing, whatever they hold; their dx is zero.  With no row left the mean is
+ * NaN (0 / 0), the sum 0, the gradients 0.
+ *
+ * The forward fills `tape` (nlfa_linear_ce_tape_bytes: packed rows, logsumexps, 16-bit copies), which the backward reads
+ * along with w, unchanged since.  `scratch` is free between the calls.  The backward runs through the vocabulary in pieces whose
+ * gradient of the logits fits 512 MiB; it forms dx (x_dtype) and dw (w_dtype), either of which may be NULL.  `grad` is the gradient of
+ * `loss`: one float, or n of them with NLFA_REDUCE_NONE.  Bit-reproducible; may be captured.  Tape, scratch, dx and dw are 16-byte aligned.  Needs compute
+ * capability 10.x. */
+#define NLFA_REDUCE_NONE 0
+#define NLFA_REDUCE_MEAN 1
+#define NLFA_REDUCE_SUM 2
+/* (w: whether the products can read the weight where it lies depends on its alignment) */
+size_t nlfa_linear_ce_tape_bytes(const void* w, int n, int V, int d, int x_dtype, int w_dtype, int dtype);
+size_t nlfa_linear_ce_scratch_bytes(int n, int V, int d, int x_dtype, int w_dtype, int dtype, int backward);
+int nlfa_linear_ce_fwd(const void* x, int x_dtype, const void* w, int w_dtype, int dtype, const void* targets,
+                       int target_bytes, int n, int V, int d, long long ignore_index, int reduction, float* loss, void* tape,
+                       size_t tape_bytes, void* scratch, size_t scratch_bytes, void* stream);
+int nlfa_linear_ce_bwd(const float* grad, const void* w, int w_dtype, int x_dtype, int dtype, const void* targets,
+                       int target_bytes, int n, int V, int d, long long ignore_index, int reduction, void* tape,
+                       size_t tape_bytes, void* dx, void* dw, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Token embedding: out [n, d] = scale * w[ids], w [V, d]; ids int32 or int64 (id_bytes 4 or 8).  Stands where nanolab's
+ * `tok_emb` stands (nanolab/model.py:205-245).  Rows of any length, contiguous.  An id outside [0, V) gives a row of NaN. */
+int nlfa_embedding_fwd(const void* ids, int id_bytes, const void* w, int dtype, void* out, int n, int V, int d, float scale,
+                       void* stream);
+
+/* Its gradient: dw_v = scale * (sum of g's rows whose id is v), all V rows (zeros where there are none).  Ids outside the table and
+ * `padding_idx` (any negative: none) get none.  Added in float32 in the order of the positions, after a sort of the ids: bit-reproducible.
+ * `scratch`, 16-byte aligned: sorted ids, partial sums. */
+size_t nlfa_embedding_scratch_bytes(int n, int V, int d);
+int nlfa_embedding_bwd(const void* g, int dtype, const void* ids, int id_bytes, void* dw, int n, int V, int d, float scale,
+                       long long padding_idx, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Norm and clip of many gradients, what `clip_grad_norm_` does after nanolab's backward (train.py:336-344):
+ *   total_norm = (sum of all elements' squares)^(1/2), or the largest |element| (NLFA_NORM_INF);
+ *   with `scale`, every gradient times min(1, max_norm / (total_norm + 1e-6)), in place or into `out` (another type allowed).
+ * In place, gradients within the limit are not touched.  The list is read during the call only.  Tensors must not overlap (an
+ * `out` may be its own gradient).  total_norm: one float on the device.  Sums are in float64 and in a fixed order: bit-reproducible. */
+typedef struct nlfa_grad {
+  const void* grad; /* n contiguous elements of `dtype`, aligned to its size */
+  void* out;        /* NULL: in place */
+  long long n;      /* >= 1 */
+  int dtype, out_dtype;
+} nlfa_grad;
+#define NLFA_NORM_INF 0
+#define NLFA_NORM_2 2
+size_t nlfa_clip_scratch_bytes(void);
+int nlfa_clip_grads(const nlfa_grad* grads, int count, float max_norm, int norm, int scale, float* total_norm, void* scratch,
+                    size_t scratch_bytes, void* stream);
+
 /* Bytes of device workspace `nlfa_selftest` needs. */
 size_t nlfa_selftest_workspace_bytes(void);
 

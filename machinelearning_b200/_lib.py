@@ -15,6 +15,7 @@ LIB_PATH = PKG / "libnlfa.so"
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 PATH_AUTO, PATH_SIMT, PATH_TENSOR = 0, 1, 2
 PASS_DELTA, PASS_DKV, PASS_DQ, PASS_ALL, PASS_FUSED = 1, 2, 4, 7, 8
+REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
 OK = 0
 ERR_DEVICE_TIMEOUT = 10
 ERR_SELFTEST_MISMATCH = 12
@@ -68,6 +69,19 @@ SIGNATURES = {
                              + [_c_void_p, _c_size_t, _c_void_p]),
     "nlfa_fwd_cached_positions": (_c_int, [_c_void_p] * 7 + [_c_int] * 7 + [_c_float] + [_c_int] * 5
                                   + [_c_void_p, _c_size_t, _c_void_p]),
+    "nlfa_linear_ce_tape_bytes": (_c_size_t, [_c_void_p] + [_c_int] * 6),
+    "nlfa_linear_ce_scratch_bytes": (_c_size_t, [_c_int] * 7),
+    "nlfa_linear_ce_fwd": (_c_int, [_c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p] + [_c_int] * 4
+                           + [ctypes.c_longlong, _c_int, _c_void_p, _c_void_p, _c_size_t, _c_void_p, _c_size_t, _c_void_p]),
+    "nlfa_linear_ce_bwd": (_c_int, [_c_void_p, _c_void_p] + [_c_int] * 3 + [_c_void_p] + [_c_int] * 4
+                           + [ctypes.c_longlong, _c_int, _c_void_p, _c_size_t, _c_void_p, _c_void_p, _c_void_p, _c_size_t,
+                              _c_void_p]),
+    "nlfa_embedding_fwd": (_c_int, [_c_void_p, _c_int, _c_void_p, _c_int, _c_void_p] + [_c_int] * 3 + [_c_float, _c_void_p]),
+    "nlfa_embedding_scratch_bytes": (_c_size_t, [_c_int] * 3),
+    "nlfa_embedding_bwd": (_c_int, [_c_void_p, _c_int, _c_void_p, _c_int, _c_void_p] + [_c_int] * 3
+                           + [_c_float, ctypes.c_longlong, _c_void_p, _c_size_t, _c_void_p]),
+    "nlfa_clip_scratch_bytes": (_c_size_t, []),
+    "nlfa_clip_grads": (_c_int, [_c_void_p, _c_int, _c_float, _c_int, _c_int, _c_void_p, _c_void_p, _c_size_t, _c_void_p]),
     "nlfa_selftest_workspace_bytes": (_c_size_t, []),
     "nlfa_selftest": (_c_int, [_c_int, _c_int, _c_void_p, _c_size_t,
                                ctypes.POINTER(_c_float), _c_void_p]),

@@ -195,3 +195,91 @@ head_gate_fwd.register_autograd(_hg_backward, setup_context=_hg_setup)
 
 def head_gate(y, gate):
     return head_gate_fwd(y.contiguous(), gate.contiguous())
+
+
+# ---------------------------------------------------------------- head with its loss, token embedding
+from . import head_loss as _hl  # noqa: E402
+from . import token_embedding as _te  # noqa: E402
+
+
+@torch.library.custom_op("nlfa::linear_ce_fwd", mutates_args=(), device_types="cuda")
+def linear_ce_fwd(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int, reduction: str,
+                  dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    return _hl.fwd(x, weight, targets, ignore_index, reduction, dtype)
+
+
+@linear_ce_fwd.register_fake
+def _(x, weight, targets, ignore_index, reduction, dtype):
+    tape = torch.library.get_ctx().new_dynamic_size()
+    return (x.new_empty(targets.shape if reduction == "none" else (), dtype=torch.float32),
+            x.new_empty((tape,), dtype=torch.uint8))
+
+
+@torch.library.custom_op("nlfa::linear_ce_bwd", mutates_args=(), device_types="cuda")
+def linear_ce_bwd(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, tape: torch.Tensor,
+                  ignore_index: int, reduction: str, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    return _hl.bwd(grad.to(torch.float32).contiguous(), x.shape, x.dtype, weight, targets, tape, ignore_index, reduction, dtype)
+
+
+@linear_ce_bwd.register_fake
+def _(grad, x, weight, targets, tape, ignore_index, reduction, dtype):
+    return torch.empty_like(x), torch.empty_like(weight)
+
+
+def _ce_setup(ctx, inputs, output):
+    x, weight, targets, ignore_index, reduction, dtype = inputs
+    ctx.save_for_backward(x, weight, targets, output[1])
+    ctx.args = (ignore_index, reduction, dtype)
+
+
+def _ce_backward(ctx, grad, gtape):
+    x, weight, targets, tape = ctx.saved_tensors
+    dx, dw = linear_ce_bwd(grad, x, weight, targets, tape, *ctx.args)
+    return dx, dw, None, None, None, None
+
+
+linear_ce_fwd.register_autograd(_ce_backward, setup_context=_ce_setup)
+
+
+def linear_cross_entropy(x, weight, targets, ignore_index, reduction, dtype):
+    """``head_loss.linear_cross_entropy`` through the registered operators."""
+    return linear_ce_fwd(x.contiguous(), weight.contiguous(), targets.contiguous(), ignore_index, reduction, dtype)[0]
+
+
+@torch.library.custom_op("nlfa::embedding_fwd", mutates_args=(), device_types="cuda")
+def embedding_fwd(idx: torch.Tensor, weight: torch.Tensor, scale: float, padding: int) -> torch.Tensor:
+    return _te.fwd(idx, weight, scale)
+
+
+@embedding_fwd.register_fake
+def _(idx, weight, scale, padding):
+    return weight.new_empty((*idx.shape, weight.shape[1]))
+
+
+@torch.library.custom_op("nlfa::embedding_bwd", mutates_args=(), device_types="cuda")
+def embedding_bwd(g: torch.Tensor, idx: torch.Tensor, rows: int, scale: float, padding: int) -> torch.Tensor:
+    return _te.bwd(g.contiguous(), idx, rows, scale, padding)
+
+
+@embedding_bwd.register_fake
+def _(g, idx, rows, scale, padding):
+    return g.new_empty((rows, g.shape[-1]))
+
+
+def _te_setup(ctx, inputs, output):
+    idx, weight, scale, padding = inputs
+    ctx.save_for_backward(idx)
+    ctx.args = (weight.shape[0], scale, padding)
+
+
+def _te_backward(ctx, g):
+    (idx,) = ctx.saved_tensors
+    return None, embedding_bwd(g, idx, *ctx.args), None, None
+
+
+embedding_fwd.register_autograd(_te_backward, setup_context=_te_setup)
+
+
+def embedding(idx, weight, scale, padding):
+    """``token_embedding.embedding`` through the registered operators."""
+    return embedding_fwd(idx.contiguous(), weight.contiguous(), scale, padding)

@@ -1,0 +1,498 @@
+// Token embedding: out_i = s w[id_i], and the table's gradient dw_v = s sum_{i: id_i = v} g_i.
+//
+// Both directions move rows and are bound by HBM.  The gradient adds the rows of a token in the order of their positions, so
+// that the same call gives the same bits: the ids are sorted first (sort_ids_kernel: one cluster, a stable radix sort whose
+// digit counts cross between its CTAs through distributed shared memory: no launch per pass and no waiting on flags),
+// then warps add runs of sorted positions (add_rows_kernel).  A token's rows that cross from one run into the next are added from the
+// runs' partial sums afterwards (join_rows_kernel), in order.  Rows of tokens that do not occur are zeroed on the way.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "ptx.cuh"
+#include "rowwise.cuh"
+
+namespace nlfa {
+namespace embedding {
+namespace {
+
+constexpr int kBlock = 256, kWarps = kBlock / 32;
+constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kMostDigitBits = 9;
+
+// W bytes of a row: 16, 8, 4 or 2, what its alignment allows
+template <int W> struct Word;
+template <> struct Word<16> { using type = uint4; };
+template <> struct Word<8> { using type = uint2; };
+template <> struct Word<4> { using type = uint32_t; };
+template <> struct Word<2> { using type = uint16_t; };
+
+__device__ __forceinline__ float as_float(float x) { return x; }
+__device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T as_type(float x);
+template <> __device__ __forceinline__ float as_type<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half as_type<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 as_type<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <typename T, int W>
+struct Vec {
+  static constexpr int N = W / static_cast<int>(sizeof(T));
+  union {
+    typename Word<W>::type w;
+    T e[N];
+  };
+  __device__ Vec() {}
+};
+
+// A thread moves words of a row; `per_row` words of W bytes, four of them in flight.
+template <typename T, int W, typename I>
+__global__ void __launch_bounds__(kBlock)
+lookup_kernel(const I* __restrict__ ids, const T* __restrict__ w, T* __restrict__ out, int n, int V, int per_row, FastDiv div, float scale) {
+  using Word_ = typename Word<W>::type;
+  using V_ = Vec<T, W>;
+  constexpr int U = 4;
+  grid_dep_wait();
+  grid_dep_release();
+  // (per CTA a run of words that fits 31 bits, wherever it starts)
+  const long long total = static_cast<long long>(n) * per_row;
+  const long long first = static_cast<long long>(blockIdx.x) * (kBlock * U);
+  const int row0 = static_cast<int>(first / per_row), col0 = static_cast<int>(first - static_cast<long long>(row0) * per_row);
+  V_ v[U];
+  long long at[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = u * kBlock + threadIdx.x;
+    at[u] = first + i;
+    if (at[u] >= total) continue;
+    const int step = div.div(col0 + i), row = row0 + step, col = col0 + i - step * per_row;
+    const long long id = static_cast<long long>(ids[row]);
+    if (id >= 0 && id < V) v[u].w = reinterpret_cast<const Word_*>(w)[id * per_row + col];
+    else {
+#pragma unroll
+      for (int e = 0; e < V_::N; ++e) v[u].e[e] = as_type<T>(__int_as_float(0x7fffffff));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (at[u] >= total) continue;
+    if (scale != 1.f) {
+#pragma unroll
+      for (int e = 0; e < V_::N; ++e) v[u].e[e] = as_type<T>(as_float(v[u].e[e]) * scale);
+    }
+    reinterpret_cast<Word_*>(out)[at[u]] = v[u].w;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ sort
+
+// (id, position) by id, positions in order; ids without a gradient (outside the table, padding) become V and end up last.
+// begin[v], end[v]: where v's positions lie; begin = -1 where there are none.  Each CTA has a run of the positions, each warp of it a run of that.
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads)
+sort_ids_kernel(const I* __restrict__ ids, int n, int V, long long padding, uint32_t* keys, uint32_t* places, int* __restrict__ begin,
+                int* __restrict__ end, int passes, int digit_bits) {
+  extern __shared__ int smem[];
+  const int digits = 1 << digit_bits;
+  int* count = smem;                                   // [warp][digit]
+  int* total = smem + kSortWarps * digits;             // [digit], read by the other CTAs
+  int* base = total + digits;
+  __shared__ int warp_sum[32];
+  grid_dep_wait();
+  grid_dep_release();
+  const int rank = static_cast<int>(cluster_rank()), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned below = (1u << lane) - 1u;
+  const int run = static_cast<int>((static_cast<long long>(n) + kSortCtas * kSortThreads - 1) / (kSortCtas * kSortThreads)) * 32;
+  const long long lo = static_cast<long long>(run) * (rank * kSortWarps + warp);
+  const int from = lo < n ? static_cast<int>(lo) : n, to = n - from < run ? n : from + run;
+
+  for (int v = rank * kSortThreads + threadIdx.x; v < V; v += kSortCtas * kSortThreads) begin[v] = -1;
+
+  uint32_t *src = keys, *src_at = places, *dst = keys + n, *dst_at = places + n;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * digit_bits;
+    auto key_at = [&](int i) -> uint32_t {
+      if (pass > 0) return __ldcg(src + i);
+      const long long id = static_cast<long long>(ids[i]);
+      return id >= 0 && id < V && id != padding ? static_cast<uint32_t>(id) : static_cast<uint32_t>(V);
+    };
+    for (int i = threadIdx.x; i < kSortWarps * digits; i += kSortThreads) count[i] = 0;
+    __syncthreads();
+    int* mine = count + warp * digits;
+    for (int i0 = from; i0 < to; i0 += 32) {
+      const bool in = i0 + lane < to;
+      const uint32_t d = in ? (key_at(i0 + lane) >> shift) & (digits - 1) : 0xffffffffu;
+      const unsigned same = __match_any_sync(0xffffffffu, d);
+      if (in && (same & below) == 0) mine[d] += __popc(same);
+      __syncwarp();
+    }
+    __syncthreads();
+    if (threadIdx.x < digits) {
+      int sum = 0;
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) {
+        const int c = count[w * digits + threadIdx.x];
+        count[w * digits + threadIdx.x] = sum;
+        sum += c;
+      }
+      total[threadIdx.x] = sum;
+    }
+    cluster_arrive();
+    cluster_wait();
+    int before = 0, all = 0;
+    if (threadIdx.x < digits) {
+#pragma unroll
+      for (int r = 0; r < kSortCtas; ++r) {
+        int v;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(smem_u32(total + threadIdx.x), r)) : "memory");
+        if (r < rank) before += v;
+        all += v;
+      }
+    }
+    int inclusive = all;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, inclusive, off);
+      if (lane >= off) inclusive += o;
+    }
+    if (lane == 31) warp_sum[warp] = inclusive;
+    __syncthreads();
+    if (threadIdx.x < digits) {
+      int ahead = 0;
+      for (int w = 0; w < warp; ++w) ahead += warp_sum[w];
+      base[threadIdx.x] = ahead + inclusive - all + before;
+    }
+    __syncthreads();
+    for (int i0 = from; i0 < to; i0 += 32) {
+      const bool in = i0 + lane < to;
+      const uint32_t key = in ? key_at(i0 + lane) : 0u;
+      const uint32_t d = in ? (key >> shift) & (digits - 1) : 0xffffffffu;
+      const unsigned same = __match_any_sync(0xffffffffu, d);
+      if (in) {
+        const int to_place = base[d] + mine[d] + __popc(same & below);
+        dst[to_place] = key;
+        dst_at[to_place] = pass > 0 ? __ldcg(src_at + i0 + lane) : static_cast<uint32_t>(i0 + lane);
+      }
+      __syncwarp();
+      if (in && (same & below) == 0) mine[d] += __popc(same);
+      __syncwarp();
+    }
+    // the next pass reads what the other CTAs wrote, and overwrites what they read
+    cluster_arrive();
+    cluster_wait();
+    uint32_t* t = src; src = dst; dst = t;
+    t = src_at; src_at = dst_at; dst_at = t;
+  }
+  for (int i = from + lane; i < to; i += 32) {
+    const uint32_t key = __ldcg(src + i);
+    if (key >= static_cast<uint32_t>(V)) continue;
+    if (i == 0 || __ldcg(src + i - 1) != key) begin[key] = i;
+    if (i == n - 1 || __ldcg(src + i + 1) != key) end[key] = i + 1;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ sums
+
+template <typename T, int W>
+struct Row {
+  using V = Vec<T, W>;
+  static constexpr int N = V::N;
+  // scaled and rounded once
+  static __device__ __forceinline__ void store(T* p, const float (&s)[N], float scale) {
+    V v;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v.e[e] = as_type<T>(s[e] * scale);
+    *reinterpret_cast<typename Word<W>::type*>(p) = v.w;
+  }
+};
+
+// Units of one warp: first (run of `run` sorted positions) x (slab of 32 words of a row), then 16 rows of the table each, of which those
+// without a position are zeroed.  partial [runs][2][d]: what a run has of a token that began in an earlier run, and of
+// one that goes on in the next.
+template <typename T, int W>
+__global__ void __launch_bounds__(kBlock)
+add_rows_kernel(const T* __restrict__ g, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ places, const int* __restrict__ begin,
+                T* __restrict__ dw, float* __restrict__ partial, int n, int V, int d, int run, int runs, int slabs, float scale) {
+  using R = Row<T, W>;
+  constexpr int N = R::N, U = 8;
+  grid_dep_wait();
+  grid_dep_release();
+  const int lane = threadIdx.x & 31;
+  const long long unit = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const long long adds = static_cast<long long>(runs) * slabs;
+  if (unit >= adds) {
+    const long long v0 = (unit - adds) * 16;
+    if (v0 >= V) return;
+    const int v = static_cast<int>(v0) + lane;
+    unsigned empty = __ballot_sync(0xffffffffu, lane < 16 && v < V && begin[v < V ? v : 0] < 0);
+    const int words = d / N;
+    typename R::V zero;
+#pragma unroll
+    for (int e = 0; e < N; ++e) zero.e[e] = as_type<T>(0.f);
+    while (empty) {
+      const int r = __ffs(empty) - 1;
+      empty &= empty - 1;
+      auto* row = reinterpret_cast<typename Word<W>::type*>(dw + (static_cast<size_t>(v0) + r) * d);
+      for (int c = lane; c < words; c += 32) row[c] = zero.w;
+    }
+    return;
+  }
+  const int c = static_cast<int>(unit / slabs), slab = static_cast<int>(unit - static_cast<long long>(c) * slabs);
+  const int col = (slab * 32 + lane) * N;
+  const bool in = col < d;
+  const int from = c * run, to = n - from < run ? n : from + run;
+  const uint32_t before = from > 0 ? keys[from - 1] : 0xffffffffu, after = to < n ? keys[to] : 0xffffffffu;
+  float sum[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) sum[e] = 0.f;
+  bool first = true;                                       // the token at hand is the run's first
+  for (int i0 = from; i0 < to; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t key = i < to ? keys[i] : 0xffffffffu;
+    const uint32_t place = i < to ? places[i] : 0u;
+    const uint32_t next = i + 1 < to ? keys[i + 1] : i + 1 == to ? after : 0xffffffffu;
+    const int live = __popc(__ballot_sync(0xffffffffu, key < static_cast<uint32_t>(V)));   // (those without a gradient stand last)
+    for (int j0 = 0; j0 < live; j0 += U) {
+      typename R::V v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t p = __shfl_sync(0xffffffffu, place, (j0 + u) & 31);
+        if (j0 + u < live && in) v[u].w = *reinterpret_cast<const typename Word<W>::type*>(g + static_cast<size_t>(p) * d + col);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u;
+        const uint32_t k = __shfl_sync(0xffffffffu, key, j & 31), k1 = __shfl_sync(0xffffffffu, next, j & 31);
+        if (j >= live) continue;
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] += as_float(v[u].e[e]);
+        const bool run_ends = i0 + j + 1 == to;
+        if (k1 == k && !run_ends) continue;
+        const bool came = first && k == before, goes = run_ends && k1 == k;
+        if (in) {
+          if (came || goes) {
+            float* o = partial + (static_cast<size_t>(2 * c) + (came ? 0 : 1)) * d + col;
+#pragma unroll
+            for (int e = 0; e < N; ++e) o[e] = sum[e];
+          } else {
+            R::store(dw + static_cast<size_t>(k) * d + col, sum, scale);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] = 0.f;
+        first = false;
+      }
+    }
+    if (live < 32) break;
+  }
+}
+
+// Tokens that begin in run c and go on: their shares of run c and of those behind, in order.  A warp per run; where there are many
+// shares the CTA's warps take an eighth each.
+template <typename T, int W>
+__global__ void __launch_bounds__(kBlock)
+join_rows_kernel(const uint32_t* __restrict__ keys, const int* __restrict__ begin, const int* __restrict__ end, const float* __restrict__ partial,
+                 T* __restrict__ dw, int n, int V, int d, int run, int runs, float scale) {
+  using R = Row<T, W>;
+  constexpr int N = R::N, kAlone = 64;
+  __shared__ float shares[kWarps][32 * N];
+  __shared__ int long_last[kWarps];
+  grid_dep_wait();
+  grid_dep_release();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = (blockIdx.y * 32 + lane) * N;
+  const bool in = col < d;
+  const int c = blockIdx.x * kWarps + warp;
+  uint32_t key = 0xffffffffu;
+  int last = 0;                                            // the last run with a share
+  if (c + 1 < runs) {
+    key = keys[(c + 1) * run - 1];
+    if (key >= static_cast<uint32_t>(V) || keys[(c + 1) * run] != key || begin[key] < c * run) key = 0xffffffffu;
+    else last = (end[key] - 1) / run;
+  }
+  auto share = [&](int r, int which, float (&s)[N]) {
+    const float* o = partial + (static_cast<size_t>(2 * r) + which) * d + col;
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] += o[e];
+  };
+  const bool alone = key != 0xffffffffu && last - c <= kAlone;
+  if (alone && in) {
+    float s[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] = 0.f;
+    share(c, 1, s);
+#pragma unroll 4
+    for (int r = c + 1; r <= last; ++r) share(r, 0, s);
+    R::store(dw + static_cast<size_t>(key) * d + col, s, scale);
+  }
+  if (lane == 0) long_last[warp] = key != 0xffffffffu && !alone ? last : -1;
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) {
+    const int l = long_last[w];
+    if (l < 0) continue;
+    const int c0 = blockIdx.x * kWarps + w, many = l - c0;                     // shares of runs c0 + 1 .. l
+    const int lo = c0 + 1 + static_cast<int>(static_cast<long long>(many) * warp / kWarps);
+    const int hi = c0 + 1 + static_cast<int>(static_cast<long long>(many) * (warp + 1) / kWarps);
+    float s[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] = 0.f;
+    if (in) {
+      if (warp == 0) share(c0, 1, s);
+#pragma unroll 4
+      for (int r = lo; r < hi; ++r) share(r, 0, s);
+#pragma unroll
+      for (int e = 0; e < N; ++e) shares[warp][lane * N + e] = s[e];
+    }
+    __syncthreads();
+    if (warp == w && in) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) s[e] = 0.f;
+      for (int x = 0; x < kWarps; ++x)
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e] += shares[x][lane * N + e];
+      R::store(dw + static_cast<size_t>(key) * d + col, s, scale);
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+
+size_t up(size_t v) { return (v + 255) / 256 * 256; }
+
+int checked(cudaError_t e) {
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e == cudaSuccess ? NLFA_OK : NLFA_ERR_CUDA;
+}
+
+int check(int n, int V, int d, int dtype) {
+  if (n < 0 || V < 1 || d < 1 || n > (1 << 30) || V > (1 << 30) || d > (1 << 24)) return NLFA_ERR_BAD_SHAPE;
+  return rowwise::dtype_ok(dtype) ? NLFA_OK : NLFA_ERR_BAD_DTYPE;
+}
+
+int element_bytes(int dtype) { return dtype == NLFA_DTYPE_F32 ? 4 : 2; }
+
+// Widest word that divides a row and both bases.
+int word_bytes(long long row_bytes, const void* a, const void* b) {
+  const unsigned long long all = static_cast<unsigned long long>(row_bytes) | reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b);
+  return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
+}
+
+// Sorted positions per warp: enough warps for the GPU, and few partial sums when there are many positions.
+int run_length(int n, int d) {
+  const long long warps = 32ll * 148, slabs = (d + 127) / 128;
+  int run = 16;
+  while (run < 128 && n * slabs / (2 * run) >= warps) run *= 2;
+  return run;
+}
+
+struct Scratch {
+  size_t keys, places, begin, end, partial, bytes;
+};
+Scratch scratch_layout(int n, int V, int d) {
+  Scratch s{};
+  size_t at = 0;
+  s.keys = at; at = up(at + static_cast<size_t>(n) * 8);
+  s.places = at; at = up(at + static_cast<size_t>(n) * 8);
+  s.begin = at; at = up(at + static_cast<size_t>(V) * 4);
+  s.end = at; at = up(at + static_cast<size_t>(V) * 4);
+  s.partial = at; at = up(at + (static_cast<size_t>(n) / run_length(n, d) + 1) * 2 * d * 4);
+  s.bytes = at;
+  return s;
+}
+
+template <typename T, int W, typename I>
+int lookup(const void* ids, const void* w, void* out, int n, int V, int d, float scale, cudaStream_t st) {
+  const int per_row = d / Vec<T, W>::N;
+  const long long ctas = (static_cast<long long>(n) * per_row + 4 * kBlock - 1) / (4 * kBlock);
+  if (ctas > 0x7fffffffll) return NLFA_ERR_BAD_SHAPE;
+  return checked(launch_kernel(lookup_kernel<T, W, I>, dim3(static_cast<unsigned>(ctas)), dim3(kBlock), 0, st, overlap_launches(kOverlapRowwise),
+                               static_cast<const I*>(ids), static_cast<const T*>(w), static_cast<T*>(out), n, V, per_row,
+                               FastDiv(per_row), scale));
+}
+
+template <typename T, int W>
+int gradient(const void* g, const Scratch& s, uint8_t* scratch, int sorted, void* dw, int n, int V, int d, float scale, cudaStream_t st) {
+  const int slabs = (d / Vec<T, W>::N + 31) / 32, run = run_length(n, d), runs = (n + run - 1) / run;
+  const uint32_t* keys = reinterpret_cast<const uint32_t*>(scratch + s.keys) + static_cast<size_t>(sorted) * n;
+  const uint32_t* places = reinterpret_cast<const uint32_t*>(scratch + s.places) + static_cast<size_t>(sorted) * n;
+  const int *begin = reinterpret_cast<const int*>(scratch + s.begin), *end = reinterpret_cast<const int*>(scratch + s.end);
+  float* partial = reinterpret_cast<float*>(scratch + s.partial);
+  const bool overlap = overlap_launches(kOverlapRowwise);
+  const long long units = static_cast<long long>(runs) * slabs + (V + 15) / 16, ctas = (units + kWarps - 1) / kWarps;
+  if (ctas > 0x7fffffffll || slabs > 65535) return NLFA_ERR_BAD_SHAPE;
+  int rc = checked(launch_kernel(add_rows_kernel<T, W>, dim3(static_cast<unsigned>(ctas)), dim3(kBlock), 0, st, overlap, static_cast<const T*>(g),
+                                 keys, places, begin, static_cast<T*>(dw), partial, n, V, d, run, runs, slabs, scale));
+  if (rc != NLFA_OK || runs < 2) return rc;
+  return checked(launch_kernel(join_rows_kernel<T, W>, dim3(static_cast<unsigned>((runs + kWarps - 1) / kWarps), static_cast<unsigned>(slabs)),
+                               dim3(kBlock), 0, st, overlap, keys, begin, end, partial, static_cast<T*>(dw), n, V, d, run, runs, scale));
+}
+
+}  // namespace
+}  // namespace embedding
+}  // namespace nlfa
+
+using namespace nlfa;
+using namespace nlfa::embedding;
+
+extern "C" {
+
+int nlfa_embedding_fwd(const void* ids, int id_bytes, const void* w, int dtype, void* out, int n, int V, int d, float scale, void* stream) {
+  const int rc = check(n, V, d, dtype);
+  if (rc != NLFA_OK) return rc;
+  if (id_bytes != 4 && id_bytes != 8) return NLFA_ERR_BAD_ARGUMENT;
+  if (n == 0) return NLFA_OK;
+  if (!ids || !w || !out) return NLFA_ERR_NULL_POINTER;
+  const int bytes = element_bytes(dtype);
+  if ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out)) % bytes != 0) return NLFA_ERR_MISALIGNED;
+  const int word = word_bytes(static_cast<long long>(d) * bytes, w, out);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+#define NLFA_GO(T, W) (id_bytes == 8 ? lookup<T, W, long long>(ids, w, out, n, V, d, scale, st) : lookup<T, W, int>(ids, w, out, n, V, d, scale, st))
+#define NLFA_16(T) (word == 16 ? NLFA_GO(T, 16) : word == 8 ? NLFA_GO(T, 8) : word == 4 ? NLFA_GO(T, 4) : NLFA_GO(T, 2))
+  if (dtype == NLFA_DTYPE_F32) return word == 16 ? NLFA_GO(float, 16) : word == 8 ? NLFA_GO(float, 8) : NLFA_GO(float, 4);
+  return dtype == NLFA_DTYPE_F16 ? NLFA_16(__half) : NLFA_16(__nv_bfloat16);
+#undef NLFA_16
+#undef NLFA_GO
+}
+
+size_t nlfa_embedding_scratch_bytes(int n, int V, int d) {
+  return check(n, V, d, NLFA_DTYPE_F32) == NLFA_OK ? scratch_layout(n, V, d).bytes : 0;
+}
+
+int nlfa_embedding_bwd(const void* g, int dtype, const void* ids, int id_bytes, void* dw, int n, int V, int d, float scale,
+                       long long padding_idx, void* scratch, size_t scratch_bytes, void* stream) {
+  int rc = check(n, V, d, dtype);
+  if (rc != NLFA_OK) return rc;
+  if (id_bytes != 4 && id_bytes != 8) return NLFA_ERR_BAD_ARGUMENT;
+  if (!dw || !scratch || (n > 0 && (!g || !ids))) return NLFA_ERR_NULL_POINTER;
+  if (!rowwise::aligned16(scratch)) return NLFA_ERR_MISALIGNED;
+  const int bytes = element_bytes(dtype);
+  if ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(dw)) % bytes != 0) return NLFA_ERR_MISALIGNED;
+  const Scratch s = scratch_layout(n, V, d);
+  if (scratch_bytes < s.bytes) return NLFA_ERR_SCRATCH_TOO_SMALL;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint8_t* at = static_cast<uint8_t*>(scratch);
+  // digits of equal width that cover 0 .. V
+  int bits = 1;
+  while (bits < 31 && (static_cast<unsigned>(V) >> bits) != 0) ++bits;
+  const int passes = (bits + kMostDigitBits - 1) / kMostDigitBits, digit_bits = (bits + passes - 1) / passes;
+  const size_t smem = static_cast<size_t>(kSortWarps + 2) * (1u << digit_bits) * sizeof(int);
+  auto sort = [&](auto* typed, auto* kernel) {
+    const int r = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), (kSortWarps + 2) * (1 << kMostDigitBits) * static_cast<int>(sizeof(int)));
+    if (r != NLFA_OK) return r;
+    return checked(launch_cluster(kernel, dim3(1, kSortCtas), dim3(kSortThreads), smem, st, overlap_launches(kOverlapRowwise), kSortCtas,
+                                  typed, n, V, padding_idx, reinterpret_cast<uint32_t*>(at + s.keys), reinterpret_cast<uint32_t*>(at + s.places),
+                                  reinterpret_cast<int*>(at + s.begin), reinterpret_cast<int*>(at + s.end), passes, digit_bits));
+  };
+  rc = id_bytes == 8 ? sort(static_cast<const long long*>(ids), sort_ids_kernel<long long>) : sort(static_cast<const int*>(ids), sort_ids_kernel<int>);
+  if (rc != NLFA_OK) return rc;
+  const int word = word_bytes(static_cast<long long>(d) * bytes, g, dw), sorted = passes & 1;
+#define NLFA_GO(T, W) gradient<T, W>(g, s, at, sorted, dw, n, V, d, scale, st)
+#define NLFA_16(T) (word == 16 ? NLFA_GO(T, 16) : word == 8 ? NLFA_GO(T, 8) : word == 4 ? NLFA_GO(T, 4) : NLFA_GO(T, 2))
+  if (dtype == NLFA_DTYPE_F32) return word == 16 ? NLFA_GO(float, 16) : word == 8 ? NLFA_GO(float, 8) : NLFA_GO(float, 4);
+  return dtype == NLFA_DTYPE_F16 ? NLFA_16(__half) : NLFA_16(__nv_bfloat16);
+#undef NLFA_16
+#undef NLFA_GO
+}
+
+}  // extern "C"

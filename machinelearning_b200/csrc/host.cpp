@@ -1,4 +1,4 @@
-// The call path between torch and the C ABI, in C++: what flash_cuda.py, qk_prologue.py and value_gate.py do per
+// The call path between torch and the C ABI, in C++: what flash_cuda.py, qk_prologue.py, value_gate.py and the modules of the step's ends do per
 // call -- checks, casts, output allocation, the autograd node, the launch -- without Python in it.
 //
 // Why: the kernels of a small call are a few microseconds, and with the Python forms of these functions (ctypes
@@ -25,6 +25,9 @@
 #include <torch/csrc/utils/object_ptr.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <ATen/MemoryOverlap.h>
+
+#include <algorithm>
 #include <cmath>
 
 #include "../../include/nlfa.h"
@@ -340,6 +343,172 @@ Tensor head_gate(const Tensor& y_in, const Tensor& gate_in) {
   return out;
 }
 
+// ------------------------------------------------------------------------------------------- head with its loss
+
+struct LinearCe {
+  int64_t ignore_index;
+  int reduction, dtype;
+};
+
+struct CeShape {
+  int n, V, d, x, w;
+};
+
+std::pair<Tensor, Tensor> linear_ce_forward(const Tensor& x, const Tensor& w, const Tensor& targets, LinearCe c) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const CeShape s{static_cast<int>(targets.numel()), static_cast<int>(w.size(0)), static_cast<int>(w.size(1)),
+                  dtype_code(x.scalar_type()), dtype_code(w.scalar_type())};
+  Tensor loss = empty(c.reduction == NLFA_REDUCE_NONE ? targets.sizes() : at::IntArrayRef{}, at::kFloat, x);
+  Tensor tape = empty({static_cast<int64_t>(nlfa_linear_ce_tape_bytes(w.data_ptr(), s.n, s.V, s.d, s.x, s.w, c.dtype))}, at::kByte, x);
+  Tensor scratch = empty({static_cast<int64_t>(nlfa_linear_ce_scratch_bytes(s.n, s.V, s.d, s.x, s.w, c.dtype, 0))}, at::kByte, x);
+  check("nlfa_linear_ce_fwd",
+        nlfa_linear_ce_fwd(x.data_ptr(), s.x, w.data_ptr(), s.w, c.dtype, targets.data_ptr(), static_cast<int>(targets.element_size()),
+                           s.n, s.V, s.d, c.ignore_index, c.reduction, static_cast<float*>(loss.data_ptr()), tape.data_ptr(),
+                           static_cast<size_t>(tape.numel()), scratch.data_ptr(), static_cast<size_t>(scratch.numel()), stream_of(x)));
+  return {loss, tape};
+}
+
+struct LinearCrossEntropyBackward : public Node {
+  SavedVariable w, targets, tape;
+  std::vector<int64_t> x_shape;
+  at::ScalarType x_dtype;
+  LinearCe call;
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return {Tensor(), Tensor()};
+    Tensor w_ = w.unpack(), t_ = targets.unpack(), tape_ = tape.unpack();
+    const c10::cuda::CUDAGuard guard(w_.device());
+    Tensor g = contiguous(cast(grads[0], at::kFloat)), dx, dw;
+    if (task_should_compute_output(0)) dx = empty(x_shape, x_dtype, w_);
+    if (task_should_compute_output(1)) dw = empty_as(w_);
+    const CeShape s{static_cast<int>(t_.numel()), static_cast<int>(w_.size(0)), static_cast<int>(w_.size(1)), dtype_code(x_dtype),
+                    dtype_code(w_.scalar_type())};
+    Tensor scratch = empty({static_cast<int64_t>(nlfa_linear_ce_scratch_bytes(s.n, s.V, s.d, s.x, s.w, call.dtype, 1))}, at::kByte, w_);
+    check("nlfa_linear_ce_bwd",
+          nlfa_linear_ce_bwd(static_cast<const float*>(g.data_ptr()), w_.data_ptr(), s.w, s.x, call.dtype, t_.data_ptr(),
+                             static_cast<int>(t_.element_size()), s.n, s.V, s.d, call.ignore_index, call.reduction, tape_.data_ptr(),
+                             static_cast<size_t>(tape_.numel()), dx.defined() ? dx.data_ptr() : nullptr,
+                             dw.defined() ? dw.data_ptr() : nullptr, scratch.data_ptr(), static_cast<size_t>(scratch.numel()), stream_of(w_)));
+    variable_list out;
+    for (const Tensor& t : {dx, dw})
+      if (t.defined()) out.push_back(t);
+    out = once(std::move(out), grads[0]);
+    size_t at = 0;
+    return {dx.defined() ? out[at++] : Tensor(), dw.defined() ? out[at] : Tensor()};
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&w, &targets, &tape}) v->reset_data();
+  }
+  std::string name() const override { return "LinearCrossEntropyBackward"; }
+};
+
+// ------------------------------------------------------------------------------------------- token embedding
+
+Tensor embedding_forward(const Tensor& ids, const Tensor& w, double scale) {
+  const c10::cuda::CUDAGuard guard(w.device());
+  std::vector<int64_t> shape = ids.sizes().vec();
+  shape.push_back(w.size(1));
+  Tensor out = empty(shape, w.scalar_type(), w);
+  check("nlfa_embedding_fwd",
+        nlfa_embedding_fwd(ids.data_ptr(), static_cast<int>(ids.element_size()), w.data_ptr(), dtype_code(w.scalar_type()), out.data_ptr(),
+                           static_cast<int>(ids.numel()), static_cast<int>(w.size(0)), static_cast<int>(w.size(1)),
+                           static_cast<float>(scale), stream_of(w)));
+  return out;
+}
+
+struct TokenEmbeddingBackward : public Node {
+  SavedVariable ids;
+  int64_t V, d, padding;
+  at::ScalarType dtype;
+  double scale;
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return {Tensor()};
+    Tensor ids_ = ids.unpack();
+    const c10::cuda::CUDAGuard guard(ids_.device());
+    Tensor g = contiguous(cast(grads[0], dtype)), dw = empty({V, d}, dtype, ids_);
+    const int n = static_cast<int>(ids_.numel()), rows = static_cast<int>(V), cols = static_cast<int>(d);
+    Tensor scratch = empty({static_cast<int64_t>(nlfa_embedding_scratch_bytes(n, rows, cols))}, at::kByte, ids_);
+    check("nlfa_embedding_bwd",
+          nlfa_embedding_bwd(g.data_ptr(), dtype_code(dtype), ids_.data_ptr(), static_cast<int>(ids_.element_size()), dw.data_ptr(), n, rows,
+                             cols, static_cast<float>(scale), padding, scratch.data_ptr(), static_cast<size_t>(scratch.numel()),
+                             stream_of(ids_)));
+    return once({dw}, grads[0]);
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    ids.reset_data();
+  }
+  std::string name() const override { return "TokenEmbeddingBackward"; }
+};
+
+// ------------------------------------------------------------------------------------------- gradient clip
+
+// Norm of the tensors, and their clip: see grad_clip.py, which documents the refusals.
+Tensor clip_grads(std::vector<Tensor> grads, const std::vector<Tensor>& outs, double max_norm, int norm, bool scale) {
+  TORCH_CHECK_VALUE(!grads.empty(), "clip_grads: no gradients");
+  TORCH_CHECK_VALUE(outs.empty() || outs.size() == grads.size(), "out: ", outs.size(), " tensors for ", grads.size(), " gradients");
+  TORCH_CHECK_VALUE(plain(grads[0]), "gradients must be plain CUDA tensors");
+  const c10::cuda::CUDAGuard guard(grads[0].device());
+  const Tensor like = grads[0];
+  std::vector<nlfa_grad> table;
+  std::vector<std::pair<Tensor, Tensor>> copies;                       // (gradient with gaps, its copy)
+  struct Span {
+    uintptr_t from, to;
+    size_t of;
+  };
+  std::vector<Span> spans;
+  table.reserve(grads.size());
+  for (size_t i = 0; i < grads.size(); ++i) {
+    Tensor g = grads[i], o = outs.empty() ? Tensor() : outs[i];
+    const Tensor given = g;
+    TORCH_CHECK_VALUE(plain(g) && g.device() == like.device() && dtype_code(g.scalar_type()) >= 0,
+                      "gradient ", i, ": needs a plain float32, float16 or bfloat16 tensor on ", like.device());
+    if (o.defined()) {
+      TORCH_CHECK_VALUE(plain(o) && o.device() == like.device() && dtype_code(o.scalar_type()) >= 0 && o.sizes() == g.sizes(),
+                        "out ", i, ": needs a plain float32, float16 or bfloat16 tensor of the gradient's shape on ", like.device());
+      TORCH_CHECK_VALUE(!o.requires_grad() || !at::GradMode::is_enabled(), "out ", i, " requires a gradient");
+      TORCH_CHECK_VALUE(o.is_non_overlapping_and_dense(), "out ", i, " must be dense");
+      if (g.strides() != o.strides()) g = at::empty_strided(o.sizes(), o.strides(), g.options()).copy_(g.detach());
+    } else if (!g.is_non_overlapping_and_dense()) {
+      Tensor c = g.detach().contiguous();
+      if (scale) {
+        TORCH_CHECK_VALUE(at::has_internal_overlap(g) != at::MemOverlap::Yes, "gradient ", i, " has elements that share memory");
+        copies.emplace_back(g, c);
+      }
+      g = c;
+    }
+    grads[i] = g;
+    if (g.numel() == 0) continue;
+    table.push_back({g.data_ptr(), o.defined() ? o.data_ptr() : nullptr, g.numel(), dtype_code(g.scalar_type()),
+                     o.defined() ? dtype_code(o.scalar_type()) : 0});
+    if (!scale) continue;
+    auto span = [&](const Tensor& t) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
+      spans.push_back({at, at + static_cast<uintptr_t>(t.numel()) * t.element_size(), i});
+    };
+    if (given.is_non_overlapping_and_dense()) span(given);
+    if (o.defined() && !(o.data_ptr() == given.data_ptr() && o.scalar_type() == given.scalar_type() && o.strides() == given.strides()))
+      span(o);
+  }
+  if (scale) {
+    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+    for (size_t i = 1; i < spans.size(); ++i)
+      TORCH_CHECK_VALUE(spans[i].from >= spans[i - 1].to, "tensors ", spans[i - 1].of, " and ", spans[i].of,
+                        " share memory (a parameter given twice?)");
+  }
+  Tensor total = empty({}, at::kFloat, like);
+  Tensor scratch = empty({static_cast<int64_t>(nlfa_clip_scratch_bytes())}, at::kByte, like);
+  check("nlfa_clip_grads", nlfa_clip_grads(table.data(), static_cast<int>(table.size()), static_cast<float>(max_norm), norm, scale ? 1 : 0,
+                                           static_cast<float*>(total.data_ptr()), scratch.data_ptr(), static_cast<size_t>(scratch.numel()),
+                                           stream_of(like)));
+  for (auto& [g, c] : copies) g.detach().copy_(c);
+  if (scale)
+    for (const Tensor& t : outs.empty() ? grads : outs) t.unsafeGetTensorImpl()->bump_version();
+  return total;
+}
+
 // ------------------------------------------------------------------------------------------- Python entries
 
 bool is_tensor(PyObject* o) { return THPVariable_Check(o); }
@@ -593,6 +762,112 @@ PyObject* py_head_gate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// linear_ce(x, weight, targets, ignore_index, reduction code) -> loss | None
+PyObject* py_linear_ce(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || !is_tensor(a[0]) || !is_tensor(a[1]) || !is_tensor(a[2])) return decline();
+  Tensor x = tensor(a[0]), w = tensor(a[1]), t = tensor(a[2]);
+  if (!plain(x) || !plain(w) || !plain(t) || !watched(x) || w.device() != x.device() || t.device() != x.device() || x.dim() < 1 ||
+      w.dim() != 2 || dtype_code(x.scalar_type()) < 0 || dtype_code(w.scalar_type()) < 0 || !PyLong_Check(a[3]))
+    return decline();
+  const auto ac = autocast_dtype();
+  if (!ac && x.scalar_type() != w.scalar_type()) return decline();
+  const int dtype = dtype_code(ac ? *ac : x.scalar_type());
+  constexpr int64_t kMost = int64_t(1) << 30;
+  if (dtype < 0 || (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt) || t.sizes() != x.sizes().slice(0, x.dim() - 1) ||
+      w.size(1) != x.size(-1) || w.size(1) < 1 || w.size(1) > (1 << 24) || w.size(0) < 1 || w.size(0) > kMost || t.numel() > kMost)
+    return decline();
+  const long long ignore = PyLong_AsLongLong(a[3]);
+  if (ignore == -1 && PyErr_Occurred()) throw python_error();
+  const LinearCe call{ignore, integer(a[4]), dtype};
+  Tensor loss;
+  {
+    py::gil_scoped_release no_gil;
+    const c10::cuda::CUDAGuard guard(x.device());
+    x = contiguous(x);
+    w = contiguous(w);
+    t = contiguous(t);
+    Tensor tape;
+    std::tie(loss, tape) = linear_ce_forward(x, w, t, call);
+    if (recording({&x, &w})) {
+      auto node = make_node<LinearCrossEntropyBackward>();
+      node->set_next_edges(torch::autograd::collect_next_edges(x, w));
+      node->w = SavedVariable(w, false);
+      node->targets = SavedVariable(t, false);
+      node->tape = SavedVariable(tape, false);
+      node->x_shape = x.sizes().vec();
+      node->x_dtype = x.scalar_type();
+      node->call = call;
+      torch::autograd::set_history(loss, node);
+    }
+  }
+  return THPVariable_Wrap(loss);
+  END_HANDLE_TH_ERRORS
+}
+
+// embedding(ids, weight, scale, padding) -> out | None
+PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4 || !is_tensor(a[0]) || !is_tensor(a[1])) return decline();
+  Tensor ids = tensor(a[0]), w = tensor(a[1]);
+  constexpr int64_t kMost = int64_t(1) << 30;
+  if (!plain(ids) || !plain(w) || ids.device() != w.device() || w.dim() != 2 || dtype_code(w.scalar_type()) < 0 ||
+      (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) || w.size(0) < 1 || w.size(0) > kMost || w.size(1) < 1 ||
+      w.size(1) > (1 << 24) || ids.numel() > kMost)
+    return decline();
+  const double scale = number(a[2]);
+  const int64_t padding = integer(a[3]);
+  Tensor out;
+  {
+    py::gil_scoped_release no_gil;
+    ids = contiguous(ids);
+    w = contiguous(w);
+    out = embedding_forward(ids, w, scale);
+    if (recording({&w})) {
+      auto node = make_node<TokenEmbeddingBackward>();
+      node->set_next_edges(torch::autograd::collect_next_edges(w));
+      node->ids = SavedVariable(ids, false);
+      node->V = w.size(0);
+      node->d = w.size(1);
+      node->padding = padding;
+      node->dtype = w.scalar_type();
+      node->scale = scale;
+      torch::autograd::set_history(out, node);
+    }
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// clip_grads(list of tensors, list of tensors | None, max_norm, norm code, scale) -> norm
+PyObject* py_clip_grads(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 5, "clip_grads takes 5 arguments");
+  auto tensors = [](PyObject* o, const char* what) {
+    std::vector<Tensor> v;
+    if (o == Py_None) return v;
+    TORCH_CHECK_TYPE(PyList_Check(o), what, " must be a list of tensors");
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(o); ++i) {
+      PyObject* t = PyList_GET_ITEM(o, i);
+      TORCH_CHECK_TYPE(is_tensor(t), what, " ", i, " must be a tensor, not ", Py_TYPE(t)->tp_name);
+      v.push_back(tensor(t));
+    }
+    return v;
+  };
+  std::vector<Tensor> grads = tensors(a[0], "gradient"), outs = tensors(a[1], "out");
+  const double max_norm = number(a[2]);
+  const int norm = integer(a[3]);
+  const bool scale = truth(a[4]);
+  TORCH_CHECK_VALUE(a[1] == Py_None || outs.size() == grads.size(), "out: ", outs.size(), " tensors for ", grads.size(), " gradients");
+  Tensor total;
+  {
+    py::gil_scoped_release no_gil;
+    total = clip_grads(std::move(grads), outs, max_norm, norm, scale);
+  }
+  return THPVariable_Wrap(total);
+  END_HANDLE_TH_ERRORS
+}
+
 // configure(check, tensor_cores): _lib.check and whether the self-test passed;  watch(device index)
 PyObject* py_configure(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -615,8 +890,9 @@ PyObject* py_watch(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define NLFA_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {NLFA_METHOD(attn),        NLFA_METHOD(attn_fwd),    NLFA_METHOD(attn_bwd),  NLFA_METHOD(attn_cached),
-                           NLFA_METHOD(qk_prologue), NLFA_METHOD(value_blend), NLFA_METHOD(head_gate), NLFA_METHOD(configure),
-                           NLFA_METHOD(watch),       {nullptr, nullptr, 0, nullptr}};
+                           NLFA_METHOD(qk_prologue), NLFA_METHOD(value_blend), NLFA_METHOD(head_gate), NLFA_METHOD(linear_ce),
+                           NLFA_METHOD(embedding),   NLFA_METHOD(clip_grads),  NLFA_METHOD(configure), NLFA_METHOD(watch),
+                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", "torch-facing call path of libnlfa (host.cpp)", -1, g_methods};
 
 }  // namespace

@@ -1,0 +1,575 @@
+// Linear cross entropy: the loss of a language model's head without its logits.
+//
+//   l_iv = x_i . w_v,  lse_i = log sum_v exp(l_iv),  loss_i = lse_i - l_i,t(i)
+//   dl_iv = g_i (exp(l_iv - lse_i) - [v == t(i)]),  dx = dl W,  dW = dl^T x
+//
+// The logits of N = 65,536 tokens over 50,304 words are 13 GB in float32.  The forward (loss_tc.cu) keeps each row's maximum
+// and sum; the backward goes through the vocabulary in pieces, forms dl of a piece in a workspace and multiplies it
+// both ways: four products of 2 N V d operations in all.  This file has what goes before and after: the rows that have a
+// target, packed (rows without one cost nothing and reach nothing, whatever they hold); 16-bit copies of operands that the products
+// cannot read as they are (float32: sums of three bf16 parts, exact to 2^-24); the sum of the losses.
+#include <climits>
+#include <cmath>
+
+#include "loss.cuh"
+#include "rowwise.cuh"
+
+namespace nlfa {
+
+unsigned* status_block();      // api.cu
+
+namespace loss {
+namespace {
+
+using rowwise::aligned16;
+using rowwise::dtype_ok;
+using rowwise::last_cta;
+
+constexpr int kScanCtas = 8, kScanThreads = 1024;
+constexpr int kBlock = 256;
+
+// ------------------------------------------------------------------------------------------------ rows with a target
+
+template <typename I>
+__device__ __forceinline__ bool counts(I t, long long ignore) { return static_cast<long long>(t) != ignore; }
+
+// One cluster: each CTA takes a run of the rows, counts those that have a target, learns the counts in front of its own from
+// the others, and writes its rows' numbers in order.  Rows behind the last one, up to a whole tile, are set empty.
+template <typename I>
+__global__ void __launch_bounds__(kScanThreads)
+pack_rows_kernel(const I* __restrict__ targets, int n, int n_rows, int V, long long ignore, Head* head, int* __restrict__ row_of,
+                 int* __restrict__ target, float* __restrict__ at_target, float* __restrict__ each, int col_tiles, int pairs,
+                 int max_splits) {
+  __shared__ int warp_count[32];
+  __shared__ int total;
+  grid_dep_wait();
+  grid_dep_release();
+  const int rank = static_cast<int>(cluster_rank());
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int run = ((n + kScanCtas - 1) / kScanCtas + kScanThreads - 1) / kScanThreads * kScanThreads;
+  const long long lo = static_cast<long long>(run) * rank;
+  const int from = lo < n ? static_cast<int>(lo) : n, to = n - from < run ? n : from + run;
+
+  int mine = 0;
+  for (int i = from + threadIdx.x; i < to; i += kScanThreads) mine += counts(targets[i], ignore) ? 1 : 0;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
+  if (lane == 0) warp_count[warp] = mine;
+  __syncthreads();
+  if (warp == 0) {
+    int v = warp_count[lane];
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    if (lane == 0) total = v;
+  }
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  int at = 0, all = 0;
+  for (int r = 0; r < kScanCtas; ++r) {
+    int v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(smem_u32(&total), r)) : "memory");
+    if (r < rank) at += v;
+    all += v;
+  }
+  cluster_arrive();                        // (the others' shared memory is no longer read)
+
+  for (int i0 = from; i0 < to; i0 += kScanThreads) {
+    const int i = i0 + threadIdx.x;
+    const bool in = i < to;
+    const long long t = in ? static_cast<long long>(targets[i]) : 0;
+    const bool has = in && counts(t, ignore);
+    const unsigned b = __ballot_sync(0xffffffffu, has);
+    __syncthreads();
+    if (lane == 0) warp_count[warp] = __popc(b);
+    __syncthreads();
+    int before = 0, sum = 0;
+    for (int w = 0; w < 32; ++w) {
+      const int c = warp_count[w];
+      if (w < warp) before += c;
+      sum += c;
+    }
+    if (has) {
+      const int r = at + before + __popc(b & ((1u << lane) - 1u));
+      row_of[r] = i;
+      // a target outside the vocabulary: its logit stays NaN, and so do its loss and its gradients (-2: see scale_rows)
+      target[r] = t >= 0 && t < V ? static_cast<int>(t) : -2;
+      at_target[r] = __int_as_float(0x7fffffff);
+    } else if (in && each != nullptr) {
+      each[i] = 0.f;
+    }
+    at += sum;
+  }
+  // rows up to the end of the last tile
+  const int end = all < kRowTile ? kRowTile : (all + kRowTile - 1) / kRowTile * kRowTile;
+  for (int r = all + rank * kScanThreads + threadIdx.x; r < end; r += kScanCtas * kScanThreads) {
+    row_of[r] = -1;
+    target[r] = -1;
+    at_target[r] = 0.f;
+  }
+  if (rank == 0 && warp == 0) {
+    // Parts of the vocabulary per row tile, so that the pairs of CTAs end together: the fewest column tiles for the busiest
+    // pair, counted with one more per unit for its start; of equals the fewest parts.
+    const int row_tiles = end / kRowTile;
+    long long best = LLONG_MAX;
+    for (int s = 1 + lane; s <= max_splits; s += 32) {
+      const long long units = (static_cast<long long>(row_tiles) * s + pairs - 1) / pairs;
+      const long long cost = units * ((col_tiles + s - 1) / s) * 4 + units;
+      if (cost < (best >> 12)) best = (cost << 12) | s;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+      const long long o = __shfl_xor_sync(0xffffffffu, best, off);
+      best = o < best ? o : best;
+    }
+    if (lane == 0) {
+      head->count = all;
+      head->splits = static_cast<int>(best & 4095);
+    }
+  }
+  cluster_wait();
+}
+
+// ------------------------------------------------------------------------------------------------ 16-bit operands
+
+template <typename T> __device__ __forceinline__ float load1(const T* p) { return static_cast<float>(*p); }
+
+// dst [planes][n_rows][d_pad] <- rows of src [*, d]: row r from row_of[r] (or r itself), zeros behind the last one and behind
+// column d.  planes = 3: dst = a + b + c, each the nearest bf16 value to what is left.  Eight columns a thread.
+template <typename S, typename T>
+__global__ void __launch_bounds__(kBlock)
+copy_rows_kernel(const S* __restrict__ src, T* __restrict__ dst, const Head* head, const int* __restrict__ row_of, int n_src,
+                 int n_rows, int d, int d_pad, int planes, int vec) {
+  grid_dep_wait();
+  grid_dep_release();
+  int end = n_src;
+  if (row_of != nullptr) {
+    const int all = head->count;
+    end = all < kRowTile ? kRowTile : (all + kRowTile - 1) / kRowTile * kRowTile;
+  }
+  const int chunks = d_pad / 8;
+  const long long total = static_cast<long long>(end) * chunks;
+  for (long long i = static_cast<long long>(blockIdx.x) * kBlock + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * kBlock) {
+    const int r = static_cast<int>(i / chunks), c = 8 * static_cast<int>(i - static_cast<long long>(r) * chunks);
+    const int from = row_of != nullptr ? row_of[r] : r;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    if (from >= 0) {
+      const S* s = src + static_cast<size_t>(from) * d + c;
+      if (vec) rowwise::Elem<S>::load(s, v);
+      else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c + j < d) v[j] = load1(s + j);
+      }
+    }
+    T* o = dst + static_cast<size_t>(r) * d_pad + c;
+    for (int part = 0; part < planes; ++part) {
+      rowwise::Elem<T>::store(o, v);
+      o += static_cast<size_t>(n_rows) * d_pad;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] -= rowwise::Elem<T>::round(v[j]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ losses
+
+// (max, sum) of a row's parts -> lse, loss.  Rows behind the last one get lse = +inf: their probabilities are zero.
+__global__ void __launch_bounds__(kBlock)
+finish_kernel(const Head* head, const float2* __restrict__ partial, const float* __restrict__ at_target, const int* __restrict__ row_of,
+              int n_rows, float* __restrict__ lse, float* __restrict__ lse_rest, float* __restrict__ each, float* __restrict__ out, double* sums, unsigned* ticket,
+              int mean) {
+  __shared__ double warp_sum[kBlock / 32];
+  __shared__ int last;
+  grid_dep_wait();
+  grid_dep_release();
+  const int all = head->count, parts = 2 * head->splits;
+  const int end = all < kRowTile ? kRowTile : (all + kRowTile - 1) / kRowTile * kRowTile;
+  double sum = 0.0;
+  for (int r = blockIdx.x * kBlock + threadIdx.x; r < end; r += gridDim.x * kBlock) {
+    if (r >= all) {
+      lse[r] = INFINITY;
+      lse_rest[r] = 0.f;
+      continue;
+    }
+    float top = -INFINITY;
+    for (int s = 0; s < parts; ++s) top = fmaxf(top, partial[static_cast<size_t>(s) * n_rows + r].x);
+    const float shift = top == -INFINITY ? 0.f : top;
+    float total = 0.f;
+    for (int s = 0; s < parts; ++s) {
+      const float2 q = partial[static_cast<size_t>(s) * n_rows + r];
+      total += q.y * expf(q.x - shift);
+    }
+    const float rest = logf(total);
+    lse[r] = shift + rest;
+    lse_rest[r] = rest - (lse[r] - shift);                // (NaN where lse is not finite)
+    const float loss = (shift - at_target[r]) + rest;
+    if (each != nullptr) each[row_of[r]] = loss;
+    sum += loss;
+  }
+  if (out == nullptr) return;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int w = 0; w < kBlock / 32; ++w) t += warp_sum[w];
+    sums[blockIdx.x] = t;
+  }
+  if (!last_cta(ticket, gridDim.x, &last)) return;
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (unsigned i = 0; i < gridDim.x; ++i) t += __ldcg(sums + i);
+    *out = static_cast<float>(mean ? t / all : t);       // (no target at all: 0 / 0)
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+
+// Factors of dl: g_i = alpha * row_scale_i with |row_scale| <= 2^14 (fp16, whose small probabilities would not be normal numbers
+// otherwise) or 1.  `grad` is one value, or one per row of the call (per_row).  One CTA.
+__global__ void __launch_bounds__(1024)
+scale_rows_kernel(const Head* head, const float* __restrict__ grad, int per_row, int mean, const int* __restrict__ row_of,
+                  const int* __restrict__ target, float* __restrict__ row_scale, float* __restrict__ alpha, float unit) {
+  __shared__ float warp_top[32];
+  grid_dep_wait();
+  grid_dep_release();
+  const int all = head->count;
+  const int end = all < kRowTile ? kRowTile : (all + kRowTile - 1) / kRowTile * kRowTile;
+  float top = 0.f;                                        // the largest finite one
+  if (per_row) {
+    for (int r = threadIdx.x; r < all; r += 1024) {
+      const float g = fabsf(grad[row_of[r]]);
+      if (g > top && g < INFINITY) top = g;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = 0.f;
+    for (int w = 0; w < 32; ++w) top = fmaxf(top, warp_top[w]);
+    if (top == 0.f) top = 1.f;
+  }
+  for (int r = threadIdx.x; r < end; r += 1024) {
+    float s = 0.f;
+    if (r < all) {
+      s = unit;
+      if (per_row) s = grad[row_of[r]] / top * unit;
+      if (target[r] == -2) s = __int_as_float(0x7fffffff);
+    }
+    row_scale[r] = s;
+  }
+  if (threadIdx.x == 0) {
+    const float g = per_row ? top : mean ? *grad / static_cast<float>(all) : *grad;
+    *alpha = all > 0 ? g / unit : 0.f;                    // (no target: gradients of zero, not 0 / 0)
+  }
+}
+
+// zeros in the rows of dx that have no target
+template <typename I>
+__global__ void __launch_bounds__(kBlock)
+clear_rows_kernel(const I* __restrict__ targets, int n, long long ignore, const Head* head, uint8_t* __restrict__ dx, long long row_bytes) {
+  grid_dep_wait();
+  grid_dep_release();
+  if (head->count == n) return;
+  const int lane = threadIdx.x & 31;
+  for (int r = blockIdx.x * (kBlock / 32) + (threadIdx.x >> 5); r < n; r += gridDim.x * (kBlock / 32)) {
+    if (counts(targets[r], ignore)) continue;
+    uint8_t* o = dx + static_cast<size_t>(r) * row_bytes;
+    if ((row_bytes & 15) == 0)
+      for (long long i = 16 * lane; i < row_bytes; i += 512) *reinterpret_cast<uint4*>(o + i) = make_uint4(0u, 0u, 0u, 0u);
+    else
+      for (long long i = 2 * lane; i < row_bytes; i += 64) *reinterpret_cast<uint16_t*>(o + i) = 0;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+
+struct Call {
+  int x_dtype, w_dtype, dtype;      // dtype: what the products read (NLFA_DTYPE_BF16 for float32: three parts)
+  int n, V, d;
+};
+
+size_t up(size_t v) { return (v + 255) / 256 * 256; }
+
+int check_call(const Call& c) {
+  if (c.n < 0 || c.V < 1 || c.d < 1 || c.n > (1 << 30) || c.V > (1 << 30) || c.d > (1 << 24)) return NLFA_ERR_BAD_SHAPE;
+  if (!dtype_ok(c.x_dtype) || !dtype_ok(c.w_dtype) || !dtype_ok(c.dtype)) return NLFA_ERR_BAD_DTYPE;
+  return NLFA_OK;
+}
+
+Layout layout(const Call& c, bool w_aligned) {
+  Layout l{};
+  l.n_rows = c.n < kRowTile ? kRowTile : (c.n + kRowTile - 1) / kRowTile * kRowTile;
+  l.d_pad = (c.d + 7) / 8 * 8;
+  l.x_planes = c.dtype == NLFA_DTYPE_F32 ? 3 : 1;
+  l.copy_w = l.x_planes == 3 || c.w_dtype != c.dtype || c.d % 8 != 0 || !w_aligned;
+  size_t at = 256;                                        // the head
+  const size_t rows = static_cast<size_t>(l.n_rows) * 4;
+  l.row_of = at; at = up(at + rows);
+  l.target = at; at = up(at + rows);
+  l.lse = at; at = up(at + rows);
+  l.lse_rest = at; at = up(at + rows);
+  l.x = at; at = up(at + static_cast<size_t>(l.x_planes) * l.n_rows * l.d_pad * 2);
+  l.w = at; if (l.copy_w) at = up(at + static_cast<size_t>(l.x_planes) * c.V * l.d_pad * 2);
+  l.tape_bytes = at;
+  // parts of the vocabulary: enough for every pair of CTAs when there is one row tile, few when there are many
+  const int col_tiles = (c.V + kColTile - 1) / kColTile, row_tiles = l.n_rows / kRowTile;
+  int most = 256 / row_tiles > 8 ? 256 / row_tiles : 8;
+  l.max_splits = most < col_tiles ? most : col_tiles;
+  at = 0;
+  l.partial = at; at = up(at + static_cast<size_t>(2 * l.max_splits) * l.n_rows * sizeof(float2));
+  l.at_target = at; at = up(at + rows);
+  l.sums = at; at = up(at + 1024 * sizeof(double));
+  l.ticket = at; at = up(at + 4);
+  l.fwd_bytes = at;
+  return l;
+}
+
+// The backward's pieces of the vocabulary: dl of one takes at most this.
+constexpr size_t kMostDl = 512ull << 20;
+
+struct BwdLayout {
+  int piece;                        // columns, a multiple of kColTile
+  size_t row_scale, alpha, dl, dx_sum, bytes;
+};
+BwdLayout bwd_layout(const Call& c, const Layout& l) {
+  BwdLayout b{};
+  const size_t column = static_cast<size_t>(l.x_planes) * l.n_rows * 2;
+  const int col_tiles = (c.V + kColTile - 1) / kColTile;
+  size_t most = kMostDl / (column * kColTile);
+  if (most < 1) most = 1;
+  const int pieces = static_cast<int>((col_tiles + most - 1) / most);
+  b.piece = (col_tiles + pieces - 1) / pieces * kColTile;
+  size_t at = 0;
+  b.row_scale = at; at = up(at + static_cast<size_t>(l.n_rows) * 4);
+  b.alpha = at; at = up(at + 4);
+  b.dl = at; at = up(at + column * b.piece);
+  b.dx_sum = at; if (pieces > 1) at = up(at + static_cast<size_t>(l.n_rows) * c.d * 4);
+  b.bytes = at;
+  return b;
+}
+
+int box_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes, int box_rows) {
+  const unsigned long long dims[4] = {static_cast<unsigned long long>(cols), static_cast<unsigned long long>(rows),
+                                      static_cast<unsigned long long>(planes), 1ull};
+  const unsigned long long strides[3] = {dims[0] * 2, dims[0] * dims[1] * 2, dims[0] * dims[1] * dims[2] * 2};
+  const unsigned box[4] = {64u, static_cast<unsigned>(box_rows), 1u, 1u};
+  return make_map(map, base, dtype, dims, strides, box);
+}
+
+int checked(cudaError_t e) {
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e == cudaSuccess ? NLFA_OK : NLFA_ERR_CUDA;
+}
+
+template <typename S, typename T>
+int copy_rows_typed(const void* src, void* dst, const Head* head, const int* row_of, int n_src, int n_rows, int d, int d_pad,
+                    int planes, cudaStream_t st) {
+  const int vec = d % 8 == 0 && aligned16(src) ? 1 : 0;
+  const long long work = static_cast<long long>(row_of != nullptr ? n_rows : n_src) * (d_pad / 8);
+  const long long most = 16ll * sm_count();
+  const long long need = (work + kBlock - 1) / kBlock;
+  return checked(launch_kernel(copy_rows_kernel<S, T>, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(kBlock), 0, st,
+                               overlap_launches(kOverlapRowwise), static_cast<const S*>(src), static_cast<T*>(dst), head, row_of,
+                               n_src, n_rows, d, d_pad, planes, vec));
+}
+int copy_rows(const void* src, int src_dtype, void* dst, int dtype, const Head* head, const int* row_of, int n_src, int n_rows,
+              int d, int d_pad, int planes, cudaStream_t st) {
+#define NLFA_TO(S) (dtype == NLFA_DTYPE_F16 ? copy_rows_typed<S, __half>(src, dst, head, row_of, n_src, n_rows, d, d_pad, planes, st) \
+                                            : copy_rows_typed<S, __nv_bfloat16>(src, dst, head, row_of, n_src, n_rows, d, d_pad, planes, st))
+  if (src_dtype == NLFA_DTYPE_F32) return NLFA_TO(float);
+  if (src_dtype == NLFA_DTYPE_F16) return NLFA_TO(__half);
+  return NLFA_TO(__nv_bfloat16);
+#undef NLFA_TO
+}
+
+struct Pointers {
+  uint8_t* tape;
+  const Layout& l;
+  Head* head() const { return reinterpret_cast<Head*>(tape); }
+  int* row_of() const { return reinterpret_cast<int*>(tape + l.row_of); }
+  int* target() const { return reinterpret_cast<int*>(tape + l.target); }
+  float* lse() const { return reinterpret_cast<float*>(tape + l.lse); }
+  float* lse_rest() const { return reinterpret_cast<float*>(tape + l.lse_rest); }
+};
+
+Params params(const Call& c, const Layout& l, const Pointers& t, unsigned* status) {
+  Params p{};
+  p.head = t.head();
+  p.V = c.V;
+  p.d = c.d;
+  p.d_pad = l.d_pad;
+  p.planes = l.x_planes;
+  p.pairs = l.x_planes == 3 ? 6 : 1;
+  p.n_rows = l.n_rows;
+  p.target = t.target();
+  p.lse = t.lse();
+  p.lse_rest = t.lse_rest();
+  p.row_of = t.row_of();
+  p.status = status;
+  return p;
+}
+
+int run_fwd(const Call& c, const void* x, const void* w, const void* targets, int target_bytes, long long ignore, int reduction,
+            float* out, uint8_t* tape, uint8_t* scratch, cudaStream_t st) {
+  const Layout l = layout(c, aligned16(w));
+  const Pointers t{tape, l};
+  unsigned* status = status_block();
+  if (!status) return NLFA_ERR_CUDA;
+  const int dtype = c.dtype == NLFA_DTYPE_F32 ? NLFA_DTYPE_BF16 : c.dtype;
+  float* at_target = reinterpret_cast<float*>(scratch + l.at_target);
+  float* each = reduction == NLFA_REDUCE_NONE ? out : nullptr;
+  const bool overlap = overlap_launches(kOverlapRowwise);
+  const int col_tiles = (c.V + kColTile - 1) / kColTile;
+  auto pack = [&](auto* typed, auto* kernel) {
+    return checked(launch_cluster(kernel, dim3(1, kScanCtas), dim3(kScanThreads), 0, st, overlap, kScanCtas, typed, c.n, l.n_rows, c.V,
+                                  ignore, t.head(), t.row_of(), t.target(), at_target, each, col_tiles, sm_count() / 2, l.max_splits));
+  };
+  int rc = target_bytes == 8 ? pack(static_cast<const long long*>(targets), pack_rows_kernel<long long>)
+                             : pack(static_cast<const int*>(targets), pack_rows_kernel<int>);
+  if (rc != NLFA_OK) return rc;
+  if (l.copy_w) {
+    rc = copy_rows(w, c.w_dtype, tape + l.w, dtype, nullptr, nullptr, c.V, c.V, c.d, l.d_pad, l.x_planes, st);
+    if (rc != NLFA_OK) return rc;
+  }
+  rc = copy_rows(x, c.x_dtype, tape + l.x, dtype, t.head(), t.row_of(), c.n, l.n_rows, c.d, l.d_pad, l.x_planes, st);
+  if (rc != NLFA_OK) return rc;
+  CUtensorMap mx, mw;
+  rc = box_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes, 64);
+  if (rc == NLFA_OK) rc = box_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes, 64);
+  if (rc != NLFA_OK) return rc;
+  Params p = params(c, l, t, status);
+  if (l.x_planes == 3 || c.d > 1024) p.chunk = l.x_planes == 3 ? 4 : 16;
+  p.partial = reinterpret_cast<float2*>(scratch + l.partial);
+  p.at_target = at_target;
+  rc = launch_product(kLse, dtype, p, mx, mw, mx, mx, st);
+  if (rc != NLFA_OK) return rc;
+  unsigned* ticket = nullptr;
+  bool captured = false;
+  if (each == nullptr) {
+    rc = launch_ticket(st, reinterpret_cast<unsigned*>(scratch + l.ticket), &ticket, &captured);
+    if (rc != NLFA_OK) return rc;
+  }
+  const int ctas = l.n_rows / kBlock < 1024 ? l.n_rows / kBlock : 1024;
+  return checked(launch_kernel(finish_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kBlock), 0, st, !captured && overlap, t.head(),
+                               p.partial, at_target, t.row_of(), l.n_rows, t.lse(), t.lse_rest(), each, each != nullptr ? nullptr : out,
+                               reinterpret_cast<double*>(scratch + l.sums), ticket, reduction == NLFA_REDUCE_MEAN ? 1 : 0));
+}
+
+int run_bwd(const Call& c, const float* grad, const void* w, const void* targets, int target_bytes, long long ignore, int reduction,
+            uint8_t* tape, void* dx, void* dw, uint8_t* scratch, cudaStream_t st) {
+  const Layout l = layout(c, aligned16(w));
+  const BwdLayout b = bwd_layout(c, l);
+  const Pointers t{tape, l};
+  unsigned* status = status_block();
+  if (!status) return NLFA_ERR_CUDA;
+  const int dtype = c.dtype == NLFA_DTYPE_F32 ? NLFA_DTYPE_BF16 : c.dtype;
+  const bool overlap = overlap_launches(kOverlapRowwise);
+  float* row_scale = reinterpret_cast<float*>(scratch + b.row_scale);
+  float* alpha = reinterpret_cast<float*>(scratch + b.alpha);
+  int rc = checked(launch_kernel(scale_rows_kernel, dim3(1), dim3(1024), 0, st, overlap, t.head(), grad,
+                                 reduction == NLFA_REDUCE_NONE ? 1 : 0, reduction == NLFA_REDUCE_MEAN ? 1 : 0, t.row_of(), t.target(),
+                                 row_scale, alpha, dtype == NLFA_DTYPE_F16 ? 16384.f : 1.f));
+  if (rc != NLFA_OK) return rc;
+  if (dx != nullptr && c.n > 0) {
+    const long long row_bytes = static_cast<long long>(c.d) * (c.x_dtype == NLFA_DTYPE_F32 ? 4 : 2);
+    const int need = (c.n + kBlock / 32 - 1) / (kBlock / 32), most = 8 * sm_count();
+    auto clear = [&](auto* typed, auto* kernel) {
+      return checked(launch_kernel(kernel, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(kBlock), 0, st, overlap, typed,
+                                   c.n, ignore, t.head(), static_cast<uint8_t*>(dx), row_bytes));
+    };
+    rc = target_bytes == 8 ? clear(static_cast<const long long*>(targets), clear_rows_kernel<long long>)
+                           : clear(static_cast<const int*>(targets), clear_rows_kernel<int>);
+    if (rc != NLFA_OK) return rc;
+  }
+  CUtensorMap mx, mw, mds, mout;
+  rc = box_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes, 64);
+  if (rc == NLFA_OK) rc = box_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes, 64);
+  if (rc == NLFA_OK) rc = box_map(&mds, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes, 64);
+  if (rc == NLFA_OK) rc = box_map(&mout, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes, 32);
+  if (rc != NLFA_OK) return rc;
+  Params p = params(c, l, t, status);
+  p.chunk = l.x_planes == 3 ? 4 : 0;
+  p.row_scale = row_scale;
+  p.alpha = alpha;
+  p.dx = dx;
+  p.dw = dw;
+  p.dx_dtype = c.x_dtype;
+  p.dw_dtype = c.w_dtype;
+  p.dx_sum = reinterpret_cast<float*>(scratch + b.dx_sum);
+  p.want_dx = dx != nullptr;
+  p.want_dw = dw != nullptr;
+  for (int v = 0; v < c.V; v += b.piece) {
+    p.v0 = v;
+    p.v1 = c.V - v < b.piece ? c.V : v + b.piece;
+    p.first = v == 0;
+    p.last = p.v1 == c.V;
+    rc = launch_product(kGrad, dtype, p, mx, mw, mds, mout, st);
+    if (rc == NLFA_OK) rc = launch_product(kProducts, dtype, p, mx, mw, mds, mout, st);
+    if (rc != NLFA_OK) return rc;
+  }
+  return NLFA_OK;
+}
+
+}  // namespace
+}  // namespace loss
+}  // namespace nlfa
+
+using namespace nlfa;
+using namespace nlfa::loss;
+using rowwise::aligned16;
+
+extern "C" {
+
+size_t nlfa_linear_ce_tape_bytes(const void* w, int n, int V, int d, int x_dtype, int w_dtype, int dtype) {
+  const Call c{x_dtype, w_dtype, dtype, n, V, d};
+  return check_call(c) == NLFA_OK ? layout(c, aligned16(w)).tape_bytes : 0;
+}
+size_t nlfa_linear_ce_scratch_bytes(int n, int V, int d, int x_dtype, int w_dtype, int dtype, int backward) {
+  const Call c{x_dtype, w_dtype, dtype, n, V, d};
+  if (check_call(c) != NLFA_OK) return 0;
+  const Layout l = layout(c, false);
+  return backward ? bwd_layout(c, l).bytes : l.fwd_bytes;
+}
+
+int nlfa_linear_ce_fwd(const void* x, int x_dtype, const void* w, int w_dtype, int dtype, const void* targets, int target_bytes,
+                       int n, int V, int d, long long ignore_index, int reduction, float* loss, void* tape, size_t tape_bytes,
+                       void* scratch, size_t scratch_bytes, void* stream) {
+  const Call c{x_dtype, w_dtype, dtype, n, V, d};
+  const int rc = check_call(c);
+  if (rc != NLFA_OK) return rc;
+  if ((target_bytes != 4 && target_bytes != 8) || reduction < NLFA_REDUCE_NONE || reduction > NLFA_REDUCE_SUM) return NLFA_ERR_BAD_ARGUMENT;
+  if (!w || !tape || !scratch || (n > 0 && (!x || !targets)) || (!loss && !(n == 0 && reduction == NLFA_REDUCE_NONE)))
+    return NLFA_ERR_NULL_POINTER;
+  if (!aligned16(tape) || !aligned16(scratch)) return NLFA_ERR_MISALIGNED;
+  const Layout l = layout(c, aligned16(w));
+  if (tape_bytes < l.tape_bytes || scratch_bytes < l.fwd_bytes) return NLFA_ERR_SCRATCH_TOO_SMALL;
+  if (!nlfa_device_supported()) return NLFA_ERR_NOT_SM100;
+  if (nlfa_peek_status() != NLFA_OK) return NLFA_ERR_DEVICE_TIMEOUT;
+  return run_fwd(c, x, w, targets, target_bytes, ignore_index, reduction, loss, static_cast<uint8_t*>(tape),
+                 static_cast<uint8_t*>(scratch), static_cast<cudaStream_t>(stream));
+}
+
+int nlfa_linear_ce_bwd(const float* grad, const void* w, int w_dtype, int x_dtype, int dtype, const void* targets, int target_bytes,
+                       int n, int V, int d, long long ignore_index, int reduction, void* tape, size_t tape_bytes, void* dx, void* dw,
+                       void* scratch, size_t scratch_bytes, void* stream) {
+  const Call c{x_dtype, w_dtype, dtype, n, V, d};
+  const int rc = check_call(c);
+  if (rc != NLFA_OK) return rc;
+  if ((target_bytes != 4 && target_bytes != 8) || reduction < NLFA_REDUCE_NONE || reduction > NLFA_REDUCE_SUM) return NLFA_ERR_BAD_ARGUMENT;
+  if (!dx && !dw) return NLFA_OK;
+  if (!w || !tape || !scratch || (n > 0 && (!targets || !grad))) return NLFA_ERR_NULL_POINTER;
+  if (!aligned16(tape) || !aligned16(scratch) || !aligned16(dx) || !aligned16(dw)) return NLFA_ERR_MISALIGNED;
+  const Layout l = layout(c, aligned16(w));
+  if (tape_bytes < l.tape_bytes || scratch_bytes < bwd_layout(c, l).bytes) return NLFA_ERR_SCRATCH_TOO_SMALL;
+  if (!nlfa_device_supported()) return NLFA_ERR_NOT_SM100;
+  if (nlfa_peek_status() != NLFA_OK) return NLFA_ERR_DEVICE_TIMEOUT;
+  return run_bwd(c, grad, w, targets, target_bytes, ignore_index, reduction, static_cast<uint8_t*>(tape), dx, dw,
+                 static_cast<uint8_t*>(scratch), static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

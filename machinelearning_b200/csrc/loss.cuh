@@ -1,0 +1,62 @@
+// Linear cross entropy (loss.cu: rows, sums, the C ABI; loss_tc.cu: the products): what the two share.
+#pragma once
+
+#include "common.cuh"
+
+namespace nlfa {
+namespace loss {
+
+constexpr int kRowTile = 256;       // rows of a product's tile: two CTAs of 128
+constexpr int kColTile = 256;       // columns of a tile
+constexpr int kK = 64;              // summands per stage
+
+// The forward leaves its tape in one buffer; counts and places, known on the device only, stand first.
+struct Head {
+  int count;                        // rows with a target
+  int splits;                       // parts of the vocabulary in the forward's units
+};
+
+// Tape and scratch, laid out for n rows.  Rows without a target are left out on the way in (`row_of` names the source
+// of each row that stays), so they cost no products and whatever stands in them reaches nothing.
+struct Layout {
+  int n_rows;                       // rows a call can hold, up to a multiple of kRowTile
+  int d_pad;                        // row length of the 16-bit copies
+  int x_planes;                     // 16-bit parts of an operand: 1, or 3 for float32
+  bool copy_w;                      // the weight is converted or re-laid (otherwise the products read the caller's)
+  size_t row_of, target, lse, lse_rest, x, w, tape_bytes;
+  int max_splits;
+  size_t partial, at_target, sums, ticket, fwd_bytes;
+};
+
+// One product's launch.
+struct Params {
+  const Head* head;
+  int V, d, d_pad;
+  int planes, pairs;                // pairs of parts whose products are added: 1 or 6
+  int chunk;                        // blocks of kK summands per chain of the tensor core (0: the whole sum)
+  int v0, v1;                       // piece of the vocabulary
+  int n_rows;
+  // forward: (max, sum) of every part of a row, logit of the target
+  float2* partial;
+  float* at_target;
+  const int* target;
+  // gradient of the logits
+  const float *lse, *lse_rest;      // lse + lse_rest: to better than float32
+  const float* row_scale;
+  // products with it: dx [N, d] by row_of, dw [V, d]
+  const int* row_of;
+  const float* alpha;
+  void *dx, *dw;
+  float* dx_sum;                    // float32 sums over the pieces, for a 16-bit dx
+  int dx_dtype, dw_dtype;
+  int first, last;                  // piece is the first / last one
+  int want_dx, want_dw;
+  unsigned* status;
+};
+
+enum { kLse = 0, kGrad = 1, kProducts = 2 };
+int launch_product(int mode, int dtype, const Params& p, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& ds,
+                   const CUtensorMap& ds_out, cudaStream_t stream);
+
+}  // namespace loss
+}  // namespace nlfa

@@ -1,0 +1,550 @@
+// The products of the linear cross entropy (loss.cu) on the tensor cores:
+//   kLse       l = x W^T, of which only each row's running maximum and sum of exponentials leave the SM, and the target's l;
+//   kGrad      l again for a piece of the vocabulary, dl = r (exp(l - lse) - [v == target]), written in 16 bits;
+//   kProducts  dx (+)= dl W and dW = dl^T x of that piece, both in one launch.
+//
+// One persistent kernel per kind, a pair of CTAs (cta_group::2) per 256 x 256 tile: each CTA holds 128 rows of A, 128
+// columns of B and 128 x 256 of the sums, so an operand byte brought into shared memory serves twice the columns
+// of a single CTA's tile.  All operands come as boxes of 64 x 64 16-bit values, K-major or MN-major by their coordinates
+// alone.  Sums are double buffered in TMEM (2 x 256 columns): the epilogue of a tile runs under the next one's products.
+//
+// The tensor core adds to its sums by truncation: a chain of K / 16 steps over positive summands comes out low by 6.6e-7 of
+// its value at K = 768, 1.1e-5 at 4,096 and 7.7e-5 at 16,384 (measured; a float32 product on the CUDA cores is off by 5e-8).  Where that shows,
+// the chain is cut (LONG): a tile's sum is formed chunk by chunk, and the chunks' sums are added in registers.
+//
+// Warps: 0 producer, 1 MMA issuer (even CTA) and TMEM owner, 2-9 epilogue: two warps per quarter of the rows, 128 columns
+// each.  Every wait is bounded (ptx.cuh); no multicast loads.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "loss.cuh"
+#include "ptx.cuh"
+
+namespace nlfa {
+namespace loss {
+namespace {
+
+constexpr int kThreads = 320;
+constexpr int kEpilogueWarps = 8;
+constexpr int kStages = 6;
+constexpr int kOperandBytes = 128 * kK * 2;                   // one CTA's half of an operand
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kStagingBytes = 4096;                           // per epilogue warp
+constexpr int kStaging = kStages * kStageBytes;
+constexpr int kBars = kStaging + kEpilogueWarps * kStagingBytes;
+constexpr int kNumBars = 2 * kStages + 4;
+constexpr int kTmemSlot = kBars + 8 * kNumBars;
+constexpr int kAbort = kTmemSlot + 4;
+constexpr int kSmem = kAbort + 4 + 1024;
+static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
+
+enum { FULL = 0, EMPTY = kStages, ACC_FULL = 2 * kStages, ACC_EMPTY = ACC_FULL + 2 };
+
+// float32 operands are sums of three bf16 parts; the products of parts, smallest first (what is left out is below 2^-24)
+__device__ __forceinline__ int part_a(int pair) { return (0x001012 >> (4 * pair)) & 15; }   // 2 1 0 1 0 0
+__device__ __forceinline__ int part_b(int pair) { return (0x010210 >> (4 * pair)) & 15; }   // 0 1 2 0 1 0
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// A tile: where it lies in A's rows and B's columns, how many stages its sum takes, which operands it has.
+struct Tile {
+  int m0, n0;
+  int k_blocks;                     // blocks of 64 summands per pair of parts
+  int dw;                           // kProducts: a tile of dW (else of dx)
+  int first, last;                  // kLse: first / last tile of a unit
+  int slot;                         // kLse: which part of the vocabulary
+};
+
+// The tiles of one pair of CTAs, in order; every role walks the same list.
+template <int MODE>
+struct Walk {
+  const Params& p;
+  int rows, row_tiles, stride, u, units;
+  int n, n_end;                     // kLse: column tiles left in the unit
+  int col_tiles, splits, dw_tiles, d_tiles;
+
+  __device__ Walk(const Params& p_, int pair, int n_pairs) : p(p_) {
+    rows = *reinterpret_cast<const volatile int*>(&p.head->count);
+    row_tiles = rows > 0 ? ceil_div(rows, kRowTile) : 1;        // (no row: one tile of zeros, which leaves zero gradients)
+    stride = n_pairs;
+    u = pair - n_pairs;
+    n = n_end = 0;
+    splits = 1;
+    if (MODE == kLse) {
+      splits = *reinterpret_cast<const volatile int*>(&p.head->splits);
+      col_tiles = ceil_div(p.V, kColTile);
+      units = row_tiles * splits;
+    } else {
+      col_tiles = ceil_div(p.v1 - p.v0, kColTile);
+      d_tiles = ceil_div(p.d, kColTile);
+      dw_tiles = MODE == kProducts && p.want_dw ? col_tiles * d_tiles : 0;
+      units = MODE == kGrad ? row_tiles * col_tiles : dw_tiles + (p.want_dx ? row_tiles * d_tiles : 0);
+    }
+  }
+
+  __device__ bool next(Tile& t) {
+    if (MODE == kLse) {
+      t.first = 0;
+      if (n == n_end) {
+        u += stride;
+        if (u >= units) return false;
+        // neighbouring pairs: the same part of the vocabulary, other rows, so that W is read from L2
+        const int part = u / row_tiles;
+        t.m0 = (u - part * row_tiles) * kRowTile;
+        t.slot = part;
+        n = static_cast<int>(static_cast<long long>(col_tiles) * part / splits);
+        n_end = static_cast<int>(static_cast<long long>(col_tiles) * (part + 1) / splits);
+        t.first = 1;
+      }
+      t.n0 = n * kColTile;
+      t.last = ++n == n_end;
+      t.k_blocks = ceil_div(p.d, kK);
+      return true;
+    }
+    u += stride;
+    if (u >= units) return false;
+    if (MODE == kGrad) {
+      // eight row tiles at a time past all columns of the piece
+      const int group = 8 * col_tiles, g = u / group, v = u - g * group;
+      const int size = row_tiles - 8 * g < 8 ? row_tiles - 8 * g : 8;
+      const int c = v / size;
+      t.m0 = (8 * g + v - c * size) * kRowTile;
+      t.n0 = p.v0 + c * kColTile;
+      t.k_blocks = ceil_div(p.d, kK);
+    } else {
+      // dW's tiles, the longest sums, first
+      t.dw = u < dw_tiles;
+      const int v = t.dw ? u : u - dw_tiles, m = v / d_tiles;
+      t.m0 = m * kRowTile;                                     // dW: columns of dl, from the piece's first
+      t.n0 = (v - m * d_tiles) * kColTile;
+      t.k_blocks = t.dw ? row_tiles * (kRowTile / kK) : ceil_div(p.v1 - p.v0, kK);
+    }
+    return true;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ float round_to(float x);
+template <>
+__device__ __forceinline__ float round_to<__nv_bfloat16>(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
+template <>
+__device__ __forceinline__ float round_to<__half>(float x) { return __half2float(__float2half_rn(x)); }
+
+// ---- epilogues: a thread has row `lane` of its warp's 32 and, 32 at a time, 128 columns
+
+// 128 columns of a thread's row: in TMEM, or (LONG) summed from the chunks' sums in registers.
+template <bool LONG>
+struct Sums {
+  uint32_t acc;
+  float v[LONG ? 128 : 1];
+  __device__ __forceinline__ void get(int col, uint32_t (&r)[32]) const {
+    if constexpr (LONG) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (col == 32 * c) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(v[32 * c + j]);
+        }
+    } else {
+      tmem_ld32(acc + col, r);
+      tc_wait_ld();
+    }
+  }
+};
+
+template <typename T, int MODE, bool LONG>
+__global__ void __launch_bounds__(kThreads, 1)
+loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+            const __grid_constant__ CUtensorMap tm_ds, const __grid_constant__ CUtensorMap tm_out, const Params p) {
+  constexpr bool kBf16 = Pack2<T>::kIsBf16;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_rank());
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  auto bar = [&](int i) -> uint32_t { return base + kBars + 8u * i; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + kAbort);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + kTmemSlot);
+  const WaitCtx wctx{abort_flag, p.status};
+
+  if (threadIdx.x == 0) {
+    *abort_flag = (*reinterpret_cast<volatile unsigned*>(p.status) != STATUS_OK) ? 1 : 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar(FULL + s), 1);
+      mbar_init(bar(EMPTY + s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(ACC_FULL + i), 1);
+      mbar_init(bar(ACC_EMPTY + i), 2 * kEpilogueWarps);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(base + kTmemSlot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const bool dead = *abort_flag != 0;
+  grid_dep_wait();
+  grid_dep_release();
+
+  if (dead) {
+    // a give-up recorded earlier makes this launch a no-op
+  } else if (warp == 0) {
+    // ============================== producer ================================
+    if (lane == 0) {
+      Walk<MODE> walk(p, pair, n_pairs);
+      Tile t;
+      int it = 0;
+      bool ok = true;
+      const uint32_t full0 = cluster_addr(bar(FULL), 0);       // loads of both CTAs are counted on the even one's
+      while (ok && walk.next(t)) {
+        const CUtensorMap* ma = MODE == kProducts ? &tm_ds : &tm_x;
+        const CUtensorMap* mb = MODE == kProducts && t.dw ? &tm_x : &tm_w;
+        const int a0 = t.m0 + 128 * rank, b0 = t.n0 + 128 * rank;
+        const int chunk = LONG ? p.chunk : t.k_blocks;
+        for (int k0 = 0; ok && k0 < t.k_blocks; k0 += chunk)
+          for (int pr = 0; ok && pr < p.pairs; ++pr) {
+            const int pa = p.pairs == 1 ? 0 : part_a(pr), pb = p.pairs == 1 ? 0 : part_b(pr);
+            const int k1 = t.k_blocks - k0 < chunk ? t.k_blocks : k0 + chunk;
+            for (int kb = k0; kb < k1; ++kb, ++it) {
+              const int s = it % kStages;
+              if (!(ok = mbar_wait(bar(EMPTY + s), ((it / kStages) & 1) ^ 1, wctx, 90))) break;
+              const uint32_t st = base + s * kStageBytes, full = full0 + 8u * s;
+              if (rank == 0) mbar_arrive_expect_tx(bar(FULL + s), 2 * kStageBytes);
+              const int k = kb * kK;
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                if (MODE == kProducts && t.dw) tma_load_4d_pair(st + j * 8192, ma, full, a0 + 64 * j, k, pa, 0);
+                else tma_load_4d_pair(st + j * 8192, ma, full, k, a0 + 64 * j, pa, 0);
+              }
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const uint32_t dst = st + kOperandBytes + j * 8192;
+                if (MODE != kProducts) tma_load_4d_pair(dst, mb, full, k, b0 + 64 * j, pb, 0);
+                else tma_load_4d_pair(dst, mb, full, b0 + 64 * j, t.dw ? k : p.v0 + k, pb, 0);
+              }
+            }
+          }
+      }
+      // the last loads of this CTA have been consumed before it may leave (after a give-up: have had time to land)
+      for (int i = 0; ok && i < kStages; ++i, ++it) ok = mbar_wait(bar(EMPTY + it % kStages), ((it / kStages) & 1) ^ 1, wctx, 91);
+      if (!ok) for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    }
+  } else if (warp == 1) {
+    // ============================= MMA issuer ===============================
+    if (rank == 0) {
+      const uint32_t leader = elect_one() ? 1u : 0u;
+      Walk<MODE> walk(p, pair, n_pairs);
+      Tile t;
+      int it = 0, sums = 0;                                    // sums: filled TMEM buffers so far
+      bool ok = true;
+      while (ok && walk.next(t)) {
+        const bool a_mn = MODE == kProducts && t.dw, b_mn = MODE == kProducts;
+        const uint32_t idesc = a_mn ? make_idesc(kBf16, 256, kColTile, true, b_mn) : make_idesc(kBf16, 256, kColTile, false, b_mn);
+        const uint32_t a_step = a_mn ? 2048u : 32u, a_lbo = a_mn ? 8192u : 16u;
+        const uint32_t b_step = b_mn ? 2048u : 32u, b_lbo = b_mn ? 8192u : 16u;
+        const int chunk = LONG ? p.chunk : t.k_blocks;
+        for (int k0 = 0; ok && k0 < t.k_blocks; k0 += chunk, ++sums) {
+          const int buf = sums & 1;
+          if (!(ok = mbar_wait(bar(ACC_EMPTY + buf), ((sums >> 1) & 1) ^ 1, wctx, 92))) break;
+          tc_fence_after();
+          const int blocks = p.pairs * (t.k_blocks - k0 < chunk ? t.k_blocks - k0 : chunk);
+          for (int kb = 0; kb < blocks; ++kb, ++it) {
+            const int s = it % kStages;
+            if (!(ok = mbar_wait(bar(FULL + s), (it / kStages) & 1, wctx, 93))) break;
+            tc_fence_after();
+            const uint32_t a = base + s * kStageBytes, b = a + kOperandBytes;
+#pragma unroll
+            for (int kk = 0; kk < kK / 16; ++kk)
+              umma_ss_pair(leader, tmem + buf * kColTile, make_smem_desc(a + kk * a_step, a_lbo, 1024),
+                           make_smem_desc(b + kk * b_step, b_lbo, 1024), idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+            umma_commit_pair(leader, bar(EMPTY + s));
+          }
+          if (ok) umma_commit_pair(leader, bar(ACC_FULL + buf));
+        }
+      }
+    }
+  } else {
+    // ============================== epilogue ================================
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t staging = base + kStaging + (warp - 2) * kStagingBytes;
+    const uint32_t acc_empty0 = cluster_addr(bar(ACC_EMPTY), 0);
+    Walk<MODE> walk(p, pair, n_pairs);
+    Tile t;
+    float run_max = 0.f, run_sum = 0.f;
+    int sums = 0;
+    bool ok = true;
+    Sums<LONG> l;
+    auto release = [&](int buf) {                              // this warp has read its part of the buffer
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * buf);
+    };
+    while (walk.next(t)) {
+      const int row0 = t.m0 + 128 * rank + 32 * q, row = row0 + lane;
+      int target = -1;
+      float lse = 0.f, rest2 = 0.f, scale = 0.f;
+      if (MODE != kProducts) target = p.target[row];
+      if (MODE == kGrad) {
+        lse = p.lse[row];
+        rest2 = p.lse_rest[row] * kLog2e;
+        scale = p.row_scale[row];
+      }
+      if (MODE == kLse && t.first) { run_max = -INFINITY; run_sum = 0.f; }
+      int buf = 0;
+      if constexpr (LONG) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j) l.v[j] = 0.f;
+        for (int k0 = 0; k0 < t.k_blocks; k0 += p.chunk, ++sums) {
+          buf = sums & 1;
+          if (!(ok = mbar_wait(bar(ACC_FULL + buf), (sums >> 1) & 1, wctx, 94))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t r[32];
+            tmem_ld32(tmem_addr(tmem, 32 * q, buf * kColTile + 128 * half + 32 * c), r);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) l.v[32 * c + j] += __uint_as_float(r[j]);
+          }
+          release(buf);
+        }
+      } else {
+        buf = sums & 1;
+        ok = mbar_wait(bar(ACC_FULL + buf), (sums >> 1) & 1, wctx, 94);
+        tc_fence_after();
+        l.acc = tmem_addr(tmem, 32 * q, buf * kColTile + 128 * half);
+        ++sums;
+      }
+      if (!ok) break;
+      const int c0 = t.n0 + 128 * half;
+
+      if constexpr (MODE == kLse) {
+#pragma unroll (LONG ? 4 : 1)
+        for (int c = 0; c < 4; ++c) {
+          const int col = c0 + 32 * c;
+          if (col >= p.V) break;
+          uint32_t r[32];
+          l.get(32 * c, r);
+          if (col + 32 > p.V) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col + j >= p.V) r[j] = __float_as_uint(-INFINITY);
+          }
+          const unsigned at = static_cast<unsigned>(target - col);
+          if (__any_sync(0xffffffffu, at < 32u)) {
+            float v = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (at == static_cast<unsigned>(j)) v = __uint_as_float(r[j]);
+            if (at < 32u) p.at_target[row] = v;
+          }
+          float top = __uint_as_float(r[0]);
+#pragma unroll
+          for (int j = 1; j < 31; j += 2) top = fmax3(top, __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+          top = fmaxf(fmaxf(top, __uint_as_float(r[31])), run_max);
+          // The difference is formed before it is scaled: fma(l, log2 e, -top log2 e) is off by the rounding of top log2 e,
+          // in every summand alike.  (every logit so far -inf: nothing to subtract)
+          const float shift = top == -INFINITY ? 0.f : top;
+          const uint64_t minus = pack_f2(-shift, -shift), by = pack_f2(kLog2e, kLog2e);
+          uint64_t part[2] = {0ull, 0ull};
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            float a, b;
+            unpack_f2(fmul2(fadd2(pack_f2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), minus), by), a, b);
+            part[j / 2 & 1] = fadd2(part[j / 2 & 1], pack_f2(fast_exp2(a), fast_exp2(b)));
+          }
+          float a, b;
+          unpack_f2(fadd2(part[0], part[1]), a, b);
+          run_sum = fmaf(run_sum, fast_exp2((run_max - shift) * kLog2e), a + b);
+          run_max = top;
+        }
+        if (t.last) p.partial[static_cast<size_t>(2 * t.slot + half) * p.n_rows + row] = make_float2(run_max, run_sum);
+      } else if constexpr (MODE == kGrad) {
+#pragma unroll (LONG ? 2 : 1)
+        for (int c2 = 0; c2 < 2; ++c2) {
+          // 64 columns: a row of the staging tile (128 bytes, swizzled as the tensor map has it)
+          float lo[2][32];                                     // what is left of the values after the parts written so far
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int col = c0 + 64 * c2 + 32 * h;
+            uint32_t r[32];
+            l.get(64 * c2 + 32 * h, r);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              float a, b;
+              unpack_f2(ffma2(fadd2(pack_f2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), pack_f2(-lse, -lse)),
+                              pack_f2(kLog2e, kLog2e), pack_f2(-rest2, -rest2)), a, b);
+              unpack_f2(fmul2(pack_f2(fast_exp2(a), fast_exp2(b)), pack_f2(scale, scale)), lo[h][j], lo[h][j + 1]);
+            }
+            if (col + 32 > p.V) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (col + j >= p.V) lo[h][j] = 0.f;
+            }
+            const unsigned at = static_cast<unsigned>(target - col);
+            if (__any_sync(0xffffffffu, at < 32u)) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (at == static_cast<unsigned>(j)) lo[h][j] -= scale;
+            }
+          }
+          for (int part = 0; part < p.planes; ++part) {
+            if (lane == 0) tma_store_wait_read();
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int j = 0; j < 32; j += 8) {
+                const float* v = lo[h] + j;
+                const uint32_t chunk = static_cast<uint32_t>((4 * h + j / 8) ^ (lane & 7));
+                st_shared_v4(staging + lane * 128 + chunk * 16, Pack2<T>::pack(v[0], v[1]), Pack2<T>::pack(v[2], v[3]),
+                             Pack2<T>::pack(v[4], v[5]), Pack2<T>::pack(v[6], v[7]));
+              }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_4d(&tm_out, staging, c0 + 64 * c2 - p.v0, row0, part, 0);
+              tma_store_commit();
+            }
+            if (part + 1 < p.planes) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 32; ++j) lo[h][j] -= round_to<T>(lo[h][j]);
+            }
+          }
+        }
+      } else {
+        // 32 x 32 values through shared memory, so that a row's columns leave side by side
+        const float alpha = *p.alpha;
+        const int rows = walk.rows;
+        const int m0 = t.dw ? p.v0 + t.m0 + 128 * rank + 32 * q : row0;
+        const int m_end = t.dw ? p.v1 : rows;
+        const int dtype = t.dw ? p.dw_dtype : p.dx_dtype;
+        void* out = t.dw ? p.dw : p.dx;
+        const bool vec = p.d % 4 == 0;
+#pragma unroll (LONG ? 4 : 1)
+        for (int c = 0; c < 4; ++c) {
+          const int col = c0 + 32 * c;
+          if (col >= p.d) break;
+          uint32_t r[32];
+          l.get(32 * c, r);
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            st_shared_v4(staging + lane * 128 + (((j / 4) ^ (lane & 7)) * 16), r[j], r[j + 1], r[j + 2], r[j + 3]);
+          __syncwarp();
+          const int cc = col + 4 * (lane & 7);
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {
+            const int lr = 4 * i + (lane >> 3), m = m0 + lr;
+            uint32_t w0, w1, w2, w3;
+            ld_shared_v4(staging + lr * 128 + (((lane & 7) ^ (lr & 7)) * 16), w0, w1, w2, w3);
+            if (m >= m_end || cc >= p.d) continue;
+            float v[4] = {__uint_as_float(w0), __uint_as_float(w1), __uint_as_float(w2), __uint_as_float(w3)};
+            const int n = p.d - cc < 4 ? p.d - cc : 4;
+            size_t at = static_cast<size_t>(m) * p.d + cc;
+            if (!t.dw && (p.first == 0 || p.last == 0)) {
+              float* sum = p.dx_sum + at;
+              if (vec) {
+                float4* s4 = reinterpret_cast<float4*>(sum);
+                if (!p.first) {
+                  const float4 b = *s4;
+                  v[0] += b.x; v[1] += b.y; v[2] += b.z; v[3] += b.w;
+                }
+                if (!p.last) *s4 = make_float4(v[0], v[1], v[2], v[3]);
+              } else {
+                for (int e = 0; e < n; ++e) {
+                  if (!p.first) v[e] += sum[e];
+                  if (!p.last) sum[e] = v[e];
+                }
+              }
+              if (!p.last) continue;
+            }
+            if (!t.dw) at = static_cast<size_t>(p.row_of[m]) * p.d + cc;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= alpha;
+            if (dtype == NLFA_DTYPE_F32) {
+              float* o = static_cast<float*>(out) + at;
+              if (vec) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+              else for (int e = 0; e < n; ++e) o[e] = v[e];
+            } else if (dtype == NLFA_DTYPE_BF16) {
+              __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out) + at;
+              if (vec) *reinterpret_cast<uint2*>(o) = make_uint2(Pack2<__nv_bfloat16>::pack(v[0], v[1]), Pack2<__nv_bfloat16>::pack(v[2], v[3]));
+              else for (int e = 0; e < n; ++e) o[e] = __float2bfloat16_rn(v[e]);
+            } else {
+              __half* o = static_cast<__half*>(out) + at;
+              if (vec) *reinterpret_cast<uint2*>(o) = make_uint2(Pack2<__half>::pack(v[0], v[1]), Pack2<__half>::pack(v[2], v[3]));
+              else for (int e = 0; e < n; ++e) o[e] = __float2half_rn(v[e]);
+            }
+          }
+          __syncwarp();
+        }
+      }
+      if (!LONG) release(buf);
+    }
+    if (MODE == kGrad && lane == 0) tma_store_wait_all();
+  }
+
+  tc_fence_before();
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
+template <typename T, int MODE, bool LONG>
+int launch_one(const Params& p, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& ds, const CUtensorMap& out,
+               cudaStream_t stream) {
+  auto* kernel = loss_kernel<T, MODE, LONG>;
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), kSmem);
+  if (rc != NLFA_OK) return rc;
+  const int pairs = sm_count() / 2;
+  // (a pair has to lie along x: along y the launch is refused)
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2u * static_cast<unsigned>(pairs));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = overlap_launches(kOverlapRowwise) ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, x, w, ds, out, p);
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e == cudaSuccess ? NLFA_OK : NLFA_ERR_CUDA;
+}
+
+}  // namespace
+
+int launch_product(int mode, int dtype, const Params& p, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& ds,
+                   const CUtensorMap& ds_out, cudaStream_t stream) {
+  const bool bf16 = dtype == NLFA_DTYPE_BF16, is_long = p.chunk > 0;
+#define NLFA_GO(T, MODE, LONG) launch_one<T, MODE, LONG>(p, x, w, ds, ds_out, stream)
+  if (mode == kLse) {
+    if (is_long) return bf16 ? NLFA_GO(__nv_bfloat16, kLse, true) : NLFA_GO(__half, kLse, true);
+    return bf16 ? NLFA_GO(__nv_bfloat16, kLse, false) : NLFA_GO(__half, kLse, false);
+  }
+  // (the gradients' sums are chunked for float32 operands alone, which are bf16 parts)
+  if (mode == kGrad)
+    return is_long ? NLFA_GO(__nv_bfloat16, kGrad, true) : bf16 ? NLFA_GO(__nv_bfloat16, kGrad, false) : NLFA_GO(__half, kGrad, false);
+  return is_long ? NLFA_GO(__nv_bfloat16, kProducts, true) : bf16 ? NLFA_GO(__nv_bfloat16, kProducts, false) : NLFA_GO(__half, kProducts, false);
+#undef NLFA_GO
+}
+
+}  // namespace loss
+}  // namespace nlfa

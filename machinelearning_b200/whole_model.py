@@ -32,7 +32,7 @@ import torch.distributed as dist
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import flash_cuda, mixer_glue, qk_prologue, value_gate
+from . import flash_cuda, grad_clip, head_loss, mixer_glue, qk_prologue, token_embedding, value_gate
 
 
 @dataclasses.dataclass
@@ -61,6 +61,8 @@ class ModelShape:
     swa_sinks: int = 0
     fused_prologue: bool = True  # with flash_cuda on: QK-norm + RoPE + cast in one kernel (qk_prologue)
     fused_epilogue: bool = True  # with flash_cuda on: value blend and head gate in one kernel each (value_gate)
+    fused_loss: bool = False     # head and cross entropy without the logits (head_loss); a training step then returns none
+    fused_embedding: bool = False  # rows of the table and their gradient by sorted tokens (token_embedding)
 
     def __post_init__(self):
         if self.n_kv_head == 0:
@@ -241,7 +243,10 @@ class GPT(nn.Module):
 
     def forward(self, idx, targets=None):
         s = self.shape
-        x = self.tok_emb(idx)
+        if s.fused_embedding and token_embedding.supports(idx, self.tok_emb.weight) and flash_cuda.is_available():
+            x = token_embedding.embedding(idx, self.tok_emb.weight)
+        else:
+            x = self.tok_emb(idx)
         key = (idx.shape[1], x.device, x.dtype)
         if key not in self._rope:
             self._rope[key] = rope_tables(idx.shape[1], s.head_dim, s.rope_base, x.device, x.dtype)
@@ -254,6 +259,8 @@ class GPT(nn.Module):
         x = self.norm_f(x)
         if targets is None:
             return self.lm_head(x[:, [-1], :]), None
+        if s.fused_loss and head_loss.supports(x, self.lm_head.weight, targets) and flash_cuda.is_available():
+            return None, head_loss.linear_cross_entropy(x, self.lm_head.weight, targets, ignore_index=-1)
         logits = self.lm_head(x)
         loss = F.cross_entropy(logits.view(-1, logits.size(-1)), targets.reshape(-1), ignore_index=-1)
         return logits, loss
@@ -302,8 +309,9 @@ class DataParallelStep:
     """
 
     def __init__(self, model: GPT, lr: float = 6e-4, weight_decay: float = 0.1, grad_clip: float = 1.0,
-                 dtype=torch.bfloat16, bucket_mb: int = 32, group=None, overlap: bool = True):
+                 dtype=torch.bfloat16, bucket_mb: int = 32, group=None, overlap: bool = True, fused_clip: bool = False):
         self.model, self.grad_clip, self.dtype, self.group = model, grad_clip, dtype, group
+        self.fused_clip = fused_clip         # the norm and the clip in two launches (grad_clip)
         self.world = dist.get_world_size(group) if dist.is_available() and dist.is_initialized() else 1
         self.bucket_elems = bucket_mb * (1 << 20) // 4
         self.overlap = overlap
@@ -434,7 +442,11 @@ class DataParallelStep:
             _, loss = self.model(idx, targets)
         loss.backward()
         self.average_gradients()
-        torch.nn.utils.clip_grad_norm_(self.model.parameters(), self.grad_clip)
+        if (self.fused_clip and grad_clip.supports([p.grad for p in self.model.parameters() if p.grad is not None])
+                and flash_cuda.is_available()):
+            grad_clip.clip_grad_norm_(self.model.parameters(), self.grad_clip)
+        else:
+            torch.nn.utils.clip_grad_norm_(self.model.parameters(), self.grad_clip)
         self.opt.step()
         self._zero_grad()
         return loss.detach()
@@ -461,6 +473,7 @@ def main(argv=None) -> int:
     """Synthetic-token micro-benchmark of the training step, after ``nanolab/bench_gpu.py:41-110``.
 
         python -m machinelearning_b200.whole_model --flash_cuda true [--batch_size 16 --iters 10 --swa_window 0]
+        ... --fused_loss true --fused_embedding true --fused_clip true     # the step's ends through their kernels as well
 
     Prints tokens/s, ms per step, the model-FLOPs estimate nanolab uses and the loss, for one GPU.
     """
@@ -470,6 +483,9 @@ def main(argv=None) -> int:
     ap = argparse.ArgumentParser()
     ap.add_argument("--flash_cuda", type=_flag, default=False)
     ap.add_argument("--fused_prologue", type=_flag, default=True)
+    ap.add_argument("--fused_loss", type=_flag, default=False)
+    ap.add_argument("--fused_embedding", type=_flag, default=False)
+    ap.add_argument("--fused_clip", type=_flag, default=False)
     ap.add_argument("--batch_size", type=int, default=16)
     ap.add_argument("--swa_window", type=int, default=0)
     ap.add_argument("--swa_sinks", type=int, default=0)
@@ -480,9 +496,9 @@ def main(argv=None) -> int:
         raise SystemExit("no CUDA device")
     torch.manual_seed(0)
     shape = ModelShape(flash_cuda=a.flash_cuda, fused_prologue=a.fused_prologue, swa_window=a.swa_window,
-                       swa_sinks=a.swa_sinks)
+                       swa_sinks=a.swa_sinks, fused_loss=a.fused_loss, fused_embedding=a.fused_embedding)
     model = GPT(shape).cuda()
-    step = DataParallelStep(model)
+    step = DataParallelStep(model, fused_clip=a.fused_clip)
     x, y = (t.cuda() for t in synthetic_tokens(shape.vocab_size, a.batch_size, shape.block_size))
     for _ in range(a.warmup):
         loss = step.step(x, y)
@@ -494,6 +510,7 @@ def main(argv=None) -> int:
     sec = (time.time() - t0) / a.iters
     tokens = a.batch_size * shape.block_size
     print(json.dumps({"flash_cuda": a.flash_cuda, "fused_prologue": a.fused_prologue and a.flash_cuda,
+                      "fused_loss": a.fused_loss, "fused_embedding": a.fused_embedding, "fused_clip": a.fused_clip,
                       "tok_s": tokens / sec, "ms_per_step": sec * 1e3, "loss": loss.item(),
                       "params_m": model.n_params() / 1e6, "flops_per_tok": model.flops_per_token(),
                       "model_tflops": model.flops_per_token() * tokens / sec / 1e12,
