@@ -17,7 +17,7 @@ namespace embedding {
 namespace {
 
 constexpr int kBlock = 256, kWarps = kBlock / 32;
-constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kMostDigitBits = 9;
 
 // W bytes of a row: 16, 8, 4 or 2, what its alignment allows
@@ -87,12 +87,14 @@ lookup_kernel(const I* __restrict__ ids, const T* __restrict__ w, T* __restrict_
 // ------------------------------------------------------------------------------------------------ sort
 
 // (id, position) by id, positions in order; ids without a gradient (outside the table, padding) become V and end up last.
-// begin[v], end[v]: where v's positions lie; begin = -1 where there are none.  Each CTA has a run of the positions, each warp of it a run of that.
+// begin[v], end[v]: where v's positions lie; begin = -1 where there are none.  One cluster: each CTA has a
+// run of the positions, each warp of it a run of that.
 template <typename I>
 __global__ void __launch_bounds__(kSortThreads)
 sort_ids_kernel(const I* __restrict__ ids, int n, int V, long long padding, uint32_t* keys, uint32_t* places, int* __restrict__ begin,
-                int* __restrict__ end, int passes, int digit_bits) {
+                int* __restrict__ end, int passes, int digit_bits, int ctas) {
   extern __shared__ int smem[];
+  constexpr int U = 8;
   const int digits = 1 << digit_bits;
   int* count = smem;                                   // [warp][digit]
   int* total = smem + kSortWarps * digits;             // [digit], read by the other CTAs
@@ -102,29 +104,47 @@ sort_ids_kernel(const I* __restrict__ ids, int n, int V, long long padding, uint
   grid_dep_release();
   const int rank = static_cast<int>(cluster_rank()), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const unsigned below = (1u << lane) - 1u;
-  const int run = static_cast<int>((static_cast<long long>(n) + kSortCtas * kSortThreads - 1) / (kSortCtas * kSortThreads)) * 32;
+  const int per_round = ctas * kSortThreads;
+  const int run = static_cast<int>((static_cast<long long>(n) + per_round - 1) / per_round) * 32;
   const long long lo = static_cast<long long>(run) * (rank * kSortWarps + warp);
   const int from = lo < n ? static_cast<int>(lo) : n, to = n - from < run ? n : from + run;
 
-  for (int v = rank * kSortThreads + threadIdx.x; v < V; v += kSortCtas * kSortThreads) begin[v] = -1;
+  for (int v = rank * kSortThreads + threadIdx.x; v < V; v += per_round) begin[v] = -1;
 
   uint32_t *src = keys, *src_at = places, *dst = keys + n, *dst_at = places + n;
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * digit_bits;
-    auto key_at = [&](int i) -> uint32_t {
-      if (pass > 0) return __ldcg(src + i);
-      const long long id = static_cast<long long>(ids[i]);
-      return id >= 0 && id < V && id != padding ? static_cast<uint32_t>(id) : static_cast<uint32_t>(V);
+    // the keys of U x 32 positions; behind the run: no digit
+    auto load_keys = [&](int i0, uint32_t (&k)[U]) {
+      if (pass > 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) k[u] = i0 + 32 * u + lane < to ? __ldcg(src + i0 + 32 * u + lane) : 0xffffffffu;
+      } else {
+        long long id[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) id[u] = i0 + 32 * u + lane < to ? static_cast<long long>(ids[i0 + 32 * u + lane]) : 0ll;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t key = id[u] >= 0 && id[u] < V && id[u] != padding ? static_cast<uint32_t>(id[u]) : static_cast<uint32_t>(V);
+          k[u] = i0 + 32 * u + lane < to ? key : 0xffffffffu;
+        }
+      }
     };
+    auto digit_of = [&](uint32_t key) { return key == 0xffffffffu ? key : (key >> shift) & (digits - 1); };
     for (int i = threadIdx.x; i < kSortWarps * digits; i += kSortThreads) count[i] = 0;
     __syncthreads();
     int* mine = count + warp * digits;
-    for (int i0 = from; i0 < to; i0 += 32) {
-      const bool in = i0 + lane < to;
-      const uint32_t d = in ? (key_at(i0 + lane) >> shift) & (digits - 1) : 0xffffffffu;
-      const unsigned same = __match_any_sync(0xffffffffu, d);
-      if (in && (same & below) == 0) mine[d] += __popc(same);
-      __syncwarp();
+    for (int i0 = from; i0 < to; i0 += 32 * U) {
+      uint32_t k[U];
+      load_keys(i0, k);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i0 + 32 * u >= to) break;
+        const uint32_t d = digit_of(k[u]);
+        const unsigned same = __match_any_sync(0xffffffffu, d);
+        if (d != 0xffffffffu && (same & below) == 0) mine[d] += __popc(same);
+        __syncwarp();
+      }
     }
     __syncthreads();
     if (threadIdx.x < digits) {
@@ -141,8 +161,8 @@ sort_ids_kernel(const I* __restrict__ ids, int n, int V, long long padding, uint
     cluster_wait();
     int before = 0, all = 0;
     if (threadIdx.x < digits) {
-#pragma unroll
-      for (int r = 0; r < kSortCtas; ++r) {
+#pragma unroll 8
+      for (int r = 0; r < ctas; ++r) {
         int v;
         asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(smem_u32(total + threadIdx.x), r)) : "memory");
         if (r < rank) before += v;
@@ -163,19 +183,30 @@ sort_ids_kernel(const I* __restrict__ ids, int n, int V, long long padding, uint
       base[threadIdx.x] = ahead + inclusive - all + before;
     }
     __syncthreads();
-    for (int i0 = from; i0 < to; i0 += 32) {
-      const bool in = i0 + lane < to;
-      const uint32_t key = in ? key_at(i0 + lane) : 0u;
-      const uint32_t d = in ? (key >> shift) & (digits - 1) : 0xffffffffu;
-      const unsigned same = __match_any_sync(0xffffffffu, d);
-      if (in) {
-        const int to_place = base[d] + mine[d] + __popc(same & below);
-        dst[to_place] = key;
-        dst_at[to_place] = pass > 0 ? __ldcg(src_at + i0 + lane) : static_cast<uint32_t>(i0 + lane);
+    for (int i0 = from; i0 < to; i0 += 32 * U) {
+      uint32_t k[U], at[U];
+      load_keys(i0, k);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + 32 * u + lane;
+        at[u] = pass > 0 ? (i < to ? __ldcg(src_at + i) : 0u) : static_cast<uint32_t>(i);
       }
-      __syncwarp();
-      if (in && (same & below) == 0) mine[d] += __popc(same);
-      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i0 + 32 * u >= to) break;
+        const uint32_t d = digit_of(k[u]);
+        const unsigned same = __match_any_sync(0xffffffffu, d);
+        const bool in = d != 0xffffffffu;
+        int to_place = 0;
+        if (in) to_place = base[d] + mine[d] + __popc(same & below);
+        __syncwarp();
+        if (in && (same & below) == 0) mine[d] += __popc(same);
+        __syncwarp();
+        if (in) {
+          dst[to_place] = k[u];
+          dst_at[to_place] = at[u];
+        }
+      }
     }
     // the next pass reads what the other CTAs wrote, and overwrites what they read
     cluster_arrive();
@@ -183,11 +214,12 @@ sort_ids_kernel(const I* __restrict__ ids, int n, int V, long long padding, uint
     uint32_t* t = src; src = dst; dst = t;
     t = src_at; src_at = dst_at; dst_at = t;
   }
+#pragma unroll 4
   for (int i = from + lane; i < to; i += 32) {
-    const uint32_t key = __ldcg(src + i);
+    const uint32_t key = __ldcg(src + i), prev = i > 0 ? __ldcg(src + i - 1) : 0xffffffffu, next = i + 1 < n ? __ldcg(src + i + 1) : 0xffffffffu;
     if (key >= static_cast<uint32_t>(V)) continue;
-    if (i == 0 || __ldcg(src + i - 1) != key) begin[key] = i;
-    if (i == n - 1 || __ldcg(src + i + 1) != key) end[key] = i + 1;
+    if (prev != key) begin[key] = i;
+    if (next != key) end[key] = i + 1;
   }
 }
 
@@ -294,7 +326,7 @@ __global__ void __launch_bounds__(kBlock)
 join_rows_kernel(const uint32_t* __restrict__ keys, const int* __restrict__ begin, const int* __restrict__ end, const float* __restrict__ partial,
                  T* __restrict__ dw, int n, int V, int d, int run, int runs, float scale) {
   using R = Row<T, W>;
-  constexpr int N = R::N, kAlone = 64;
+  constexpr int N = R::N, kAlone = 8;
   __shared__ float shares[kWarps][32 * N];
   __shared__ int long_last[kWarps];
   grid_dep_wait();
@@ -321,7 +353,7 @@ join_rows_kernel(const uint32_t* __restrict__ keys, const int* __restrict__ begi
 #pragma unroll
     for (int e = 0; e < N; ++e) s[e] = 0.f;
     share(c, 1, s);
-#pragma unroll 4
+#pragma unroll 8
     for (int r = c + 1; r <= last; ++r) share(r, 0, s);
     R::store(dw + static_cast<size_t>(key) * d + col, s, scale);
   }
@@ -338,7 +370,7 @@ join_rows_kernel(const uint32_t* __restrict__ keys, const int* __restrict__ begi
     for (int e = 0; e < N; ++e) s[e] = 0.f;
     if (in) {
       if (warp == 0) share(c0, 1, s);
-#pragma unroll 4
+#pragma unroll 8
       for (int r = lo; r < hi; ++r) share(r, 0, s);
 #pragma unroll
       for (int e = 0; e < N; ++e) shares[warp][lane * N + e] = s[e];
@@ -380,7 +412,7 @@ int word_bytes(long long row_bytes, const void* a, const void* b) {
 
 // Sorted positions per warp: enough warps for the GPU, and few partial sums when there are many positions.
 int run_length(int n, int d) {
-  const long long warps = 32ll * 148, slabs = (d + 127) / 128;
+  const long long warps = 64ll * 148, slabs = (d + 127) / 128;
   int run = 16;
   while (run < 128 && n * slabs / (2 * run) >= warps) run *= 2;
   return run;
@@ -480,9 +512,10 @@ int nlfa_embedding_bwd(const void* g, int dtype, const void* ids, int id_bytes, 
   auto sort = [&](auto* typed, auto* kernel) {
     const int r = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), (kSortWarps + 2) * (1 << kMostDigitBits) * static_cast<int>(sizeof(int)));
     if (r != NLFA_OK) return r;
-    return checked(launch_cluster(kernel, dim3(1, kSortCtas), dim3(kSortThreads), smem, st, overlap_launches(kOverlapRowwise), kSortCtas,
+    const int ctas = resident_clusters(reinterpret_cast<const void*>(kernel), kSortThreads, static_cast<int>(smem), 16) > 0 ? 16 : 8;
+    return checked(launch_cluster(kernel, dim3(1, static_cast<unsigned>(ctas)), dim3(kSortThreads), smem, st, overlap_launches(kOverlapRowwise), ctas,
                                   typed, n, V, padding_idx, reinterpret_cast<uint32_t*>(at + s.keys), reinterpret_cast<uint32_t*>(at + s.places),
-                                  reinterpret_cast<int*>(at + s.begin), reinterpret_cast<int*>(at + s.end), passes, digit_bits));
+                                  reinterpret_cast<int*>(at + s.begin), reinterpret_cast<int*>(at + s.end), passes, digit_bits, ctas));
   };
   rc = id_bytes == 8 ? sort(static_cast<const long long*>(ids), sort_ids_kernel<long long>) : sort(static_cast<const int*>(ids), sort_ids_kernel<int>);
   if (rc != NLFA_OK) return rc;

@@ -2,10 +2,10 @@
 // g <- c g where c < 1 (or out <- c g).
 //
 // Bound by HBM: one read for the norm, one read and one write where the gradients change.  The tensors come as a table in the
-// launch's parameters (nothing is copied to the device, and a captured launch keeps its table); a CTA takes pieces of 8,192
-// elements of whichever tensor.  Squares are added eight at a time in float32 and the eights in float64; an eight whose sum leaves float32's
+// launch's parameters (nothing is copied to the device, and a captured launch keeps its table); a CTA takes pieces of 32 KB
+// of whichever tensor.  Squares are added eight at a time in float32 and the eights in float64; an eight whose sum leaves float32's
 // safe range is squared in float64 (gradients of 1e20, or of 1e-20, have a norm).  The sums of the CTAs are added in order by the one that ends
-// last, so the same call gives the same bits.  The clip goes through the tensors backwards: what the norm read last is still in L2.
+// last, so the same call gives the same bits.  The clip goes through the pieces backwards: what the norm read last is still in L2.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -19,10 +19,8 @@ namespace nlfa {
 namespace clip {
 namespace {
 
-using rowwise::Elem;
-
 constexpr int kBlock = 256;
-constexpr int kPiece = 8192;                    // elements
+constexpr int kPieceBytes = 32768;              // of a gradient
 constexpr int kCtasPerSm = 6;
 constexpr int kMostTables = 64;                 // launches of one call
 
@@ -63,9 +61,9 @@ __device__ __forceinline__ Piece piece_of(const Table<K>& t, int piece) {
   const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(p.src) & 15u);
   p.head = skew == 0 ? 0 : (16 - skew) / element_bytes(p.dtype);
   if (p.head > p.n) p.head = static_cast<int>(p.n);
-  const int at = piece - t.first[lo];
-  p.from = p.head + static_cast<long long>(at) * kPiece;
-  p.to = p.from + kPiece;
+  const int at = piece - t.first[lo], size = kPieceBytes / element_bytes(p.dtype);
+  p.from = p.head + static_cast<long long>(at) * size;
+  p.to = p.from + size;
   p.first = at == 0;
   p.last = p.to >= p.n;
   if (p.last) p.to = p.n;
@@ -110,28 +108,42 @@ struct Largest {
   static __device__ __forceinline__ double finish(double s) { return s; }
 };
 
+// 16 bytes of a gradient a thread and step, as many steps of a piece in flight.
+constexpr int kSteps = kPieceBytes / 16 / kBlock;
+
 template <typename S, typename Norm>
-__device__ __forceinline__ void norm_of(const Piece& p, Norm& acc) {
-  const S* src = static_cast<const S*>(p.src);
-  if (p.first && static_cast<int>(threadIdx.x) < p.head) acc.add(value(src[threadIdx.x]));
-  const int vectors = static_cast<int>((p.to - p.from) / 8);
-  const S* body = src + p.from;
-  constexpr int U = kPiece / 8 / kBlock;
-  typename Elem<S>::Raw raw[U];
+__device__ __forceinline__ void add_words(const uint4 (&raw)[kSteps], Norm& acc) {
+  constexpr int N = 16 / sizeof(S);
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = u * kBlock + threadIdx.x;
-    raw[u] = i < vectors ? Elem<S>::load_raw(body + 8 * i) : Elem<S>::zero();
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
+  for (int u = 0; u < kSteps; u += 8 / N) {
     float v[8];
-    Elem<S>::unpack(raw[u], v);
+#pragma unroll
+    for (int w = 0; w < 8 / N; ++w) {
+      S e[N];
+      *reinterpret_cast<uint4*>(e) = raw[u + w];
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[N * w + j] = value(e[j]);
+    }
     acc.add(v);
   }
+}
+template <typename S, typename Norm>
+__device__ __forceinline__ void add_ends(const Piece& p, Norm& acc) {
+  constexpr int N = 16 / sizeof(S);
+  const S* src = static_cast<const S*>(p.src);
+  if (p.first && static_cast<int>(threadIdx.x) < p.head) acc.add(value(src[threadIdx.x]));
   if (p.last) {
-    const long long i = p.from + 8ll * vectors + threadIdx.x;
+    const long long i = p.from + (p.to - p.from) / N * N + threadIdx.x;
     if (i < p.to) acc.add(value(src[i]));
+  }
+}
+__device__ __forceinline__ void load_words(const Piece& p, uint4 (&raw)[kSteps]) {
+  const int bytes = element_bytes(p.dtype), words = static_cast<int>((p.to - p.from) * bytes / 16);
+  const uint4* body = reinterpret_cast<const uint4*>(static_cast<const char*>(p.src) + p.from * bytes);
+#pragma unroll
+  for (int u = 0; u < kSteps; ++u) {
+    const int i = u * kBlock + threadIdx.x;
+    raw[u] = i < words ? __ldcs(body + i) : make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
@@ -148,11 +160,14 @@ norm_kernel(const __grid_constant__ Table<K> t, double* __restrict__ partial, in
   grid_dep_wait();
   grid_dep_release();
   Norm acc;
-  for (int i = blockIdx.x; i < t.pieces; i += gridDim.x) {
+  const int step = gridDim.x;
+  for (int i = blockIdx.x; i < t.pieces; i += step) {
     const Piece p = piece_of(t, i);
-    if (p.dtype == NLFA_DTYPE_F32) norm_of<float>(p, acc);
-    else if (p.dtype == NLFA_DTYPE_F16) norm_of<__half>(p, acc);
-    else norm_of<__nv_bfloat16>(p, acc);
+    uint4 raw[kSteps];
+    load_words(p, raw);
+    if (p.dtype == NLFA_DTYPE_F32) { add_ends<float>(p, acc); add_words<float>(raw, acc); }
+    else if (p.dtype == NLFA_DTYPE_F16) { add_ends<__half>(p, acc); add_words<__half>(raw, acc); }
+    else { add_ends<__nv_bfloat16>(p, acc); add_words<__nv_bfloat16>(raw, acc); }
   }
   auto block = [&](double v) {
 #pragma unroll
@@ -179,62 +194,83 @@ norm_kernel(const __grid_constant__ Table<K> t, double* __restrict__ partial, in
   }
 }
 
+// N scaled values to their place, N elements of D: 8 to 32 bytes, aligned to 16 at least
+template <typename D, int N>
+__device__ __forceinline__ void put(D* p, const float (&v)[N]) {
+  if constexpr (sizeof(D) == 4) {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+  } else {
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int j = 0; j < N; j += 2) w[j / 2] = Pack2<D>::pack(v[j], v[j + 1]);
+    if constexpr (N == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  }
+}
+// ... a whole sector in one store (16-bit gradients into float32: two stores of half a sector each took ... us more)
+__device__ __forceinline__ void put_sector(float* p, const float (&v)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+}
+
 template <typename S, typename D>
-__device__ __forceinline__ void scale_of(const Piece& p, float c) {
+__device__ __forceinline__ void scale_of(const Piece& p, const uint4 (&raw)[kSteps], float c) {
+  constexpr int N = 16 / sizeof(S);
   const S* src = static_cast<const S*>(p.src);
   D* dst = static_cast<D*>(p.dst);
-  if (p.first)
-    for (int i = threadIdx.x; i < p.head; i += kBlock) dst[i] = static_cast<D>(value(src[i]) * c);
-  if ((reinterpret_cast<uintptr_t>(dst + p.head) & 15u) != 0) {          // out lies otherwise than the gradient
-    for (long long i = p.from + threadIdx.x; i < p.to; i += kBlock) dst[i] = static_cast<D>(value(src[i]) * c);
-    return;
-  }
-  const int vectors = static_cast<int>((p.to - p.from) / 8);
-  const S* body = src + p.from;
-  D* out = dst + p.from;
-  constexpr int U = kPiece / 8 / kBlock;
-  typename Elem<S>::Raw raw[U];
+  const uintptr_t at = reinterpret_cast<uintptr_t>(dst + p.from);
+  const bool words = at % (N * sizeof(D) < 16 ? N * sizeof(D) : 16) == 0, sectors = at % 32 == 0;
+  const int whole = words ? static_cast<int>((p.to - p.from) / N) : 0;     // (out lies otherwise than the gradient: one by one)
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
+  for (int u = 0; u < kSteps; ++u) {
     const int i = u * kBlock + threadIdx.x;
-    if (i < vectors) raw[u] = Elem<S>::load_raw(body + 8 * i);
-  }
+    alignas(16) S e[N];
+    *reinterpret_cast<uint4*>(e) = raw[u];
+    float v[N];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = u * kBlock + threadIdx.x;
-    if (i >= vectors) break;
-    float v[8];
-    Elem<S>::unpack(raw[u], v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= c;
-    Elem<D>::store(out + 8 * i, v);
+    for (int j = 0; j < N; ++j) v[j] = value(e[j]) * c;
+    if (i >= whole) continue;
+    if constexpr (N == 8 && sizeof(D) == 4) {
+      if (sectors) {
+        put_sector(dst + p.from + N * i, v);
+        continue;
+      }
+    }
+    put(dst + p.from + N * i, v);
   }
-  if (p.last) {
-    const long long i = p.from + 8ll * vectors + threadIdx.x;
-    if (i < p.to) dst[i] = static_cast<D>(value(src[i]) * c);
-  }
+  auto one = [&](long long i) { dst[i] = static_cast<D>(value(src[i]) * c); };
+  if (p.first && static_cast<int>(threadIdx.x) < p.head) one(threadIdx.x);
+  if (!words || p.last)
+#pragma unroll 1
+    for (long long i = p.from + static_cast<long long>(N) * whole + threadIdx.x; i < p.to; i += kBlock) one(i);
 }
 
 template <typename S>
-__device__ __forceinline__ void scale_from(const Piece& p, float c) {
-  if (p.out_dtype == NLFA_DTYPE_F32) scale_of<S, float>(p, c);
-  else if (p.out_dtype == NLFA_DTYPE_F16) scale_of<S, __half>(p, c);
-  else scale_of<S, __nv_bfloat16>(p, c);
+__device__ __forceinline__ void scale_from(const Piece& p, const uint4 (&raw)[kSteps], float c) {
+  if (p.out_dtype == NLFA_DTYPE_F32) scale_of<S, float>(p, raw, c);
+  else if (p.out_dtype == NLFA_DTYPE_F16) scale_of<S, __half>(p, raw, c);
+  else scale_of<S, __nv_bfloat16>(p, raw, c);
 }
 
 template <int K>
-__global__ void __launch_bounds__(kBlock, 4)
+__global__ void __launch_bounds__(kBlock)
 scale_kernel(const __grid_constant__ Table<K> t, const Result* result, int in_place) {
   grid_dep_wait();
   grid_dep_release();
   const float c = result->factor;
   if (in_place && c == 1.f) return;
-  for (int i = t.pieces - 1 - static_cast<int>(blockIdx.x); i >= 0; i -= gridDim.x) {
-    const Piece p = piece_of(t, i);
-    if (c == 1.f && p.src == p.dst) continue;
-    if (p.dtype == NLFA_DTYPE_F32) scale_from<float>(p, c);
-    else if (p.dtype == NLFA_DTYPE_F16) scale_from<__half>(p, c);
-    else scale_from<__nv_bfloat16>(p, c);
+  const int step = gridDim.x;
+  int i = t.pieces - 1 - static_cast<int>(blockIdx.x);
+  for (Piece p = piece_of(t, i), next; i >= 0; i -= step, p = next) {
+    uint4 raw[kSteps];
+    const bool change = c != 1.f || p.src != p.dst;
+    if (change) load_words(p, raw);
+    if (i >= step) next = piece_of(t, i - step);
+    if (!change) continue;
+    if (p.dtype == NLFA_DTYPE_F32) scale_from<float>(p, raw, c);
+    else if (p.dtype == NLFA_DTYPE_F16) scale_from<__half>(p, raw, c);
+    else scale_from<__nv_bfloat16>(p, raw, c);
   }
 }
 
@@ -264,7 +300,8 @@ int run(const nlfa_grad* grads, int count, float max_norm, int norm, int scale, 
       long long body = g.n - (skew == 0 ? 0 : (16 - skew) / bytes_of(g.dtype));
       if (body < 1) body = 1;
       t.first[j] = static_cast<int>(pieces);
-      pieces += (body + kPiece - 1) / kPiece;
+      const int size = kPieceBytes / bytes_of(g.dtype);
+      pieces += (body + size - 1) / size;
       t.dtype[j] = static_cast<unsigned char>(g.dtype);
       t.out_dtype[j] = static_cast<unsigned char>(g.out != nullptr ? g.out_dtype : g.dtype);
       t.n[j] = g.n;

@@ -445,55 +445,67 @@ struct TokenEmbeddingBackward : public Node {
 
 // ------------------------------------------------------------------------------------------- gradient clip
 
-// Norm of the tensors, and their clip: see grad_clip.py, which documents the refusals.
-Tensor clip_grads(std::vector<Tensor> grads, const std::vector<Tensor>& outs, double max_norm, int norm, bool scale) {
-  TORCH_CHECK_VALUE(!grads.empty(), "clip_grads: no gradients");
-  TORCH_CHECK_VALUE(outs.empty() || outs.size() == grads.size(), "out: ", outs.size(), " tensors for ", grads.size(), " gradients");
-  TORCH_CHECK_VALUE(plain(grads[0]), "gradients must be plain CUDA tensors");
-  const c10::cuda::CUDAGuard guard(grads[0].device());
-  const Tensor like = grads[0];
+// Norm of the tensors, and their clip: see grad_clip.py, which documents the refusals.  A model has hundreds of gradients, and the
+// kernels take 10 us per 50 MB of them: what is done per tensor is kept to reads of its fields.
+Tensor clip_grads(const std::vector<const Tensor*>& grads, const std::vector<const Tensor*>& outs, double max_norm, int norm, bool scale) {
+  TORCH_CHECK_VALUE(!grads.empty() && plain(*grads[0]), "gradients must be plain CUDA tensors");
+  const Tensor& like = *grads[0];
+  const c10::cuda::CUDAGuard guard(like.device());
   std::vector<nlfa_grad> table;
-  std::vector<std::pair<Tensor, Tensor>> copies;                       // (gradient with gaps, its copy)
+  std::vector<Tensor> held;                                            // copies the launches read
+  std::vector<std::pair<const Tensor*, Tensor>> back;                  // (gradient with gaps, its copy)
   struct Span {
     uintptr_t from, to;
     size_t of;
   };
   std::vector<Span> spans;
   table.reserve(grads.size());
+  spans.reserve(grads.size() + outs.size());
+  auto takes = [&](const Tensor& t) {
+    const auto* impl = t.unsafeGetTensorImpl();
+    return t.defined() && t.is_cuda() && t.device() == like.device() && t.layout() == at::kStrided && !impl->is_python_dispatch() &&
+           dtype_code(t.scalar_type()) >= 0;
+  };
+  auto span = [&](const Tensor& t, size_t i) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    spans.push_back({at, at + static_cast<uintptr_t>(t.numel()) * t.element_size(), i});
+  };
   for (size_t i = 0; i < grads.size(); ++i) {
-    Tensor g = grads[i], o = outs.empty() ? Tensor() : outs[i];
-    const Tensor given = g;
-    TORCH_CHECK_VALUE(plain(g) && g.device() == like.device() && dtype_code(g.scalar_type()) >= 0,
-                      "gradient ", i, ": needs a plain float32, float16 or bfloat16 tensor on ", like.device());
-    if (o.defined()) {
-      TORCH_CHECK_VALUE(plain(o) && o.device() == like.device() && dtype_code(o.scalar_type()) >= 0 && o.sizes() == g.sizes(),
+    const Tensor& given = *grads[i];
+    TORCH_CHECK_VALUE(takes(given), "gradient ", i, ": needs a plain float32, float16 or bfloat16 tensor on ", like.device());
+    const bool dense = given.is_contiguous() || given.is_non_overlapping_and_dense();
+    const int dtype = dtype_code(given.scalar_type());
+    const void* from = given.data_ptr();
+    void* to = nullptr;
+    int out_dtype = 0;
+    if (!outs.empty()) {
+      const Tensor& o = *outs[i];
+      TORCH_CHECK_VALUE(takes(o) && o.sizes() == given.sizes(),
                         "out ", i, ": needs a plain float32, float16 or bfloat16 tensor of the gradient's shape on ", like.device());
-      TORCH_CHECK_VALUE(!o.requires_grad() || !at::GradMode::is_enabled(), "out ", i, " requires a gradient");
+      TORCH_CHECK_VALUE(!o.requires_grad(), "out ", i, " requires a gradient");
       TORCH_CHECK_VALUE(o.is_non_overlapping_and_dense(), "out ", i, " must be dense");
-      if (g.strides() != o.strides()) g = at::empty_strided(o.sizes(), o.strides(), g.options()).copy_(g.detach());
-    } else if (!g.is_non_overlapping_and_dense()) {
-      Tensor c = g.detach().contiguous();
-      if (scale) {
-        TORCH_CHECK_VALUE(at::has_internal_overlap(g) != at::MemOverlap::Yes, "gradient ", i, " has elements that share memory");
-        copies.emplace_back(g, c);
+      to = o.data_ptr();
+      out_dtype = dtype_code(o.scalar_type());
+      if (given.strides() != o.strides()) {
+        held.push_back(at::empty_strided(o.sizes(), o.strides(), given.options()).copy_(given.detach()));
+        from = held.back().data_ptr();
       }
-      g = c;
+      if (given.numel() && !(to == given.data_ptr() && out_dtype == dtype && given.strides() == o.strides())) span(o, i);
+    } else if (!dense) {
+      held.push_back(given.detach().contiguous());
+      from = held.back().data_ptr();
+      if (scale) {
+        TORCH_CHECK_VALUE(at::has_internal_overlap(given) != at::MemOverlap::Yes, "gradient ", i, " has elements that share memory");
+        back.emplace_back(&given, held.back());
+      }
     }
-    grads[i] = g;
-    if (g.numel() == 0) continue;
-    table.push_back({g.data_ptr(), o.defined() ? o.data_ptr() : nullptr, g.numel(), dtype_code(g.scalar_type()),
-                     o.defined() ? dtype_code(o.scalar_type()) : 0});
-    if (!scale) continue;
-    auto span = [&](const Tensor& t) {
-      const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
-      spans.push_back({at, at + static_cast<uintptr_t>(t.numel()) * t.element_size(), i});
-    };
-    if (given.is_non_overlapping_and_dense()) span(given);
-    if (o.defined() && !(o.data_ptr() == given.data_ptr() && o.scalar_type() == given.scalar_type() && o.strides() == given.strides()))
-      span(o);
+    if (given.numel() == 0) continue;
+    if (dense) span(given, i);
+    table.push_back({from, to, given.numel(), dtype, out_dtype});
   }
   if (scale) {
-    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+    const auto first = [](const Span& a, const Span& b) { return a.from < b.from; };
+    if (!std::is_sorted(spans.begin(), spans.end(), first)) std::sort(spans.begin(), spans.end(), first);
     for (size_t i = 1; i < spans.size(); ++i)
       TORCH_CHECK_VALUE(spans[i].from >= spans[i - 1].to, "tensors ", spans[i - 1].of, " and ", spans[i].of,
                         " share memory (a parameter given twice?)");
@@ -503,9 +515,9 @@ Tensor clip_grads(std::vector<Tensor> grads, const std::vector<Tensor>& outs, do
   check("nlfa_clip_grads", nlfa_clip_grads(table.data(), static_cast<int>(table.size()), static_cast<float>(max_norm), norm, scale ? 1 : 0,
                                            static_cast<float*>(total.data_ptr()), scratch.data_ptr(), static_cast<size_t>(scratch.numel()),
                                            stream_of(like)));
-  for (auto& [g, c] : copies) g.detach().copy_(c);
+  for (auto& [g, c] : back) g->detach().copy_(c);
   if (scale)
-    for (const Tensor& t : outs.empty() ? grads : outs) t.unsafeGetTensorImpl()->bump_version();
+    for (const Tensor* t : outs.empty() ? grads : outs) t->unsafeGetTensorImpl()->bump_version();
   return total;
 }
 
@@ -839,31 +851,36 @@ PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// clip_grads(list of tensors, list of tensors | None, max_norm, norm code, scale) -> norm
+// clip_grads(list of tensors, list of tensors | None, max_norm, norm code, scale, of_parameters) -> norm | None
+// of_parameters: the tensors' gradients, where they have one (None: none has).
 PyObject* py_clip_grads(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK(n == 5, "clip_grads takes 5 arguments");
-  auto tensors = [](PyObject* o, const char* what) {
-    std::vector<Tensor> v;
+  TORCH_CHECK(n == 6, "clip_grads takes 6 arguments");
+  const bool of_parameters = truth(a[5]);
+  auto tensors = [](PyObject* o, const char* what, bool grads) {
+    std::vector<const Tensor*> v;
     if (o == Py_None) return v;
     TORCH_CHECK_TYPE(PyList_Check(o), what, " must be a list of tensors");
-    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(o); ++i) {
+    const Py_ssize_t count = PyList_GET_SIZE(o);
+    v.reserve(count);
+    for (Py_ssize_t i = 0; i < count; ++i) {
       PyObject* t = PyList_GET_ITEM(o, i);
       TORCH_CHECK_TYPE(is_tensor(t), what, " ", i, " must be a tensor, not ", Py_TYPE(t)->tp_name);
-      v.push_back(tensor(t));
+      const Tensor& x = tensor(t);
+      if (!grads) v.push_back(&x);
+      else if (x.grad().defined()) v.push_back(&x.grad());
     }
     return v;
   };
-  std::vector<Tensor> grads = tensors(a[0], "gradient"), outs = tensors(a[1], "out");
+  const std::vector<const Tensor*> grads = tensors(a[0], of_parameters ? "parameter" : "tensor", of_parameters);
+  const std::vector<const Tensor*> outs = tensors(a[1], "out", false);
   const double max_norm = number(a[2]);
   const int norm = integer(a[3]);
   const bool scale = truth(a[4]);
   TORCH_CHECK_VALUE(a[1] == Py_None || outs.size() == grads.size(), "out: ", outs.size(), " tensors for ", grads.size(), " gradients");
-  Tensor total;
-  {
-    py::gil_scoped_release no_gil;
-    total = clip_grads(std::move(grads), outs, max_norm, norm, scale);
-  }
+  if (grads.empty()) return decline();
+  // (the lists are the caller's and hold their tensors for as long as the interpreter lock is held)
+  const Tensor total = clip_grads(grads, outs, max_norm, norm, scale);
   return THPVariable_Wrap(total);
   END_HANDLE_TH_ERRORS
 }

@@ -155,7 +155,7 @@ copy_rows_kernel(const S* __restrict__ src, T* __restrict__ dst, const Head* hea
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = 0.f;
-    if (from >= 0) {
+    if (from >= 0 && c < d) {
       const S* s = src + static_cast<size_t>(from) * d + c;
       if (vec) rowwise::Elem<S>::load(s, v);
       else {
@@ -176,35 +176,44 @@ copy_rows_kernel(const S* __restrict__ src, T* __restrict__ dst, const Head* hea
 
 // ------------------------------------------------------------------------------------------------ losses
 
-// (max, sum) of a row's parts -> lse, loss.  Rows behind the last one get lse = +inf: their probabilities are zero.
+// (max, sum) of a row's parts -> lse, loss.  Rows behind the last one get lse = +inf: their probabilities are zero.  `lanes` threads per
+// row (a power of two up to 32): few rows have many parts.
 __global__ void __launch_bounds__(kBlock)
 finish_kernel(const Head* head, const float2* __restrict__ partial, const float* __restrict__ at_target, const int* __restrict__ row_of,
-              int n_rows, float* __restrict__ lse, float* __restrict__ lse_rest, float* __restrict__ each, float* __restrict__ out, double* sums, unsigned* ticket,
-              int mean) {
+              int n_rows, float* __restrict__ lse, float* __restrict__ lse_rest, float* __restrict__ each, float* __restrict__ out, double* sums,
+              unsigned* ticket, int mean, int lanes) {
   __shared__ double warp_sum[kBlock / 32];
   __shared__ int last;
   grid_dep_wait();
   grid_dep_release();
   const int all = head->count, parts = 2 * head->splits;
   const int end = all < kRowTile ? kRowTile : (all + kRowTile - 1) / kRowTile * kRowTile;
+  const int mine = threadIdx.x & (lanes - 1), rows = kBlock / lanes;
   double sum = 0.0;
-  for (int r = blockIdx.x * kBlock + threadIdx.x; r < end; r += gridDim.x * kBlock) {
-    if (r >= all) {
-      lse[r] = INFINITY;
-      lse_rest[r] = 0.f;
-      continue;
-    }
+  for (int r0 = blockIdx.x * rows; r0 < end; r0 += gridDim.x * rows) {
+    const int r = r0 + threadIdx.x / lanes;               // (end is a multiple of rows: whole warps stay together)
+    const bool live = r < all;
     float top = -INFINITY;
-    for (int s = 0; s < parts; ++s) top = fmaxf(top, partial[static_cast<size_t>(s) * n_rows + r].x);
+    if (live) {
+#pragma unroll 4
+      for (int s = mine; s < parts; s += lanes) top = fmaxf(top, partial[static_cast<size_t>(s) * n_rows + r].x);
+    }
+    for (int off = lanes / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
     const float shift = top == -INFINITY ? 0.f : top;
     float total = 0.f;
-    for (int s = 0; s < parts; ++s) {
-      const float2 q = partial[static_cast<size_t>(s) * n_rows + r];
-      total += q.y * expf(q.x - shift);
+    if (live) {
+#pragma unroll 4
+      for (int s = mine; s < parts; s += lanes) {
+        const float2 q = partial[static_cast<size_t>(s) * n_rows + r];
+        total += q.y * expf(q.x - shift);
+      }
     }
-    const float rest = logf(total);
-    lse[r] = shift + rest;
-    lse_rest[r] = rest - (lse[r] - shift);                // (NaN where lse is not finite)
+    for (int off = lanes / 2; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+    if (mine != 0) continue;
+    const float rest = logf(total), whole = shift + rest;
+    lse[r] = live ? whole : INFINITY;
+    lse_rest[r] = live ? rest - (whole - shift) : 0.f;    // (NaN where lse is not finite)
+    if (!live) continue;
     const float loss = (shift - at_target[r]) + rest;
     if (each != nullptr) each[row_of[r]] = loss;
     sum += loss;
@@ -229,52 +238,81 @@ finish_kernel(const Head* head, const float2* __restrict__ partial, const float*
 
 // ------------------------------------------------------------------------------------------------ backward
 
-// Factors of dl: g_i = alpha * row_scale_i with |row_scale| <= 2^14 (fp16, whose small probabilities would not be normal numbers
-// otherwise) or 1.  `grad` is one value, or one per row of the call (per_row).  One CTA.
+// The largest finite |grad| (1 if there is none): one CTA.
 __global__ void __launch_bounds__(1024)
-scale_rows_kernel(const Head* head, const float* __restrict__ grad, int per_row, int mean, const int* __restrict__ row_of,
-                  const int* __restrict__ target, float* __restrict__ row_scale, float* __restrict__ alpha, float unit) {
+largest_kernel(const Head* head, const float* __restrict__ grad, const int* __restrict__ row_of, float* __restrict__ largest) {
   __shared__ float warp_top[32];
   grid_dep_wait();
   grid_dep_release();
-  const int all = head->count;
-  const int end = all < kRowTile ? kRowTile : (all + kRowTile - 1) / kRowTile * kRowTile;
-  float top = 0.f;                                        // the largest finite one
-  if (per_row) {
-    for (int r = threadIdx.x; r < all; r += 1024) {
-      const float g = fabsf(grad[row_of[r]]);
-      if (g > top && g < INFINITY) top = g;
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
-    __syncthreads();
-    top = 0.f;
-    for (int w = 0; w < 32; ++w) top = fmaxf(top, warp_top[w]);
-    if (top == 0.f) top = 1.f;
+  float top = 0.f;
+#pragma unroll 4
+  for (int r = threadIdx.x; r < head->count; r += 1024) {
+    const float g = fabsf(grad[row_of[r]]);
+    if (g > top && g < INFINITY) top = g;
   }
-  for (int r = threadIdx.x; r < end; r += 1024) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < 32; ++w) top = fmaxf(top, warp_top[w]);
+  *largest = top > 0.f ? top : 1.f;
+}
+
+// In how many parts the sums of `rest` tiles of k blocks are formed, by one warp: the fewest blocks for the busiest pair of CTAs, with
+// kShare more for every share written and added.
+__device__ int choose_parts(int rest, int k, int pairs) {
+  constexpr int kShare = 4;
+  const int lane = threadIdx.x & 31, most = rest > 0 ? kPartsPerPair * pairs / rest : 1;
+  long long best = LLONG_MAX;
+  for (int s = 1 + lane; s <= most && s <= k; s += 32) {
+    const long long units = (rest * s + pairs - 1) / pairs, cost = units * ((k + s - 1) / s + (s > 1 ? kShare : 0)) + (s > 1 ? s : 0);
+    if (cost < best >> 8) best = cost << 8 | s;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, off));
+  return best == LLONG_MAX ? 1 : static_cast<int>(best & 255);
+}
+
+// Factors of dl: g_i = alpha row_scale_i.  `grad` is one value, which alpha takes, or one per row of the call (per_row), which row_scale
+// takes.  fp16: small probabilities would not be normal numbers, so dl is held times 2^14 (`unit`) over the largest |g| (`largest`).
+// Rows of dx that have no target become zeros on the way.
+template <typename I>
+__global__ void __launch_bounds__(kBlock)
+scale_rows_kernel(const Head* head, const float* __restrict__ grad, int per_row, int mean, const int* __restrict__ row_of,
+                  const int* __restrict__ target, float* __restrict__ row_scale, float* __restrict__ alpha, Parts* parts, const float* __restrict__ largest,
+                  float unit, const I* __restrict__ targets, int n, long long ignore, uint8_t* __restrict__ dx, long long row_bytes, int V,
+                  int d, int piece, int want_dw, int pairs) {
+  grid_dep_wait();
+  grid_dep_release();
+  const int all = head->count, stride = gridDim.x * kBlock;
+  const int end = all < kRowTile ? kRowTile : (all + kRowTile - 1) / kRowTile * kRowTile;
+  const float top = largest != nullptr ? *largest : 1.f;
+  for (int r = blockIdx.x * kBlock + threadIdx.x; r < end; r += stride) {
     float s = 0.f;
     if (r < all) {
-      s = unit;
-      if (per_row) s = grad[row_of[r]] / top * unit;
+      s = per_row ? grad[row_of[r]] / top * unit : unit;
       if (target[r] == -2) s = __int_as_float(0x7fffffff);
     }
     row_scale[r] = s;
   }
-  if (threadIdx.x == 0) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
     const float g = per_row ? top : mean ? *grad / static_cast<float>(all) : *grad;
     *alpha = all > 0 ? g / unit : 0.f;                    // (no target: gradients of zero, not 0 / 0)
   }
-}
-
-// zeros in the rows of dx that have no target
-template <typename I>
-__global__ void __launch_bounds__(kBlock)
-clear_rows_kernel(const I* __restrict__ targets, int n, long long ignore, const Head* head, uint8_t* __restrict__ dx, long long row_bytes) {
-  grid_dep_wait();
-  grid_dep_release();
-  if (head->count == n) return;
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x < 32) {
+    const int d_tiles = (d + kColTile - 1) / kColTile, rest_x = dx != nullptr ? end / kRowTile * d_tiles % pairs : 0;
+    for (int last = 0; last < 2; ++last) {
+      const int cols = last ? V - (V - 1) / piece * piece : piece;
+      const int rest_w = want_dw ? (cols + kColTile - 1) / kColTile * d_tiles % pairs : 0;
+      const int parts_w = choose_parts(rest_w, end / kK, pairs), parts_x = choose_parts(rest_x, (cols + kK - 1) / kK, pairs);
+      if (threadIdx.x == 0) {
+        parts->dw[last] = parts_w;
+        parts->dx[last] = parts_x;
+      }
+    }
+  }
+  if (dx == nullptr || all == n) return;
   const int lane = threadIdx.x & 31;
   for (int r = blockIdx.x * (kBlock / 32) + (threadIdx.x >> 5); r < n; r += gridDim.x * (kBlock / 32)) {
     if (counts(targets[r], ignore)) continue;
@@ -304,9 +342,9 @@ int check_call(const Call& c) {
 Layout layout(const Call& c, bool w_aligned) {
   Layout l{};
   l.n_rows = c.n < kRowTile ? kRowTile : (c.n + kRowTile - 1) / kRowTile * kRowTile;
-  l.d_pad = (c.d + 7) / 8 * 8;
+  l.d_pad = (c.d + 63) / 64 * 64;
   l.x_planes = c.dtype == NLFA_DTYPE_F32 ? 3 : 1;
-  l.copy_w = l.x_planes == 3 || c.w_dtype != c.dtype || c.d % 8 != 0 || !w_aligned;
+  l.copy_w = l.x_planes == 3 || c.w_dtype != c.dtype || c.d % 64 != 0 || !w_aligned;
   size_t at = 256;                                        // the head
   const size_t rows = static_cast<size_t>(l.n_rows) * 4;
   l.row_of = at; at = up(at + rows);
@@ -334,7 +372,7 @@ constexpr size_t kMostDl = 512ull << 20;
 
 struct BwdLayout {
   int piece;                        // columns, a multiple of kColTile
-  size_t row_scale, alpha, dl, dx_sum, bytes;
+  size_t row_scale, alpha, parts, dl, shares, dx_sum, bytes;
 };
 BwdLayout bwd_layout(const Call& c, const Layout& l) {
   BwdLayout b{};
@@ -346,18 +384,21 @@ BwdLayout bwd_layout(const Call& c, const Layout& l) {
   b.piece = (col_tiles + pieces - 1) / pieces * kColTile;
   size_t at = 0;
   b.row_scale = at; at = up(at + static_cast<size_t>(l.n_rows) * 4);
-  b.alpha = at; at = up(at + 4);
+  b.alpha = at; at = up(at + 8);                          // (and the largest |grad|)
+  b.parts = at; at = up(at + sizeof(Parts));
   b.dl = at; at = up(at + column * b.piece);
+  b.shares = at; at = up(at + share_bytes());
   b.dx_sum = at; if (pieces > 1) at = up(at + static_cast<size_t>(l.n_rows) * c.d * 4);
   b.bytes = at;
   return b;
 }
 
-int box_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes, int box_rows) {
-  const unsigned long long dims[4] = {static_cast<unsigned long long>(cols), static_cast<unsigned long long>(rows),
-                                      static_cast<unsigned long long>(planes), 1ull};
-  const unsigned long long strides[3] = {dims[0] * 2, dims[0] * dims[1] * 2, dims[0] * dims[1] * dims[2] * 2};
-  const unsigned box[4] = {64u, static_cast<unsigned>(box_rows), 1u, 1u};
+// [planes][rows][cols], cols a multiple of 64, as (64 columns, rows, blocks of 64 columns, planes)
+int box_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes, int box_rows, int box_blocks) {
+  const unsigned long long pitch = static_cast<unsigned long long>(cols) * 2, r = static_cast<unsigned long long>(rows);
+  const unsigned long long dims[4] = {64ull, r, pitch / 128, static_cast<unsigned long long>(planes)};
+  const unsigned long long strides[3] = {pitch, 128ull, pitch * r};
+  const unsigned box[4] = {64u, static_cast<unsigned>(box_rows), static_cast<unsigned>(box_blocks), 1u};
   return make_map(map, base, dtype, dims, strides, box);
 }
 
@@ -427,7 +468,7 @@ int run_fwd(const Call& c, const void* x, const void* w, const void* targets, in
   const int col_tiles = (c.V + kColTile - 1) / kColTile;
   auto pack = [&](auto* typed, auto* kernel) {
     return checked(launch_cluster(kernel, dim3(1, kScanCtas), dim3(kScanThreads), 0, st, overlap, kScanCtas, typed, c.n, l.n_rows, c.V,
-                                  ignore, t.head(), t.row_of(), t.target(), at_target, each, col_tiles, sm_count() / 2, l.max_splits));
+                                  ignore, t.head(), t.row_of(), t.target(), at_target, each, col_tiles, most_pairs(), l.max_splits));
   };
   int rc = target_bytes == 8 ? pack(static_cast<const long long*>(targets), pack_rows_kernel<long long>)
                              : pack(static_cast<const int*>(targets), pack_rows_kernel<int>);
@@ -439,11 +480,11 @@ int run_fwd(const Call& c, const void* x, const void* w, const void* targets, in
   rc = copy_rows(x, c.x_dtype, tape + l.x, dtype, t.head(), t.row_of(), c.n, l.n_rows, c.d, l.d_pad, l.x_planes, st);
   if (rc != NLFA_OK) return rc;
   CUtensorMap mx, mw;
-  rc = box_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes, 64);
-  if (rc == NLFA_OK) rc = box_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes, 64);
+  rc = box_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes, 128, kK / 64);
+  if (rc == NLFA_OK) rc = box_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes, 128, kK / 64);
   if (rc != NLFA_OK) return rc;
   Params p = params(c, l, t, status);
-  if (l.x_planes == 3 || c.d > 1024) p.chunk = l.x_planes == 3 ? 4 : 16;
+  if (l.x_planes == 3 || c.d > 1024) p.chunk = l.x_planes == 3 ? 2 : 8;
   p.partial = reinterpret_cast<float2*>(scratch + l.partial);
   p.at_target = at_target;
   rc = launch_product(kLse, dtype, p, mx, mw, mx, mx, st);
@@ -454,10 +495,12 @@ int run_fwd(const Call& c, const void* x, const void* w, const void* targets, in
     rc = launch_ticket(st, reinterpret_cast<unsigned*>(scratch + l.ticket), &ticket, &captured);
     if (rc != NLFA_OK) return rc;
   }
-  const int ctas = l.n_rows / kBlock < 1024 ? l.n_rows / kBlock : 1024;
+  int lanes = 1;
+  while (lanes < 32 && 2 * l.max_splits > 4 * lanes) lanes *= 2;
+  const int need = l.n_rows / (kBlock / lanes), ctas = need < 1024 ? need : 1024;
   return checked(launch_kernel(finish_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kBlock), 0, st, !captured && overlap, t.head(),
                                p.partial, at_target, t.row_of(), l.n_rows, t.lse(), t.lse_rest(), each, each != nullptr ? nullptr : out,
-                               reinterpret_cast<double*>(scratch + l.sums), ticket, reduction == NLFA_REDUCE_MEAN ? 1 : 0));
+                               reinterpret_cast<double*>(scratch + l.sums), ticket, reduction == NLFA_REDUCE_MEAN ? 1 : 0, lanes));
 }
 
 int run_bwd(const Call& c, const float* grad, const void* w, const void* targets, int target_bytes, long long ignore, int reduction,
@@ -471,35 +514,40 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
   const bool overlap = overlap_launches(kOverlapRowwise);
   float* row_scale = reinterpret_cast<float*>(scratch + b.row_scale);
   float* alpha = reinterpret_cast<float*>(scratch + b.alpha);
-  int rc = checked(launch_kernel(scale_rows_kernel, dim3(1), dim3(1024), 0, st, overlap, t.head(), grad,
-                                 reduction == NLFA_REDUCE_NONE ? 1 : 0, reduction == NLFA_REDUCE_MEAN ? 1 : 0, t.row_of(), t.target(),
-                                 row_scale, alpha, dtype == NLFA_DTYPE_F16 ? 16384.f : 1.f));
+  Parts* parts = reinterpret_cast<Parts*>(scratch + b.parts);
+  const int per_row = reduction == NLFA_REDUCE_NONE ? 1 : 0;
+  float* largest = per_row && dtype == NLFA_DTYPE_F16 ? alpha + 1 : nullptr;
+  int rc = NLFA_OK;
+  if (largest != nullptr)
+    rc = checked(launch_kernel(largest_kernel, dim3(1), dim3(1024), 0, st, overlap, t.head(), grad, t.row_of(), largest));
   if (rc != NLFA_OK) return rc;
-  if (dx != nullptr && c.n > 0) {
-    const long long row_bytes = static_cast<long long>(c.d) * (c.x_dtype == NLFA_DTYPE_F32 ? 4 : 2);
-    const int need = (c.n + kBlock / 32 - 1) / (kBlock / 32), most = 8 * sm_count();
-    auto clear = [&](auto* typed, auto* kernel) {
-      return checked(launch_kernel(kernel, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(kBlock), 0, st, overlap, typed,
-                                   c.n, ignore, t.head(), static_cast<uint8_t*>(dx), row_bytes));
-    };
-    rc = target_bytes == 8 ? clear(static_cast<const long long*>(targets), clear_rows_kernel<long long>)
-                           : clear(static_cast<const int*>(targets), clear_rows_kernel<int>);
-    if (rc != NLFA_OK) return rc;
-  }
+  const long long row_bytes = static_cast<long long>(c.d) * (c.x_dtype == NLFA_DTYPE_F32 ? 4 : 2);
+  const int need = l.n_rows / (kBlock / 32), most = 4 * sm_count();
+  auto scale = [&](auto* typed, auto* kernel) {
+    return checked(launch_kernel(kernel, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(kBlock), 0, st, overlap, t.head(), grad,
+                                 per_row, reduction == NLFA_REDUCE_MEAN ? 1 : 0, t.row_of(), t.target(), row_scale, alpha, parts, largest,
+                                 dtype == NLFA_DTYPE_F16 ? 16384.f : 1.f, typed, c.n, ignore, static_cast<uint8_t*>(dx), row_bytes, c.V, c.d, b.piece, dw != nullptr ? 1 : 0,
+                                 most_pairs()));
+  };
+  rc = target_bytes == 8 ? scale(static_cast<const long long*>(targets), scale_rows_kernel<long long>)
+                         : scale(static_cast<const int*>(targets), scale_rows_kernel<int>);
+  if (rc != NLFA_OK) return rc;
   CUtensorMap mx, mw, mds, mout;
-  rc = box_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes, 64);
-  if (rc == NLFA_OK) rc = box_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes, 64);
-  if (rc == NLFA_OK) rc = box_map(&mds, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes, 64);
-  if (rc == NLFA_OK) rc = box_map(&mout, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes, 32);
+  rc = box_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes, 128, kK / 64);
+  if (rc == NLFA_OK) rc = box_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes, 128, kK / 64);
+  if (rc == NLFA_OK) rc = box_map(&mds, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes, 128, kK / 64);
+  if (rc == NLFA_OK) rc = box_map(&mout, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes, 32, 1);
   if (rc != NLFA_OK) return rc;
   Params p = params(c, l, t, status);
-  p.chunk = l.x_planes == 3 ? 4 : 0;
+  p.chunk = l.x_planes == 3 ? 2 : 0;
   p.row_scale = row_scale;
   p.alpha = alpha;
+  p.parts = parts;
   p.dx = dx;
   p.dw = dw;
   p.dx_dtype = c.x_dtype;
   p.dw_dtype = c.w_dtype;
+  p.shares = reinterpret_cast<float*>(scratch + b.shares);
   p.dx_sum = reinterpret_cast<float*>(scratch + b.dx_sum);
   p.want_dx = dx != nullptr;
   p.want_dw = dw != nullptr;

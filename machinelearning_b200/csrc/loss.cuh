@@ -8,19 +8,24 @@ namespace loss {
 
 constexpr int kRowTile = 256;       // rows of a product's tile: two CTAs of 128
 constexpr int kColTile = 256;       // columns of a tile
-constexpr int kK = 64;              // summands per stage
+constexpr int kK = 128;             // summands per stage
+constexpr int kPartsPerPair = 2;    // shares of dW's, and of dx's, odd tiles there is room for, per pair of CTAs
 
 // The forward leaves its tape in one buffer; counts and places, known on the device only, stand first.
 struct Head {
   int count;                        // rows with a target
   int splits;                       // parts of the vocabulary in the forward's units
 };
+// In how many parts the sums of dW's and dx's odd tiles are formed, in all pieces of the vocabulary but the last, and in the last.
+struct Parts {
+  int dw[2], dx[2];
+};
 
 // Tape and scratch, laid out for n rows.  Rows without a target are left out on the way in (`row_of` names the source
 // of each row that stays), so they cost no products and whatever stands in them reaches nothing.
 struct Layout {
   int n_rows;                       // rows a call can hold, up to a multiple of kRowTile
-  int d_pad;                        // row length of the 16-bit copies
+  int d_pad;                        // row length of the 16-bit copies, a multiple of 64
   int x_planes;                     // 16-bit parts of an operand: 1, or 3 for float32
   bool copy_w;                      // the weight is converted or re-laid (otherwise the products read the caller's)
   size_t row_of, target, lse, lse_rest, x, w, tape_bytes;
@@ -48,12 +53,16 @@ struct Params {
   const float* alpha;
   void *dx, *dw;
   float* dx_sum;                    // float32 sums over the pieces, for a 16-bit dx
+  const Parts* parts;
+  float* shares;                    // of tiles formed in parts
   int dx_dtype, dw_dtype;
   int first, last;                  // piece is the first / last one
   int want_dx, want_dw;
   unsigned* status;
 };
 
+int most_pairs();                   // of CTAs that run at once
+size_t share_bytes();
 enum { kLse = 0, kGrad = 1, kProducts = 2 };
 int launch_product(int mode, int dtype, const Params& p, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& ds,
                    const CUtensorMap& ds_out, cudaStream_t stream);

@@ -5,8 +5,9 @@
 //
 // One persistent kernel per kind, a pair of CTAs (cta_group::2) per 256 x 256 tile: each CTA holds 128 rows of A, 128
 // columns of B and 128 x 256 of the sums, so an operand byte brought into shared memory serves twice the columns
-// of a single CTA's tile.  All operands come as boxes of 64 x 64 16-bit values, K-major or MN-major by their coordinates
-// alone.  Sums are double buffered in TMEM (2 x 256 columns): the epilogue of a tile runs under the next one's products.
+// of a single CTA's tile.  A stage is 128 summands, each operand of it one box of 32 KB: 128 rows x 2 blocks of 64 columns, K-major or
+// MN-major by what its coordinates mean.  (Loads bound these kernels, and how many there are counts as much as their bytes:
+// forward of 16,384 x 50,304 x 768 at 1,490 TFLOP/s with boxes of 8 KB, 1,583 with 16 KB, ... with 32 KB; as fast with four stages as with six.)  Sums are double buffered in TMEM (2 x 256 columns): the epilogue of a tile runs under the next one's products.
 //
 // The tensor core adds to its sums by truncation: a chain of K / 16 steps over positive summands comes out low by 6.6e-7 of
 // its value at K = 768, 1.1e-5 at 4,096 and 7.7e-5 at 16,384 (measured; a float32 product on the CUDA cores is off by 5e-8).  Where that shows,
@@ -26,7 +27,8 @@ namespace {
 
 constexpr int kThreads = 320;
 constexpr int kEpilogueWarps = 8;
-constexpr int kStages = 6;
+constexpr int kStages = 3;
+constexpr int kBlockBytes = 128 * 128;                        // 128 rows of 64 columns
 constexpr int kOperandBytes = 128 * kK * 2;                   // one CTA's half of an operand
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kStagingBytes = 4096;                           // per epilogue warp
@@ -49,10 +51,66 @@ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; 
 // A tile: where it lies in A's rows and B's columns, how many stages its sum takes, which operands it has.
 struct Tile {
   int m0, n0;
-  int k_blocks;                     // blocks of 64 summands per pair of parts
+  int k0, k1;                       // its blocks of kK summands (per pair of parts): all, or of a shared tile this pair's
   int dw;                           // kProducts: a tile of dW (else of dx)
   int first, last;                  // kLse: first / last tile of a unit
-  int slot;                         // kLse: which part of the vocabulary
+  int slot;                         // kLse: which part of the vocabulary; kProducts: where a share of a tile goes (-1: the tile is whole)
+};
+
+// kProducts: the units are dW's tiles and then dx's, handed out in turn: whole tiles, as many of each kind as all pairs of CTAs get,
+// and the rest, whose sums are cut into parts so that every pair is busy (loss.cu: choose_parts; fold_kernel adds the shares).  Parts of one
+// index stand together: they read the same summands, from L2.  (Cut into one line of equal lengths instead, they read everything from
+// HBM: products of 16,384 tokens over 12,800 words 768 wide 427 us with whole tiles only, 468 us so, ... us as it is.)
+struct Plan {
+  int d_tiles, kw, kx;
+  int dw_whole, dw_rest, dw_parts, dx_whole, dx_rest, dx_parts;
+  int u1, u2, u3, u4;               // ends of the four kinds of units
+  int dx_slot;                      // dx's first share
+  Plan() = default;
+  __device__ Plan(const Params& p, int rows, int pairs) {
+    const int row_tiles = rows > 0 ? ceil_div(rows, kRowTile) : 1;
+    d_tiles = ceil_div(p.d, kColTile);
+    const int dw_tiles = p.want_dw ? ceil_div(p.v1 - p.v0, kColTile) * d_tiles : 0, dx_tiles = p.want_dx ? row_tiles * d_tiles : 0;
+    kw = row_tiles * (kRowTile / kK);
+    kx = ceil_div(p.v1 - p.v0, kK);
+    dw_whole = dw_tiles / pairs * pairs;
+    dx_whole = dx_tiles / pairs * pairs;
+    dw_rest = dw_tiles - dw_whole;
+    dx_rest = dx_tiles - dx_whole;
+    dw_parts = p.parts->dw[p.last];
+    dx_parts = p.parts->dx[p.last];
+    u1 = dw_whole;
+    u2 = u1 + dw_rest * dw_parts;
+    u3 = u2 + dx_whole;
+    u4 = u3 + dx_rest * dx_parts;
+    dx_slot = kPartsPerPair * pairs;
+  }
+  __device__ bool unit(int u, Tile& t) const {
+    if (u >= u4) return false;
+    t.dw = u < u2;
+    const int first = t.dw ? 0 : u2, whole = t.dw ? dw_whole : dx_whole, rest = t.dw ? dw_rest : dx_rest;
+    const int parts = t.dw ? dw_parts : dx_parts, k = t.dw ? kw : kx, i = u - first - whole;
+    int v = u - first;
+    t.k0 = 0;
+    t.k1 = k;
+    t.slot = -1;
+    if (i >= 0) {
+      const int part = i / rest;
+      v = whole + i - part * rest;
+      if (parts > 1) {
+        t.k0 = static_cast<int>(static_cast<long long>(k) * part / parts);
+        t.k1 = static_cast<int>(static_cast<long long>(k) * (part + 1) / parts);
+        t.slot = (t.dw ? 0 : dx_slot) + i;
+      }
+    }
+    place(v, t);
+    return true;
+  }
+  __device__ void place(int v, Tile& t) const {
+    const int m = v / d_tiles;
+    t.m0 = m * kRowTile;                                       // dW: columns of dl, from the piece's first
+    t.n0 = (v - m * d_tiles) * kColTile;
+  }
 };
 
 // The tiles of one pair of CTAs, in order; every role walks the same list.
@@ -61,28 +119,29 @@ struct Walk {
   const Params& p;
   int rows, row_tiles, stride, u, units;
   int n, n_end;                     // kLse: column tiles left in the unit
-  int col_tiles, splits, dw_tiles, d_tiles;
+  int col_tiles, splits;
+  Plan plan;                        // kProducts
 
-  __device__ Walk(const Params& p_, int pair, int n_pairs) : p(p_) {
-    rows = *reinterpret_cast<const volatile int*>(&p.head->count);
+  __device__ Walk(const Params& p_, int pair, int n_pairs) : p(p_), rows(p_.head->count), stride(n_pairs) {
     row_tiles = rows > 0 ? ceil_div(rows, kRowTile) : 1;        // (no row: one tile of zeros, which leaves zero gradients)
-    stride = n_pairs;
     u = pair - n_pairs;
     n = n_end = 0;
     splits = 1;
     if (MODE == kLse) {
-      splits = *reinterpret_cast<const volatile int*>(&p.head->splits);
+      splits = p.head->splits;
       col_tiles = ceil_div(p.V, kColTile);
       units = row_tiles * splits;
-    } else {
+    } else if (MODE == kGrad) {
       col_tiles = ceil_div(p.v1 - p.v0, kColTile);
-      d_tiles = ceil_div(p.d, kColTile);
-      dw_tiles = MODE == kProducts && p.want_dw ? col_tiles * d_tiles : 0;
-      units = MODE == kGrad ? row_tiles * col_tiles : dw_tiles + (p.want_dx ? row_tiles * d_tiles : 0);
+      units = row_tiles * col_tiles;
+    } else {
+      plan = Plan(p, rows, n_pairs);
     }
   }
 
   __device__ bool next(Tile& t) {
+    t.k0 = 0;
+    if (MODE != kProducts) t.k1 = ceil_div(p.d, kK);
     if (MODE == kLse) {
       t.first = 0;
       if (n == n_end) {
@@ -98,28 +157,20 @@ struct Walk {
       }
       t.n0 = n * kColTile;
       t.last = ++n == n_end;
-      t.k_blocks = ceil_div(p.d, kK);
       return true;
     }
     u += stride;
-    if (u >= units) return false;
     if (MODE == kGrad) {
+      if (u >= units) return false;
       // eight row tiles at a time past all columns of the piece
       const int group = 8 * col_tiles, g = u / group, v = u - g * group;
       const int size = row_tiles - 8 * g < 8 ? row_tiles - 8 * g : 8;
       const int c = v / size;
       t.m0 = (8 * g + v - c * size) * kRowTile;
       t.n0 = p.v0 + c * kColTile;
-      t.k_blocks = ceil_div(p.d, kK);
-    } else {
-      // dW's tiles, the longest sums, first
-      t.dw = u < dw_tiles;
-      const int v = t.dw ? u : u - dw_tiles, m = v / d_tiles;
-      t.m0 = m * kRowTile;                                     // dW: columns of dl, from the piece's first
-      t.n0 = (v - m * d_tiles) * kColTile;
-      t.k_blocks = t.dw ? row_tiles * (kRowTile / kK) : ceil_div(p.v1 - p.v0, kK);
+      return true;
     }
-    return true;
+    return plan.unit(u, t);
   }
 };
 
@@ -129,6 +180,89 @@ template <>
 __device__ __forceinline__ float round_to<__nv_bfloat16>(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
 template <>
 __device__ __forceinline__ float round_to<__half>(float x) { return __half2float(__float2half_rn(x)); }
+
+// Where a product's values go: four of row `m` of its tiles' rows, columns cc ..
+struct Out {
+  const Params& p;
+  int dw, dtype, m_end;
+  float alpha;
+  void* to;
+  bool vec;
+  __device__ Out(const Params& p_, int dw_, int rows) : p(p_), dw(dw_) {
+    dtype = dw ? p.dw_dtype : p.dx_dtype;
+    m_end = dw ? p.v1 - p.v0 : rows;
+    alpha = *p.alpha;
+    to = dw ? p.dw : p.dx;
+    vec = p.d % 4 == 0;
+  }
+  __device__ __forceinline__ void put(int m, int cc, float (&v)[4]) const {
+    if (m >= m_end || cc >= p.d) return;
+    const int n = p.d - cc < 4 ? p.d - cc : 4;
+    size_t at = static_cast<size_t>(dw ? p.v0 + m : m) * p.d + cc;
+    if (!dw && !(p.first && p.last)) {                         // dx is summed over the pieces
+      float* sum = p.dx_sum + at;
+      if (vec) {
+        float4* s4 = reinterpret_cast<float4*>(sum);
+        if (!p.first) {
+          const float4 b = *s4;
+          v[0] += b.x; v[1] += b.y; v[2] += b.z; v[3] += b.w;
+        }
+        if (!p.last) *s4 = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+        for (int e = 0; e < n; ++e) {
+          if (!p.first) v[e] += sum[e];
+          if (!p.last) sum[e] = v[e];
+        }
+      }
+      if (!p.last) return;
+    }
+    if (!dw) at = static_cast<size_t>(p.row_of[m]) * p.d + cc;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= alpha;
+    if (dtype == NLFA_DTYPE_F32) {
+      float* o = static_cast<float*>(to) + at;
+      if (vec) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+      else for (int e = 0; e < n; ++e) o[e] = v[e];
+    } else if (dtype == NLFA_DTYPE_BF16) {
+      __nv_bfloat16* o = static_cast<__nv_bfloat16*>(to) + at;
+      if (vec) *reinterpret_cast<uint2*>(o) = make_uint2(Pack2<__nv_bfloat16>::pack(v[0], v[1]), Pack2<__nv_bfloat16>::pack(v[2], v[3]));
+      else for (int e = 0; e < n; ++e) o[e] = __float2bfloat16_rn(v[e]);
+    } else {
+      __half* o = static_cast<__half*>(to) + at;
+      if (vec) *reinterpret_cast<uint2*>(o) = make_uint2(Pack2<__half>::pack(v[0], v[1]), Pack2<__half>::pack(v[2], v[3]));
+      else for (int e = 0; e < n; ++e) o[e] = __float2half_rn(v[e]);
+    }
+  }
+};
+
+// The shares of a tile formed in parts (blockIdx.x), added in order; 4 rows a CTA.
+constexpr int kFoldThreads = 256, kFoldRows = 4;
+__global__ void __launch_bounds__(kFoldThreads)
+fold_kernel(const Params p, int pairs) {
+  grid_dep_wait();
+  grid_dep_release();
+  const Plan plan(p, p.head->count, pairs);
+  int i = blockIdx.x;
+  Tile t;
+  t.dw = i < plan.dw_rest;
+  if (!t.dw) i -= plan.dw_rest;
+  const int rest = t.dw ? plan.dw_rest : plan.dx_rest, parts = t.dw ? plan.dw_parts : plan.dx_parts;
+  if (i >= rest || parts < 2) return;
+  plan.place((t.dw ? plan.dw_whole : plan.dx_whole) + i, t);
+  const Out out(p, t.dw, p.head->count);
+  const int cc = 4 * (threadIdx.x & 63);
+  if (t.n0 + cc >= p.d) return;
+  const float* shares = p.shares + (static_cast<size_t>(t.dw ? 0 : plan.dx_slot) + i) * (kRowTile * kColTile) + cc;
+  const int r = blockIdx.y * kFoldRows + (threadIdx.x >> 6);
+  if (t.m0 + r >= out.m_end) return;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int part = 0; part < parts; ++part) {
+    const float4 x = *reinterpret_cast<const float4*>(shares + (static_cast<size_t>(part) * rest * kRowTile + r) * kColTile);
+    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+  }
+  out.put(t.m0 + r, t.n0 + cc, v);
+}
 
 // ---- epilogues: a thread has row `lane` of its warp's 32 and, 32 at a time, 128 columns
 
@@ -209,28 +343,22 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
         const CUtensorMap* ma = MODE == kProducts ? &tm_ds : &tm_x;
         const CUtensorMap* mb = MODE == kProducts && t.dw ? &tm_x : &tm_w;
         const int a0 = t.m0 + 128 * rank, b0 = t.n0 + 128 * rank;
-        const int chunk = LONG ? p.chunk : t.k_blocks;
-        for (int k0 = 0; ok && k0 < t.k_blocks; k0 += chunk)
+        const int chunk = LONG ? p.chunk : t.k1 - t.k0;
+        for (int k0 = t.k0; ok && k0 < t.k1; k0 += chunk)
           for (int pr = 0; ok && pr < p.pairs; ++pr) {
             const int pa = p.pairs == 1 ? 0 : part_a(pr), pb = p.pairs == 1 ? 0 : part_b(pr);
-            const int k1 = t.k_blocks - k0 < chunk ? t.k_blocks : k0 + chunk;
+            const int k1 = t.k1 - k0 < chunk ? t.k1 : k0 + chunk;
             for (int kb = k0; kb < k1; ++kb, ++it) {
               const int s = it % kStages;
               if (!(ok = mbar_wait(bar(EMPTY + s), ((it / kStages) & 1) ^ 1, wctx, 90))) break;
               const uint32_t st = base + s * kStageBytes, full = full0 + 8u * s;
               if (rank == 0) mbar_arrive_expect_tx(bar(FULL + s), 2 * kStageBytes);
-              const int k = kb * kK;
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                if (MODE == kProducts && t.dw) tma_load_4d_pair(st + j * 8192, ma, full, a0 + 64 * j, k, pa, 0);
-                else tma_load_4d_pair(st + j * 8192, ma, full, k, a0 + 64 * j, pa, 0);
-              }
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const uint32_t dst = st + kOperandBytes + j * 8192;
-                if (MODE != kProducts) tma_load_4d_pair(dst, mb, full, k, b0 + 64 * j, pb, 0);
-                else tma_load_4d_pair(dst, mb, full, b0 + 64 * j, t.dw ? k : p.v0 + k, pb, 0);
-              }
+              // boxes at (row, block of 64 columns): the sum runs along the columns, or (MN-major) along the rows
+              const int blk = kb * (kK / 64), a_blk = a0 / 64, b_blk = b0 / 64;
+              if (MODE == kProducts && t.dw) tma_load_4d_pair(st, ma, full, 0, kb * kK, a_blk, pa);
+              else tma_load_4d_pair(st, ma, full, 0, a0, blk, pa);
+              if (MODE != kProducts) tma_load_4d_pair(st + kOperandBytes, mb, full, 0, b0, blk, pb);
+              else tma_load_4d_pair(st + kOperandBytes, mb, full, 0, (t.dw ? 0 : p.v0) + kb * kK, b_blk, pb);
             }
           }
       }
@@ -249,23 +377,25 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
       while (ok && walk.next(t)) {
         const bool a_mn = MODE == kProducts && t.dw, b_mn = MODE == kProducts;
         const uint32_t idesc = a_mn ? make_idesc(kBf16, 256, kColTile, true, b_mn) : make_idesc(kBf16, 256, kColTile, false, b_mn);
-        const uint32_t a_step = a_mn ? 2048u : 32u, a_lbo = a_mn ? 8192u : 16u;
-        const uint32_t b_step = b_mn ? 2048u : 32u, b_lbo = b_mn ? 8192u : 16u;
-        const int chunk = LONG ? p.chunk : t.k_blocks;
-        for (int k0 = 0; ok && k0 < t.k_blocks; k0 += chunk, ++sums) {
+        // 16 summands on: 32 bytes along a row, four times per block of 64 columns, or 16 rows
+        const uint32_t a_lbo = a_mn ? kBlockBytes : 16u, b_lbo = b_mn ? kBlockBytes : 16u;
+        const int chunk = LONG ? p.chunk : t.k1 - t.k0;
+        for (int k0 = t.k0; ok && k0 < t.k1; k0 += chunk, ++sums) {
           const int buf = sums & 1;
           if (!(ok = mbar_wait(bar(ACC_EMPTY + buf), ((sums >> 1) & 1) ^ 1, wctx, 92))) break;
           tc_fence_after();
-          const int blocks = p.pairs * (t.k_blocks - k0 < chunk ? t.k_blocks - k0 : chunk);
+          const int blocks = p.pairs * (t.k1 - k0 < chunk ? t.k1 - k0 : chunk);
           for (int kb = 0; kb < blocks; ++kb, ++it) {
             const int s = it % kStages;
             if (!(ok = mbar_wait(bar(FULL + s), (it / kStages) & 1, wctx, 93))) break;
             tc_fence_after();
             const uint32_t a = base + s * kStageBytes, b = a + kOperandBytes;
 #pragma unroll
-            for (int kk = 0; kk < kK / 16; ++kk)
-              umma_ss_pair(leader, tmem + buf * kColTile, make_smem_desc(a + kk * a_step, a_lbo, 1024),
-                           make_smem_desc(b + kk * b_step, b_lbo, 1024), idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < kK / 16; ++kk) {
+              const uint32_t along_rows = (kk / 4) * kBlockBytes + (kk % 4) * 32u, along_k = kk * 2048u;
+              umma_ss_pair(leader, tmem + buf * kColTile, make_smem_desc(a + (a_mn ? along_k : along_rows), a_lbo, 1024),
+                           make_smem_desc(b + (b_mn ? along_k : along_rows), b_lbo, 1024), idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+            }
             umma_commit_pair(leader, bar(EMPTY + s));
           }
           if (ok) umma_commit_pair(leader, bar(ACC_FULL + buf));
@@ -303,7 +433,7 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
       if constexpr (LONG) {
 #pragma unroll
         for (int j = 0; j < 128; ++j) l.v[j] = 0.f;
-        for (int k0 = 0; k0 < t.k_blocks; k0 += p.chunk, ++sums) {
+        for (int k0 = t.k0; k0 < t.k1; k0 += p.chunk, ++sums) {
           buf = sums & 1;
           if (!(ok = mbar_wait(bar(ACC_FULL + buf), (sums >> 1) & 1, wctx, 94))) break;
           tc_fence_after();
@@ -412,7 +542,7 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_4d(&tm_out, staging, c0 + 64 * c2 - p.v0, row0, part, 0);
+              tma_store_4d(&tm_out, staging, 0, row0, (c0 + 64 * c2 - p.v0) / 64, part);
               tma_store_commit();
             }
             if (part + 1 < p.planes) {
@@ -425,13 +555,9 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
         }
       } else {
         // 32 x 32 values through shared memory, so that a row's columns leave side by side
-        const float alpha = *p.alpha;
-        const int rows = walk.rows;
-        const int m0 = t.dw ? p.v0 + t.m0 + 128 * rank + 32 * q : row0;
-        const int m_end = t.dw ? p.v1 : rows;
-        const int dtype = t.dw ? p.dw_dtype : p.dx_dtype;
-        void* out = t.dw ? p.dw : p.dx;
-        const bool vec = p.d % 4 == 0;
+        const Out out(p, t.dw, walk.rows);
+        const int local = 128 * rank + 32 * q;
+        float* share = t.slot < 0 ? nullptr : p.shares + (static_cast<size_t>(t.slot) * kRowTile + local) * kColTile;
 #pragma unroll (LONG ? 4 : 1)
         for (int c = 0; c < 4; ++c) {
           const int col = c0 + 32 * c;
@@ -446,46 +572,12 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
           const int cc = col + 4 * (lane & 7);
 #pragma unroll 1
           for (int i = 0; i < 8; ++i) {
-            const int lr = 4 * i + (lane >> 3), m = m0 + lr;
+            const int lr = 4 * i + (lane >> 3);
             uint32_t w0, w1, w2, w3;
             ld_shared_v4(staging + lr * 128 + (((lane & 7) ^ (lr & 7)) * 16), w0, w1, w2, w3);
-            if (m >= m_end || cc >= p.d) continue;
             float v[4] = {__uint_as_float(w0), __uint_as_float(w1), __uint_as_float(w2), __uint_as_float(w3)};
-            const int n = p.d - cc < 4 ? p.d - cc : 4;
-            size_t at = static_cast<size_t>(m) * p.d + cc;
-            if (!t.dw && (p.first == 0 || p.last == 0)) {
-              float* sum = p.dx_sum + at;
-              if (vec) {
-                float4* s4 = reinterpret_cast<float4*>(sum);
-                if (!p.first) {
-                  const float4 b = *s4;
-                  v[0] += b.x; v[1] += b.y; v[2] += b.z; v[3] += b.w;
-                }
-                if (!p.last) *s4 = make_float4(v[0], v[1], v[2], v[3]);
-              } else {
-                for (int e = 0; e < n; ++e) {
-                  if (!p.first) v[e] += sum[e];
-                  if (!p.last) sum[e] = v[e];
-                }
-              }
-              if (!p.last) continue;
-            }
-            if (!t.dw) at = static_cast<size_t>(p.row_of[m]) * p.d + cc;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= alpha;
-            if (dtype == NLFA_DTYPE_F32) {
-              float* o = static_cast<float*>(out) + at;
-              if (vec) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-              else for (int e = 0; e < n; ++e) o[e] = v[e];
-            } else if (dtype == NLFA_DTYPE_BF16) {
-              __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out) + at;
-              if (vec) *reinterpret_cast<uint2*>(o) = make_uint2(Pack2<__nv_bfloat16>::pack(v[0], v[1]), Pack2<__nv_bfloat16>::pack(v[2], v[3]));
-              else for (int e = 0; e < n; ++e) o[e] = __float2bfloat16_rn(v[e]);
-            } else {
-              __half* o = static_cast<__half*>(out) + at;
-              if (vec) *reinterpret_cast<uint2*>(o) = make_uint2(Pack2<__half>::pack(v[0], v[1]), Pack2<__half>::pack(v[2], v[3]));
-              else for (int e = 0; e < n; ++e) o[e] = __float2half_rn(v[e]);
-            }
+            if (share != nullptr) *reinterpret_cast<float4*>(share + static_cast<size_t>(lr) * kColTile + (cc - t.n0)) = make_float4(v[0], v[1], v[2], v[3]);
+            else out.put(t.m0 + local + lr, cc, v);
           }
           __syncwarp();
         }
@@ -509,7 +601,7 @@ int launch_one(const Params& p, const CUtensorMap& x, const CUtensorMap& w, cons
   auto* kernel = loss_kernel<T, MODE, LONG>;
   const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), kSmem);
   if (rc != NLFA_OK) return rc;
-  const int pairs = sm_count() / 2;
+  const int pairs = most_pairs();
   // (a pair has to lie along x: along y the launch is refused)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2u * static_cast<unsigned>(pairs));
@@ -524,12 +616,18 @@ int launch_one(const Params& p, const CUtensorMap& x, const CUtensorMap& w, cons
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = overlap_launches(kOverlapRowwise) ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, x, w, ds, out, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, x, w, ds, out, p);
+  if (MODE == kProducts && e == cudaSuccess)
+    e = launch_kernel(fold_kernel, dim3(2u * static_cast<unsigned>(pairs), kRowTile / kFoldRows), dim3(kFoldThreads), 0, stream,
+                      overlap_launches(kOverlapRowwise), p, pairs);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? NLFA_OK : NLFA_ERR_CUDA;
 }
 
 }  // namespace
+
+int most_pairs() { return sm_count() / 2; }
+size_t share_bytes() { return static_cast<size_t>(2 * kPartsPerPair * most_pairs()) * kRowTile * kColTile * sizeof(float); }
 
 int launch_product(int mode, int dtype, const Params& p, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& ds,
                    const CUtensorMap& ds_out, cudaStream_t stream) {

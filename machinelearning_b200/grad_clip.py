@@ -32,17 +32,15 @@ def _norm_code(norm_type) -> int:
     return code
 
 
-def _host():
+def _run(tensors, out, max_norm, code, scale, of_parameters):
     if flash_cuda._load() is None:
+        grads = [t.grad for t in tensors if t.grad is not None] if of_parameters else tensors
+        if not grads:
+            return None
+        if not supports(grads):
+            raise ValueError("gradients must be plain float32, float16 or bfloat16 tensors on one CUDA device")
         raise RuntimeError(f"flash_cuda is unavailable ({flash_cuda.unavailable_reason()})")
-    return flash_cuda._host
-
-
-def _run(grads, out, max_norm, code, scale):
-    if not supports(grads):
-        raise ValueError("gradients must be float32, float16 or bfloat16 tensors on one CUDA device "
-                         f"(at most {MAX_TENSORS} of them)")
-    return _host().clip_grads(grads, out, max_norm, code, scale)
+    return flash_cuda._host.clip_grads(tensors, out, max_norm, code, scale, of_parameters)
 
 
 def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
@@ -51,7 +49,7 @@ def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     grads = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not grads:
         return torch.tensor(0.0)
-    return _run(grads, None, 0.0, code, False)
+    return _run(grads, None, 0.0, code, False, False)
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False, *,
@@ -65,16 +63,16 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     """
     code = _norm_code(norm_type)
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    grads = [p.grad for p in parameters if p.grad is not None]
     out = None if out is None else list(out)
-    if out is not None and len(out) != len(grads):
-        raise ValueError(f"out: {len(out)} tensors for {len(grads)} gradients")
-    if not grads:
-        return torch.tensor(0.0)
     if error_if_nonfinite:
-        norm = _run(grads, None, 0.0, code, False)
-        if not math.isfinite(norm.item()):
+        norm = _run(parameters, None, 0.0, code, False, True)
+        if norm is not None and not math.isfinite(norm.item()):
             raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients from `parameters` is non-finite, "
                                "so it cannot be clipped. To disable this error and scale the gradients by the non-finite "
                                "norm anyway, set `error_if_nonfinite=False`")
-    return _run(grads, out, float(max_norm), code, True)
+    norm = _run(parameters, out, float(max_norm), code, True, True)
+    if norm is None:                                  # no gradients
+        if out:
+            raise ValueError(f"out: {len(out)} tensors for 0 gradients")
+        return torch.tensor(0.0)
+    return norm

@@ -56,8 +56,6 @@ def test_python_call_refuses_what_it_does_not_take():
         grad_clip.clip_grad_norm_([p], 1.0)
     with pytest.raises(ValueError, match="norm_type"):
         grad_clip.clip_grad_norm_([p], 1.0, norm_type=1.0)
-    with pytest.raises(ValueError, match="out"):
-        grad_clip.clip_grad_norm_([p], 1.0, out=[])
 
 
 SHAPES = [(1,), (768,), (8193,), (333, 77), (), (16384,), (5, 7, 11), (100003,), (2,)]
@@ -208,6 +206,12 @@ def test_layouts_and_refusals():
         grad_clip.clip_grad_norm_([p, d], 0.1)
     with pytest.raises(ValueError, match="out"):
         grad_clip.clip_grad_norm_([p], 0.1, out=[torch.zeros(5, 8, device="cuda")])
+    with pytest.raises(ValueError, match="0 tensors for 1"):
+        grad_clip.clip_grad_norm_([p], 0.1, out=[])
+    with pytest.raises(TypeError, match="must be a tensor"):
+        grad_clip.clip_grad_norm_([p, 3.0], 0.1)
+    with pytest.raises(ValueError, match="CUDA"):
+        grad_clip.grad_norm([torch.ones(3)])
     with pytest.raises(ValueError, match="share memory"):
         grad_clip.clip_grad_norm_([p, one], 0.1, out=[torch.zeros(6, 8, device="cuda"), p.grad])
 
