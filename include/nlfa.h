@@ -328,7 +328,7 @@ int nlfa_fwd_cached_positions(const void* q, const void* k_cache, const void* v_
  *
  * The forward fills `tape` (nlfa_linear_ce_tape_bytes: packed rows, logsumexps, 16-bit copies), which the backward reads
  * along with w, unchanged since.  `scratch` is free between the calls.  The backward runs through the vocabulary in pieces whose
- * gradient of the logits fits 512 MiB; it forms dx (x_dtype) and dw (w_dtype), either of which may be NULL.  `grad` is the gradient of
+ * gradient of the logits fits 1 GiB; it forms dx (x_dtype) and dw (w_dtype), either of which may be NULL.  `grad` is the gradient of
  * `loss`: one float, or n of them with NLFA_REDUCE_NONE.  Bit-reproducible; may be captured.  Tape, scratch, dx and dw are 16-byte aligned.  Needs compute
  * capability 10.x. */
 #define NLFA_REDUCE_NONE 0

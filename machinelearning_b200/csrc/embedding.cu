@@ -4,7 +4,7 @@
 // that the same call gives the same bits: the ids are sorted first (sort_ids_kernel: one cluster, a stable radix sort whose
 // digit counts cross between its CTAs through distributed shared memory: no launch per pass and no waiting on flags),
 // then warps add runs of sorted positions (add_rows_kernel).  A token's rows that cross from one run into the next are added from the
-// runs' partial sums afterwards (join_rows_kernel), in order.  Rows of tokens that do not occur are zeroed on the way.
+// runs' partial sums afterwards (join_rows_kernel), in order.  The rows of tokens that do not occur have been zeroed beside the sort.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -17,7 +17,7 @@ namespace embedding {
 namespace {
 
 constexpr int kBlock = 256, kWarps = kBlock / 32;
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kSortThreads = 1024;
 constexpr int kMostDigitBits = 9;
 
 // W bytes of a row: 16, 8, 4 or 2, what its alignment allows
@@ -87,38 +87,54 @@ lookup_kernel(const I* __restrict__ ids, const T* __restrict__ w, T* __restrict_
 // ------------------------------------------------------------------------------------------------ sort
 
 // (id, position) by id, positions in order; ids without a gradient (outside the table, padding) become V and end up last.
-// begin[v], end[v]: where v's positions lie; begin = -1 where there are none.  One cluster: each CTA has a
-// run of the positions, each warp of it a run of that.
+// begin[v], end[v]: where v's positions lie; begin = -1 where there are none.  The first cluster of
+// the grid: each of its CTAs has a run of the positions, each warp of it a run of that.  The other clusters write zeros over dw
+// meanwhile (it is the larger part of the memory traffic where the table is; the sort is all latency).
 template <typename I>
 __global__ void __launch_bounds__(kSortThreads)
-sort_ids_kernel(const I* __restrict__ ids, int n, int V, long long padding, uint32_t* keys, uint32_t* places, int* __restrict__ begin,
-                int* __restrict__ end, int passes, int digit_bits, int ctas) {
+sort_ids_kernel(const I* __restrict__ ids, int n, int V, long long padding, uint2* pairs, int* __restrict__ begin,
+                int* __restrict__ end, int passes, int digit_bits, int ctas, uint8_t* __restrict__ dw, long long dw_bytes) {
   extern __shared__ int smem[];
   constexpr int U = 8;
   const int digits = 1 << digit_bits;
   int* count = smem;                                   // [warp][digit]
-  int* total = smem + kSortWarps * digits;             // [digit], read by the other CTAs
+  int* total = smem + (blockDim.x / 32) * digits;             // [digit], read by the other CTAs
   int* base = total + digits;
   __shared__ int warp_sum[32];
   grid_dep_wait();
   grid_dep_release();
   const int rank = static_cast<int>(cluster_rank()), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int threads = blockDim.x, warps = threads / 32;
+  if (blockIdx.x > 0) {
+    const long long i0 = ((static_cast<long long>(blockIdx.x) - 1) * ctas + rank) * threads + threadIdx.x;
+    const long long step = static_cast<long long>(gridDim.x - 1) * ctas * threads;
+    const int head = static_cast<int>(-reinterpret_cast<uintptr_t>(dw) & 15u);             // to a 16-byte border, in whole elements
+    const long long body = dw_bytes > head ? (dw_bytes - head) / 16 : 0, tail = dw_bytes > head ? head + 16 * body : 0;
+    uint4* words = reinterpret_cast<uint4*>(dw + head);
+#pragma unroll 8
+    for (long long i = i0; i < body; i += step) words[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (long long b = 2 * i0; b < 16 && b < dw_bytes; b += 2 * step) {
+      if (b < head || tail == 0) *reinterpret_cast<uint16_t*>(dw + b) = 0;
+      if (tail + b < dw_bytes) *reinterpret_cast<uint16_t*>(dw + tail + b) = 0;
+    }
+    return;
+  }
   const unsigned below = (1u << lane) - 1u;
-  const int per_round = ctas * kSortThreads;
+  const int per_round = ctas * threads;
   const int run = static_cast<int>((static_cast<long long>(n) + per_round - 1) / per_round) * 32;
-  const long long lo = static_cast<long long>(run) * (rank * kSortWarps + warp);
+  const long long lo = static_cast<long long>(run) * (rank * warps + warp);
   const int from = lo < n ? static_cast<int>(lo) : n, to = n - from < run ? n : from + run;
 
-  for (int v = rank * kSortThreads + threadIdx.x; v < V; v += per_round) begin[v] = -1;
+  for (int v = rank * threads + threadIdx.x; v < V; v += per_round) begin[v] = -1;
 
-  uint32_t *src = keys, *src_at = places, *dst = keys + n, *dst_at = places + n;
+  uint2 *src = pairs, *dst = pairs + n;
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * digit_bits;
     // the keys of U x 32 positions; behind the run: no digit
     auto load_keys = [&](int i0, uint32_t (&k)[U]) {
       if (pass > 0) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) k[u] = i0 + 32 * u + lane < to ? __ldcg(src + i0 + 32 * u + lane) : 0xffffffffu;
+        for (int u = 0; u < U; ++u) k[u] = i0 + 32 * u + lane < to ? __ldcg(&src[i0 + 32 * u + lane].x) : 0xffffffffu;
       } else {
         long long id[U];
 #pragma unroll
@@ -131,7 +147,18 @@ sort_ids_kernel(const I* __restrict__ ids, int n, int V, long long padding, uint
       }
     };
     auto digit_of = [&](uint32_t key) { return key == 0xffffffffu ? key : (key >> shift) & (digits - 1); };
-    for (int i = threadIdx.x; i < kSortWarps * digits; i += kSortThreads) count[i] = 0;
+    // the lanes with this lane's digit, bit by bit (match.any in its place: the whole sort of 131,072 ids ... us, so ... us)
+    auto same_digit = [&](uint32_t d) {
+      const unsigned valid = __ballot_sync(0xffffffffu, d != 0xffffffffu);
+      unsigned same = d != 0xffffffffu ? valid : ~valid;
+      for (int b = 0; b < digit_bits; ++b) {
+        const bool bit = d >> b & 1u;
+        const unsigned set = __ballot_sync(0xffffffffu, bit);
+        same &= bit ? set : ~set;
+      }
+      return same;
+    };
+    for (int i = threadIdx.x; i < warps * digits; i += threads) count[i] = 0;
     __syncthreads();
     int* mine = count + warp * digits;
     for (int i0 = from; i0 < to; i0 += 32 * U) {
@@ -141,82 +168,87 @@ sort_ids_kernel(const I* __restrict__ ids, int n, int V, long long padding, uint
       for (int u = 0; u < U; ++u) {
         if (i0 + 32 * u >= to) break;
         const uint32_t d = digit_of(k[u]);
-        const unsigned same = __match_any_sync(0xffffffffu, d);
+        const unsigned same = same_digit(d);
         if (d != 0xffffffffu && (same & below) == 0) mine[d] += __popc(same);
         __syncwarp();
       }
     }
     __syncthreads();
-    if (threadIdx.x < digits) {
+    for (int d = threadIdx.x; d < digits; d += threads) {
       int sum = 0;
 #pragma unroll 8
-      for (int w = 0; w < kSortWarps; ++w) {
-        const int c = count[w * digits + threadIdx.x];
-        count[w * digits + threadIdx.x] = sum;
+      for (int w = 0; w < warps; ++w) {
+        const int c = count[w * digits + d];
+        count[w * digits + d] = sum;
         sum += c;
       }
-      total[threadIdx.x] = sum;
+      total[d] = sum;
     }
     cluster_arrive();
     cluster_wait();
-    int before = 0, all = 0;
-    if (threadIdx.x < digits) {
+    int carry = 0;                                       // positions of the digits below d0
+    for (int d0 = 0; d0 < digits; d0 += threads) {
+      const int d = d0 + threadIdx.x;
+      int before = 0, all = 0;
+      if (d < digits) {
 #pragma unroll 8
-      for (int r = 0; r < ctas; ++r) {
-        int v;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(smem_u32(total + threadIdx.x), r)) : "memory");
-        if (r < rank) before += v;
-        all += v;
+        for (int r = 0; r < ctas; ++r) {
+          int v;
+          asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(smem_u32(total + d), r)) : "memory");
+          if (r < rank) before += v;
+          all += v;
+        }
       }
-    }
-    int inclusive = all;
+      int inclusive = all;
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, inclusive, off);
-      if (lane >= off) inclusive += o;
+      for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, inclusive, off);
+        if (lane >= off) inclusive += o;
+      }
+      if (lane == 31) warp_sum[warp] = inclusive;
+      __syncthreads();
+      int ahead = 0, sum = 0;
+      for (int w = 0; w < warps; ++w) {
+        const int v = warp_sum[w];
+        if (w < warp) ahead += v;
+        sum += v;
+      }
+      if (d < digits) base[d] = carry + ahead + inclusive - all + before;
+      carry += sum;
+      __syncthreads();
     }
-    if (lane == 31) warp_sum[warp] = inclusive;
-    __syncthreads();
-    if (threadIdx.x < digits) {
-      int ahead = 0;
-      for (int w = 0; w < warp; ++w) ahead += warp_sum[w];
-      base[threadIdx.x] = ahead + inclusive - all + before;
-    }
-    __syncthreads();
     for (int i0 = from; i0 < to; i0 += 32 * U) {
       uint32_t k[U], at[U];
       load_keys(i0, k);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = i0 + 32 * u + lane;
-        at[u] = pass > 0 ? (i < to ? __ldcg(src_at + i) : 0u) : static_cast<uint32_t>(i);
+        at[u] = pass > 0 ? (i < to ? __ldcg(&src[i].y) : 0u) : static_cast<uint32_t>(i);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (i0 + 32 * u >= to) break;
         const uint32_t d = digit_of(k[u]);
-        const unsigned same = __match_any_sync(0xffffffffu, d);
+        const unsigned same = same_digit(d);
         const bool in = d != 0xffffffffu;
         int to_place = 0;
         if (in) to_place = base[d] + mine[d] + __popc(same & below);
         __syncwarp();
         if (in && (same & below) == 0) mine[d] += __popc(same);
         __syncwarp();
-        if (in) {
-          dst[to_place] = k[u];
-          dst_at[to_place] = at[u];
-        }
+        if (in) dst[to_place] = make_uint2(k[u], at[u]);      // (one store: the scattered sectors are what this loop waits for)
       }
     }
     // the next pass reads what the other CTAs wrote, and overwrites what they read
     cluster_arrive();
     cluster_wait();
-    uint32_t* t = src; src = dst; dst = t;
-    t = src_at; src_at = dst_at; dst_at = t;
+    uint2* t = src;
+    src = dst;
+    dst = t;
   }
 #pragma unroll 4
   for (int i = from + lane; i < to; i += 32) {
-    const uint32_t key = __ldcg(src + i), prev = i > 0 ? __ldcg(src + i - 1) : 0xffffffffu, next = i + 1 < n ? __ldcg(src + i + 1) : 0xffffffffu;
+    const uint32_t key = __ldcg(&src[i].x), prev = i > 0 ? __ldcg(&src[i - 1].x) : 0xffffffffu, next = i + 1 < n ? __ldcg(&src[i + 1].x) : 0xffffffffu;
     if (key >= static_cast<uint32_t>(V)) continue;
     if (prev != key) begin[key] = i;
     if (next != key) end[key] = i + 1;
@@ -238,69 +270,53 @@ struct Row {
   }
 };
 
-// Units of one warp: first (run of `run` sorted positions) x (slab of 32 words of a row), then 16 rows of the table each, of which those
-// without a position are zeroed.  partial [runs][2][d]: what a run has of a token that began in an earlier run, and of
-// one that goes on in the next.
+// A warp adds a run of `run` sorted positions, a slab of 32 words of each row.  partial [runs][2][d]: what a run has of a token that
+// began in an earlier run, and of one that goes on in the next.  Where tokens end is found for 32 positions at once, so that a row costs its
+// load and its additions (131,072 rows of 1,024 in bf16 ... us, with the two tokens compared at each row 86).
 template <typename T, int W>
 __global__ void __launch_bounds__(kBlock)
-add_rows_kernel(const T* __restrict__ g, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ places, const int* __restrict__ begin,
-                T* __restrict__ dw, float* __restrict__ partial, int n, int V, int d, int run, int runs, int slabs, float scale) {
+add_rows_kernel(const T* __restrict__ g, const uint2* __restrict__ pairs, T* __restrict__ dw,
+                float* __restrict__ partial, int n, int V, int d, int run, int runs, int slabs, float scale) {
   using R = Row<T, W>;
   constexpr int N = R::N, U = 8;
   grid_dep_wait();
   grid_dep_release();
   const int lane = threadIdx.x & 31;
   const long long unit = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const long long adds = static_cast<long long>(runs) * slabs;
-  if (unit >= adds) {
-    const long long v0 = (unit - adds) * 16;
-    if (v0 >= V) return;
-    const int v = static_cast<int>(v0) + lane;
-    unsigned empty = __ballot_sync(0xffffffffu, lane < 16 && v < V && begin[v < V ? v : 0] < 0);
-    const int words = d / N;
-    typename R::V zero;
-#pragma unroll
-    for (int e = 0; e < N; ++e) zero.e[e] = as_type<T>(0.f);
-    while (empty) {
-      const int r = __ffs(empty) - 1;
-      empty &= empty - 1;
-      auto* row = reinterpret_cast<typename Word<W>::type*>(dw + (static_cast<size_t>(v0) + r) * d);
-      for (int c = lane; c < words; c += 32) row[c] = zero.w;
-    }
-    return;
-  }
+  if (unit >= static_cast<long long>(runs) * slabs) return;
   const int c = static_cast<int>(unit / slabs), slab = static_cast<int>(unit - static_cast<long long>(c) * slabs);
   const int col = (slab * 32 + lane) * N;
   const bool in = col < d;
   const int from = c * run, to = n - from < run ? n : from + run;
-  const uint32_t before = from > 0 ? keys[from - 1] : 0xffffffffu, after = to < n ? keys[to] : 0xffffffffu;
+  const uint32_t before = from > 0 ? pairs[from - 1].x : 0xffffffffu, after = to < n ? pairs[to].x : 0xffffffffu;
+  const T* rows = g + (in ? col : 0);
   float sum[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) sum[e] = 0.f;
   bool first = true;                                       // the token at hand is the run's first
   for (int i0 = from; i0 < to; i0 += 32) {
     const int i = i0 + lane;
-    const uint32_t key = i < to ? keys[i] : 0xffffffffu;
-    const uint32_t place = i < to ? places[i] : 0u;
-    const uint32_t next = i + 1 < to ? keys[i + 1] : i + 1 == to ? after : 0xffffffffu;
+    const uint2 at = i < to ? pairs[i] : make_uint2(0xffffffffu, 0u);
+    const uint32_t key = at.x, place = at.y;
+    const uint32_t next = i + 1 < to ? pairs[i + 1].x : 0xffffffffu;         // (behind the run: another)
     const int live = __popc(__ballot_sync(0xffffffffu, key < static_cast<uint32_t>(V)));   // (those without a gradient stand last)
+    const unsigned ends = __ballot_sync(0xffffffffu, next != key);
     for (int j0 = 0; j0 < live; j0 += U) {
       typename R::V v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const uint32_t p = __shfl_sync(0xffffffffu, place, (j0 + u) & 31);
-        if (j0 + u < live && in) v[u].w = *reinterpret_cast<const typename Word<W>::type*>(g + static_cast<size_t>(p) * d + col);
+        if (j0 + u < live) v[u].w = *reinterpret_cast<const typename Word<W>::type*>(rows + static_cast<size_t>(p) * d);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int j = j0 + u;
-        const uint32_t k = __shfl_sync(0xffffffffu, key, j & 31), k1 = __shfl_sync(0xffffffffu, next, j & 31);
-        if (j >= live) continue;
+        if (j >= live) break;
 #pragma unroll
         for (int e = 0; e < N; ++e) sum[e] += as_float(v[u].e[e]);
-        const bool run_ends = i0 + j + 1 == to;
-        if (k1 == k && !run_ends) continue;
-        const bool came = first && k == before, goes = run_ends && k1 == k;
+        if (!(ends >> j & 1u)) continue;
+        const uint32_t k = __shfl_sync(0xffffffffu, key, j);
+        const bool came = first && k == before, goes = i0 + j + 1 == to && k == after;
         if (in) {
           if (came || goes) {
             float* o = partial + (static_cast<size_t>(2 * c) + (came ? 0 : 1)) * d + col;
@@ -323,7 +339,7 @@ add_rows_kernel(const T* __restrict__ g, const uint32_t* __restrict__ keys, cons
 // shares the CTA's warps take an eighth each.
 template <typename T, int W>
 __global__ void __launch_bounds__(kBlock)
-join_rows_kernel(const uint32_t* __restrict__ keys, const int* __restrict__ begin, const int* __restrict__ end, const float* __restrict__ partial,
+join_rows_kernel(const uint2* __restrict__ pairs, const int* __restrict__ begin, const int* __restrict__ end, const float* __restrict__ partial,
                  T* __restrict__ dw, int n, int V, int d, int run, int runs, float scale) {
   using R = Row<T, W>;
   constexpr int N = R::N, kAlone = 8;
@@ -338,8 +354,8 @@ join_rows_kernel(const uint32_t* __restrict__ keys, const int* __restrict__ begi
   uint32_t key = 0xffffffffu;
   int last = 0;                                            // the last run with a share
   if (c + 1 < runs) {
-    key = keys[(c + 1) * run - 1];
-    if (key >= static_cast<uint32_t>(V) || keys[(c + 1) * run] != key || begin[key] < c * run) key = 0xffffffffu;
+    key = pairs[(c + 1) * run - 1].x;
+    if (key >= static_cast<uint32_t>(V) || pairs[(c + 1) * run].x != key || begin[key] < c * run) key = 0xffffffffu;
     else last = (end[key] - 1) / run;
   }
   auto share = [&](int r, int which, float (&s)[N]) {
@@ -419,13 +435,12 @@ int run_length(int n, int d) {
 }
 
 struct Scratch {
-  size_t keys, places, begin, end, partial, bytes;
+  size_t pairs, begin, end, partial, bytes;
 };
 Scratch scratch_layout(int n, int V, int d) {
   Scratch s{};
   size_t at = 0;
-  s.keys = at; at = up(at + static_cast<size_t>(n) * 8);
-  s.places = at; at = up(at + static_cast<size_t>(n) * 8);
+  s.pairs = at; at = up(at + static_cast<size_t>(n) * 16);         // two of (id, position), from one pass to the next
   s.begin = at; at = up(at + static_cast<size_t>(V) * 4);
   s.end = at; at = up(at + static_cast<size_t>(V) * 4);
   s.partial = at; at = up(at + (static_cast<size_t>(n) / run_length(n, d) + 1) * 2 * d * 4);
@@ -446,18 +461,18 @@ int lookup(const void* ids, const void* w, void* out, int n, int V, int d, float
 template <typename T, int W>
 int gradient(const void* g, const Scratch& s, uint8_t* scratch, int sorted, void* dw, int n, int V, int d, float scale, cudaStream_t st) {
   const int slabs = (d / Vec<T, W>::N + 31) / 32, run = run_length(n, d), runs = (n + run - 1) / run;
-  const uint32_t* keys = reinterpret_cast<const uint32_t*>(scratch + s.keys) + static_cast<size_t>(sorted) * n;
-  const uint32_t* places = reinterpret_cast<const uint32_t*>(scratch + s.places) + static_cast<size_t>(sorted) * n;
+  const uint2* pairs = reinterpret_cast<const uint2*>(scratch + s.pairs) + static_cast<size_t>(sorted) * n;
   const int *begin = reinterpret_cast<const int*>(scratch + s.begin), *end = reinterpret_cast<const int*>(scratch + s.end);
   float* partial = reinterpret_cast<float*>(scratch + s.partial);
   const bool overlap = overlap_launches(kOverlapRowwise);
-  const long long units = static_cast<long long>(runs) * slabs + (V + 15) / 16, ctas = (units + kWarps - 1) / kWarps;
+  const long long units = static_cast<long long>(runs) * slabs, ctas = (units + kWarps - 1) / kWarps;
   if (ctas > 0x7fffffffll || slabs > 65535) return NLFA_ERR_BAD_SHAPE;
+  if (n == 0) return NLFA_OK;                              // (the zeros are written)
   int rc = checked(launch_kernel(add_rows_kernel<T, W>, dim3(static_cast<unsigned>(ctas)), dim3(kBlock), 0, st, overlap, static_cast<const T*>(g),
-                                 keys, places, begin, static_cast<T*>(dw), partial, n, V, d, run, runs, slabs, scale));
+                                 pairs, static_cast<T*>(dw), partial, n, V, d, run, runs, slabs, scale));
   if (rc != NLFA_OK || runs < 2) return rc;
   return checked(launch_kernel(join_rows_kernel<T, W>, dim3(static_cast<unsigned>((runs + kWarps - 1) / kWarps), static_cast<unsigned>(slabs)),
-                               dim3(kBlock), 0, st, overlap, keys, begin, end, partial, static_cast<T*>(dw), n, V, d, run, runs, scale));
+                               dim3(kBlock), 0, st, overlap, pairs, begin, end, partial, static_cast<T*>(dw), n, V, d, run, runs, scale));
 }
 
 }  // namespace
@@ -508,14 +523,19 @@ int nlfa_embedding_bwd(const void* g, int dtype, const void* ids, int id_bytes, 
   int bits = 1;
   while (bits < 31 && (static_cast<unsigned>(V) >> bits) != 0) ++bits;
   const int passes = (bits + kMostDigitBits - 1) / kMostDigitBits, digit_bits = (bits + passes - 1) / passes;
-  const size_t smem = static_cast<size_t>(kSortWarps + 2) * (1u << digit_bits) * sizeof(int);
+  // few positions: fewer warps, whose counts are added one after the other
+  const int threads = n <= 32768 ? 256 : kSortThreads;
+  const size_t smem = static_cast<size_t>(threads / 32 + 2) * (1u << digit_bits) * sizeof(int);
   auto sort = [&](auto* typed, auto* kernel) {
-    const int r = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), (kSortWarps + 2) * (1 << kMostDigitBits) * static_cast<int>(sizeof(int)));
+    const int r = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), (kSortThreads / 32 + 2) * (1 << kMostDigitBits) * static_cast<int>(sizeof(int)));
     if (r != NLFA_OK) return r;
-    const int ctas = resident_clusters(reinterpret_cast<const void*>(kernel), kSortThreads, static_cast<int>(smem), 16) > 0 ? 16 : 8;
-    return checked(launch_cluster(kernel, dim3(1, static_cast<unsigned>(ctas)), dim3(kSortThreads), smem, st, overlap_launches(kOverlapRowwise), ctas,
-                                  typed, n, V, padding_idx, reinterpret_cast<uint32_t*>(at + s.keys), reinterpret_cast<uint32_t*>(at + s.places),
-                                  reinterpret_cast<int*>(at + s.begin), reinterpret_cast<int*>(at + s.end), passes, digit_bits, ctas));
+    const int ctas = resident_clusters(reinterpret_cast<const void*>(kernel), kSortThreads, (kSortThreads / 32 + 2) * (1 << kMostDigitBits) * 4, 16) > 0 ? 16 : 8;
+    const long long dw_bytes = static_cast<long long>(V) * d * bytes, each = 16ll * threads * ctas * 8;   // (eight words a thread)
+    const long long most = 8 * (kSortThreads / threads), want = dw_bytes / each;
+    const int clusters = static_cast<int>(want < 1 ? 1 : want > most ? most : want);
+    return checked(launch_cluster(kernel, dim3(static_cast<unsigned>(1 + clusters), static_cast<unsigned>(ctas)), dim3(static_cast<unsigned>(threads)), smem, st, overlap_launches(kOverlapRowwise), ctas,
+                                  typed, n, V, padding_idx, reinterpret_cast<uint2*>(at + s.pairs),
+                                  reinterpret_cast<int*>(at + s.begin), reinterpret_cast<int*>(at + s.end), passes, digit_bits, ctas, static_cast<uint8_t*>(dw), dw_bytes));
   };
   rc = id_bytes == 8 ? sort(static_cast<const long long*>(ids), sort_ids_kernel<long long>) : sort(static_cast<const int*>(ids), sort_ids_kernel<int>);
   if (rc != NLFA_OK) return rc;
