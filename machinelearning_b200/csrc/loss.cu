@@ -259,14 +259,13 @@ largest_kernel(const Head* head, const float* __restrict__ grad, const int* __re
   *largest = top > 0.f ? top : 1.f;
 }
 
-// In how many parts the sums of `rest` tiles of k blocks are formed, by one warp: the fewest blocks for the busiest pair of CTAs, with
-// kShare more for every share written and added.
-__device__ int choose_parts(int rest, int k, int pairs) {
-  constexpr int kShare = 4;
+// In how many parts the sums of `rest` tiles of k blocks are formed, by one warp: the fewest stages for the busiest pair of CTAs, with
+// `share` more for every share written and added.
+__device__ int choose_parts(int rest, int k, int pairs, int share) {
   const int lane = threadIdx.x & 31, most = rest > 0 ? kPartsPerPair * pairs / rest : 1;
   long long best = LLONG_MAX;
   for (int s = 1 + lane; s <= most && s <= k; s += 32) {
-    const long long units = (rest * s + pairs - 1) / pairs, cost = units * ((k + s - 1) / s + (s > 1 ? kShare : 0)) + (s > 1 ? s : 0);
+    const long long units = (rest * s + pairs - 1) / pairs, cost = units * ((k + s - 1) / s + (s > 1 ? share : 0)) + (s > 1 ? s : 0);
     if (cost < best >> 8) best = cost << 8 | s;
   }
 #pragma unroll
@@ -282,7 +281,7 @@ __global__ void __launch_bounds__(kBlock)
 scale_rows_kernel(const Head* head, const float* __restrict__ grad, int per_row, int mean, const int* __restrict__ row_of,
                   const int* __restrict__ target, float* __restrict__ row_scale, float* __restrict__ alpha, Parts* parts, const float* __restrict__ largest,
                   float unit, const I* __restrict__ targets, int n, long long ignore, uint8_t* __restrict__ dx, long long row_bytes, int V,
-                  int d, int piece, int want_dw, int pairs) {
+                  int d, int piece, int want_dw, int pairs, int planes) {
   grid_dep_wait();
   grid_dep_release();
   const int all = head->count, stride = gridDim.x * kBlock;
@@ -301,11 +300,12 @@ scale_rows_kernel(const Head* head, const float* __restrict__ grad, int per_row,
     *alpha = all > 0 ? g / unit : 0.f;                    // (no target: gradients of zero, not 0 / 0)
   }
   if (blockIdx.x == gridDim.x - 1 && threadIdx.x < 32) {
+    const int k = summands(planes), share = planes == 3 ? 1 : 4;          // (a stage of three parts is three times as long)
     const int d_tiles = (d + kColTile - 1) / kColTile, rest_x = dx != nullptr ? end / kRowTile * d_tiles % pairs : 0;
     for (int last = 0; last < 2; ++last) {
       const int cols = last ? V - (V - 1) / piece * piece : piece;
       const int rest_w = want_dw ? (cols + kColTile - 1) / kColTile * d_tiles % pairs : 0;
-      const int parts_w = choose_parts(rest_w, end / kK, pairs), parts_x = choose_parts(rest_x, (cols + kK - 1) / kK, pairs);
+      const int parts_w = choose_parts(rest_w, end / k, pairs, share), parts_x = choose_parts(rest_x, (cols + k - 1) / k, pairs, share);
       if (threadIdx.x == 0) {
         parts->dw[last] = parts_w;
         parts->dx[last] = parts_x;
@@ -395,12 +395,21 @@ BwdLayout bwd_layout(const Call& c, const Layout& l) {
 }
 
 // [planes][rows][cols], cols a multiple of 64, as (64 columns, rows, blocks of 64 columns, planes)
-int box_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes, int box_rows, int box_blocks) {
+int box_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes, int box_rows, int box_blocks,
+            int box_planes) {
   const unsigned long long pitch = static_cast<unsigned long long>(cols) * 2, r = static_cast<unsigned long long>(rows);
   const unsigned long long dims[4] = {64ull, r, pitch / 128, static_cast<unsigned long long>(planes)};
   const unsigned long long strides[3] = {pitch, 128ull, pitch * r};
-  const unsigned box[4] = {64u, static_cast<unsigned>(box_rows), static_cast<unsigned>(box_blocks), 1u};
+  const unsigned box[4] = {64u, static_cast<unsigned>(box_rows), static_cast<unsigned>(box_blocks), static_cast<unsigned>(box_planes)};
   return make_map(map, base, dtype, dims, strides, box);
+}
+// One CTA's half of an operand, a stage of it, in all its parts: 128 rows, the summands along the columns ...
+int column_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes) {
+  return box_map(map, base, dtype, cols, rows, planes, 128, summands(planes) / 64, planes);
+}
+// ... or 128 columns, the summands along the rows.
+int row_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes) {
+  return box_map(map, base, dtype, cols, rows, planes, summands(planes), 2, planes);
 }
 
 int checked(cudaError_t e) {
@@ -446,7 +455,6 @@ Params params(const Call& c, const Layout& l, const Pointers& t, unsigned* statu
   p.d = c.d;
   p.d_pad = l.d_pad;
   p.planes = l.x_planes;
-  p.pairs = l.x_planes == 3 ? 6 : 1;
   p.n_rows = l.n_rows;
   p.target = t.target();
   p.lse = t.lse();
@@ -481,11 +489,11 @@ int run_fwd(const Call& c, const void* x, const void* w, const void* targets, in
   rc = copy_rows(x, c.x_dtype, tape + l.x, dtype, t.head(), t.row_of(), c.n, l.n_rows, c.d, l.d_pad, l.x_planes, st);
   if (rc != NLFA_OK) return rc;
   CUtensorMap mx, mw;
-  rc = box_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes, 128, kK / 64);
-  if (rc == NLFA_OK) rc = box_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes, 128, kK / 64);
+  rc = column_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes);
+  if (rc == NLFA_OK) rc = column_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes);
   if (rc != NLFA_OK) return rc;
   Params p = params(c, l, t, status);
-  if (l.x_planes == 3 || c.d > 1024) p.chunk = l.x_planes == 3 ? 2 : 8;
+  p.chunk = l.x_planes == 3 ? 1 : c.d > 1024 ? 8 : 0;
   p.partial = reinterpret_cast<float2*>(scratch + l.partial);
   p.at_target = at_target;
   rc = launch_product(kLse, dtype, p, mx, mw, mx, mx, st);
@@ -528,19 +536,23 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
     return checked(launch_kernel(kernel, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(kBlock), 0, st, overlap, t.head(), grad,
                                  per_row, reduction == NLFA_REDUCE_MEAN ? 1 : 0, t.row_of(), t.target(), row_scale, alpha, parts, largest,
                                  dtype == NLFA_DTYPE_F16 ? 16384.f : 1.f, typed, c.n, ignore, static_cast<uint8_t*>(dx), row_bytes, c.V, c.d, b.piece, dw != nullptr ? 1 : 0,
-                                 most_pairs()));
+                                 most_pairs(), l.x_planes));
   };
   rc = target_bytes == 8 ? scale(static_cast<const long long*>(targets), scale_rows_kernel<long long>)
                          : scale(static_cast<const int*>(targets), scale_rows_kernel<int>);
   if (rc != NLFA_OK) return rc;
-  CUtensorMap mx, mw, mds, mout;
-  rc = box_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes, 128, kK / 64);
-  if (rc == NLFA_OK) rc = box_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes, 128, kK / 64);
-  if (rc == NLFA_OK) rc = box_map(&mds, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes, 128, kK / 64);
-  if (rc == NLFA_OK) rc = box_map(&mout, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes, 32, 1);
+  CUtensorMap x_columns, w_columns, out, x_rows, w_rows, dl_columns, dl_rows;
+  const void* wp = l.copy_w ? tape + l.w : w;
+  rc = column_map(&x_columns, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes);
+  if (rc == NLFA_OK) rc = column_map(&w_columns, wp, dtype, l.d_pad, c.V, l.x_planes);
+  if (rc == NLFA_OK) rc = row_map(&x_rows, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes);
+  if (rc == NLFA_OK) rc = row_map(&w_rows, wp, dtype, l.d_pad, c.V, l.x_planes);
+  if (rc == NLFA_OK) rc = column_map(&dl_columns, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes);
+  if (rc == NLFA_OK) rc = row_map(&dl_rows, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes);
+  if (rc == NLFA_OK) rc = box_map(&out, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes, 32, 1, 1);
   if (rc != NLFA_OK) return rc;
   Params p = params(c, l, t, status);
-  p.chunk = l.x_planes == 3 ? 2 : 0;
+  p.chunk = l.x_planes == 3 ? 1 : 0;
   p.row_scale = row_scale;
   p.alpha = alpha;
   p.parts = parts;
@@ -557,8 +569,8 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
     p.v1 = c.V - v < b.piece ? c.V : v + b.piece;
     p.first = v == 0;
     p.last = p.v1 == c.V;
-    rc = launch_product(kGrad, dtype, p, mx, mw, mds, mout, st);
-    if (rc == NLFA_OK) rc = launch_product(kProducts, dtype, p, mx, mw, mds, mout, st);
+    rc = launch_product(kGrad, dtype, p, x_columns, w_columns, out, out, st);
+    if (rc == NLFA_OK) rc = launch_product(kProducts, dtype, p, x_rows, w_rows, dl_columns, dl_rows, st);
     if (rc != NLFA_OK) return rc;
   }
   return NLFA_OK;

@@ -8,7 +8,8 @@ namespace loss {
 
 constexpr int kRowTile = 256;       // rows of a product's tile: two CTAs of 128
 constexpr int kColTile = 256;       // columns of a tile
-constexpr int kK = 128;             // summands per stage
+// Summands per stage of a product's pipeline: 128, or 64 of operands in three parts.
+__host__ __device__ constexpr int summands(int planes) { return planes == 3 ? 64 : 128; }
 constexpr int kPartsPerPair = 2;    // shares of dW's, and of dx's, odd tiles there is room for, per pair of CTAs
 
 // The forward leaves its tape in one buffer; counts and places, known on the device only, stand first.
@@ -37,8 +38,8 @@ struct Layout {
 struct Params {
   const Head* head;
   int V, d, d_pad;
-  int planes, pairs;                // pairs of parts whose products are added: 1 or 6
-  int chunk;                        // blocks of kK summands per chain of the tensor core (0: the whole sum)
+  int planes;                       // parts of an operand: 1 or 3
+  int chunk;                        // stages per chain of the tensor core (0: the whole sum)
   int v0, v1;                       // piece of the vocabulary
   int n_rows;
   // forward: (max, sum) of every part of a row, logit of the target
@@ -64,6 +65,8 @@ struct Params {
 int most_pairs();                   // of CTAs that run at once
 size_t share_bytes();
 enum { kLse = 0, kGrad = 1, kProducts = 2 };
+// Maps: kLse and kGrad: x and w as operands along the columns, kGrad: ds_out to store dl; kProducts: x and w as operands along the rows,
+// dl along the columns (ds) and along the rows (ds_out).
 int launch_product(int mode, int dtype, const Params& p, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& ds,
                    const CUtensorMap& ds_out, cudaStream_t stream);
 

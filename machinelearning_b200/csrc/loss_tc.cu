@@ -27,20 +27,29 @@ namespace {
 
 constexpr int kThreads = 320;
 constexpr int kEpilogueWarps = 8;
-constexpr int kStages = 3;
 constexpr int kBlockBytes = 128 * 128;                        // 128 rows of 64 columns
-constexpr int kOperandBytes = 128 * kK * 2;                   // one CTA's half of an operand
-constexpr int kStageBytes = 2 * kOperandBytes;
+// PARTS = 1: three stages of 128 summands.  PARTS = 3 (float32 operands, sums of three bf16 parts): two stages of 64 summands in all
+// parts, each of which is multiplied with two or three of the other operand's: a pair of parts a stage loads everything twice.
+template <int PARTS>
+struct Ring {
+  static constexpr int kStages = PARTS == 3 ? 2 : 3;
+  static constexpr int kSummands = summands(PARTS);
+  static constexpr int kBlocks = PARTS == 3 ? 3 : kSummands / 64;
+  static constexpr int kOperandBytes = kBlocks * kBlockBytes;   // one CTA's half of an operand
+  static constexpr int kStageBytes = 2 * kOperandBytes;
+};
+constexpr int kMostStages = 3;
 constexpr int kStagingBytes = 4096;                           // per epilogue warp
-constexpr int kStaging = kStages * kStageBytes;
+constexpr int kStaging = 12 * kBlockBytes;
+static_assert(Ring<1>::kStages * Ring<1>::kStageBytes <= kStaging && Ring<3>::kStages * Ring<3>::kStageBytes <= kStaging, "stages");
 constexpr int kBars = kStaging + kEpilogueWarps * kStagingBytes;
-constexpr int kNumBars = 2 * kStages + 4;
+constexpr int kNumBars = 2 * kMostStages + 4;
 constexpr int kTmemSlot = kBars + 8 * kNumBars;
 constexpr int kAbort = kTmemSlot + 4;
 constexpr int kSmem = kAbort + 4 + 1024;
 static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
 
-enum { FULL = 0, EMPTY = kStages, ACC_FULL = 2 * kStages, ACC_EMPTY = ACC_FULL + 2 };
+enum { FULL = 0, EMPTY = kMostStages, ACC_FULL = 2 * kMostStages, ACC_EMPTY = ACC_FULL + 2 };
 
 // float32 operands are sums of three bf16 parts; the products of parts, smallest first (what is left out is below 2^-24)
 __device__ __forceinline__ int part_a(int pair) { return (0x001012 >> (4 * pair)) & 15; }   // 2 1 0 1 0 0
@@ -51,7 +60,7 @@ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; 
 // A tile: where it lies in A's rows and B's columns, how many stages its sum takes, which operands it has.
 struct Tile {
   int m0, n0;
-  int k0, k1;                       // its blocks of kK summands (per pair of parts): all, or of a shared tile this pair's
+  int k0, k1;                       // its blocks of summands (a stage each): all, or of a shared tile this pair's
   int dw;                           // kProducts: a tile of dW (else of dx)
   int first, last;                  // kLse: first / last tile of a unit
   int slot;                         // kLse: which part of the vocabulary; kProducts: where a share of a tile goes (-1: the tile is whole)
@@ -71,8 +80,8 @@ struct Plan {
     const int row_tiles = rows > 0 ? ceil_div(rows, kRowTile) : 1;
     d_tiles = ceil_div(p.d, kColTile);
     const int dw_tiles = p.want_dw ? ceil_div(p.v1 - p.v0, kColTile) * d_tiles : 0, dx_tiles = p.want_dx ? row_tiles * d_tiles : 0;
-    kw = row_tiles * (kRowTile / kK);
-    kx = ceil_div(p.v1 - p.v0, kK);
+    kw = row_tiles * (kRowTile / summands(p.planes));
+    kx = ceil_div(p.v1 - p.v0, summands(p.planes));
     dw_whole = dw_tiles / pairs * pairs;
     dx_whole = dx_tiles / pairs * pairs;
     dw_rest = dw_tiles - dw_whole;
@@ -141,7 +150,7 @@ struct Walk {
 
   __device__ bool next(Tile& t) {
     t.k0 = 0;
-    if (MODE != kProducts) t.k1 = ceil_div(p.d, kK);
+    if (MODE != kProducts) t.k1 = ceil_div(p.d, summands(p.planes));
     if (MODE == kLse) {
       t.first = 0;
       if (n == n_end) {
@@ -286,11 +295,13 @@ struct Sums {
   }
 };
 
-template <typename T, int MODE, bool LONG>
+template <typename T, int MODE, bool LONG, int PARTS>
 __global__ void __launch_bounds__(kThreads, 1)
 loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
             const __grid_constant__ CUtensorMap tm_ds, const __grid_constant__ CUtensorMap tm_out, const Params p) {
   constexpr bool kBf16 = Pack2<T>::kIsBf16;
+  using R = Ring<PARTS>;
+  constexpr int kStages = R::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -339,28 +350,25 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
       int it = 0;
       bool ok = true;
       const uint32_t full0 = cluster_addr(bar(FULL), 0);       // loads of both CTAs are counted on the even one's
+      auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t full, int row, int col) {
+        tma_load_4d_pair(dst, map, full, 0, row, col / 64, 0);
+      };
       while (ok && walk.next(t)) {
-        const CUtensorMap* ma = MODE == kProducts ? &tm_ds : &tm_x;
+        const CUtensorMap* ma = MODE != kProducts ? &tm_x : t.dw ? &tm_out : &tm_ds;
         const CUtensorMap* mb = MODE == kProducts && t.dw ? &tm_x : &tm_w;
         const int a0 = t.m0 + 128 * rank, b0 = t.n0 + 128 * rank;
-        const int chunk = LONG ? p.chunk : t.k1 - t.k0;
-        for (int k0 = t.k0; ok && k0 < t.k1; k0 += chunk)
-          for (int pr = 0; ok && pr < p.pairs; ++pr) {
-            const int pa = p.pairs == 1 ? 0 : part_a(pr), pb = p.pairs == 1 ? 0 : part_b(pr);
-            const int k1 = t.k1 - k0 < chunk ? t.k1 : k0 + chunk;
-            for (int kb = k0; kb < k1; ++kb, ++it) {
-              const int s = it % kStages;
-              if (!(ok = mbar_wait(bar(EMPTY + s), ((it / kStages) & 1) ^ 1, wctx, 90))) break;
-              const uint32_t st = base + s * kStageBytes, full = full0 + 8u * s;
-              if (rank == 0) mbar_arrive_expect_tx(bar(FULL + s), 2 * kStageBytes);
-              // boxes at (row, block of 64 columns): the sum runs along the columns, or (MN-major) along the rows
-              const int blk = kb * (kK / 64), a_blk = a0 / 64, b_blk = b0 / 64;
-              if (MODE == kProducts && t.dw) tma_load_4d_pair(st, ma, full, 0, kb * kK, a_blk, pa);
-              else tma_load_4d_pair(st, ma, full, 0, a0, blk, pa);
-              if (MODE != kProducts) tma_load_4d_pair(st + kOperandBytes, mb, full, 0, b0, blk, pb);
-              else tma_load_4d_pair(st + kOperandBytes, mb, full, 0, (t.dw ? 0 : p.v0) + kb * kK, b_blk, pb);
-            }
-          }
+        for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
+          const int s = it % kStages;
+          if (!(ok = mbar_wait(bar(EMPTY + s), ((it / kStages) & 1) ^ 1, wctx, 90))) break;
+          const uint32_t st = base + s * R::kStageBytes, full = full0 + 8u * s;
+          if (rank == 0) mbar_arrive_expect_tx(bar(FULL + s), 2 * R::kStageBytes);
+          // boxes at (row, block of 64 columns): the sum runs along the columns, or (MN-major) along the rows
+          const int k = kb * R::kSummands;
+          if (MODE == kProducts && t.dw) load(st, ma, full, k, a0);
+          else load(st, ma, full, a0, k);
+          if (MODE != kProducts) load(st + R::kOperandBytes, mb, full, b0, k);
+          else load(st + R::kOperandBytes, mb, full, (t.dw ? 0 : p.v0) + k, b0);
+        }
       }
       // the last loads of this CTA have been consumed before it may leave (after a give-up: have had time to land)
       for (int i = 0; ok && i < kStages; ++i, ++it) ok = mbar_wait(bar(EMPTY + it % kStages), ((it / kStages) & 1) ^ 1, wctx, 91);
@@ -377,24 +385,30 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
       while (ok && walk.next(t)) {
         const bool a_mn = MODE == kProducts && t.dw, b_mn = MODE == kProducts;
         const uint32_t idesc = a_mn ? make_idesc(kBf16, 256, kColTile, true, b_mn) : make_idesc(kBf16, 256, kColTile, false, b_mn);
-        // 16 summands on: 32 bytes along a row, four times per block of 64 columns, or 16 rows
-        const uint32_t a_lbo = a_mn ? kBlockBytes : 16u, b_lbo = b_mn ? kBlockBytes : 16u;
+        // 16 summands on: 32 bytes along a row, then the next block of 64 columns; or (MN-major) 16 rows
+        constexpr uint32_t kMnBlock = PARTS == 3 ? kBlockBytes / 2 : kBlockBytes;     // (of 64 summands: 64 rows)
+        const uint32_t a_lbo = a_mn ? kMnBlock : 16u, b_lbo = b_mn ? kMnBlock : 16u;
         const int chunk = LONG ? p.chunk : t.k1 - t.k0;
         for (int k0 = t.k0; ok && k0 < t.k1; k0 += chunk, ++sums) {
           const int buf = sums & 1;
           if (!(ok = mbar_wait(bar(ACC_EMPTY + buf), ((sums >> 1) & 1) ^ 1, wctx, 92))) break;
           tc_fence_after();
-          const int blocks = p.pairs * (t.k1 - k0 < chunk ? t.k1 - k0 : chunk);
-          for (int kb = 0; kb < blocks; ++kb, ++it) {
+          const int stages = t.k1 - k0 < chunk ? t.k1 - k0 : chunk;
+          for (int kb = 0; kb < stages; ++kb, ++it) {
             const int s = it % kStages;
             if (!(ok = mbar_wait(bar(FULL + s), (it / kStages) & 1, wctx, 93))) break;
             tc_fence_after();
-            const uint32_t a = base + s * kStageBytes, b = a + kOperandBytes;
+            const uint32_t a = base + s * R::kStageBytes, b = a + R::kOperandBytes;
 #pragma unroll
-            for (int kk = 0; kk < kK / 16; ++kk) {
-              const uint32_t along_rows = (kk / 4) * kBlockBytes + (kk % 4) * 32u, along_k = kk * 2048u;
-              umma_ss_pair(leader, tmem + buf * kColTile, make_smem_desc(a + (a_mn ? along_k : along_rows), a_lbo, 1024),
-                           make_smem_desc(b + (b_mn ? along_k : along_rows), b_lbo, 1024), idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+            for (int pr = 0; pr < (PARTS == 3 ? 6 : 1); ++pr) {
+              const uint32_t a_part = PARTS == 3 ? part_a(pr) * kBlockBytes : 0u, b_part = PARTS == 3 ? part_b(pr) * kBlockBytes : 0u;
+#pragma unroll
+              for (int kk = 0; kk < R::kSummands / 16; ++kk) {
+                const uint32_t along_rows = (kk / 4) * kBlockBytes + (kk % 4) * 32u, along_k = kk * 2048u;
+                umma_ss_pair(leader, tmem + buf * kColTile, make_smem_desc(a + a_part + (a_mn ? along_k : along_rows), a_lbo, 1024),
+                             make_smem_desc(b + b_part + (b_mn ? along_k : along_rows), b_lbo, 1024), idesc,
+                             (kb > 0 || pr > 0 || kk > 0) ? 1u : 0u);
+              }
             }
             umma_commit_pair(leader, bar(EMPTY + s));
           }
@@ -595,10 +609,10 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
-template <typename T, int MODE, bool LONG>
+template <typename T, int MODE, bool LONG, int PARTS = 1>
 int launch_one(const Params& p, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& ds, const CUtensorMap& out,
                cudaStream_t stream) {
-  auto* kernel = loss_kernel<T, MODE, LONG>;
+  auto* kernel = loss_kernel<T, MODE, LONG, PARTS>;
   const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), kSmem);
   if (rc != NLFA_OK) return rc;
   const int pairs = most_pairs();
@@ -631,16 +645,16 @@ size_t share_bytes() { return static_cast<size_t>(2 * kPartsPerPair * most_pairs
 
 int launch_product(int mode, int dtype, const Params& p, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& ds,
                    const CUtensorMap& ds_out, cudaStream_t stream) {
-  const bool bf16 = dtype == NLFA_DTYPE_BF16, is_long = p.chunk > 0;
-#define NLFA_GO(T, MODE, LONG) launch_one<T, MODE, LONG>(p, x, w, ds, ds_out, stream)
-  if (mode == kLse) {
-    if (is_long) return bf16 ? NLFA_GO(__nv_bfloat16, kLse, true) : NLFA_GO(__half, kLse, true);
-    return bf16 ? NLFA_GO(__nv_bfloat16, kLse, false) : NLFA_GO(__half, kLse, false);
-  }
-  // (the gradients' sums are chunked for float32 operands alone, which are bf16 parts)
-  if (mode == kGrad)
-    return is_long ? NLFA_GO(__nv_bfloat16, kGrad, true) : bf16 ? NLFA_GO(__nv_bfloat16, kGrad, false) : NLFA_GO(__half, kGrad, false);
-  return is_long ? NLFA_GO(__nv_bfloat16, kProducts, true) : bf16 ? NLFA_GO(__nv_bfloat16, kProducts, false) : NLFA_GO(__half, kProducts, false);
+  const bool bf16 = dtype == NLFA_DTYPE_BF16;
+#define NLFA_GO(...) launch_one<__VA_ARGS__>(p, x, w, ds, ds_out, stream)
+  if (p.planes == 3)                                          // float32 operands: parts in bf16
+    return mode == kLse ? NLFA_GO(__nv_bfloat16, kLse, true, 3)
+           : mode == kGrad ? NLFA_GO(__nv_bfloat16, kGrad, true, 3)
+                           : NLFA_GO(__nv_bfloat16, kProducts, true, 3);
+  if (mode == kLse && p.chunk > 0) return bf16 ? NLFA_GO(__nv_bfloat16, kLse, true) : NLFA_GO(__half, kLse, true);
+  if (mode == kLse) return bf16 ? NLFA_GO(__nv_bfloat16, kLse, false) : NLFA_GO(__half, kLse, false);
+  if (mode == kGrad) return bf16 ? NLFA_GO(__nv_bfloat16, kGrad, false) : NLFA_GO(__half, kGrad, false);
+  return bf16 ? NLFA_GO(__nv_bfloat16, kProducts, false) : NLFA_GO(__half, kProducts, false);
 #undef NLFA_GO
 }
 

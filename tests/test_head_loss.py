@@ -163,9 +163,9 @@ def test_gradients_against_differences():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,n,V,d", [("bf16", 16500, 17000, 64), ("fp32", 9000, 10500, 40)])
+@pytest.mark.parametrize("dtype,n,V,d", [("bf16", 24100, 25000, 64), ("fp32", 14000, 14500, 40)])
 def test_vocabulary_in_pieces(dtype, n, V, d):
-    """Sizes whose gradient of the logits does not fit the workspace: dx is summed over the pieces."""
+    """Sizes whose gradient of the logits does not fit the workspace (1 GiB): dx is summed over the pieces."""
     from machinelearning_b200 import _lib, head_loss
     lib = _lib.load()
     code = {"bf16": 2, "fp32": 0}[dtype]
