@@ -10,6 +10,7 @@
 // cannot read as they are (float32: sums of three bf16 parts, exact to 2^-24); the sum of the losses.
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "loss.cuh"
 #include "rowwise.cuh"
@@ -27,6 +28,56 @@ using rowwise::last_cta;
 
 constexpr int kScanCtas = 8, kScanThreads = 1024;
 constexpr int kBlock = 256;
+
+// ------------------------------------------------------------------------------------------------ 16-bit operands
+
+template <typename T> __device__ __forceinline__ float load1(const T* p) { return static_cast<float>(*p); }
+
+// Eight columns (from c) of row `from` of src [*, d] (-1: zeros) to row r of dst [planes][n_rows][d_pad]; planes = 3: dst = a + b + c,
+// each the nearest bf16 value to what is left.
+template <typename S, typename T>
+__device__ __forceinline__ void copy_chunk(const S* __restrict__ src, T* __restrict__ dst, int from, int r, int c, int n_rows, int d, int d_pad,
+                                           int planes, int vec) {
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  if (from >= 0 && c < d) {
+    const S* s = src + static_cast<size_t>(from) * d + c;
+    if (vec) rowwise::Elem<S>::load(s, v);
+    else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < d) v[j] = load1(s + j);
+    }
+  }
+  T* o = dst + static_cast<size_t>(r) * d_pad + c;
+  for (int part = 0; part < planes; ++part) {
+    rowwise::Elem<T>::store(o, v);
+    o += static_cast<size_t>(n_rows) * d_pad;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] -= rowwise::Elem<T>::round(v[j]);
+  }
+}
+
+// Rows from row_of (or r itself), zeros behind the last one up to a whole tile and behind column d.
+template <typename S, typename T>
+__global__ void __launch_bounds__(kBlock)
+copy_rows_kernel(const S* __restrict__ src, T* __restrict__ dst, const Head* head, const int* __restrict__ row_of, int n_src,
+                 int n_rows, int d, int d_pad, int planes, int vec) {
+  grid_dep_wait();
+  grid_dep_release();
+  int end = n_src;
+  if (row_of != nullptr) {
+    const int all = head->count;
+    end = all < kRowTile ? kRowTile : (all + kRowTile - 1) / kRowTile * kRowTile;
+  }
+  const int chunks = d_pad / 8;
+  const long long total = static_cast<long long>(end) * chunks;
+  for (long long i = static_cast<long long>(blockIdx.x) * kBlock + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * kBlock) {
+    const int r = static_cast<int>(i / chunks), c = 8 * static_cast<int>(i - static_cast<long long>(r) * chunks);
+    copy_chunk(src, dst, row_of != nullptr ? row_of[r] : r, r, c, n_rows, d, d_pad, planes, vec);
+  }
+}
 
 // ------------------------------------------------------------------------------------------------ rows with a target
 
@@ -130,47 +181,55 @@ pack_rows_kernel(const I* __restrict__ targets, int n, int n_rows, int V, long l
   cluster_wait();
 }
 
-// ------------------------------------------------------------------------------------------------ 16-bit operands
-
-template <typename T> __device__ __forceinline__ float load1(const T* p) { return static_cast<float>(*p); }
-
-// dst [planes][n_rows][d_pad] <- rows of src [*, d]: row r from row_of[r] (or r itself), zeros behind the last one and behind
-// column d.  planes = 3: dst = a + b + c, each the nearest bf16 value to what is left.  Eight columns a thread.
-template <typename S, typename T>
+// Up to kFewRows rows, packed and copied in one launch: every CTA finds the rows for itself and copies its part of the tile.
+template <typename I, typename S, typename T>
 __global__ void __launch_bounds__(kBlock)
-copy_rows_kernel(const S* __restrict__ src, T* __restrict__ dst, const Head* head, const int* __restrict__ row_of, int n_src,
-                 int n_rows, int d, int d_pad, int planes, int vec) {
+pack_few_kernel(const I* __restrict__ targets, int n, int V, long long ignore, Head* head, int* __restrict__ row_of, int* __restrict__ target,
+                float* __restrict__ at_target, float* __restrict__ each, const S* __restrict__ x, T* __restrict__ copy, int n_rows, int d, int d_pad,
+                int planes, int vec) {
+  __shared__ int source[kFewRows];
+  __shared__ unsigned has[kFewRows / 32];
   grid_dep_wait();
   grid_dep_release();
-  int end = n_src;
-  if (row_of != nullptr) {
-    const int all = head->count;
-    end = all < kRowTile ? kRowTile : (all + kRowTile - 1) / kRowTile * kRowTile;
+  const int i = threadIdx.x, lane = i & 31;
+  const bool in = i < n;
+  const long long t = in ? static_cast<long long>(targets[i]) : 0;
+  const bool mine = in && counts(t, ignore);
+  if (i < kFewRows) {
+    const unsigned b = __ballot_sync(0xffffffffu, mine);
+    if (lane == 0) has[i / 32] = b;
   }
+  __syncthreads();
+  int all = 0, r = 0;                      // rows with a target, and those in front of this one
+  for (int w = 0; w < kFewRows / 32; ++w) {
+    if (w < i / 32) r += __popc(has[w]);
+    if (w == i / 32) r += __popc(has[w] & ((1u << lane) - 1u));
+    all += __popc(has[w]);
+  }
+  if (mine) source[r] = i;
+  if (blockIdx.x == 0) {
+    if (mine) {
+      row_of[r] = i;
+      target[r] = t >= 0 && t < V ? static_cast<int>(t) : -2;
+      at_target[r] = __int_as_float(0x7fffffff);
+    } else if (in && each != nullptr) {
+      each[i] = 0.f;
+    }
+    if (i >= all && i < kRowTile) {
+      row_of[i] = -1;
+      target[i] = -1;
+      at_target[i] = 0.f;
+    }
+    if (i == 0) {
+      head->count = all;
+      head->splits = 1;
+    }
+  }
+  __syncthreads();
   const int chunks = d_pad / 8;
-  const long long total = static_cast<long long>(end) * chunks;
-  for (long long i = static_cast<long long>(blockIdx.x) * kBlock + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * kBlock) {
-    const int r = static_cast<int>(i / chunks), c = 8 * static_cast<int>(i - static_cast<long long>(r) * chunks);
-    const int from = row_of != nullptr ? row_of[r] : r;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.f;
-    if (from >= 0 && c < d) {
-      const S* s = src + static_cast<size_t>(from) * d + c;
-      if (vec) rowwise::Elem<S>::load(s, v);
-      else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c + j < d) v[j] = load1(s + j);
-      }
-    }
-    T* o = dst + static_cast<size_t>(r) * d_pad + c;
-    for (int part = 0; part < planes; ++part) {
-      rowwise::Elem<T>::store(o, v);
-      o += static_cast<size_t>(n_rows) * d_pad;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] -= rowwise::Elem<T>::round(v[j]);
-    }
+  for (int c = blockIdx.x * kBlock + i; c < kRowTile * chunks; c += gridDim.x * kBlock) {
+    const int row = c / chunks;
+    copy_chunk(x, copy, row < all ? source[row] : -1, row, 8 * (c - row * chunks), n_rows, d, d_pad, planes, vec);
   }
 }
 
@@ -181,12 +240,12 @@ copy_rows_kernel(const S* __restrict__ src, T* __restrict__ dst, const Head* hea
 __global__ void __launch_bounds__(kBlock)
 finish_kernel(const Head* head, const float2* __restrict__ partial, const float* __restrict__ at_target, const int* __restrict__ row_of,
               int n_rows, float* __restrict__ lse, float* __restrict__ lse_rest, float* __restrict__ each, float* __restrict__ out, double* sums,
-              unsigned* ticket, int mean, int lanes) {
+              unsigned* ticket, int mean, int lanes, int few_parts) {
   __shared__ double warp_sum[kBlock / 32];
   __shared__ int last;
   grid_dep_wait();
   grid_dep_release();
-  const int all = head->count, parts = 2 * head->splits;
+  const int all = head->count, parts = few_parts > 0 ? few_parts : 2 * head->splits;
   const int end = all < kRowTile ? kRowTile : (all + kRowTile - 1) / kRowTile * kRowTile;
   const int mine = threadIdx.x & (lanes - 1), rows = kBlock / lanes;
   double sum = 0.0;
@@ -259,17 +318,28 @@ largest_kernel(const Head* head, const float* __restrict__ grad, const int* __re
   *largest = top > 0.f ? top : 1.f;
 }
 
-// In how many parts the sums of `rest` tiles of k blocks are formed, by one warp: the fewest stages for the busiest pair of CTAs, with
-// `share` more for every share written and added.
-__device__ int choose_parts(int rest, int k, int pairs, int share) {
+// In how many parts the sums of `rest` tiles of k stages are formed, by one warp: the fewest stages for the busiest pair of CTAs, with
+// `share` more for every share written and added.  The units are handed out in turn behind `ahead` units of `length` stages.
+__device__ int choose_parts(int rest, int k, int pairs, int share, int ahead, int length) {
   const int lane = threadIdx.x & 31, most = rest > 0 ? kPartsPerPair * pairs / rest : 1;
   long long best = LLONG_MAX;
   for (int s = 1 + lane; s <= most && s <= k; s += 32) {
-    const long long units = (rest * s + pairs - 1) / pairs, cost = units * ((k + s - 1) / s + (s > 1 ? share : 0)) + (s > 1 ? s : 0);
+    const int end = ahead + rest * s, mine = (k + s - 1) / s + (s > 1 ? share : 0);
+    long long cost = 0;
+    for (int i = 0; i < 3; ++i) {                          // the first pair, and the first that gets one unit less of either kind
+      const int b = i == 0 ? 0 : (i == 1 ? ahead : end) % pairs;
+      const int first = (ahead + pairs - 1 - b) / pairs, both = (end + pairs - 1 - b) / pairs;
+      const long long c = static_cast<long long>(first) * length + static_cast<long long>(both - first) * mine;
+      cost = c > cost ? c : cost;
+    }
+    cost += s > 1 ? s : 0;
     if (cost < best >> 8) best = cost << 8 | s;
   }
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, off));
+  for (int off = 16; off > 0; off >>= 1) {
+    const long long o = __shfl_xor_sync(0xffffffffu, best, off);
+    best = o < best ? o : best;
+  }
   return best == LLONG_MAX ? 1 : static_cast<int>(best & 255);
 }
 
@@ -305,7 +375,9 @@ scale_rows_kernel(const Head* head, const float* __restrict__ grad, int per_row,
     for (int last = 0; last < 2; ++last) {
       const int cols = last ? V - (V - 1) / piece * piece : piece;
       const int rest_w = want_dw ? (cols + kColTile - 1) / kColTile * d_tiles % pairs : 0;
-      const int parts_w = choose_parts(rest_w, end / k, pairs, share), parts_x = choose_parts(rest_x, (cols + k - 1) / k, pairs, share);
+      const int kw = end / k, parts_w = choose_parts(rest_w, kw, pairs, share, 0, 0);
+      const int length = (kw + parts_w - 1) / parts_w + (parts_w > 1 ? share : 0);
+      const int parts_x = choose_parts(rest_x, (cols + k - 1) / k, pairs, share, rest_w * parts_w, length);
       if (threadIdx.x == 0) {
         parts->dw[last] = parts_w;
         parts->dx[last] = parts_x;
@@ -358,8 +430,9 @@ Layout layout(const Call& c, bool w_aligned) {
   const int col_tiles = (c.V + kColTile - 1) / kColTile, row_tiles = l.n_rows / kRowTile;
   int most = 256 / row_tiles > 8 ? 256 / row_tiles : 8;
   l.max_splits = most < col_tiles ? most : col_tiles;
+  l.max_parts = c.n <= kFewRows ? 2 * most_pairs() : 2 * l.max_splits;
   at = 0;
-  l.partial = at; at = up(at + static_cast<size_t>(2 * l.max_splits) * l.n_rows * sizeof(float2));
+  l.partial = at; at = up(at + static_cast<size_t>(l.max_parts) * l.n_rows * sizeof(float2));
   l.at_target = at; at = up(at + rows);
   l.sums = at; at = up(at + 1024 * sizeof(double));
   l.ticket = at; at = up(at + 4);
@@ -475,28 +548,46 @@ int run_fwd(const Call& c, const void* x, const void* w, const void* targets, in
   float* each = reduction == NLFA_REDUCE_NONE ? out : nullptr;
   const bool overlap = overlap_launches(kOverlapRowwise);
   const int col_tiles = (c.V + kColTile - 1) / kColTile;
-  auto pack = [&](auto* typed, auto* kernel) {
-    return checked(launch_cluster(kernel, dim3(1, kScanCtas), dim3(kScanThreads), 0, st, overlap, kScanCtas, typed, c.n, l.n_rows, c.V,
-                                  ignore, t.head(), t.row_of(), t.target(), at_target, each, col_tiles, most_pairs(), l.max_splits));
+  const bool few = c.n <= kFewRows;
+  const int vec = c.d % 8 == 0 && aligned16(x) ? 1 : 0;
+  auto pack_few = [&](auto* kernel, auto* typed, auto* from, auto* to) {
+    const int need = (kRowTile * (l.d_pad / 8) + kBlock - 1) / kBlock, ctas = need < sm_count() ? need : sm_count();
+    return checked(launch_kernel(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kBlock), 0, st, overlap, typed, c.n, c.V, ignore, t.head(),
+                                 t.row_of(), t.target(), at_target, each, from, to, l.n_rows, c.d, l.d_pad, l.x_planes, vec));
   };
-  int rc = target_bytes == 8 ? pack(static_cast<const long long*>(targets), pack_rows_kernel<long long>)
-                             : pack(static_cast<const int*>(targets), pack_rows_kernel<int>);
+  auto pack = [&](auto* typed) {
+    using I = std::remove_const_t<std::remove_pointer_t<decltype(typed)>>;
+    auto from = [&](auto* rows) {
+      using S = std::remove_const_t<std::remove_pointer_t<decltype(rows)>>;
+      return dtype == NLFA_DTYPE_F16 ? pack_few(pack_few_kernel<I, S, __half>, typed, rows, reinterpret_cast<__half*>(tape + l.x))
+                                     : pack_few(pack_few_kernel<I, S, __nv_bfloat16>, typed, rows, reinterpret_cast<__nv_bfloat16*>(tape + l.x));
+    };
+    if (few)
+      return c.x_dtype == NLFA_DTYPE_F32 ? from(static_cast<const float*>(x))
+             : c.x_dtype == NLFA_DTYPE_F16 ? from(static_cast<const __half*>(x)) : from(static_cast<const __nv_bfloat16*>(x));
+    return checked(launch_cluster(pack_rows_kernel<I>, dim3(1, kScanCtas), dim3(kScanThreads), 0, st, overlap, kScanCtas, typed, c.n, l.n_rows,
+                                  c.V, ignore, t.head(), t.row_of(), t.target(), at_target, each, col_tiles, most_pairs(), l.max_splits));
+  };
+  int rc = target_bytes == 8 ? pack(static_cast<const long long*>(targets)) : pack(static_cast<const int*>(targets));
   if (rc != NLFA_OK) return rc;
   if (l.copy_w) {
     rc = copy_rows(w, c.w_dtype, tape + l.w, dtype, nullptr, nullptr, c.V, c.V, c.d, l.d_pad, l.x_planes, st);
     if (rc != NLFA_OK) return rc;
   }
-  rc = copy_rows(x, c.x_dtype, tape + l.x, dtype, t.head(), t.row_of(), c.n, l.n_rows, c.d, l.d_pad, l.x_planes, st);
+  if (!few) rc = copy_rows(x, c.x_dtype, tape + l.x, dtype, t.head(), t.row_of(), c.n, l.n_rows, c.d, l.d_pad, l.x_planes, st);
   if (rc != NLFA_OK) return rc;
   CUtensorMap mx, mw;
-  rc = column_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes);
+  rc = few ? box_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes, kFewRows / 2, summands(l.x_planes) / 64, l.x_planes)
+           : column_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes);
   if (rc == NLFA_OK) rc = column_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes);
   if (rc != NLFA_OK) return rc;
   Params p = params(c, l, t, status);
   p.chunk = l.x_planes == 3 ? 1 : c.d > 1024 ? 8 : 0;
   p.partial = reinterpret_cast<float2*>(scratch + l.partial);
+  p.w_stands = l.copy_w ? 0 : 1;
   p.at_target = at_target;
-  rc = launch_product(kLse, dtype, p, mx, mw, mx, mx, st);
+  // few rows: W is read once, as the operand with 256 rows a tile; a tile of 256 rows of x would be read again for each of W's
+  rc = launch_product(few ? kFew : kLse, dtype, p, mx, mw, mx, mx, st);
   if (rc != NLFA_OK) return rc;
   unsigned* ticket = nullptr;
   bool captured = false;
@@ -505,11 +596,11 @@ int run_fwd(const Call& c, const void* x, const void* w, const void* targets, in
     if (rc != NLFA_OK) return rc;
   }
   int lanes = 1;
-  while (lanes < 32 && 2 * l.max_splits > 4 * lanes) lanes *= 2;
+  while (lanes < 32 && l.max_parts > 4 * lanes) lanes *= 2;
   const int need = l.n_rows / (kBlock / lanes), ctas = need < 1024 ? need : 1024;
   return checked(launch_kernel(finish_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kBlock), 0, st, !captured && overlap, t.head(),
                                p.partial, at_target, t.row_of(), l.n_rows, t.lse(), t.lse_rest(), each, each != nullptr ? nullptr : out,
-                               reinterpret_cast<double*>(scratch + l.sums), ticket, reduction == NLFA_REDUCE_MEAN ? 1 : 0, lanes));
+                               reinterpret_cast<double*>(scratch + l.sums), ticket, reduction == NLFA_REDUCE_MEAN ? 1 : 0, lanes, few ? l.max_parts : 0));
 }
 
 int run_bwd(const Call& c, const float* grad, const void* w, const void* targets, int target_bytes, long long ignore, int reduction,

@@ -32,6 +32,7 @@ struct Layout {
   size_t row_of, target, lse, lse_rest, x, w, tape_bytes;
   int max_splits;
   size_t partial, at_target, sums, ticket, fwd_bytes;
+  int max_parts;                    // (maximum, sum) pairs per row
 };
 
 // One product's launch.
@@ -42,6 +43,7 @@ struct Params {
   int chunk;                        // stages per chain of the tensor core (0: the whole sum)
   int v0, v1;                       // piece of the vocabulary
   int n_rows;
+  int w_stands;                     // kFew: w is the caller's, not a copy made by the launch before
   // forward: (max, sum) of every part of a row, logit of the target
   float2* partial;
   float* at_target;
@@ -64,8 +66,9 @@ struct Params {
 
 int most_pairs();                   // of CTAs that run at once
 size_t share_bytes();
-enum { kLse = 0, kGrad = 1, kProducts = 2 };
-// Maps: kLse and kGrad: x and w as operands along the columns, kGrad: ds_out to store dl; kProducts: x and w as operands along the rows,
+enum { kLse = 0, kGrad = 1, kProducts = 2, kFew = 3 };
+constexpr int kFewRows = 64;        // rows of a call that kFew takes
+// Maps: kLse, kFew and kGrad: x and w as operands along the columns, kGrad: ds_out to store dl; kProducts: x and w as operands along the rows,
 // dl along the columns (ds) and along the rows (ds_out).
 int launch_product(int mode, int dtype, const Params& p, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& ds,
                    const CUtensorMap& ds_out, cudaStream_t stream);

@@ -1,7 +1,8 @@
 // The products of the linear cross entropy (loss.cu) on the tensor cores:
 //   kLse       l = x W^T, of which only each row's running maximum and sum of exponentials leave the SM, and the target's l;
 //   kGrad      l again for a piece of the vocabulary, dl = r (exp(l - lse) - [v == target]), written in 16 bits;
-//   kProducts  dx (+)= dl W and dW = dl^T x of that piece, both in one launch.
+//   kProducts  dx (+)= dl W and dW = dl^T x of that piece, both in one launch;
+//   kFew       kLse of up to 64 rows with the operands exchanged: l^T = W x^T, 256 words x 64 rows a tile.
 //
 // One persistent kernel per kind, a pair of CTAs (cta_group::2) per 256 x 256 tile: each CTA holds 128 rows of A, 128
 // columns of B and 128 x 256 of the sums, so an operand byte brought into shared memory serves twice the columns
@@ -15,6 +16,8 @@
 //
 // Warps: 0 producer, 1 MMA issuer (even CTA) and TMEM owner, 2-9 epilogue: two warps per quarter of the rows, 128 columns
 // each.  Every wait is bounded (ptx.cuh); no multicast loads.
+#include <cfloat>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -30,18 +33,20 @@ constexpr int kEpilogueWarps = 8;
 constexpr int kBlockBytes = 128 * 128;                        // 128 rows of 64 columns
 // PARTS = 1: three stages of 128 summands.  PARTS = 3 (float32 operands, sums of three bf16 parts): two stages of 64 summands in all
 // parts, each of which is multiplied with two or three of the other operand's: a pair of parts a stage loads everything twice.
-template <int PARTS>
+// kFew: four stages, A as above, B 32 rows of a CTA.
+template <int MODE, int PARTS>
 struct Ring {
-  static constexpr int kStages = PARTS == 3 ? 2 : 3;
+  static constexpr int kStages = PARTS == 3 ? 2 : MODE == kFew ? 4 : 3;
   static constexpr int kSummands = summands(PARTS);
   static constexpr int kBlocks = PARTS == 3 ? 3 : kSummands / 64;
-  static constexpr int kOperandBytes = kBlocks * kBlockBytes;   // one CTA's half of an operand
-  static constexpr int kStageBytes = 2 * kOperandBytes;
+  static constexpr int kOperandBytes = kBlocks * kBlockBytes;   // one CTA's half of A
+  static constexpr int kBBlockBytes = MODE == kFew ? kBlockBytes / 4 : kBlockBytes;
+  static constexpr int kStageBytes = kOperandBytes + kBlocks * kBBlockBytes;
+  static_assert(kStages * kStageBytes <= 12 * kBlockBytes, "stages");
 };
-constexpr int kMostStages = 3;
+constexpr int kMostStages = 4;
 constexpr int kStagingBytes = 4096;                           // per epilogue warp
 constexpr int kStaging = 12 * kBlockBytes;
-static_assert(Ring<1>::kStages * Ring<1>::kStageBytes <= kStaging && Ring<3>::kStages * Ring<3>::kStageBytes <= kStaging, "stages");
 constexpr int kBars = kStaging + kEpilogueWarps * kStagingBytes;
 constexpr int kNumBars = 2 * kMostStages + 4;
 constexpr int kTmemSlot = kBars + 8 * kNumBars;
@@ -55,7 +60,7 @@ enum { FULL = 0, EMPTY = kMostStages, ACC_FULL = 2 * kMostStages, ACC_EMPTY = AC
 __device__ __forceinline__ int part_a(int pair) { return (0x001012 >> (4 * pair)) & 15; }   // 2 1 0 1 0 0
 __device__ __forceinline__ int part_b(int pair) { return (0x010210 >> (4 * pair)) & 15; }   // 0 1 2 0 1 0
 
-__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+__host__ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // A tile: where it lies in A's rows and B's columns, how many stages its sum takes, which operands it has.
 struct Tile {
@@ -140,6 +145,11 @@ struct Walk {
       splits = p.head->splits;
       col_tiles = ceil_div(p.V, kColTile);
       units = row_tiles * splits;
+    } else if (MODE == kFew) {
+      // a run of W's tiles for every pair
+      col_tiles = ceil_div(p.V, kRowTile);
+      n = static_cast<int>(static_cast<long long>(col_tiles) * pair / n_pairs);
+      n_end = static_cast<int>(static_cast<long long>(col_tiles) * (pair + 1) / n_pairs);
     } else if (MODE == kGrad) {
       col_tiles = ceil_div(p.v1 - p.v0, kColTile);
       units = row_tiles * col_tiles;
@@ -166,6 +176,12 @@ struct Walk {
       }
       t.n0 = n * kColTile;
       t.last = ++n == n_end;
+      return true;
+    }
+    if (MODE == kFew) {
+      if (n == n_end) return false;
+      t.m0 = n++ * kRowTile;
+      t.n0 = 0;
       return true;
     }
     u += stride;
@@ -300,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
             const __grid_constant__ CUtensorMap tm_ds, const __grid_constant__ CUtensorMap tm_out, const Params p) {
   constexpr bool kBf16 = Pack2<T>::kIsBf16;
-  using R = Ring<PARTS>;
+  using R = Ring<MODE, PARTS>;
   constexpr int kStages = R::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -314,6 +330,10 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + kTmemSlot);
   const WaitCtx wctx{abort_flag, p.status};
 
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_w);
+  }
   if (threadIdx.x == 0) {
     *abort_flag = (*reinterpret_cast<volatile unsigned*>(p.status) != STATUS_OK) ? 1 : 0;
     for (int s = 0; s < kStages; ++s) {
@@ -337,6 +357,12 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const bool dead = *abort_flag != 0;
+  if (MODE == kFew && p.w_stands && threadIdx.x == 0) {
+    // while the rows are packed, W comes into L2
+    const int tiles = ceil_div(p.V, kRowTile), n_end = static_cast<int>(static_cast<long long>(tiles) * (pair + 1) / n_pairs);
+    for (int n = static_cast<int>(static_cast<long long>(tiles) * pair / n_pairs); n < n_end; ++n)
+      for (int k = 0; k < p.d; k += R::kSummands) tma_prefetch_4d(&tm_w, 0, n * kRowTile + 128 * rank, k / 64, 0);
+  }
   grid_dep_wait();
   grid_dep_release();
 
@@ -354,9 +380,9 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
         tma_load_4d_pair(dst, map, full, 0, row, col / 64, 0);
       };
       while (ok && walk.next(t)) {
-        const CUtensorMap* ma = MODE != kProducts ? &tm_x : t.dw ? &tm_out : &tm_ds;
-        const CUtensorMap* mb = MODE == kProducts && t.dw ? &tm_x : &tm_w;
-        const int a0 = t.m0 + 128 * rank, b0 = t.n0 + 128 * rank;
+        const CUtensorMap* ma = MODE == kFew ? &tm_w : MODE != kProducts ? &tm_x : t.dw ? &tm_out : &tm_ds;
+        const CUtensorMap* mb = MODE == kFew || (MODE == kProducts && t.dw) ? &tm_x : &tm_w;
+        const int a0 = t.m0 + 128 * rank, b0 = t.n0 + (MODE == kFew ? kFewRows / 2 : 128) * rank;
         for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
           const int s = it % kStages;
           if (!(ok = mbar_wait(bar(EMPTY + s), ((it / kStages) & 1) ^ 1, wctx, 90))) break;
@@ -384,7 +410,8 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
       bool ok = true;
       while (ok && walk.next(t)) {
         const bool a_mn = MODE == kProducts && t.dw, b_mn = MODE == kProducts;
-        const uint32_t idesc = a_mn ? make_idesc(kBf16, 256, kColTile, true, b_mn) : make_idesc(kBf16, 256, kColTile, false, b_mn);
+        constexpr int kN = MODE == kFew ? kFewRows : kColTile;
+        const uint32_t idesc = a_mn ? make_idesc(kBf16, 256, kN, true, b_mn) : make_idesc(kBf16, 256, kN, false, b_mn);
         // 16 summands on: 32 bytes along a row, then the next block of 64 columns; or (MN-major) 16 rows
         constexpr uint32_t kMnBlock = PARTS == 3 ? kBlockBytes / 2 : kBlockBytes;     // (of 64 summands: 64 rows)
         const uint32_t a_lbo = a_mn ? kMnBlock : 16u, b_lbo = b_mn ? kMnBlock : 16u;
@@ -401,12 +428,13 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
             const uint32_t a = base + s * R::kStageBytes, b = a + R::kOperandBytes;
 #pragma unroll
             for (int pr = 0; pr < (PARTS == 3 ? 6 : 1); ++pr) {
-              const uint32_t a_part = PARTS == 3 ? part_a(pr) * kBlockBytes : 0u, b_part = PARTS == 3 ? part_b(pr) * kBlockBytes : 0u;
+              const uint32_t a_part = PARTS == 3 ? part_a(pr) * kBlockBytes : 0u, b_part = PARTS == 3 ? part_b(pr) * R::kBBlockBytes : 0u;
 #pragma unroll
               for (int kk = 0; kk < R::kSummands / 16; ++kk) {
-                const uint32_t along_rows = (kk / 4) * kBlockBytes + (kk % 4) * 32u, along_k = kk * 2048u;
-                umma_ss_pair(leader, tmem + buf * kColTile, make_smem_desc(a + a_part + (a_mn ? along_k : along_rows), a_lbo, 1024),
-                             make_smem_desc(b + b_part + (b_mn ? along_k : along_rows), b_lbo, 1024), idesc,
+                const uint32_t along_a = a_mn ? kk * 2048u : (kk / 4) * kBlockBytes + (kk % 4) * 32u;
+                const uint32_t along_b = b_mn ? kk * 2048u : (kk / 4) * R::kBBlockBytes + (kk % 4) * 32u;
+                umma_ss_pair(leader, tmem + buf * kColTile, make_smem_desc(a + a_part + along_a, a_lbo, 1024),
+                             make_smem_desc(b + b_part + along_b, b_lbo, 1024), idesc,
                              (kb > 0 || pr > 0 || kk > 0) ? 1u : 0u);
               }
             }
@@ -426,6 +454,17 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
     float run_max = 0.f, run_sum = 0.f;
     int sums = 0;
     bool ok = true;
+    constexpr int kMine = kFewRows / 2;                        // kFew: a thread has one word and, of each tile, this many rows
+    float few_max[MODE == kFew ? kMine : 1], few_sum[MODE == kFew ? kMine : 1];
+    int few_target = -1;
+    if constexpr (MODE == kFew) {
+#pragma unroll
+      for (int j = 0; j < kMine; ++j) {
+        few_max[j] = -FLT_MAX;
+        few_sum[j] = 0.f;
+      }
+      few_target = p.target[kMine * half + lane];
+    }
     Sums<LONG> l;
     auto release = [&](int buf) {                              // this warp has read its part of the buffer
       tc_fence_before();
@@ -436,7 +475,7 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
       const int row0 = t.m0 + 128 * rank + 32 * q, row = row0 + lane;
       int target = -1;
       float lse = 0.f, rest2 = 0.f, scale = 0.f;
-      if (MODE != kProducts) target = p.target[row];
+      if (MODE == kLse || MODE == kGrad) target = p.target[row];
       if (MODE == kGrad) {
         lse = p.lse[row];
         rest2 = p.lse_rest[row] * kLog2e;
@@ -454,7 +493,8 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t r[32];
-            tmem_ld32(tmem_addr(tmem, 32 * q, buf * kColTile + 128 * half + 32 * c), r);
+            if (MODE == kFew && c > 0) break;
+            tmem_ld32(tmem_addr(tmem, 32 * q, buf * kColTile + (MODE == kFew ? kMine : 128) * half + 32 * c), r);
             tc_wait_ld();
 #pragma unroll
             for (int j = 0; j < 32; ++j) l.v[32 * c + j] += __uint_as_float(r[j]);
@@ -465,13 +505,25 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
         buf = sums & 1;
         ok = mbar_wait(bar(ACC_FULL + buf), (sums >> 1) & 1, wctx, 94);
         tc_fence_after();
-        l.acc = tmem_addr(tmem, 32 * q, buf * kColTile + 128 * half);
+        l.acc = tmem_addr(tmem, 32 * q, buf * kColTile + (MODE == kFew ? kMine : 128) * half);
         ++sums;
       }
       if (!ok) break;
       const int c0 = t.n0 + 128 * half;
 
-      if constexpr (MODE == kLse) {
+      if constexpr (MODE == kFew) {
+        uint32_t r[32];
+        l.get(0, r);
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+          if (kMine * half + j >= walk.rows) break;
+          const float x = row < p.V ? __uint_as_float(r[j]) : -INFINITY;
+          if (__shfl_sync(0xffffffffu, few_target, j) == row) p.at_target[kMine * half + j] = x;
+          const float top = fmaxf(few_max[j], x);
+          few_sum[j] = fmaf(few_sum[j], fast_exp2((few_max[j] - top) * kLog2e), fast_exp2((x - top) * kLog2e));
+          few_max[j] = top;
+        }
+      } else if constexpr (MODE == kLse) {
 #pragma unroll (LONG ? 4 : 1)
         for (int c = 0; c < 4; ++c) {
           const int col = c0 + 32 * c;
@@ -598,6 +650,33 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
       }
       if (!LONG) release(buf);
     }
+    if constexpr (MODE == kFew) {
+      // the 128 words of a CTA's four warps as one part (a pair without tiles has an empty one)
+      float2* parts = reinterpret_cast<float2*>(gen + kStaging);          // [quarter][row]
+#pragma unroll
+      for (int j = 0; j < kMine; ++j) {
+        if (kMine * half + j >= walk.rows) break;
+        float top = few_max[j];
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        float sum = few_sum[j] * fast_exp2((few_max[j] - top) * kLog2e);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (lane == 0) parts[kFewRows * q + kMine * half + j] = make_float2(top, sum);
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
+      const int row = kMine * half + lane;
+      if (q == 0 && row < walk.rows) {
+        float2 all = parts[row];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) {
+          const float2 x = parts[kFewRows * i + row];
+          const float top = fmaxf(all.x, x.x);
+          all = make_float2(top, fmaf(all.y, fast_exp2((all.x - top) * kLog2e), x.y * fast_exp2((x.x - top) * kLog2e)));
+        }
+        p.partial[static_cast<size_t>(2 * pair + rank) * p.n_rows + row] = all;
+      }
+    }
     if (MODE == kGrad && lane == 0) tma_store_wait_all();
   }
 
@@ -631,9 +710,12 @@ int launch_one(const Params& p, const CUtensorMap& x, const CUtensorMap& w, cons
   cfg.attrs = attr;
   cfg.numAttrs = overlap_launches(kOverlapRowwise) ? 2 : 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, x, w, ds, out, p);
-  if (MODE == kProducts && e == cudaSuccess)
-    e = launch_kernel(fold_kernel, dim3(2u * static_cast<unsigned>(pairs), kRowTile / kFoldRows), dim3(kFoldThreads), 0, stream,
-                      overlap_launches(kOverlapRowwise), p, pairs);
+  if (MODE == kProducts && e == cudaSuccess) {
+    const int d_tiles = ceil_div(p.d, kColTile), dw_rest = p.want_dw ? ceil_div(p.v1 - p.v0, kColTile) * d_tiles % pairs : 0;
+    const int dx_tiles = p.want_dx ? p.n_rows / kRowTile * d_tiles : 0, most = dw_rest + (dx_tiles < pairs ? dx_tiles : pairs);
+    e = launch_kernel(fold_kernel, dim3(static_cast<unsigned>(most > 0 ? most : 1), kRowTile / kFoldRows), dim3(kFoldThreads), 0,
+                      stream, overlap_launches(kOverlapRowwise), p, pairs);
+  }
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? NLFA_OK : NLFA_ERR_CUDA;
 }
@@ -648,9 +730,12 @@ int launch_product(int mode, int dtype, const Params& p, const CUtensorMap& x, c
   const bool bf16 = dtype == NLFA_DTYPE_BF16;
 #define NLFA_GO(...) launch_one<__VA_ARGS__>(p, x, w, ds, ds_out, stream)
   if (p.planes == 3)                                          // float32 operands: parts in bf16
-    return mode == kLse ? NLFA_GO(__nv_bfloat16, kLse, true, 3)
+    return mode == kFew ? NLFA_GO(__nv_bfloat16, kFew, true, 3)
+           : mode == kLse ? NLFA_GO(__nv_bfloat16, kLse, true, 3)
            : mode == kGrad ? NLFA_GO(__nv_bfloat16, kGrad, true, 3)
                            : NLFA_GO(__nv_bfloat16, kProducts, true, 3);
+  if (mode == kFew && p.chunk > 0) return bf16 ? NLFA_GO(__nv_bfloat16, kFew, true) : NLFA_GO(__half, kFew, true);
+  if (mode == kFew) return bf16 ? NLFA_GO(__nv_bfloat16, kFew, false) : NLFA_GO(__half, kFew, false);
   if (mode == kLse && p.chunk > 0) return bf16 ? NLFA_GO(__nv_bfloat16, kLse, true) : NLFA_GO(__half, kLse, true);
   if (mode == kLse) return bf16 ? NLFA_GO(__nv_bfloat16, kLse, false) : NLFA_GO(__half, kLse, false);
   if (mode == kGrad) return bf16 ? NLFA_GO(__nv_bfloat16, kGrad, false) : NLFA_GO(__half, kGrad, false);
