@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kBlock)
 scale_rows_kernel(const Head* head, const float* __restrict__ grad, int per_row, int mean, const int* __restrict__ row_of,
                   const int* __restrict__ target, float* __restrict__ row_scale, float* __restrict__ alpha, Parts* parts, const float* __restrict__ largest,
                   float unit, const I* __restrict__ targets, int n, long long ignore, uint8_t* __restrict__ dx, long long row_bytes, int V,
-                  int d, int piece, int want_dw, int pairs, int planes) {
+                  int d, int piece, int want_dw, int pairs, int planes, int again) {
   grid_dep_wait();
   grid_dep_release();
   const int all = head->count, stride = gridDim.x * kBlock;
@@ -375,9 +375,9 @@ scale_rows_kernel(const Head* head, const float* __restrict__ grad, int per_row,
     for (int last = 0; last < 2; ++last) {
       const int cols = last ? V - (V - 1) / piece * piece : piece;
       const int rest_w = want_dw ? (cols + kColTile - 1) / kColTile * d_tiles % pairs : 0;
-      const int kw = end / k, parts_w = choose_parts(rest_w, kw, pairs, share, 0, 0);
+      const int kw = again * end / k, parts_w = choose_parts(rest_w, kw, pairs, share, 0, 0);
       const int length = (kw + parts_w - 1) / parts_w + (parts_w > 1 ? share : 0);
-      const int parts_x = choose_parts(rest_x, (cols + k - 1) / k, pairs, share, rest_w * parts_w, length);
+      const int parts_x = choose_parts(rest_x, again * ((cols + k - 1) / k), pairs, share, rest_w * parts_w, length);
       if (threadIdx.x == 0) {
         parts->dw[last] = parts_w;
         parts->dx[last] = parts_x;
@@ -444,13 +444,18 @@ Layout layout(const Call& c, bool w_aligned) {
 // 1 GiB and with 4: between pieces the GPU runs empty, and dx is summed in memory).
 constexpr size_t kMostDl = 1024ull << 20;
 
+// dl is held in 16 bits.  Its roundings (half a step, 2^-8 in bf16) are independent and largely cancel in sums over many rows or words:
+// gradients of 513 rows are off by 2.2e-3 as a whole, 1.7e-3 of that by their own rounding.  A row's own target has most of its dl,
+// though, and in a sum of a few rows one such rounding shows (3.3e-3 for one row): up to a tile of rows dl is held in two parts.
 struct BwdLayout {
   int piece;                        // columns, a multiple of kColTile
+  int dl_planes;
   size_t row_scale, alpha, parts, dl, shares, dx_sum, bytes;
 };
 BwdLayout bwd_layout(const Call& c, const Layout& l) {
   BwdLayout b{};
-  const size_t column = static_cast<size_t>(l.x_planes) * l.n_rows * 2;
+  b.dl_planes = l.x_planes == 3 ? 3 : c.n <= kRowTile ? 2 : 1;
+  const size_t column = static_cast<size_t>(b.dl_planes) * l.n_rows * 2;
   const int col_tiles = (c.V + kColTile - 1) / kColTile;
   size_t most = kMostDl / (column * kColTile);
   if (most < 1) most = 1;
@@ -478,11 +483,11 @@ int box_map(CUtensorMap* map, const void* base, int dtype, long long cols, long 
 }
 // One CTA's half of an operand, a stage of it, in all its parts: 128 rows, the summands along the columns ...
 int column_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes) {
-  return box_map(map, base, dtype, cols, rows, planes, 128, summands(planes) / 64, planes);
+  return box_map(map, base, dtype, cols, rows, planes, 128, summands(planes) / 64, planes == 3 ? 3 : 1);
 }
 // ... or 128 columns, the summands along the rows.
 int row_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes) {
-  return box_map(map, base, dtype, cols, rows, planes, summands(planes), 2, planes);
+  return box_map(map, base, dtype, cols, rows, planes, summands(planes), 2, planes == 3 ? 3 : 1);
 }
 
 int checked(cudaError_t e) {
@@ -627,7 +632,7 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
     return checked(launch_kernel(kernel, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(kBlock), 0, st, overlap, t.head(), grad,
                                  per_row, reduction == NLFA_REDUCE_MEAN ? 1 : 0, t.row_of(), t.target(), row_scale, alpha, parts, largest,
                                  dtype == NLFA_DTYPE_F16 ? 16384.f : 1.f, typed, c.n, ignore, static_cast<uint8_t*>(dx), row_bytes, c.V, c.d, b.piece, dw != nullptr ? 1 : 0,
-                                 most_pairs(), l.x_planes));
+                                 most_pairs(), l.x_planes, l.x_planes == 1 ? b.dl_planes : 1));
   };
   rc = target_bytes == 8 ? scale(static_cast<const long long*>(targets), scale_rows_kernel<long long>)
                          : scale(static_cast<const int*>(targets), scale_rows_kernel<int>);
@@ -638,12 +643,13 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
   if (rc == NLFA_OK) rc = column_map(&w_columns, wp, dtype, l.d_pad, c.V, l.x_planes);
   if (rc == NLFA_OK) rc = row_map(&x_rows, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes);
   if (rc == NLFA_OK) rc = row_map(&w_rows, wp, dtype, l.d_pad, c.V, l.x_planes);
-  if (rc == NLFA_OK) rc = column_map(&dl_columns, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes);
-  if (rc == NLFA_OK) rc = row_map(&dl_rows, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes);
-  if (rc == NLFA_OK) rc = box_map(&out, scratch + b.dl, dtype, b.piece, l.n_rows, l.x_planes, 32, 1, 1);
+  if (rc == NLFA_OK) rc = column_map(&dl_columns, scratch + b.dl, dtype, b.piece, l.n_rows, b.dl_planes);
+  if (rc == NLFA_OK) rc = row_map(&dl_rows, scratch + b.dl, dtype, b.piece, l.n_rows, b.dl_planes);
+  if (rc == NLFA_OK) rc = box_map(&out, scratch + b.dl, dtype, b.piece, l.n_rows, b.dl_planes, 32, 1, 1);
   if (rc != NLFA_OK) return rc;
   Params p = params(c, l, t, status);
   p.chunk = l.x_planes == 3 ? 1 : 0;
+  p.dl_planes = b.dl_planes;
   p.row_scale = row_scale;
   p.alpha = alpha;
   p.parts = parts;

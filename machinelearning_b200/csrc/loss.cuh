@@ -40,6 +40,7 @@ struct Params {
   const Head* head;
   int V, d, d_pad;
   int planes;                       // parts of an operand: 1 or 3
+  int dl_planes;                    // parts of dl: 1, 3 with operands in three, or 2 where gradients are sums of few rows (loss.cu)
   int chunk;                        // stages per chain of the tensor core (0: the whole sum)
   int v0, v1;                       // piece of the vocabulary
   int n_rows;

@@ -8,7 +8,8 @@
 // columns of B and 128 x 256 of the sums, so an operand byte brought into shared memory serves twice the columns
 // of a single CTA's tile.  A stage is 128 summands, each operand of it one box of 32 KB: 128 rows x 2 blocks of 64 columns, K-major or
 // MN-major by what its coordinates mean.  (Loads bound these kernels, and how many there are counts as much as their bytes:
-// forward of 16,384 x 50,304 x 768 at 1,490 TFLOP/s with boxes of 8 KB, 1,583 with 16 KB, ... with 32 KB; as fast with four stages as with six.)  Sums are double buffered in TMEM (2 x 256 columns): the epilogue of a tile runs under the next one's products.
+// forward of 16,384 x 50,304 x 768 at 1,490 TFLOP/s with boxes of 8 KB, 1,583 with 16 KB, 1,605 with
+// 32 KB; with half of the bytes 1,780.)  Sums are double buffered in TMEM (2 x 256 columns): the epilogue of a tile runs under the next one's products.
 //
 // The tensor core adds to its sums by truncation: a chain of K / 16 steps over positive summands comes out low by 6.6e-7 of
 // its value at K = 768, 1.1e-5 at 4,096 and 7.7e-5 at 16,384 (measured; a float32 product on the CUDA cores is off by 5e-8).  Where that shows,
@@ -66,6 +67,7 @@ __host__ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b -
 struct Tile {
   int m0, n0;
   int k0, k1;                       // its blocks of summands (a stage each): all, or of a shared tile this pair's
+  int length;                       // kProducts: blocks per part of dl (the parts follow one another)
   int dw;                           // kProducts: a tile of dW (else of dx)
   int first, last;                  // kLse: first / last tile of a unit
   int slot;                         // kLse: which part of the vocabulary; kProducts: where a share of a tile goes (-1: the tile is whole)
@@ -73,10 +75,11 @@ struct Tile {
 
 // kProducts: the units are dW's tiles and then dx's, handed out in turn: whole tiles, as many of each kind as all pairs of CTAs get,
 // and the rest, whose sums are cut into parts so that every pair is busy (loss.cu: choose_parts; fold_kernel adds the shares).  Parts of one
-// index stand together: they read the same summands, from L2.  (Cut into one line of equal lengths instead, they read everything from
-// HBM: products of 16,384 tokens over 12,800 words 768 wide 427 us with whole tiles only, 468 us so, ... us as it is.)
+// index stand together: they read the same summands, from L2.  Backward with whole tiles only, and as it is: 65,536 rows x 50,304 words
+// x 768 12.9 and 11.9 ms, 4,096 rows 0.74 and 0.69, 300 rows 0.36 and 0.14.  (The rest as one line of stages cut into equal lengths balances
+// better, but every pair then reads summands of its own from HBM: slower than whole tiles at 16,384 rows.)
 struct Plan {
-  int d_tiles, kw, kx;
+  int d_tiles, kw, kx, again;
   int dw_whole, dw_rest, dw_parts, dx_whole, dx_rest, dx_parts;
   int u1, u2, u3, u4;               // ends of the four kinds of units
   int dx_slot;                      // dx's first share
@@ -85,8 +88,9 @@ struct Plan {
     const int row_tiles = rows > 0 ? ceil_div(rows, kRowTile) : 1;
     d_tiles = ceil_div(p.d, kColTile);
     const int dw_tiles = p.want_dw ? ceil_div(p.v1 - p.v0, kColTile) * d_tiles : 0, dx_tiles = p.want_dx ? row_tiles * d_tiles : 0;
-    kw = row_tiles * (kRowTile / summands(p.planes));
-    kx = ceil_div(p.v1 - p.v0, summands(p.planes));
+    again = p.planes == 1 ? p.dl_planes : 1;
+    kw = again * row_tiles * (kRowTile / summands(p.planes));
+    kx = again * ceil_div(p.v1 - p.v0, summands(p.planes));
     dw_whole = dw_tiles / pairs * pairs;
     dx_whole = dx_tiles / pairs * pairs;
     dw_rest = dw_tiles - dw_whole;
@@ -107,6 +111,7 @@ struct Plan {
     int v = u - first;
     t.k0 = 0;
     t.k1 = k;
+    t.length = k / again;
     t.slot = -1;
     if (i >= 0) {
       const int part = i / rest;
@@ -376,8 +381,8 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
       int it = 0;
       bool ok = true;
       const uint32_t full0 = cluster_addr(bar(FULL), 0);       // loads of both CTAs are counted on the even one's
-      auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t full, int row, int col) {
-        tma_load_4d_pair(dst, map, full, 0, row, col / 64, 0);
+      auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t full, int row, int col, int plane) {
+        tma_load_4d_pair(dst, map, full, 0, row, col / 64, plane);
       };
       while (ok && walk.next(t)) {
         const CUtensorMap* ma = MODE == kFew ? &tm_w : MODE != kProducts ? &tm_x : t.dw ? &tm_out : &tm_ds;
@@ -389,11 +394,12 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
           const uint32_t st = base + s * R::kStageBytes, full = full0 + 8u * s;
           if (rank == 0) mbar_arrive_expect_tx(bar(FULL + s), 2 * R::kStageBytes);
           // boxes at (row, block of 64 columns): the sum runs along the columns, or (MN-major) along the rows
-          const int k = kb * R::kSummands;
-          if (MODE == kProducts && t.dw) load(st, ma, full, k, a0);
-          else load(st, ma, full, a0, k);
-          if (MODE != kProducts) load(st + R::kOperandBytes, mb, full, b0, k);
-          else load(st + R::kOperandBytes, mb, full, (t.dw ? 0 : p.v0) + k, b0);
+          const int plane = MODE == kProducts && PARTS == 1 ? kb / t.length : 0;
+          const int k = (kb - (plane > 0 ? plane * t.length : 0)) * R::kSummands;
+          if (MODE == kProducts && t.dw) load(st, ma, full, k, a0, plane);
+          else load(st, ma, full, a0, k, plane);
+          if (MODE != kProducts) load(st + R::kOperandBytes, mb, full, b0, k, 0);
+          else load(st + R::kOperandBytes, mb, full, (t.dw ? 0 : p.v0) + k, b0, 0);
         }
       }
       // the last loads of this CTA have been consumed before it may leave (after a give-up: have had time to land)
@@ -592,8 +598,13 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
               for (int j = 0; j < 32; ++j)
                 if (at == static_cast<unsigned>(j)) lo[h][j] -= scale;
             }
+            if (__any_sync(0xffffffffu, target == -1)) {     // behind the last row: zeros, whatever W holds (0 inf would not be)
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (target == -1) lo[h][j] = 0.f;
+            }
           }
-          for (int part = 0; part < p.planes; ++part) {
+          for (int part = 0; part < p.dl_planes; ++part) {
             if (lane == 0) tma_store_wait_read();
             __syncwarp();
 #pragma unroll
@@ -611,7 +622,7 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
               tma_store_4d(&tm_out, staging, 0, row0, (c0 + 64 * c2 - p.v0) / 64, part);
               tma_store_commit();
             }
-            if (part + 1 < p.planes) {
+            if (part + 1 < p.dl_planes) {
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll

@@ -8,7 +8,7 @@ float32 is three bf16 parts: 2^-24) and u_out that of the output:
   c = min(d, 1024) / 16 steps (float32: 256 / 16 and three parts of it) and the chunks' own additions |dl| <= e = (c + 8 + d / 256) 2^-23 S;
 * a loss is the difference of a logarithm and a logit: |d loss| <= 2 e + 2^-21 (1 + |loss|) (ex2.approx is off by 2^-22, log by less);
 * a probability is off by a factor exp(2 e) 2^-21: r = 2 e + 2^-20;
-* dx = dl W: u on each dl, r on each p, the chain over V (k = V / 16, float32: 32 + V / 256) in steps of 2^-23, and the output's rounding:
+* dx = dl W: u on each dl (u^2 where dl is held in two parts: up to 256 rows), r on each p, the chain over V (k = V / 16, float32: 32 + V / 256) in steps of 2^-23, and the output's rounding:
   u_out |dx| + (u + k 2^-23) sum |dl w| + r sum p |w|; dw the same over the rows.  fp16: dl is held times 2^14 / max |g|, so what
   underflows is below 2^-25 2^-14 max |g| each, and outputs below the normal range are off by 2^-25.
 """
@@ -91,9 +91,10 @@ def _np(t):
     return t.detach().double().cpu().numpy()
 
 
-def _check(dtype, x, w, t, loss, dx, dw, reduction, grad=None, compute=None):
-    """Against the bounds of this file's head; ``compute``: what the products ran in, where it is not ``dtype``."""
+def _check(dtype, x, w, t, loss, dx, dw, reduction, grad=None, compute=None, dl_step=None):
+    """Against the bounds of this file's head; ``compute``: what the products ran in, where it is not ``dtype``; ``dl_step``: u."""
     compute = compute or dtype
+    dl_step = dl_step or HALF_STEP[compute]
     xs, ws = _np(x.to(DT[compute])), _np(w.to(DT[compute]))
     xs, ts = xs.reshape(-1, xs.shape[-1]), t.reshape(-1).cpu().numpy()
     up = None if grad is None else _np(grad).reshape(-1) if reduction == "none" else _np(grad)
@@ -114,7 +115,7 @@ def _check(dtype, x, w, t, loss, dx, dw, reduction, grad=None, compute=None):
         got = _np(got).reshape(want.shape)
         out = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, torch.float32: 2.0**-24}[like.dtype]
         k = 32 + k / 256 if compute == "fp32" else k / 16
-        bound = out * np.abs(want) + (HALF_STEP[compute] + (k + 8) * 2.0**-23) * total + (2 * e + 2.0**-20) * prob
+        bound = out * np.abs(want) + (dl_step + (k + 8) * 2.0**-23) * total + (2 * e + 2.0**-20) * prob
         if compute == "fp16":
             other = np.abs(ws).sum(0) if name == "dx" else np.abs(xs).sum(0)
             bound = bound + 2.0**-39 * gmax * other
@@ -141,6 +142,18 @@ def test_loss_and_gradients(dtype, n, V, d, reduction):
     _check(dtype, x, w, t, loss, dx, dw, reduction, up)
     with torch.no_grad():
         assert torch.equal(head_loss.linear_cross_entropy(x, w, t, reduction=reduction), loss)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 5, 64, 65, 256])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_few_rows_hold_the_gradient_of_the_logits_in_two_parts(dtype, n):
+    """Up to 256 rows: u is half a step of the second part (bf16 2^-16, fp16 2^-22)."""
+    from machinelearning_b200 import head_loss
+    x, w, t = _inputs(dtype, n, 1500, 200, seed=n)
+    loss = head_loss.linear_cross_entropy(x, w, t, reduction="sum")
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    _check(dtype, x, w, t, loss, dx, dw, "sum", dl_step=HALF_STEP[dtype] ** 2)
 
 
 @pytest.mark.gpu
@@ -250,6 +263,8 @@ def test_logits_of_any_size():
     keep = [i for i in range(300) if i != 7]
     want = step_f64.linear_cross_entropy(_np(x), _np(w2)[keep], [0, 149, 298], reduction="none")["loss"]
     assert np.abs(_np(each) - want).max() <= 2.0**-12
+    (dw,) = torch.autograd.grad(each.sum(), w2)
+    assert bool(torch.isfinite(dw.float()).all()) and bool((dw[7] == 0).all())
 
 
 @pytest.mark.gpu
