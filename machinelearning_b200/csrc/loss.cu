@@ -446,15 +446,17 @@ constexpr size_t kMostDl = 1024ull << 20;
 
 // dl is held in 16 bits.  Its roundings (half a step, 2^-8 in bf16) are independent and largely cancel in sums over many rows or words:
 // gradients of 513 rows are off by 2.2e-3 as a whole, 1.7e-3 of that by their own rounding.  A row's own target has most of its dl,
-// though, and in a sum of a few rows one such rounding shows (3.3e-3 for one row): up to a tile of rows dl is held in two parts.
+// though, and in a sum of a few rows one such rounding shows (3.3e-3 for one row): up to a tile of rows dl is held in two parts, and up
+// to kTwoParts where the rows' gradients differ, so that a few of them can be most of the sum (2.5e-3 for 160 rows).
+constexpr int kTwoParts = 1024;
 struct BwdLayout {
   int piece;                        // columns, a multiple of kColTile
-  int dl_planes;
+  int dl_planes;                    // there is room for
   size_t row_scale, alpha, parts, dl, shares, dx_sum, bytes;
 };
 BwdLayout bwd_layout(const Call& c, const Layout& l) {
   BwdLayout b{};
-  b.dl_planes = l.x_planes == 3 ? 3 : c.n <= kRowTile ? 2 : 1;
+  b.dl_planes = l.x_planes == 3 ? 3 : c.n <= kTwoParts ? 2 : 1;
   const size_t column = static_cast<size_t>(b.dl_planes) * l.n_rows * 2;
   const int col_tiles = (c.V + kColTile - 1) / kColTile;
   size_t most = kMostDl / (column * kColTile);
@@ -587,7 +589,8 @@ int run_fwd(const Call& c, const void* x, const void* w, const void* targets, in
   if (rc == NLFA_OK) rc = column_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes);
   if (rc != NLFA_OK) return rc;
   Params p = params(c, l, t, status);
-  p.chunk = l.x_planes == 3 ? 1 : c.d > 1024 ? 8 : 0;
+  // chains of 64 summands for float32, of 256 for few rows (whose losses are not averaged; W's bandwidth hides it), else of up to 1,024
+  p.chunk = l.x_planes == 3 ? 1 : few ? (c.d > 256 ? 2 : 0) : c.d > 1024 ? 8 : 0;
   p.partial = reinterpret_cast<float2*>(scratch + l.partial);
   p.w_stands = l.copy_w ? 0 : 1;
   p.at_target = at_target;
@@ -617,6 +620,7 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
   if (!status) return NLFA_ERR_CUDA;
   const int dtype = c.dtype == NLFA_DTYPE_F32 ? NLFA_DTYPE_BF16 : c.dtype;
   const bool overlap = overlap_launches(kOverlapRowwise);
+  const int dl_planes = l.x_planes == 3 ? 3 : c.n <= kRowTile || (reduction == NLFA_REDUCE_NONE && c.n <= kTwoParts) ? 2 : 1;
   float* row_scale = reinterpret_cast<float*>(scratch + b.row_scale);
   float* alpha = reinterpret_cast<float*>(scratch + b.alpha);
   Parts* parts = reinterpret_cast<Parts*>(scratch + b.parts);
@@ -632,7 +636,7 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
     return checked(launch_kernel(kernel, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(kBlock), 0, st, overlap, t.head(), grad,
                                  per_row, reduction == NLFA_REDUCE_MEAN ? 1 : 0, t.row_of(), t.target(), row_scale, alpha, parts, largest,
                                  dtype == NLFA_DTYPE_F16 ? 16384.f : 1.f, typed, c.n, ignore, static_cast<uint8_t*>(dx), row_bytes, c.V, c.d, b.piece, dw != nullptr ? 1 : 0,
-                                 most_pairs(), l.x_planes, l.x_planes == 1 ? b.dl_planes : 1));
+                                 most_pairs(), l.x_planes, l.x_planes == 1 ? dl_planes : 1));
   };
   rc = target_bytes == 8 ? scale(static_cast<const long long*>(targets), scale_rows_kernel<long long>)
                          : scale(static_cast<const int*>(targets), scale_rows_kernel<int>);
@@ -643,13 +647,13 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
   if (rc == NLFA_OK) rc = column_map(&w_columns, wp, dtype, l.d_pad, c.V, l.x_planes);
   if (rc == NLFA_OK) rc = row_map(&x_rows, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes);
   if (rc == NLFA_OK) rc = row_map(&w_rows, wp, dtype, l.d_pad, c.V, l.x_planes);
-  if (rc == NLFA_OK) rc = column_map(&dl_columns, scratch + b.dl, dtype, b.piece, l.n_rows, b.dl_planes);
-  if (rc == NLFA_OK) rc = row_map(&dl_rows, scratch + b.dl, dtype, b.piece, l.n_rows, b.dl_planes);
-  if (rc == NLFA_OK) rc = box_map(&out, scratch + b.dl, dtype, b.piece, l.n_rows, b.dl_planes, 32, 1, 1);
+  if (rc == NLFA_OK) rc = column_map(&dl_columns, scratch + b.dl, dtype, b.piece, l.n_rows, dl_planes);
+  if (rc == NLFA_OK) rc = row_map(&dl_rows, scratch + b.dl, dtype, b.piece, l.n_rows, dl_planes);
+  if (rc == NLFA_OK) rc = box_map(&out, scratch + b.dl, dtype, b.piece, l.n_rows, dl_planes, 32, 1, 1);
   if (rc != NLFA_OK) return rc;
   Params p = params(c, l, t, status);
   p.chunk = l.x_planes == 3 ? 1 : 0;
-  p.dl_planes = b.dl_planes;
+  p.dl_planes = dl_planes;
   p.row_scale = row_scale;
   p.alpha = alpha;
   p.parts = parts;

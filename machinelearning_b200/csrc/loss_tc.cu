@@ -13,7 +13,7 @@
 //
 // The tensor core adds to its sums by truncation: a chain of K / 16 steps over positive summands comes out low by 6.6e-7 of
 // its value at K = 768, 1.1e-5 at 4,096 and 7.7e-5 at 16,384 (measured; a float32 product on the CUDA cores is off by 5e-8).  Where that shows,
-// the chain is cut (LONG): a tile's sum is formed chunk by chunk, and the chunks' sums are added in registers.
+// the chain is cut (LONG; where: loss.cu): a tile's sum is formed chunk by chunk, and the chunks' sums are added in registers.
 //
 // Warps: 0 producer, 1 MMA issuer (even CTA) and TMEM owner, 2-9 epilogue: two warps per quarter of the rows, 128 columns
 // each.  Every wait is bounded (ptx.cuh); no multicast loads.
@@ -296,15 +296,15 @@ fold_kernel(const Params p, int pairs) {
 
 // ---- epilogues: a thread has row `lane` of its warp's 32 and, 32 at a time, 128 columns
 
-// 128 columns of a thread's row: in TMEM, or (LONG) summed from the chunks' sums in registers.
-template <bool LONG>
+// The columns of a thread's row: in TMEM, or (LONG) summed from the chunks' sums in registers.
+template <bool LONG, int COLS>
 struct Sums {
   uint32_t acc;
-  float v[LONG ? 128 : 1];
+  float v[LONG ? COLS : 1];
   __device__ __forceinline__ void get(int col, uint32_t (&r)[32]) const {
     if constexpr (LONG) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < COLS / 32; ++c)
         if (col == 32 * c) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(v[32 * c + j]);
@@ -471,7 +471,8 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
       }
       few_target = p.target[kMine * half + lane];
     }
-    Sums<LONG> l;
+    constexpr int kCols = MODE == kFew ? kMine : 128;
+    Sums<LONG, kCols> l;
     auto release = [&](int buf) {                              // this warp has read its part of the buffer
       tc_fence_before();
       __syncwarp();
@@ -480,27 +481,26 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
     while (walk.next(t)) {
       const int row0 = t.m0 + 128 * rank + 32 * q, row = row0 + lane;
       int target = -1;
-      float lse = 0.f, rest2 = 0.f, scale = 0.f;
+      float lse = 0.f, rest = 0.f, scale = 0.f;
       if (MODE == kLse || MODE == kGrad) target = p.target[row];
       if (MODE == kGrad) {
         lse = p.lse[row];
-        rest2 = p.lse_rest[row] * kLog2e;
+        rest = p.lse_rest[row];
         scale = p.row_scale[row];
       }
       if (MODE == kLse && t.first) { run_max = -INFINITY; run_sum = 0.f; }
       int buf = 0;
       if constexpr (LONG) {
 #pragma unroll
-        for (int j = 0; j < 128; ++j) l.v[j] = 0.f;
+        for (int j = 0; j < kCols; ++j) l.v[j] = 0.f;
         for (int k0 = t.k0; k0 < t.k1; k0 += p.chunk, ++sums) {
           buf = sums & 1;
           if (!(ok = mbar_wait(bar(ACC_FULL + buf), (sums >> 1) & 1, wctx, 94))) break;
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < kCols / 32; ++c) {
             uint32_t r[32];
-            if (MODE == kFew && c > 0) break;
-            tmem_ld32(tmem_addr(tmem, 32 * q, buf * kColTile + (MODE == kFew ? kMine : 128) * half + 32 * c), r);
+            tmem_ld32(tmem_addr(tmem, 32 * q, buf * kColTile + kCols * half + 32 * c), r);
             tc_wait_ld();
 #pragma unroll
             for (int j = 0; j < 32; ++j) l.v[32 * c + j] += __uint_as_float(r[j]);
@@ -511,7 +511,7 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
         buf = sums & 1;
         ok = mbar_wait(bar(ACC_FULL + buf), (sums >> 1) & 1, wctx, 94);
         tc_fence_after();
-        l.acc = tmem_addr(tmem, 32 * q, buf * kColTile + (MODE == kFew ? kMine : 128) * half);
+        l.acc = tmem_addr(tmem, 32 * q, buf * kColTile + kCols * half);
         ++sums;
       }
       if (!ok) break;
@@ -584,7 +584,7 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
             for (int j = 0; j < 32; j += 2) {
               float a, b;
               unpack_f2(ffma2(fadd2(pack_f2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), pack_f2(-lse, -lse)),
-                              pack_f2(kLog2e, kLog2e), pack_f2(-rest2, -rest2)), a, b);
+                              pack_f2(kLog2e, kLog2e), pack_f2(-rest * kLog2e, -rest * kLog2e)), a, b);
               unpack_f2(fmul2(pack_f2(fast_exp2(a), fast_exp2(b)), pack_f2(scale, scale)), lo[h][j], lo[h][j + 1]);
             }
             if (col + 32 > p.V) {
@@ -594,9 +594,15 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
             }
             const unsigned at = static_cast<unsigned>(target - col);
             if (__any_sync(0xffffffffu, at < 32u)) {
+              float top = 0.f;                                 // the target's logit
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                if (at == static_cast<unsigned>(j)) lo[h][j] -= scale;
+                if (at == static_cast<unsigned>(j)) top = __uint_as_float(r[j]);
+              // (p - 1 of a token the model is sure of: not by a difference)
+              const float v = expm1f((top - lse) - rest) * scale;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (at == static_cast<unsigned>(j)) lo[h][j] = v;
             }
             if (__any_sync(0xffffffffu, target == -1)) {     // behind the last row: zeros, whatever W holds (0 inf would not be)
 #pragma unroll
