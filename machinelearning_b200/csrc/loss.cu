@@ -33,7 +33,7 @@ constexpr int kBlock = 256;
 
 template <typename T> __device__ __forceinline__ float load1(const T* p) { return static_cast<float>(*p); }
 
-// Eight columns (from c) of row `from` of src [*, d] (-1: zeros) to row r of dst [planes][n_rows][d_pad]; planes = 3: dst = a + b + c,
+// Eight columns (from c) of row `from` of src [*, d] (-1: zeros) to row r of dst [planes][d_pad / 64][n_rows][64]; planes = 3: dst = a + b + c,
 // each the nearest bf16 value to what is left.
 template <typename S, typename T>
 __device__ __forceinline__ void copy_chunk(const S* __restrict__ src, T* __restrict__ dst, int from, int r, int c, int n_rows, int d, int d_pad,
@@ -50,7 +50,7 @@ __device__ __forceinline__ void copy_chunk(const S* __restrict__ src, T* __restr
         if (c + j < d) v[j] = load1(s + j);
     }
   }
-  T* o = dst + static_cast<size_t>(r) * d_pad + c;
+  T* o = dst + (static_cast<size_t>(c / 64) * n_rows + r) * 64 + c % 64;
   for (int part = 0; part < planes; ++part) {
     rowwise::Elem<T>::store(o, v);
     o += static_cast<size_t>(n_rows) * d_pad;
@@ -474,22 +474,23 @@ BwdLayout bwd_layout(const Call& c, const Layout& l) {
   return b;
 }
 
-// [planes][rows][cols], cols a multiple of 64, as (64 columns, rows, blocks of 64 columns, planes)
+// What lies in tape and scratch lies in blocks, [planes][blocks of 64 columns][rows][64], so that a box is contiguous; the caller's w is
+// [rows][cols].  Either as (64 columns, rows, blocks of 64 columns, planes), cols a multiple of 64.
 int box_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes, int box_rows, int box_blocks,
-            int box_planes) {
+            int box_planes, bool blocked) {
   const unsigned long long pitch = static_cast<unsigned long long>(cols) * 2, r = static_cast<unsigned long long>(rows);
   const unsigned long long dims[4] = {64ull, r, pitch / 128, static_cast<unsigned long long>(planes)};
-  const unsigned long long strides[3] = {pitch, 128ull, pitch * r};
+  const unsigned long long strides[3] = {blocked ? 128ull : pitch, blocked ? 128ull * r : 128ull, pitch * r};
   const unsigned box[4] = {64u, static_cast<unsigned>(box_rows), static_cast<unsigned>(box_blocks), static_cast<unsigned>(box_planes)};
   return make_map(map, base, dtype, dims, strides, box);
 }
 // One CTA's half of an operand, a stage of it, in all its parts: 128 rows, the summands along the columns ...
-int column_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes) {
-  return box_map(map, base, dtype, cols, rows, planes, 128, summands(planes) / 64, planes == 3 ? 3 : 1);
+int column_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes, bool blocked = true) {
+  return box_map(map, base, dtype, cols, rows, planes, 128, summands(planes) / 64, planes == 3 ? 3 : 1, blocked);
 }
 // ... or 128 columns, the summands along the rows.
-int row_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes) {
-  return box_map(map, base, dtype, cols, rows, planes, summands(planes), 2, planes == 3 ? 3 : 1);
+int row_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes, bool blocked = true) {
+  return box_map(map, base, dtype, cols, rows, planes, summands(planes), 2, planes == 3 ? 3 : 1, blocked);
 }
 
 int checked(cudaError_t e) {
@@ -584,13 +585,14 @@ int run_fwd(const Call& c, const void* x, const void* w, const void* targets, in
   if (!few) rc = copy_rows(x, c.x_dtype, tape + l.x, dtype, t.head(), t.row_of(), c.n, l.n_rows, c.d, l.d_pad, l.x_planes, st);
   if (rc != NLFA_OK) return rc;
   CUtensorMap mx, mw;
-  rc = few ? box_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes, kFewRows / 2, summands(l.x_planes) / 64, l.x_planes)
+  rc = few ? box_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes, kFewRows / 2, summands(l.x_planes) / 64, l.x_planes, true)
            : column_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes);
-  if (rc == NLFA_OK) rc = column_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes);
+  if (rc == NLFA_OK) rc = column_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes, l.copy_w);
   if (rc != NLFA_OK) return rc;
   Params p = params(c, l, t, status);
-  // chains of 64 summands for float32, of 256 for few rows (whose losses are not averaged; W's bandwidth hides it), else of up to 1,024
-  p.chunk = l.x_planes == 3 ? 1 : few ? (c.d > 256 ? 2 : 0) : c.d > 1024 ? 8 : 0;
+  // chains of 64 summands for float32, of 384 for few rows (whose losses are not averaged; 26.1 us with one chain, 27.6
+  // so, 29.5 with 256, for 8 rows of 50,304 x 768), else of up to 1,024
+  p.chunk = l.x_planes == 3 ? 1 : few ? (c.d > 384 ? 3 : 0) : c.d > 1024 ? 8 : 0;
   p.partial = reinterpret_cast<float2*>(scratch + l.partial);
   p.w_stands = l.copy_w ? 0 : 1;
   p.at_target = at_target;
@@ -644,12 +646,12 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
   CUtensorMap x_columns, w_columns, out, x_rows, w_rows, dl_columns, dl_rows;
   const void* wp = l.copy_w ? tape + l.w : w;
   rc = column_map(&x_columns, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes);
-  if (rc == NLFA_OK) rc = column_map(&w_columns, wp, dtype, l.d_pad, c.V, l.x_planes);
+  if (rc == NLFA_OK) rc = column_map(&w_columns, wp, dtype, l.d_pad, c.V, l.x_planes, l.copy_w);
   if (rc == NLFA_OK) rc = row_map(&x_rows, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes);
-  if (rc == NLFA_OK) rc = row_map(&w_rows, wp, dtype, l.d_pad, c.V, l.x_planes);
+  if (rc == NLFA_OK) rc = row_map(&w_rows, wp, dtype, l.d_pad, c.V, l.x_planes, l.copy_w);
   if (rc == NLFA_OK) rc = column_map(&dl_columns, scratch + b.dl, dtype, b.piece, l.n_rows, dl_planes);
   if (rc == NLFA_OK) rc = row_map(&dl_rows, scratch + b.dl, dtype, b.piece, l.n_rows, dl_planes);
-  if (rc == NLFA_OK) rc = box_map(&out, scratch + b.dl, dtype, b.piece, l.n_rows, dl_planes, 32, 1, 1);
+  if (rc == NLFA_OK) rc = box_map(&out, scratch + b.dl, dtype, b.piece, l.n_rows, dl_planes, 32, 1, 1, true);
   if (rc != NLFA_OK) return rc;
   Params p = params(c, l, t, status);
   p.chunk = l.x_planes == 3 ? 1 : 0;
