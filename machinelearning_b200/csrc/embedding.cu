@@ -492,7 +492,8 @@ int nlfa_embedding_fwd(const void* ids, int id_bytes, const void* w, int dtype, 
   if (n == 0) return NLFA_OK;
   if (!ids || !w || !out) return NLFA_ERR_NULL_POINTER;
   const int bytes = element_bytes(dtype);
-  if ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out)) % bytes != 0) return NLFA_ERR_MISALIGNED;
+  if ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out)) % bytes != 0 || reinterpret_cast<uintptr_t>(ids) % id_bytes != 0)
+    return NLFA_ERR_MISALIGNED;
   const int word = word_bytes(static_cast<long long>(d) * bytes, w, out);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define NLFA_GO(T, W) (id_bytes == 8 ? lookup<T, W, long long>(ids, w, out, n, V, d, scale, st) : lookup<T, W, int>(ids, w, out, n, V, d, scale, st))
@@ -515,7 +516,8 @@ int nlfa_embedding_bwd(const void* g, int dtype, const void* ids, int id_bytes, 
   if (!dw || !scratch || (n > 0 && (!g || !ids))) return NLFA_ERR_NULL_POINTER;
   if (!rowwise::aligned16(scratch)) return NLFA_ERR_MISALIGNED;
   const int bytes = element_bytes(dtype);
-  if ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(dw)) % bytes != 0) return NLFA_ERR_MISALIGNED;
+  if ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(dw)) % bytes != 0 || reinterpret_cast<uintptr_t>(ids) % id_bytes != 0)
+    return NLFA_ERR_MISALIGNED;
   const Scratch s = scratch_layout(n, V, d);
   if (scratch_bytes < s.bytes) return NLFA_ERR_SCRATCH_TOO_SMALL;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -354,7 +354,7 @@ int nlfa_clip_grads(const nlfa_grad* grads, int count, float max_norm, int norm,
                     size_t scratch_bytes, void* stream) {
   if (count < 0 || (norm != NLFA_NORM_2 && norm != NLFA_NORM_INF)) return NLFA_ERR_BAD_ARGUMENT;
   if (!total_norm || !scratch || (count > 0 && !grads)) return NLFA_ERR_NULL_POINTER;
-  if (!rowwise::aligned16(scratch)) return NLFA_ERR_MISALIGNED;
+  if (!rowwise::aligned16(scratch) || reinterpret_cast<uintptr_t>(total_norm) % 4 != 0) return NLFA_ERR_MISALIGNED;
   if (scratch_bytes < nlfa_clip_scratch_bytes()) return NLFA_ERR_SCRATCH_TOO_SMALL;
   if (static_cast<long long>(count) > static_cast<long long>(kMostTables) * kLargeTable || sm_count() > 160) return NLFA_ERR_BAD_SHAPE;
   int in_place = 1;

@@ -404,6 +404,8 @@ struct Call {
 };
 
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
+int element_bytes(int dtype) { return dtype == NLFA_DTYPE_F32 ? 4 : 2; }
+bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 int check_call(const Call& c) {
   if (c.n < 0 || c.V < 1 || c.d < 1 || c.n > (1 << 30) || c.V > (1 << 30) || c.d > (1 << 24)) return NLFA_ERR_BAD_SHAPE;
@@ -632,7 +634,7 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
   if (largest != nullptr)
     rc = checked(launch_kernel(largest_kernel, dim3(1), dim3(1024), 0, st, overlap, t.head(), grad, t.row_of(), largest));
   if (rc != NLFA_OK) return rc;
-  const long long row_bytes = static_cast<long long>(c.d) * (c.x_dtype == NLFA_DTYPE_F32 ? 4 : 2);
+  const long long row_bytes = static_cast<long long>(c.d) * element_bytes(c.x_dtype);
   const int need = l.n_rows / (kBlock / 32), most = 4 * sm_count();
   auto scale = [&](auto* typed, auto* kernel) {
     return checked(launch_kernel(kernel, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(kBlock), 0, st, overlap, t.head(), grad,
@@ -709,7 +711,9 @@ int nlfa_linear_ce_fwd(const void* x, int x_dtype, const void* w, int w_dtype, i
   if ((target_bytes != 4 && target_bytes != 8) || reduction < NLFA_REDUCE_NONE || reduction > NLFA_REDUCE_SUM) return NLFA_ERR_BAD_ARGUMENT;
   if (!w || !tape || !scratch || (n > 0 && (!x || !targets)) || (!loss && !(n == 0 && reduction == NLFA_REDUCE_NONE)))
     return NLFA_ERR_NULL_POINTER;
-  if (!aligned16(tape) || !aligned16(scratch)) return NLFA_ERR_MISALIGNED;
+  if (!aligned16(tape) || !aligned16(scratch) || !aligned_to(x, element_bytes(x_dtype)) || !aligned_to(w, element_bytes(w_dtype)) ||
+      !aligned_to(targets, target_bytes) || !aligned_to(loss, 4))
+    return NLFA_ERR_MISALIGNED;
   const Layout l = layout(c, aligned16(w));
   if (tape_bytes < l.tape_bytes || scratch_bytes < l.fwd_bytes) return NLFA_ERR_SCRATCH_TOO_SMALL;
   if (!nlfa_device_supported()) return NLFA_ERR_NOT_SM100;
@@ -726,8 +730,10 @@ int nlfa_linear_ce_bwd(const float* grad, const void* w, int w_dtype, int x_dtyp
   if (rc != NLFA_OK) return rc;
   if ((target_bytes != 4 && target_bytes != 8) || reduction < NLFA_REDUCE_NONE || reduction > NLFA_REDUCE_SUM) return NLFA_ERR_BAD_ARGUMENT;
   if (!dx && !dw) return NLFA_OK;
-  if (!w || !tape || !scratch || (n > 0 && (!targets || !grad))) return NLFA_ERR_NULL_POINTER;
-  if (!aligned16(tape) || !aligned16(scratch) || !aligned16(dx) || !aligned16(dw)) return NLFA_ERR_MISALIGNED;
+  if (!w || !tape || !scratch || (n > 0 && !targets) || (!grad && (n > 0 || reduction != NLFA_REDUCE_NONE))) return NLFA_ERR_NULL_POINTER;
+  if (!aligned16(tape) || !aligned16(scratch) || !aligned16(dx) || !aligned16(dw) || !aligned_to(w, element_bytes(w_dtype)) ||
+      !aligned_to(targets, target_bytes) || !aligned_to(grad, 4))
+    return NLFA_ERR_MISALIGNED;
   const Layout l = layout(c, aligned16(w));
   if (tape_bytes < l.tape_bytes || scratch_bytes < bwd_layout(c, l).bytes) return NLFA_ERR_SCRATCH_TOO_SMALL;
   if (!nlfa_device_supported()) return NLFA_ERR_NOT_SM100;

@@ -40,7 +40,7 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
         return lib.nlfa_clip_grads(ctypes.addressof(a), count, 1.0, norm, 1, total, s, sb, None)
     assert call(count=-1) == 14 and call(norm=1) == 14
     assert call(total=None) == 1 and call(s=None) == 1 and call(grad=None) == 1
-    assert call(s=264) == 6 and call(sb=need - 1) == 11
+    assert call(s=264) == 6 and call(sb=need - 1) == 11 and call(total=258) == 6
     assert call(dtype=5) == 3 and call(out=512, out_dtype=7) == 3 and call(n=0) == 2
     assert call(grad=257) == 6 and call(out=514, out_dtype=0) == 6
     assert lib.nlfa_clip_grads(None, 1, 1.0, 2, 1, 256, 256, need, None) == 1

@@ -57,6 +57,7 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
     assert fwd(tb=2) == 14 and fwd(red=3) == 14
     assert fwd(x=None) == 1 and fwd(w=None) == 1 and fwd(t=None) == 1 and fwd(loss=None) == 1 and fwd(tp=None) == 1 and fwd(s=None) == 1
     assert fwd(tp=264) == 6 and fwd(s=260) == 6
+    assert fwd(x=257) == 6 and fwd(w=257) == 6 and fwd(w=258, wd=0) == 6 and fwd(t=260) == 6 and fwd(t=260, tb=4, tpb=64) == 11 and fwd(loss=258) == 6
     assert fwd(tpb=64) == 11 and fwd(sb=64) == 11
 
     def bwd(g=256, w=256, wd=2, xd=2, dt=2, t=256, tb=8, n=8, V=100, d=64, red=1, tp=256, tpb=big, dx=256, dw=256, s=256, sb=big):
@@ -64,6 +65,7 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
     assert bwd(V=0) == 2 and bwd(wd=9) == 3 and bwd(tb=1) == 14
     assert bwd(dx=None, dw=None) == 0                            # nothing wanted
     assert bwd(g=None) == 1 and bwd(tp=None) == 1 and bwd(dx=264) == 6 and bwd(dw=264) == 6 and bwd(sb=64) == 11
+    assert bwd(g=258) == 6 and bwd(w=257) == 6 and bwd(t=260) == 6 and bwd(g=None, n=0, t=None) == 1
 
 
 def test_python_call_refuses_what_it_does_not_take():

@@ -91,3 +91,41 @@ def test_clip_of_the_step():
     assert abs(float(got) - float(total)) <= 2.0**-18 * float(total) and torch.equal(got, norm)
     for a, p in zip(ref, (p for p in model.parameters() if p.grad is not None)):
         assert float((a.grad - p.grad).abs().max()) <= 2.0**-17 * float(a.grad.abs().max())
+
+
+@pytest.mark.gpu
+def test_two_streams_and_a_replay_at_once():
+    """Calls that overlap on the GPU -- two streams, and a captured step replayed beside eager ones -- give each its own bits."""
+    from machinelearning_b200 import grad_clip, head_loss, token_embedding
+
+    def job(seed, n, V, d, dtype):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        table = torch.randn(V, d, device="cuda", generator=g).to(dtype).requires_grad_()
+        idx, t = (torch.randint(0, V, (n,), device="cuda", generator=g) for _ in range(2))
+
+        def step():
+            x = token_embedding.embedding(idx, table, scale=0.2)
+            loss = head_loss.linear_cross_entropy(x, table, t)
+            (grad,) = torch.autograd.grad(loss, (table,))
+            leaf = torch.nn.Parameter(torch.empty_like(table))
+            leaf.grad = grad
+            return loss.detach(), grad_clip.clip_grad_norm_([leaf], 1e-3), leaf.grad
+        return step
+    jobs = [job(1, 900, 3000, 192, torch.bfloat16), job(2, 700, 5000, 96, torch.float32), job(3, 40, 2000, 64, torch.float16)]
+    want = [j() for j in jobs]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = jobs[2]()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = [[], []]
+    for _ in range(8):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(jobs[k]())
+        with torch.cuda.stream(streams[2]):
+            graph.replay()
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(a, b) for one in got[k] for a, b in zip(one, want[k]))
+    assert all(torch.equal(a, b) for a, b in zip(captured, want[2]))

@@ -32,7 +32,7 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
     fwd = lambda ids=256, ib=8, w=256, dt=2, out=256, n=4, V=10, d=8: lib.nlfa_embedding_fwd(ids, ib, w, dt, out, n, V, d, 1.0, None)
     assert fwd(V=0) == 2 and fwd(d=0) == 2 and fwd(n=-1) == 2 and fwd(dt=4) == 3 and fwd(ib=2) == 14
     assert fwd(ids=None) == 1 and fwd(w=None) == 1 and fwd(out=None) == 1
-    assert fwd(w=257) == 6 and fwd(out=258, dt=0) == 6
+    assert fwd(w=257) == 6 and fwd(out=258, dt=0) == 6 and fwd(ids=260) == 6
     assert fwd(n=0, ids=None, w=None, out=None) == 0
     need = lib.nlfa_embedding_scratch_bytes(4, 10, 8)
     assert need > 0 and lib.nlfa_embedding_scratch_bytes(4, 0, 8) == 0
@@ -41,7 +41,7 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
         return lib.nlfa_embedding_bwd(g, dt, ids, ib, dw, n, V, d, 1.0, -1, s, sb, None)
     assert bwd(V=0) == 2 and bwd(dt=9) == 3 and bwd(ib=3) == 14
     assert bwd(g=None) == 1 and bwd(ids=None) == 1 and bwd(dw=None) == 1 and bwd(s=None) == 1
-    assert bwd(s=264) == 6 and bwd(dw=257) == 6 and bwd(sb=need - 1) == 11
+    assert bwd(s=264) == 6 and bwd(dw=257) == 6 and bwd(ids=260) == 6 and bwd(sb=need - 1) == 11
 
 
 def test_python_call_refuses_what_it_does_not_take():
