@@ -294,6 +294,14 @@ fold_kernel(const Params p, int pairs) {
   out.put(t.m0 + r, t.n0 + cc, v);
 }
 
+// exp(x) - 1 for x <= 0: near 0 -- a token the model is sure of -- by its series (six terms, off by x^6 / 5040: 5e-8 at 1/4), elsewhere
+// as the difference (1.2e-7 of 0.22).  1,000 x 5,003 x 384 in float32, the gradient of the logits: 51 us, 53.5 with expm1f and 44.6
+// with the difference alone, whose p - 1 loses all digits of a sure token's gradient (three parts: the registers are used up).
+__device__ __forceinline__ float less_one(float x) {
+  const float series = x * fmaf(x * 0.5f, fmaf(x * (1.f / 3.f), fmaf(x * 0.25f, fmaf(x * 0.2f, fmaf(x, 1.f / 6.f, 1.f), 1.f), 1.f), 1.f), 1.f);
+  return x > -0.25f ? series : fast_exp2(x * kLog2e) - 1.f;
+}
+
 // ---- epilogues: a thread has row `lane` of its warp's 32 and, 32 at a time, 128 columns
 
 // The columns of a thread's row: in TMEM, or (LONG) summed from the chunks' sums in registers.
@@ -581,6 +589,14 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
             const int col = c0 + 64 * c2 + 32 * h;
             uint32_t r[32];
             l.get(64 * c2 + 32 * h, r);
+            const unsigned at = static_cast<unsigned>(target - col);
+            const bool hit = __any_sync(0xffffffffu, at < 32u);
+            float top = 0.f;                                   // the target's logit, taken before r's registers are needed
+            if (hit) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (at == static_cast<unsigned>(j)) top = __uint_as_float(r[j]);
+            }
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
               float a, b;
@@ -593,14 +609,8 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
               for (int j = 0; j < 32; ++j)
                 if (col + j >= p.V) lo[h][j] = 0.f;
             }
-            const unsigned at = static_cast<unsigned>(target - col);
-            if (__any_sync(0xffffffffu, at < 32u)) {
-              float top = 0.f;                                 // the target's logit
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (at == static_cast<unsigned>(j)) top = __uint_as_float(r[j]);
-              // (p - 1 of a token the model is sure of: not by a difference)
-              const float v = expm1f((top - lse) - rest) * scale;
+            if (hit) {
+              const float v = less_one((top - lse) - rest) * scale;
 #pragma unroll
               for (int j = 0; j < 32; ++j)
                 if (at == static_cast<unsigned>(j)) lo[h][j] = v;
