@@ -445,6 +445,47 @@ struct TokenEmbeddingBackward : public Node {
 
 // ------------------------------------------------------------------------------------------- gradient clip
 
+struct Span {
+  uintptr_t from, to;
+  size_t of;
+};
+
+// A tensor's runs of elements without gaps, one Span each.
+void runs_of(const Tensor& t, size_t of, std::vector<Span>& spans) {
+  const int64_t size = t.element_size();
+  std::vector<std::pair<int64_t, int64_t>> dims;                       // (stride, size), the smallest stride first
+  for (int64_t k = 0; k < t.dim(); ++k)
+    if (t.size(k) > 1) dims.emplace_back(t.stride(k), t.size(k));
+  std::sort(dims.begin(), dims.end());
+  size_t outer = 0;
+  int64_t run = 1;
+  for (; outer < dims.size() && dims[outer].first == run; ++outer) run *= dims[outer].second;
+  std::vector<int64_t> at(dims.size(), 0);
+  const uintptr_t base = reinterpret_cast<uintptr_t>(t.data_ptr());
+  int64_t from = 0;
+  for (;;) {
+    const uintptr_t start = base + static_cast<uintptr_t>(from * size);
+    spans.push_back({start, start + static_cast<uintptr_t>(run * size), of});
+    size_t k = outer;
+    for (; k < dims.size(); ++k) {
+      from += dims[k].first;
+      if (++at[k] < dims[k].second) break;
+      from -= dims[k].first * dims[k].second;
+      at[k] = 0;
+    }
+    if (k == dims.size()) return;
+  }
+}
+
+// Of two Spans that share memory the second in the order of addresses, nullptr if none do; sorts them.
+const Span* shared(std::vector<Span>& spans) {
+  const auto first = [](const Span& a, const Span& b) { return a.from < b.from; };
+  if (!std::is_sorted(spans.begin(), spans.end(), first)) std::sort(spans.begin(), spans.end(), first);
+  for (size_t i = 1; i < spans.size(); ++i)
+    if (spans[i].from < spans[i - 1].to) return &spans[i];
+  return nullptr;
+}
+
 // Norm of the tensors, and their clip: see grad_clip.py, which documents the refusals.  A model has hundreds of gradients, and the
 // kernels take 10 us per 50 MB of them: what is done per tensor is kept to reads of its fields.
 Tensor clip_grads(const std::vector<const Tensor*>& grads, const std::vector<const Tensor*>& outs, double max_norm, int norm, bool scale) {
@@ -454,11 +495,8 @@ Tensor clip_grads(const std::vector<const Tensor*>& grads, const std::vector<con
   std::vector<nlfa_grad> table;
   std::vector<Tensor> held;                                            // copies the launches read
   std::vector<std::pair<const Tensor*, Tensor>> back;                  // (gradient with gaps, its copy)
-  struct Span {
-    uintptr_t from, to;
-    size_t of;
-  };
   std::vector<Span> spans;
+  std::vector<size_t> gapped;                                          // whose Span, from end to end, holds gaps
   table.reserve(grads.size());
   spans.reserve(grads.size() + outs.size());
   auto takes = [&](const Tensor& t) {
@@ -469,6 +507,13 @@ Tensor clip_grads(const std::vector<const Tensor*>& grads, const std::vector<con
   auto span = [&](const Tensor& t, size_t i) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
     spans.push_back({at, at + static_cast<uintptr_t>(t.numel()) * t.element_size(), i});
+  };
+  auto span_with_gaps = [&](const Tensor& t, size_t i) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    int64_t last = 0;
+    for (int64_t k = 0; k < t.dim(); ++k) last += (t.size(k) - 1) * t.stride(k);
+    spans.push_back({at, at + static_cast<uintptr_t>(last + 1) * t.element_size(), i});
+    gapped.push_back(i);
   };
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor& given = *grads[i];
@@ -497,6 +542,7 @@ Tensor clip_grads(const std::vector<const Tensor*>& grads, const std::vector<con
       if (scale) {
         TORCH_CHECK_VALUE(at::has_internal_overlap(given) != at::MemOverlap::Yes, "gradient ", i, " has elements that share memory");
         back.emplace_back(&given, held.back());
+        span_with_gaps(given, i);
       }
     }
     if (given.numel() == 0) continue;
@@ -504,11 +550,15 @@ Tensor clip_grads(const std::vector<const Tensor*>& grads, const std::vector<con
     table.push_back({from, to, given.numel(), dtype, out_dtype});
   }
   if (scale) {
-    const auto first = [](const Span& a, const Span& b) { return a.from < b.from; };
-    if (!std::is_sorted(spans.begin(), spans.end(), first)) std::sort(spans.begin(), spans.end(), first);
-    for (size_t i = 1; i < spans.size(); ++i)
-      TORCH_CHECK_VALUE(spans[i].from >= spans[i - 1].to, "tensors ", spans[i - 1].of, " and ", spans[i].of,
-                        " share memory (a parameter given twice?)");
+    const Span* found = shared(spans);
+    if (found != nullptr && !gapped.empty()) {                         // (they may only lie between one another's elements)
+      spans.erase(std::remove_if(spans.begin(), spans.end(), [&](const Span& x) {
+        return std::binary_search(gapped.begin(), gapped.end(), x.of);
+      }), spans.end());
+      for (size_t i : gapped) runs_of(*grads[i], i, spans);
+      found = shared(spans);
+    }
+    TORCH_CHECK_VALUE(found == nullptr, "tensors ", found[-1].of, " and ", found->of, " share memory (a parameter given twice?)");
   }
   Tensor total = empty({}, at::kFloat, like);
   Tensor scratch = empty({static_cast<int64_t>(nlfa_clip_scratch_bytes())}, at::kByte, like);

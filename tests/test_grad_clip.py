@@ -217,6 +217,33 @@ def test_layouts_and_refusals():
 
 
 @pytest.mark.gpu
+def test_gradients_with_gaps_that_share_memory():
+    """Refused as dense ones are; gradients that lie in one another's gaps are taken."""
+    from machinelearning_b200 import grad_clip
+
+    def clip(*views):
+        ps = [torch.nn.Parameter(torch.zeros(v.shape, device="cuda")) for v in views]
+        for p, v in zip(ps, views):
+            p.grad = v
+        return grad_clip.clip_grad_norm_(ps, 0.1)
+
+    wide = torch.randn(6, 20, 4, device="cuda", generator=torch.Generator(device="cuda").manual_seed(0))
+    rest = wide.clone()
+    left = wide[:, 3:11]
+    for views in ((left, left), (left, wide[:, 10:15]), (wide[:, 12:], left, wide[4]), (wide[2, 3:5], left), (wide[:, ::2], wide[:, ::3]),
+                  (wide[:, :, 1], wide[3, 7:8])):
+        with pytest.raises(ValueError, match="share memory"):
+            clip(*views)
+    assert torch.equal(wide, rest)
+    for views in ((left, wide[:, 11:], wide[:, :3]), (wide[:, ::2], wide[:, 1::2]), (wide[2, 11:15], left, wide[5, 11]),
+                  (wide[..., 0], wide[..., 2], wide[..., 3])):
+        before = [v.clone() for v in views]
+        total = clip(*views)
+        _check(before, views, total, 0.1)
+        wide.copy_(rest)
+
+
+@pytest.mark.gpu
 def test_reproducible_captured_and_on_another_stream():
     from machinelearning_b200 import grad_clip
     ps = _params([(300, 400), (4097,), (9,)], [torch.float32])
