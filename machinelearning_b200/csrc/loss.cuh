@@ -29,7 +29,7 @@ struct Layout {
   int d_pad;                        // row length of the 16-bit copies, a multiple of 64
   int x_planes;                     // 16-bit parts of an operand: 1, or 3 for float32
   bool copy_w;                      // the weight is converted or re-laid (otherwise the products read the caller's)
-  size_t row_of, target, lse, lse_rest, x, w, tape_bytes;
+  size_t row_of, target, lse, lse_rest, own, x, w, tape_bytes;
   int max_splits;
   size_t partial, at_target, sums, ticket, fwd_bytes;
   int max_parts;                    // (maximum, sum) pairs per row
@@ -51,6 +51,7 @@ struct Params {
   const int* target;
   // gradient of the logits
   const float *lse, *lse_rest;      // lse + lse_rest: to better than float32
+  const float* own;                 // p - 1 of the row's target
   const float* row_scale;
   // products with it: dx [N, d] by row_of, dw [V, d]
   const int* row_of;

@@ -294,14 +294,6 @@ fold_kernel(const Params p, int pairs) {
   out.put(t.m0 + r, t.n0 + cc, v);
 }
 
-// exp(x) - 1 for x <= 0: near 0 -- a token the model is sure of -- by its series (six terms, off by x^6 / 5040: 5e-8 at 1/4), elsewhere
-// as the difference (1.2e-7 of 0.22).  1,000 x 5,003 x 384 in float32, the gradient of the logits: 51 us, 53.5 with expm1f and 44.6
-// with the difference alone, whose p - 1 loses all digits of a sure token's gradient (three parts: the registers are used up).
-__device__ __forceinline__ float less_one(float x) {
-  const float series = x * fmaf(x * 0.5f, fmaf(x * (1.f / 3.f), fmaf(x * 0.25f, fmaf(x * 0.2f, fmaf(x, 1.f / 6.f, 1.f), 1.f), 1.f), 1.f), 1.f);
-  return x > -0.25f ? series : fast_exp2(x * kLog2e) - 1.f;
-}
-
 // ---- epilogues: a thread has row `lane` of its warp's 32 and, 32 at a time, 128 columns
 
 // The columns of a thread's row: in TMEM, or (LONG) summed from the chunks' sums in registers.
@@ -490,12 +482,13 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
     while (walk.next(t)) {
       const int row0 = t.m0 + 128 * rank + 32 * q, row = row0 + lane;
       int target = -1;
-      float lse = 0.f, rest = 0.f, scale = 0.f;
+      float lse = 0.f, rest2 = 0.f, scale = 0.f, own = 0.f;
       if (MODE == kLse || MODE == kGrad) target = p.target[row];
       if (MODE == kGrad) {
         lse = p.lse[row];
-        rest = p.lse_rest[row];
+        rest2 = p.lse_rest[row] * kLog2e;
         scale = p.row_scale[row];
+        own = p.own[row] * scale;                              // dl of the row's target
       }
       if (MODE == kLse && t.first) { run_max = -INFINITY; run_sum = 0.f; }
       int buf = 0;
@@ -589,19 +582,11 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
             const int col = c0 + 64 * c2 + 32 * h;
             uint32_t r[32];
             l.get(64 * c2 + 32 * h, r);
-            const unsigned at = static_cast<unsigned>(target - col);
-            const bool hit = __any_sync(0xffffffffu, at < 32u);
-            float top = 0.f;                                   // the target's logit, taken before r's registers are needed
-            if (hit) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (at == static_cast<unsigned>(j)) top = __uint_as_float(r[j]);
-            }
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
               float a, b;
               unpack_f2(ffma2(fadd2(pack_f2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), pack_f2(-lse, -lse)),
-                              pack_f2(kLog2e, kLog2e), pack_f2(-rest * kLog2e, -rest * kLog2e)), a, b);
+                              pack_f2(kLog2e, kLog2e), pack_f2(-rest2, -rest2)), a, b);
               unpack_f2(fmul2(pack_f2(fast_exp2(a), fast_exp2(b)), pack_f2(scale, scale)), lo[h][j], lo[h][j + 1]);
             }
             if (col + 32 > p.V) {
@@ -609,11 +594,13 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
               for (int j = 0; j < 32; ++j)
                 if (col + j >= p.V) lo[h][j] = 0.f;
             }
-            if (hit) {
-              const float v = less_one((top - lse) - rest) * scale;
+            const unsigned at = static_cast<unsigned>(target - col);
+            // (three parts leave no registers: written as a product and sum the kernel takes 44.1 us, as a choice 48.7, at 1,000 x 5,003 x
+            // 384; one part: 11.48 and 11.26 ms, the backward of 65,536 x 50,304 x 768.  p is finite unless own is NaN too)
+            if (__any_sync(0xffffffffu, at < 32u)) {
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                if (at == static_cast<unsigned>(j)) lo[h][j] = v;
+                if (at == static_cast<unsigned>(j)) lo[h][j] = PARTS == 3 ? fmaf(lo[h][j], 0.f, own) : own;
             }
             if (__any_sync(0xffffffffu, target == -1)) {     // behind the last row: zeros, whatever W holds (0 inf would not be)
 #pragma unroll
