@@ -556,6 +556,21 @@ Params params(const Call& c, const Layout& l, const Pointers& t, unsigned* statu
   return p;
 }
 
+// Stages per chain of the tensor core (loss_tc.cu) where logits are formed, in the forward and again in the backward: exp(l - lse) would
+// show any difference between the two.  Chains of 64 summands for float32, of 384 for few rows (whose losses are not averaged; 26.1 us
+// with one chain, 27.6 so, 29.5 with 256, for 8 rows of 50,304 x 768), else of up to 1,024.
+int logit_chain(const Call& c, const Layout& l) {
+  return l.x_planes == 3 ? 1 : c.n <= kFewRows ? (c.d > 384 ? 3 : 0) : c.d > 1024 ? 8 : 0;
+}
+// ... and in the products with dl, whose sums run over rows or words without end.  Where dl is held in one part its roundings leave 2^-8 / sqrt(3)
+// (bf16; 2^-11 in fp16) over sqrt(4,096) of a sum of as many values of one sign, 3.5e-5 (4.4e-6): a chain of 4,096 summands, low by 1.1e-5,
+// hides under that, in fp16 one of 2,048.  In two parts nothing hides it: 1,024.  (65,536 x 50,304 x 768, forward and backward: 16.05 ms with one chain
+// however long, 16.25 with 4,096; 16.7 with 2,048; 17.1 with 1,024: adding costs power.
+// One chain over a piece of 131,072 words of one sign left dx low by 8.5e-5.)
+int product_chain(const Layout& l, int dl_planes, int dtype) {
+  return l.x_planes == 3 ? 1 : dl_planes == 2 ? 8 : dtype == NLFA_DTYPE_F16 ? 16 : 32;
+}
+
 int run_fwd(const Call& c, const void* x, const void* w, const void* targets, int target_bytes, long long ignore, int reduction,
             float* out, uint8_t* tape, uint8_t* scratch, cudaStream_t st) {
   const Layout l = layout(c, aligned16(w));
@@ -601,9 +616,7 @@ int run_fwd(const Call& c, const void* x, const void* w, const void* targets, in
   if (rc == NLFA_OK) rc = column_map(&mw, l.copy_w ? tape + l.w : w, dtype, l.d_pad, c.V, l.x_planes, l.copy_w);
   if (rc != NLFA_OK) return rc;
   Params p = params(c, l, t, status);
-  // chains of 64 summands for float32, of 384 for few rows (whose losses are not averaged; 26.1 us with one chain, 27.6
-  // so, 29.5 with 256, for 8 rows of 50,304 x 768), else of up to 1,024
-  p.chunk = l.x_planes == 3 ? 1 : few ? (c.d > 384 ? 3 : 0) : c.d > 1024 ? 8 : 0;
+  p.chunk = logit_chain(c, l);
   p.partial = reinterpret_cast<float2*>(scratch + l.partial);
   p.w_stands = l.copy_w ? 0 : 1;
   p.at_target = at_target;
@@ -665,7 +678,6 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
   if (rc == NLFA_OK) rc = box_map(&out, scratch + b.dl, dtype, b.piece, l.n_rows, dl_planes, 32, 1, 1, true);
   if (rc != NLFA_OK) return rc;
   Params p = params(c, l, t, status);
-  p.chunk = l.x_planes == 3 ? 1 : 0;
   p.dl_planes = dl_planes;
   p.row_scale = row_scale;
   p.alpha = alpha;
@@ -683,7 +695,9 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
     p.v1 = c.V - v < b.piece ? c.V : v + b.piece;
     p.first = v == 0;
     p.last = p.v1 == c.V;
+    p.chunk = logit_chain(c, l);
     rc = launch_product(kGrad, dtype, p, x_columns, w_columns, out, out, st);
+    p.chunk = product_chain(l, dl_planes, dtype);
     if (rc == NLFA_OK) rc = launch_product(kProducts, dtype, p, x_rows, w_rows, dl_columns, dl_rows, st);
     if (rc != NLFA_OK) return rc;
   }

@@ -41,7 +41,7 @@ struct Params {
   int V, d, d_pad;
   int planes;                       // parts of an operand: 1 or 3
   int dl_planes;                    // parts of dl: 1, 3 with operands in three, or 2 where gradients are sums of few rows (loss.cu)
-  int chunk;                        // stages per chain of the tensor core (0: the whole sum)
+  int chunk;                        // stages per chain of the tensor core (0: the whole sum; kProducts: never)
   int v0, v1;                       // piece of the vocabulary
   int n_rows;
   int w_stands;                     // kFew: w is the caller's, not a copy made by the launch before

@@ -505,7 +505,9 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
             tmem_ld32(tmem_addr(tmem, 32 * q, buf * kColTile + kCols * half + 32 * c), r);
             tc_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) l.v[32 * c + j] += __uint_as_float(r[j]);
+            for (int j = 0; j < 32; j += 2)
+              unpack_f2(fadd2(pack_f2(l.v[32 * c + j], l.v[32 * c + j + 1]), pack_f2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]))),
+                        l.v[32 * c + j], l.v[32 * c + j + 1]);
           }
           release(buf);
         }
@@ -753,8 +755,9 @@ int launch_product(int mode, int dtype, const Params& p, const CUtensorMap& x, c
   if (mode == kFew) return bf16 ? NLFA_GO(__nv_bfloat16, kFew, false) : NLFA_GO(__half, kFew, false);
   if (mode == kLse && p.chunk > 0) return bf16 ? NLFA_GO(__nv_bfloat16, kLse, true) : NLFA_GO(__half, kLse, true);
   if (mode == kLse) return bf16 ? NLFA_GO(__nv_bfloat16, kLse, false) : NLFA_GO(__half, kLse, false);
+  if (mode == kGrad && p.chunk > 0) return bf16 ? NLFA_GO(__nv_bfloat16, kGrad, true) : NLFA_GO(__half, kGrad, true);
   if (mode == kGrad) return bf16 ? NLFA_GO(__nv_bfloat16, kGrad, false) : NLFA_GO(__half, kGrad, false);
-  return bf16 ? NLFA_GO(__nv_bfloat16, kProducts, false) : NLFA_GO(__half, kProducts, false);
+  return bf16 ? NLFA_GO(__nv_bfloat16, kProducts, true) : NLFA_GO(__half, kProducts, true);
 #undef NLFA_GO
 }
 
