@@ -235,10 +235,10 @@ pack_few_kernel(const I* __restrict__ targets, int n, int V, long long ignore, H
 
 // ------------------------------------------------------------------------------------------------ losses
 
-// (max, sum) of a row's parts -> lse, loss, and own = p - 1 of the target as exp(-loss) - 1: as a difference a sure token's gradient would
-// lose its digits.  (Here, not where dl is formed: expm1 in that epilogue, which has no registers left, made it 44.6 -> 53.5 us at 1,000 x
-// 5,003 x 384 in float32.)  Rows behind the last one get lse = +inf: their probabilities are zero.  `lanes` threads per row (a power of
-// two up to 32): few rows have many parts.
+// (max, sum) of a row's parts, the target left out of them, and the target's logit t -> lse, loss, and own = p - 1 of the target.  With
+// e = sum_{v != t} exp(l_v - t):  lse = t + log(1 + e),  loss = log(1 + e),  own = -e / (1 + e).  (A sum that held the target's own 1 would keep
+// of e what 2^-24 leaves: at e = 1e-7 own would be off by a fifth, and at 5e-8 nothing would be left of it.)  Rows behind the last one get
+// lse = +inf: their probabilities are zero.  `lanes` threads per row (a power of two up to 32): few rows have many parts.
 __global__ void __launch_bounds__(kBlock)
 finish_kernel(const Head* head, const float2* __restrict__ partial, const float* __restrict__ at_target, const int* __restrict__ row_of,
               int n_rows, float* __restrict__ lse, float* __restrict__ lse_rest, float* __restrict__ own, float* __restrict__ each, float* __restrict__ out, double* sums,
@@ -271,15 +271,29 @@ finish_kernel(const Head* head, const float2* __restrict__ partial, const float*
     }
     for (int off = lanes / 2; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
     if (mine != 0) continue;
-    const float rest = logf(total), whole = shift + rest;
-    lse[r] = live ? whole : INFINITY;
-    lse_rest[r] = live ? rest - (whole - shift) : 0.f;    // (NaN where lse is not finite)
     if (!live) {
-      own[r] = 0.f;
+      lse[r] = INFINITY;
+      lse_rest[r] = own[r] = 0.f;
       continue;
     }
-    const float loss = (shift - at_target[r]) + rest;
-    own[r] = expm1f(-loss);
+    const float t = at_target[r];
+    float base = t, rest, loss, p_less_1;
+    if (t > top) {
+      const float e = total * expf(top - t), bad = t - t;   // (a logit of +inf: NaN, as its softmax is)
+      rest = log1pf(e);
+      loss = rest + bad;
+      p_less_1 = -e / (1.f + e) + bad;
+    } else {
+      const float with_t = total + expf(t - top);
+      base = top;
+      rest = logf(with_t);
+      loss = (top - t) + rest;
+      p_less_1 = -total / with_t;
+    }
+    const float whole = base + rest;
+    lse[r] = whole;
+    lse_rest[r] = rest - (whole - base);                   // (NaN where lse is not finite)
+    own[r] = p_less_1;
     if (each != nullptr) each[row_of[r]] = loss;
     sum += loss;
   }

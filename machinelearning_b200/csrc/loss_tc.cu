@@ -1,5 +1,6 @@
 // The products of the linear cross entropy (loss.cu) on the tensor cores:
-//   kLse       l = x W^T, of which only each row's running maximum and sum of exponentials leave the SM, and the target's l;
+//   kLse       l = x W^T, of which only each row's running maximum and sum of exponentials, both without the target's, leave the SM, and
+//              the target's l;
 //   kGrad      l again for a piece of the vocabulary, dl = r (exp(l - lse) - [v == target]), written in 16 bits;
 //   kProducts  dx (+)= dl W and dW = dl^T x of that piece, both in one launch;
 //   kFew       kLse of up to 64 rows with the operands exchanged: l^T = W x^T, 256 words x 64 rows a tile.
@@ -527,8 +528,11 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
           if (kMine * half + j >= walk.rows) break;
-          const float x = row < p.V ? __uint_as_float(r[j]) : -INFINITY;
-          if (__shfl_sync(0xffffffffu, few_target, j) == row) p.at_target[kMine * half + j] = x;
+          float x = row < p.V ? __uint_as_float(r[j]) : -INFINITY;
+          if (__shfl_sync(0xffffffffu, few_target, j) == row) {
+            p.at_target[kMine * half + j] = x;
+            x = -INFINITY;
+          }
           const float top = fmaxf(few_max[j], x);
           few_sum[j] = fmaf(few_sum[j], fast_exp2((few_max[j] - top) * kLog2e), fast_exp2((x - top) * kLog2e));
           few_max[j] = top;
@@ -550,7 +554,10 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
             float v = 0.f;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (at == static_cast<unsigned>(j)) v = __uint_as_float(r[j]);
+              if (at == static_cast<unsigned>(j)) {
+                v = __uint_as_float(r[j]);
+                r[j] = __float_as_uint(-INFINITY);
+              }
             if (at < 32u) p.at_target[row] = v;
           }
           float top = __uint_as_float(r[0]);

@@ -71,3 +71,75 @@ def test_both_passes_form_the_same_logits(dtype, n, V, d):
         loss = head_loss.linear_cross_entropy(xf, wf, t, reduction="sum")
     dx, dw = torch.autograd.grad(loss, (xf, wf))
     _check("fp32", xf, wf, t, loss, dx, dw, "sum", compute=dtype, dl_step=HALF_STEP[dtype] ** 2)
+
+
+MARGINS = [0.0, 1.0, 5.0, 12.0, 15.0, 17.0, 20.0, 25.0, 40.0, 60.0, -3.0, -12.0, -25.0]
+
+
+def _sure(dtype, n, V, target, d=72):
+    """Rows of known logits: x_0 is the margin by which the target's logit lies above the others' (w_0 is 1 for the target, -1/64, 0 or 1/64 for
+    the others).  w_1 is 1 for the target alone and w_2 for the others alone, with x_1 = x_2 = 0: dx_1 is p - 1 of the target, dx_2 the others'
+    sum of p."""
+    w = torch.zeros(V, d, device="cuda")
+    w[:, 0] = (torch.arange(V, device="cuda") % 3 - 1) / 64
+    w[:, 2] = 1
+    w[target, :3] = torch.tensor([1.0, 1.0, 0.0], device="cuda")
+    x = torch.zeros(n, d, device="cuda")
+    x[:, 0] = torch.tensor(MARGINS, device="cuda").repeat(n // len(MARGINS) + 1)[:n]
+    t = torch.full((n,), target, device="cuda")
+    if dtype != "fp32":
+        assert torch.equal(x, x.to(DT[dtype]).float()) and torch.equal(w, w.to(DT[dtype]).float())
+    return x.requires_grad_(), w.requires_grad_(), t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,V,target", [(13, 1000, 0), (13, 1000, 777), (64, 300, 299), (200, 1000, 777), (200, 1, 0), (13, 1, 0), (200, 1000, 999)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_tokens_the_model_is_sure_of(dtype, n, V, target):
+    """Losses and p - 1 down to 1e-26, in relative terms: exp2(z log2 e) with z rounded to half a step is off by |z| 2^-24 twice (product and
+    constant), ex2 and exp by 2^-22 each, sums of 1,000 and their joining by 2^-20, the logarithm and the quotient by 2^-22.  Gradients: u^2 of two parts
+    in 16 bits (u = 2^-8, 2^-11), 2^-24 in float32; in fp16 what lies below 2^-25 2^-14 is lost."""
+    from machinelearning_b200 import head_loss
+    x, w, t = _sure(dtype, n, V, target)
+    with torch.autocast("cuda", dtype=DT[dtype], enabled=dtype != "fp32"):
+        each = head_loss.linear_cross_entropy(x, w, t, reduction="none")
+        total = head_loss.linear_cross_entropy(x, w, t, reduction="sum")
+    (dx,) = torch.autograd.grad(total, x)
+    l = x.detach().double() @ w.detach().double().t()
+    others = torch.cat([l[:, :target], l[:, target + 1:]], 1)
+    e = torch.exp(others - l[:, target:target + 1]).sum(1)       # (margins of up to 60: no overflow)
+    loss, own = torch.log1p(e), -e / (1 + e)
+    z = 2 * x.detach()[:, 0].abs().double() + 2
+    off = 2 * z * 2.0**-24 + 2.0**-20 + 3 * 2.0**-22
+    assert bool(((each.double() - loss).abs() <= off * loss).all())
+    assert abs(float(total.detach().double() - loss.sum())) <= float((off * loss).sum() + 2.0**-24 * loss.sum())
+    held = 2.0**-24 if dtype == "fp32" else HALF_STEP[dtype] ** 2
+    small = 2.0**-39 * V if dtype == "fp16" else 0.0
+    for got, want in ((dx[:, 1], own), (dx[:, 2], -own)):        # (sums of V equal signs: steps of 2^-23 on top)
+        assert bool(((got.double() - want).abs() <= (off + held + 64 * 2.0**-23) * want.abs() + small).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 100])
+@pytest.mark.parametrize("target_logit,other,rest", [
+    (float("inf"), 0.0, 0.0), (-float("inf"), 0.0, 0.0), (0.0, float("inf"), 0.0), (0.0, -float("inf"), 0.0),
+    (0.0, -float("inf"), -float("inf")), (-float("inf"), -float("inf"), -float("inf")), (float("nan"), 0.0, 0.0), (0.0, float("nan"), 0.0)])
+def test_logits_that_are_not_finite(n, target_logit, other, rest):
+    """Losses and gradients of the rows are infinite, NaN or finite where torch's are."""
+    from machinelearning_b200 import head_loss
+    V, d, target = 300, 8, 150
+    w = torch.zeros(V, d, device="cuda", dtype=torch.bfloat16)
+    w[:, 0], w[target, 0], w[7, 0] = rest, target_logit, other
+    x = torch.zeros(n, d, device="cuda", dtype=torch.bfloat16)
+    x[:, 0] = 1
+    x.requires_grad_(), w.requires_grad_()
+    t = torch.full((n,), target, device="cuda")
+    each = head_loss.linear_cross_entropy(x, w, t, reduction="none")
+    logits = w.detach()[:, 0].float().expand(n, V)               # (x W^T without 0 x inf)
+    want = torch.nn.functional.cross_entropy(logits, t, reduction="none")
+    assert torch.allclose(each, want, rtol=2.0**-18, atol=2.0**-18, equal_nan=True)
+    (dw,) = torch.autograd.grad(each.sum(), w)
+    dl = torch.softmax(logits, 1)
+    dl[:, target] -= 1
+    got, dl = dw[:, 0].float(), dl.sum(0)
+    assert torch.equal(got.isnan(), dl.isnan()) and torch.allclose(got.nan_to_num(), dl.nan_to_num(), rtol=2.0**-7, atol=2.0**-7)
