@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kBlock)
 scale_rows_kernel(const Head* head, const float* __restrict__ grad, int per_row, int mean, const int* __restrict__ row_of,
                   const int* __restrict__ target, float* __restrict__ row_scale, float* __restrict__ alpha, Parts* parts, const float* __restrict__ largest,
                   float unit, const I* __restrict__ targets, int n, long long ignore, uint8_t* __restrict__ dx, long long row_bytes, int V,
-                  int d, int piece, int want_dw, int pairs, int planes, int again) {
+                  int d, int piece, int want_dw, int pairs, int planes) {
   grid_dep_wait();
   grid_dep_release();
   const int all = head->count, stride = gridDim.x * kBlock;
@@ -390,6 +390,7 @@ scale_rows_kernel(const Head* head, const float* __restrict__ grad, int per_row,
     *alpha = all > 0 ? g / unit : 0.f;                    // (no target: gradients of zero, not 0 / 0)
   }
   if (blockIdx.x == gridDim.x - 1 && threadIdx.x < 32) {
+    const int again = planes == 1 ? dl_parts(planes, per_row, all) : 1;
     const int k = summands(planes), share = planes == 3 ? 1 : 4;          // (a stage of three parts is three times as long)
     const int d_tiles = (d + kColTile - 1) / kColTile, rest_x = dx != nullptr ? end / kRowTile * d_tiles % pairs : 0;
     for (int last = 0; last < 2; ++last) {
@@ -467,20 +468,16 @@ Layout layout(const Call& c, bool w_aligned) {
 // 1 GiB and with 4: between pieces the GPU runs empty, and dx is summed in memory).
 constexpr size_t kMostDl = 1024ull << 20;
 
-// dl is held in 16 bits.  Its roundings (half a step, 2^-8 in bf16) are independent and largely cancel in sums over many rows or words:
-// gradients of 513 rows are off by 2.2e-3 as a whole, 1.7e-3 of that by their own rounding.  A row's own target has most of its dl,
-// though, and in a sum of a few rows one such rounding shows (3.3e-3 for one row): up to a tile of rows dl is held in two parts, and up
-// to kTwoParts where the rows' gradients differ, so that a few of them can be most of the sum (2.5e-3 for 160 rows).
-constexpr int kTwoParts = 1024;
 struct BwdLayout {
   int piece;                        // columns, a multiple of kColTile
-  int dl_planes;                    // there is room for
+  int dl_rows, dl_second;           // rows of dl's buffer, and where the second part begins if there is one: only the device knows (dl_parts)
   size_t row_scale, alpha, parts, dl, shares, dx_sum, bytes;
 };
 BwdLayout bwd_layout(const Call& c, const Layout& l) {
   BwdLayout b{};
-  b.dl_planes = l.x_planes == 3 ? 3 : c.n <= kTwoParts ? 2 : 1;
-  const size_t column = static_cast<size_t>(b.dl_planes) * l.n_rows * 2;
+  b.dl_second = l.n_rows < kTwoParts ? l.n_rows : kTwoParts;
+  b.dl_rows = l.x_planes == 3 || l.n_rows > 2 * b.dl_second ? l.n_rows : 2 * b.dl_second;
+  const size_t column = static_cast<size_t>(l.x_planes) * b.dl_rows * 2;
   const int col_tiles = (c.V + kColTile - 1) / kColTile;
   size_t most = kMostDl / (column * kColTile);
   if (most < 1) most = 1;
@@ -578,12 +575,10 @@ int logit_chain(const Call& c, const Layout& l) {
 }
 // ... and in the products with dl, whose sums run over rows or words without end.  Where dl is held in one part its roundings leave 2^-8 / sqrt(3)
 // (bf16; 2^-11 in fp16) over sqrt(4,096) of a sum of as many values of one sign, 3.5e-5 (4.4e-6): a chain of 4,096 summands, low by 1.1e-5,
-// hides under that, in fp16 one of 2,048.  In two parts nothing hides it: 1,024.  (65,536 x 50,304 x 768, forward and backward: 16.05 ms with one chain
+// hides under that, in fp16 one of 2,048.  In two parts nothing hides it: 1,024 (loss_tc.cu: Plan).  (65,536 x 50,304 x 768, forward and backward: 16.05 ms with one chain
 // however long, 16.25 with 4,096; 16.7 with 2,048; 17.1 with 1,024: adding costs power.
 // One chain over a piece of 131,072 words of one sign left dx low by 8.5e-5.)
-int product_chain(const Layout& l, int dl_planes, int dtype) {
-  return l.x_planes == 3 ? 1 : dl_planes == 2 ? 8 : dtype == NLFA_DTYPE_F16 ? 16 : 32;
-}
+int product_chain(const Layout& l, int dtype) { return l.x_planes == 3 ? 1 : dtype == NLFA_DTYPE_F16 ? 16 : 32; }
 
 int run_fwd(const Call& c, const void* x, const void* w, const void* targets, int target_bytes, long long ignore, int reduction,
             float* out, uint8_t* tape, uint8_t* scratch, cudaStream_t st) {
@@ -660,7 +655,6 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
   if (!status) return NLFA_ERR_CUDA;
   const int dtype = c.dtype == NLFA_DTYPE_F32 ? NLFA_DTYPE_BF16 : c.dtype;
   const bool overlap = overlap_launches(kOverlapRowwise);
-  const int dl_planes = l.x_planes == 3 ? 3 : c.n <= kRowTile || (reduction == NLFA_REDUCE_NONE && c.n <= kTwoParts) ? 2 : 1;
   float* row_scale = reinterpret_cast<float*>(scratch + b.row_scale);
   float* alpha = reinterpret_cast<float*>(scratch + b.alpha);
   Parts* parts = reinterpret_cast<Parts*>(scratch + b.parts);
@@ -676,7 +670,7 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
     return checked(launch_kernel(kernel, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(kBlock), 0, st, overlap, t.head(), grad,
                                  per_row, reduction == NLFA_REDUCE_MEAN ? 1 : 0, t.row_of(), t.target(), row_scale, alpha, parts, largest,
                                  dtype == NLFA_DTYPE_F16 ? 16384.f : 1.f, typed, c.n, ignore, static_cast<uint8_t*>(dx), row_bytes, c.V, c.d, b.piece, dw != nullptr ? 1 : 0,
-                                 most_pairs(), l.x_planes, l.x_planes == 1 ? dl_planes : 1));
+                                 most_pairs(), l.x_planes));
   };
   rc = target_bytes == 8 ? scale(static_cast<const long long*>(targets), scale_rows_kernel<long long>)
                          : scale(static_cast<const int*>(targets), scale_rows_kernel<int>);
@@ -687,12 +681,13 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
   if (rc == NLFA_OK) rc = column_map(&w_columns, wp, dtype, l.d_pad, c.V, l.x_planes, l.copy_w);
   if (rc == NLFA_OK) rc = row_map(&x_rows, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes);
   if (rc == NLFA_OK) rc = row_map(&w_rows, wp, dtype, l.d_pad, c.V, l.x_planes, l.copy_w);
-  if (rc == NLFA_OK) rc = column_map(&dl_columns, scratch + b.dl, dtype, b.piece, l.n_rows, dl_planes);
-  if (rc == NLFA_OK) rc = row_map(&dl_rows, scratch + b.dl, dtype, b.piece, l.n_rows, dl_planes);
-  if (rc == NLFA_OK) rc = box_map(&out, scratch + b.dl, dtype, b.piece, l.n_rows, dl_planes, 32, 1, 1, true);
+  if (rc == NLFA_OK) rc = column_map(&dl_columns, scratch + b.dl, dtype, b.piece, b.dl_rows, l.x_planes);
+  if (rc == NLFA_OK) rc = row_map(&dl_rows, scratch + b.dl, dtype, b.piece, b.dl_rows, l.x_planes);
+  if (rc == NLFA_OK) rc = box_map(&out, scratch + b.dl, dtype, b.piece, b.dl_rows, l.x_planes, 32, 1, 1, true);
   if (rc != NLFA_OK) return rc;
   Params p = params(c, l, t, status);
-  p.dl_planes = dl_planes;
+  p.per_row = per_row;
+  p.dl_second = b.dl_second;
   p.row_scale = row_scale;
   p.alpha = alpha;
   p.parts = parts;
@@ -711,7 +706,7 @@ int run_bwd(const Call& c, const float* grad, const void* w, const void* targets
     p.last = p.v1 == c.V;
     p.chunk = logit_chain(c, l);
     rc = launch_product(kGrad, dtype, p, x_columns, w_columns, out, out, st);
-    p.chunk = product_chain(l, dl_planes, dtype);
+    p.chunk = product_chain(l, dtype);
     if (rc == NLFA_OK) rc = launch_product(kProducts, dtype, p, x_rows, w_rows, dl_columns, dl_rows, st);
     if (rc != NLFA_OK) return rc;
   }

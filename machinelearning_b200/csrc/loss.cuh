@@ -10,6 +10,14 @@ constexpr int kRowTile = 256;       // rows of a product's tile: two CTAs of 128
 constexpr int kColTile = 256;       // columns of a tile
 // Summands per stage of a product's pipeline: 128, or 64 of operands in three parts.
 __host__ __device__ constexpr int summands(int planes) { return planes == 3 ? 64 : 128; }
+// dl is held in 16 bits.  Its roundings (half a step, 2^-8 in bf16) are independent and largely cancel in sums over many rows or words:
+// gradients of 513 rows are off by 2.2e-3 as a whole, 1.7e-3 of that by their own rounding.  A row's own target has most of its dl,
+// though, and in a sum of a few rows one such rounding shows (3.3e-3 for one row): up to a tile of rows with a target dl is held in two
+// parts, and up to kTwoParts where the rows' gradients differ, so that a few of them can be most of the sum (2.5e-3 for 160 rows).
+constexpr int kTwoParts = 1024;
+__device__ __forceinline__ int dl_parts(int planes, int per_row, int rows) {
+  return planes == 3 ? 3 : rows <= (per_row ? kTwoParts : kRowTile) ? 2 : 1;
+}
 constexpr int kPartsPerPair = 2;    // shares of dW's, and of dx's, odd tiles there is room for, per pair of CTAs
 
 // The forward leaves its tape in one buffer; counts and places, known on the device only, stand first.
@@ -40,8 +48,9 @@ struct Params {
   const Head* head;
   int V, d, d_pad;
   int planes;                       // parts of an operand: 1 or 3
-  int dl_planes;                    // parts of dl: 1, 3 with operands in three, or 2 where gradients are sums of few rows (loss.cu)
-  int chunk;                        // stages per chain of the tensor core (0: the whole sum; kProducts: never)
+  int per_row;                      // a gradient for each row (dl_parts)
+  int dl_second;                    // rows between the first and the second part of dl
+  int chunk;                        // stages per chain of the tensor core (0: the whole sum; kProducts: of dl in one part, or three)
   int v0, v1;                       // piece of the vocabulary
   int n_rows;
   int w_stands;                     // kFew: w is the caller's, not a copy made by the launch before

@@ -81,6 +81,7 @@ struct Tile {
 // better, but every pair then reads summands of its own from HBM: slower than whole tiles at 16,384 rows.)
 struct Plan {
   int d_tiles, kw, kx, again;
+  int chunk;                        // stages per chain
   int dw_whole, dw_rest, dw_parts, dx_whole, dx_rest, dx_parts;
   int u1, u2, u3, u4;               // ends of the four kinds of units
   int dx_slot;                      // dx's first share
@@ -89,7 +90,8 @@ struct Plan {
     const int row_tiles = rows > 0 ? ceil_div(rows, kRowTile) : 1;
     d_tiles = ceil_div(p.d, kColTile);
     const int dw_tiles = p.want_dw ? ceil_div(p.v1 - p.v0, kColTile) * d_tiles : 0, dx_tiles = p.want_dx ? row_tiles * d_tiles : 0;
-    again = p.planes == 1 ? p.dl_planes : 1;
+    again = p.planes == 1 ? dl_parts(p.planes, p.per_row, rows) : 1;
+    chunk = again == 2 ? 8 : p.chunk;                          // (loss.cu: product_chain)
     kw = again * row_tiles * (kRowTile / summands(p.planes));
     kx = again * ceil_div(p.v1 - p.v0, summands(p.planes));
     dw_whole = dw_tiles / pairs * pairs;
@@ -164,6 +166,7 @@ struct Walk {
     }
   }
 
+  __device__ int chunk() const { return MODE == kProducts ? plan.chunk : p.chunk; }
   __device__ bool next(Tile& t) {
     t.k0 = 0;
     if (MODE != kProducts) t.k1 = ceil_div(p.d, summands(p.planes));
@@ -383,8 +386,8 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
       int it = 0;
       bool ok = true;
       const uint32_t full0 = cluster_addr(bar(FULL), 0);       // loads of both CTAs are counted on the even one's
-      auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t full, int row, int col, int plane) {
-        tma_load_4d_pair(dst, map, full, 0, row, col / 64, plane);
+      auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t full, int row, int col) {
+        tma_load_4d_pair(dst, map, full, 0, row, col / 64, 0);
       };
       while (ok && walk.next(t)) {
         const CUtensorMap* ma = MODE == kFew ? &tm_w : MODE != kProducts ? &tm_x : t.dw ? &tm_out : &tm_ds;
@@ -396,12 +399,12 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
           const uint32_t st = base + s * R::kStageBytes, full = full0 + 8u * s;
           if (rank == 0) mbar_arrive_expect_tx(bar(FULL + s), 2 * R::kStageBytes);
           // boxes at (row, block of 64 columns): the sum runs along the columns, or (MN-major) along the rows
-          const int plane = MODE == kProducts && PARTS == 1 ? kb / t.length : 0;
-          const int k = (kb - (plane > 0 ? plane * t.length : 0)) * R::kSummands;
-          if (MODE == kProducts && t.dw) load(st, ma, full, k, a0, plane);
-          else load(st, ma, full, a0, k, plane);
-          if (MODE != kProducts) load(st + R::kOperandBytes, mb, full, b0, k, 0);
-          else load(st + R::kOperandBytes, mb, full, (t.dw ? 0 : p.v0) + k, b0, 0);
+          const bool second = MODE == kProducts && PARTS == 1 && kb >= t.length;            // part of dl
+          const int k = (kb - (second ? t.length : 0)) * R::kSummands, part = second ? p.dl_second : 0;
+          if (MODE == kProducts && t.dw) load(st, ma, full, part + k, a0);
+          else load(st, ma, full, part + a0, k);
+          if (MODE != kProducts) load(st + R::kOperandBytes, mb, full, b0, k);
+          else load(st + R::kOperandBytes, mb, full, (t.dw ? 0 : p.v0) + k, b0);
         }
       }
       // the last loads of this CTA have been consumed before it may leave (after a give-up: have had time to land)
@@ -423,7 +426,7 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
         // 16 summands on: 32 bytes along a row, then the next block of 64 columns; or (MN-major) 16 rows
         constexpr uint32_t kMnBlock = PARTS == 3 ? kBlockBytes / 2 : kBlockBytes;     // (of 64 summands: 64 rows)
         const uint32_t a_lbo = a_mn ? kMnBlock : 16u, b_lbo = b_mn ? kMnBlock : 16u;
-        const int chunk = LONG ? p.chunk : t.k1 - t.k0;
+        const int chunk = LONG ? walk.chunk() : t.k1 - t.k0;
         for (int k0 = t.k0; ok && k0 < t.k1; k0 += chunk, ++sums) {
           const int buf = sums & 1;
           if (!(ok = mbar_wait(bar(ACC_EMPTY + buf), ((sums >> 1) & 1) ^ 1, wctx, 92))) break;
@@ -496,7 +499,7 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
       if constexpr (LONG) {
 #pragma unroll
         for (int j = 0; j < kCols; ++j) l.v[j] = 0.f;
-        for (int k0 = t.k0; k0 < t.k1; k0 += p.chunk, ++sums) {
+        for (int k0 = t.k0; k0 < t.k1; k0 += walk.chunk(), ++sums) {
           buf = sums & 1;
           if (!(ok = mbar_wait(bar(ACC_FULL + buf), (sums >> 1) & 1, wctx, 94))) break;
           tc_fence_after();
@@ -617,7 +620,9 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
                 if (target == -1) lo[h][j] = 0.f;
             }
           }
-          for (int part = 0; part < p.dl_planes; ++part) {
+          const int held = dl_parts(PARTS, p.per_row, walk.rows);
+#pragma unroll 1
+          for (int part = 0; part < held; ++part) {
             if (lane == 0) tma_store_wait_read();
             __syncwarp();
 #pragma unroll
@@ -632,10 +637,10 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_4d(&tm_out, staging, 0, row0, (c0 + 64 * c2 - p.v0) / 64, part);
+              tma_store_4d(&tm_out, staging, 0, row0 + (PARTS == 1 && part > 0 ? p.dl_second : 0), (c0 + 64 * c2 - p.v0) / 64, PARTS == 1 ? 0 : part);
               tma_store_commit();
             }
-            if (part + 1 < p.dl_planes) {
+            if (part + 1 < held) {
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll

@@ -7,7 +7,7 @@ addition is off by at most 2^-23 of the sum of magnitudes.
 import pytest
 import torch
 
-from test_head_loss import DT, HALF_STEP, _check
+from test_head_loss import DT, HALF_STEP, _check, _inputs
 
 
 def _gradients(x, w, t, **kw):
@@ -143,3 +143,27 @@ def test_logits_that_are_not_finite(n, target_logit, other, rest):
     dl[:, target] -= 1
     got, dl = dw[:, 0].float(), dl.sum(0)
     assert torch.equal(got.isnan(), dl.isnan()) and torch.allclose(got.nan_to_num(), dl.nan_to_num(), rtol=2.0**-7, atol=2.0**-7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("reduction,n,kept", [
+    ("mean", 2000, 1), ("sum", 2000, 200), ("sum", 700, 256), ("mean", 5000, 256), ("none", 257, 257), ("none", 1024, 1024), ("none", 1025, 1000),
+    ("none", 1500, 1024), ("none", 6000, 700), ("sum", 1300, 0), ("none", 64, 3)])
+def test_gradients_of_few_rows_in_a_call_of_many(dtype, reduction, n, kept):
+    """What counts is the rows with a target: up to 256 of them, up to 1,024 with a gradient each, hold the gradient of the logits in two parts."""
+    from machinelearning_b200 import head_loss
+    x, w, t = _inputs(dtype, n, 900, 136, seed=n)
+    g = torch.Generator(device="cuda").manual_seed(n)
+    drop = torch.randperm(n, device="cuda", generator=g)[kept:]
+    t[drop] = -1
+    # a few of the rows are most of the sums
+    up = torch.exp2(-8 * torch.rand(n, device="cuda", generator=g)) if reduction == "none" else None
+    xf, wf = x.detach().float().requires_grad_(), w.detach().float().requires_grad_()
+    with torch.autocast("cuda", dtype=DT[dtype]):
+        loss = head_loss.linear_cross_entropy(xf, wf, t, reduction=reduction)
+    dx, dw = torch.autograd.grad(loss, (xf, wf), up)
+    if kept == 0:
+        assert bool((dx == 0).all()) and bool((dw == 0).all())
+        return
+    _check("fp32", xf, wf, t, loss, dx, dw, reduction, up, compute=dtype, dl_step=HALF_STEP[dtype] ** 2)
