@@ -450,12 +450,19 @@ struct Span {
   size_t of;
 };
 
+Span end_to_end(const Tensor& t, size_t of) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
+  int64_t last = 0;
+  for (int64_t k = 0; k < t.dim(); ++k) last += (t.size(k) - 1) * t.stride(k);
+  return {at, at + static_cast<uintptr_t>(last + 1) * t.element_size(), of};
+}
+
 // A tensor's runs of elements without gaps, one Span each.
 void runs_of(const Tensor& t, size_t of, std::vector<Span>& spans) {
   const int64_t size = t.element_size();
   std::vector<std::pair<int64_t, int64_t>> dims;                       // (stride, size), the smallest stride first
   for (int64_t k = 0; k < t.dim(); ++k)
-    if (t.size(k) > 1) dims.emplace_back(t.stride(k), t.size(k));
+    if (t.size(k) > 1 && t.stride(k) != 0) dims.emplace_back(t.stride(k), t.size(k));     // (broadcast: the same memory again)
   std::sort(dims.begin(), dims.end());
   size_t outer = 0;
   int64_t run = 1;
@@ -486,6 +493,21 @@ const Span* shared(std::vector<Span>& spans) {
   return nullptr;
 }
 
+// Of the Spans `written`, which share no memory with one another and are sorted here, one that reaches into a tensor; nullptr if none does.
+const Span* reaches_into(std::vector<Span>& written, const Tensor& t) {
+  std::sort(written.begin(), written.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+  const auto hit = [&](const Span& r) -> const Span* {
+    auto behind = std::lower_bound(written.begin(), written.end(), r.to, [](const Span& w, uintptr_t at) { return w.from < at; });
+    return behind != written.begin() && behind[-1].to > r.from ? &behind[-1] : nullptr;
+  };
+  if (hit(end_to_end(t, 0)) == nullptr) return nullptr;
+  std::vector<Span> runs;
+  runs_of(t, 0, runs);
+  for (const Span& r : runs)
+    if (const Span* w = hit(r)) return w;
+  return nullptr;
+}
+
 // Norm of the tensors, and their clip: see grad_clip.py, which documents the refusals.  A model has hundreds of gradients, and the
 // kernels take 10 us per 50 MB of them: what is done per tensor is kept to reads of its fields.
 Tensor clip_grads(const std::vector<const Tensor*>& grads, const std::vector<const Tensor*>& outs, double max_norm, int norm, bool scale) {
@@ -496,7 +518,7 @@ Tensor clip_grads(const std::vector<const Tensor*>& grads, const std::vector<con
   std::vector<Tensor> held;                                            // copies the launches read
   std::vector<std::pair<const Tensor*, Tensor>> back;                  // (gradient with gaps, its copy)
   std::vector<Span> spans;
-  std::vector<size_t> gapped;                                          // whose Span, from end to end, holds gaps
+  std::vector<size_t> gapped;                                          // whose Span, from end to end, holds gaps; with `out` they have none
   table.reserve(grads.size());
   spans.reserve(grads.size() + outs.size());
   auto takes = [&](const Tensor& t) {
@@ -507,13 +529,6 @@ Tensor clip_grads(const std::vector<const Tensor*>& grads, const std::vector<con
   auto span = [&](const Tensor& t, size_t i) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
     spans.push_back({at, at + static_cast<uintptr_t>(t.numel()) * t.element_size(), i});
-  };
-  auto span_with_gaps = [&](const Tensor& t, size_t i) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
-    int64_t last = 0;
-    for (int64_t k = 0; k < t.dim(); ++k) last += (t.size(k) - 1) * t.stride(k);
-    spans.push_back({at, at + static_cast<uintptr_t>(last + 1) * t.element_size(), i});
-    gapped.push_back(i);
   };
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor& given = *grads[i];
@@ -535,6 +550,7 @@ Tensor clip_grads(const std::vector<const Tensor*>& grads, const std::vector<con
         held.push_back(at::empty_strided(o.sizes(), o.strides(), given.options()).copy_(given.detach()));
         from = held.back().data_ptr();
       }
+      if (given.numel() && !dense) gapped.push_back(i);
       if (given.numel() && !(to == given.data_ptr() && out_dtype == dtype && given.strides() == o.strides())) span(o, i);
     } else if (!dense) {
       held.push_back(given.detach().contiguous());
@@ -542,7 +558,8 @@ Tensor clip_grads(const std::vector<const Tensor*>& grads, const std::vector<con
       if (scale) {
         TORCH_CHECK_VALUE(at::has_internal_overlap(given) != at::MemOverlap::Yes, "gradient ", i, " has elements that share memory");
         back.emplace_back(&given, held.back());
-        span_with_gaps(given, i);
+        spans.push_back(end_to_end(given, i));
+        gapped.push_back(i);
       }
     }
     if (given.numel() == 0) continue;
@@ -551,7 +568,7 @@ Tensor clip_grads(const std::vector<const Tensor*>& grads, const std::vector<con
   }
   if (scale) {
     const Span* found = shared(spans);
-    if (found != nullptr && !gapped.empty()) {                         // (they may only lie between one another's elements)
+    if (found != nullptr && outs.empty() && !gapped.empty()) {                         // (they may only lie between one another's elements)
       spans.erase(std::remove_if(spans.begin(), spans.end(), [&](const Span& x) {
         return std::binary_search(gapped.begin(), gapped.end(), x.of);
       }), spans.end());
@@ -559,6 +576,15 @@ Tensor clip_grads(const std::vector<const Tensor*>& grads, const std::vector<con
       found = shared(spans);
     }
     TORCH_CHECK_VALUE(found == nullptr, "tensors ", found[-1].of, " and ", found->of, " share memory (a parameter given twice?)");
+    if (!outs.empty() && !gapped.empty()) {                            // gradients with gaps are read and stay: no out may lie over one
+      std::vector<Span> written;
+      for (size_t i = 0; i < outs.size(); ++i)
+        if (outs[i]->numel()) written.push_back(end_to_end(*outs[i], i));
+      for (size_t i : gapped) {
+        const Span* over = reaches_into(written, *grads[i]);
+        TORCH_CHECK_VALUE(over == nullptr, "gradient ", i, " and out ", over->of, " share memory");
+      }
+    }
   }
   Tensor total = empty({}, at::kFloat, like);
   Tensor scratch = empty({static_cast<int64_t>(nlfa_clip_scratch_bytes())}, at::kByte, like);
