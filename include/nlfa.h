@@ -322,6 +322,8 @@ int nlfa_fwd_cached_positions(const void* q, const void* k_cache, const void* v_
  * nanolab's `lm_head` and `F.cross_entropy` stand (nanolab/model.py:364-453).  Every extent may be of any size; x and w
  * are contiguous, of x_dtype and w_dtype; `dtype` is what the products run in (the autocast type, say): 16-bit types on
  * the tensor cores, NLFA_DTYPE_F32 on the tensor cores as sums of three bf16 parts.  Sums are float32, and so is `loss`.
+ * Infinities have their softmax in 16 bits.  NLFA_DTYPE_F32 is for finite values below 3.39e38, bf16's largest:
+ * other values have no three parts, and every logit they enter is NaN: a word of -inf makes the losses of all rows NaN, where it has no probability in 16 bits.
  * Targets are int32 or int64 (target_bytes 4 or 8).  A target outside [0, V) that is not ignore_index gives a NaN loss and
  * NaN gradients.  Rows that are ignored cost nothing and reach nothing, whatever they hold; their dx is zero.  With no row left the mean is
  * NaN (0 / 0), the sum 0, the gradients 0.

@@ -34,7 +34,7 @@ constexpr int kBlock = 256;
 template <typename T> __device__ __forceinline__ float load1(const T* p) { return static_cast<float>(*p); }
 
 // Eight columns (from c) of row `from` of src [*, d] (-1: zeros) to row r of dst [planes][d_pad / 64][n_rows][64]; planes = 3: dst = a + b + c,
-// each the nearest bf16 value to what is left.
+// each the nearest bf16 value to what is left (of infinity: NaN; and its products with the other operand's small parts would be NaN whatever was left).
 template <typename S, typename T>
 __device__ __forceinline__ void copy_chunk(const S* __restrict__ src, T* __restrict__ dst, int from, int r, int c, int n_rows, int d, int d_pad,
                                            int planes, int vec) {

@@ -99,6 +99,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     ``"sum"``, or ``"none"`` (the shape of ``targets``, zero where ignored).  The loss is float32; gradients have the
     dtypes of ``x`` and ``weight``.  Under CUDA autocast the products run in the autocast dtype, whatever the tensors'.
     A target outside the vocabulary gives a NaN loss and NaN gradients; rows that are ignored reach nothing, whatever ``x`` holds there.
+    Where the products run in float32, infinities (and values above bf16's largest, 3.39e38) make every logit they enter NaN, also the -inf
+    that masks a word: a word is masked in 16 bits, or left out of ``weight``.
     """
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction must be one of {tuple(REDUCTIONS)}, got {reduction!r}")

@@ -167,3 +167,22 @@ def test_gradients_of_few_rows_in_a_call_of_many(dtype, reduction, n, kept):
         assert bool((dx == 0).all()) and bool((dw == 0).all())
         return
     _check("fp32", xf, wf, t, loss, dx, dw, reduction, up, compute=dtype, dl_step=HALF_STEP[dtype] ** 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [5, 90])
+def test_float32_values_without_three_parts_show_as_nan(n):
+    """Infinities and what rounds to one in bf16: NaN in every logit they enter, no finite number."""
+    from machinelearning_b200 import head_loss
+    x, w, t = _inputs("fp32", n, 200, 24)
+    for bad in (-float("inf"), float("inf"), 3.4e38):
+        w2, x2 = w.detach().clone(), x.detach().clone()
+        w2[7, 3], x2[2, 5] = bad, bad
+        each = head_loss.linear_cross_entropy(x.detach(), w2, t, reduction="none")
+        assert bool(each.isnan().all())
+        leaf = x2.requires_grad_()
+        each = head_loss.linear_cross_entropy(leaf, w.detach(), t, reduction="none")
+        want = head_loss.linear_cross_entropy(x, w, t, reduction="none")
+        assert bool(each[2].isnan()) and torch.equal(each[3:], want[3:]) and torch.equal(each[:2], want[:2])
+        (dx,) = torch.autograd.grad(each.sum(), leaf)
+        assert bool(dx[2].isnan().all()) and not bool(dx[:2].isnan().any()) and not bool(dx[3:].isnan().any())
