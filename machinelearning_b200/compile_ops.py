@@ -217,13 +217,17 @@ def _(x, weight, targets, ignore_index, reduction, dtype):
 
 @torch.library.custom_op("nlfa::linear_ce_bwd", mutates_args=(), device_types="cuda")
 def linear_ce_bwd(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, tape: torch.Tensor,
-                  ignore_index: int, reduction: str, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
-    return _hl.bwd(grad.to(torch.float32).contiguous(), x.shape, x.dtype, weight, targets, tape, ignore_index, reduction, dtype)
+                  ignore_index: int, reduction: str, dtype: torch.dtype, want_dx: bool,
+                  want_dw: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """A gradient that is not wanted costs nothing and comes back without elements."""
+    dx, dw = _hl.bwd(grad.to(torch.float32).contiguous(), x.shape, x.dtype, weight, targets, tape, ignore_index, reduction, dtype,
+                     want_dx, want_dw)
+    return dx if want_dx else x.new_empty(0), dw if want_dw else weight.new_empty(0)
 
 
 @linear_ce_bwd.register_fake
-def _(grad, x, weight, targets, tape, ignore_index, reduction, dtype):
-    return torch.empty_like(x), torch.empty_like(weight)
+def _(grad, x, weight, targets, tape, ignore_index, reduction, dtype, want_dx, want_dw):
+    return torch.empty_like(x) if want_dx else x.new_empty(0), torch.empty_like(weight) if want_dw else weight.new_empty(0)
 
 
 def _ce_setup(ctx, inputs, output):
@@ -234,8 +238,9 @@ def _ce_setup(ctx, inputs, output):
 
 def _ce_backward(ctx, grad, gtape):
     x, weight, targets, tape = ctx.saved_tensors
-    dx, dw = linear_ce_bwd(grad, x, weight, targets, tape, *ctx.args)
-    return dx, dw, None, None, None, None
+    want_dx, want_dw = ctx.needs_input_grad[:2]
+    dx, dw = linear_ce_bwd(grad, x, weight, targets, tape, *ctx.args, want_dx, want_dw)
+    return dx if want_dx else None, dw if want_dw else None, None, None, None, None
 
 
 linear_ce_fwd.register_autograd(_ce_backward, setup_context=_ce_setup)

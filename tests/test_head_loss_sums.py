@@ -186,3 +186,20 @@ def test_float32_values_without_three_parts_show_as_nan(n):
         assert bool(each[2].isnan()) and torch.equal(each[3:], want[3:]) and torch.equal(each[:2], want[:2])
         (dx,) = torch.autograd.grad(each.sum(), leaf)
         assert bool(dx[2].isnan().all()) and not bool(dx[:2].isnan().any()) and not bool(dx[3:].isnan().any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("frozen", ["weight", "x", "none"])
+def test_compiled_callers_form_the_gradients_that_are_wanted(monkeypatch, frozen):
+    from machinelearning_b200 import flash_cuda, head_loss
+    assert flash_cuda.is_available()
+    x, w, t = _inputs("bf16", 90, 300, 64)
+    x, w = x.detach().requires_grad_(frozen != "x"), w.detach().requires_grad_(frozen != "weight")
+    leaves = [l for l in (x, w) if l.requires_grad]
+    want = torch.autograd.grad(head_loss.linear_cross_entropy(x, w, t), leaves)
+    asked, bwd = [], head_loss.bwd
+    monkeypatch.setattr(head_loss, "bwd", lambda *a: (asked.append(a[-2:]), bwd(*a))[1])
+    compiled = torch.compile(lambda x, w, t: head_loss.linear_cross_entropy(x, w, t), backend="aot_eager", fullgraph=True)
+    got = torch.autograd.grad(compiled(x, w, t), leaves)
+    assert asked == [(frozen != "x", frozen != "weight")]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
