@@ -349,9 +349,10 @@ join_rows_kernel(const uint2* __restrict__ pairs, const int* __restrict__ begin,
   grid_dep_wait();
   grid_dep_release();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int col = (blockIdx.y * 32 + lane) * N;
+  const int groups = (runs + kWarps - 1) / kWarps, slab = static_cast<int>(blockIdx.x) / groups, group = static_cast<int>(blockIdx.x) - slab * groups;
+  const int col = (slab * 32 + lane) * N;
   const bool in = col < d;
-  const int c = blockIdx.x * kWarps + warp;
+  const int c = group * kWarps + warp;
   uint32_t key = 0xffffffffu;
   int last = 0;                                            // the last run with a share
   if (c + 1 < runs) {
@@ -379,7 +380,7 @@ join_rows_kernel(const uint2* __restrict__ pairs, const int* __restrict__ begin,
   for (int w = 0; w < kWarps; ++w) {
     const int l = long_last[w];
     if (l < 0) continue;
-    const int c0 = blockIdx.x * kWarps + w, many = l - c0;                     // shares of runs c0 + 1 .. l
+    const int c0 = group * kWarps + w, many = l - c0;                     // shares of runs c0 + 1 .. l
     const int lo = c0 + 1 + static_cast<int>(static_cast<long long>(many) * warp / kWarps);
     const int hi = c0 + 1 + static_cast<int>(static_cast<long long>(many) * (warp + 1) / kWarps);
     float s[N];
@@ -427,7 +428,8 @@ int word_bytes(long long row_bytes, const void* a, const void* b) {
   return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
 }
 
-// Sorted positions per warp: enough warps for the GPU, and few partial sums when there are many positions.
+// Sorted positions per warp: enough warps for the GPU (148 SMs as a constant: the runs decide the order of additions and the size of the
+// scratch, so neither depends on the device that is asked), and few partial sums when there are many positions.
 int run_length(int n, int d) {
   const long long warps = 64ll * 148, slabs = (d + 127) / 128;
   int run = 16;
@@ -467,13 +469,14 @@ int gradient(const void* g, const Scratch& s, uint8_t* scratch, int sorted, void
   float* partial = reinterpret_cast<float*>(scratch + s.partial);
   const bool overlap = overlap_launches(kOverlapRowwise);
   const long long units = static_cast<long long>(runs) * slabs, ctas = (units + kWarps - 1) / kWarps;
-  if (ctas > 0x7fffffffll || slabs > 65535) return NLFA_ERR_BAD_SHAPE;
+  const long long join = static_cast<long long>((runs + kWarps - 1) / kWarps) * slabs;
+  if (join > 0x7fffffffll) return NLFA_ERR_BAD_SHAPE;      // (no fewer than `ctas`)
   if (n == 0) return NLFA_OK;                              // (the zeros are written)
   int rc = checked(launch_kernel(add_rows_kernel<T, W>, dim3(static_cast<unsigned>(ctas)), dim3(kBlock), 0, st, overlap, static_cast<const T*>(g),
                                  pairs, static_cast<T*>(dw), partial, n, V, d, run, runs, slabs, scale));
   if (rc != NLFA_OK || runs < 2) return rc;
-  return checked(launch_kernel(join_rows_kernel<T, W>, dim3(static_cast<unsigned>((runs + kWarps - 1) / kWarps), static_cast<unsigned>(slabs)),
-                               dim3(kBlock), 0, st, overlap, pairs, begin, end, partial, static_cast<T*>(dw), n, V, d, run, runs, scale));
+  return checked(launch_kernel(join_rows_kernel<T, W>, dim3(static_cast<unsigned>(join)), dim3(kBlock), 0, st, overlap, pairs, begin, end, partial,
+                               static_cast<T*>(dw), n, V, d, run, runs, scale));
 }
 
 }  // namespace
