@@ -464,7 +464,7 @@ Layout layout(const Call& c, bool w_aligned) {
   return l;
 }
 
-// The backward's pieces of the vocabulary: dl of one takes at most this (65,536 x 50,304 x 768: backward 13.8 ms with 512 MiB, 12.6 with
+// The backward's pieces of the vocabulary: dl of one takes at most this (65,536 x 50,304 x 768: backward 13.7 ms with 512 MiB, 12.4 with
 // 1 GiB and with 4: between pieces the GPU runs empty, and dx is summed in memory).
 constexpr size_t kMostDl = 1024ull << 20;
 
@@ -568,8 +568,8 @@ Params params(const Call& c, const Layout& l, const Pointers& t, unsigned* statu
 }
 
 // Stages per chain of the tensor core (loss_tc.cu) where logits are formed, in the forward and again in the backward: exp(l - lse) would
-// show any difference between the two.  Chains of 64 summands for float32, of 384 for few rows (whose losses are not averaged; 26.1 us
-// with one chain, 27.6 so, 29.5 with 256, for 8 rows of 50,304 x 768), else of up to 1,024.
+// show any difference between the two.  Chains of 64 summands for float32, of 384 for few rows (whose losses are not averaged; 22.5 us
+// with one chain, 24.3 so, 25.9 with 256, for 8 rows of 50,304 x 768), else of up to 1,024.
 int logit_chain(const Call& c, const Layout& l) {
   return l.x_planes == 3 ? 1 : c.n <= kFewRows ? (c.d > 384 ? 3 : 0) : c.d > 1024 ? 8 : 0;
 }

@@ -66,7 +66,7 @@ struct Params {
   const int* row_of;
   const float* alpha;
   void *dx, *dw;
-  float* dx_sum;                    // float32 sums over the pieces, for a 16-bit dx
+  float* dx_sum;                    // float32 sums of dx over the pieces
   const Parts* parts;
   float* shares;                    // of tiles formed in parts
   int dx_dtype, dw_dtype;

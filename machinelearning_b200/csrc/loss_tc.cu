@@ -78,7 +78,7 @@ struct Tile {
 // kProducts: the units are dW's tiles and then dx's, handed out in turn: whole tiles, as many of each kind as all pairs of CTAs get,
 // and the rest, whose sums are cut into parts so that every pair is busy (loss.cu: choose_parts; fold_kernel adds the shares).  Parts of one
 // index stand together: they read the same summands, from L2.  Backward with whole tiles only, and as it is: 65,536 rows x 50,304 words
-// x 768 12.9 and 11.9 ms, 4,096 rows 0.74 and 0.69, 300 rows 0.36 and 0.14.  (The rest as one line of stages cut into equal lengths balances
+// x 768 13.5 and 12.4 ms, 4,096 rows 0.86 and 0.82, 300 rows 0.38 and 0.15.  (The rest as one line of stages cut into equal lengths balances
 // better, but every pair then reads summands of its own from HBM: slower than whole tiles at 16,384 rows.)
 struct Plan {
   int d_tiles, kw, kx, again;
@@ -614,8 +614,8 @@ loss_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CU
                 if (col + j >= p.V) lo[h][j] = 0.f;
             }
             const unsigned at = static_cast<unsigned>(target - col);
-            // (three parts leave no registers: written as a product and sum the kernel takes 44.1 us, as a choice 48.7, at 1,000 x 5,003 x
-            // 384; one part: 11.48 and 11.26 ms, the backward of 65,536 x 50,304 x 768.  p is finite unless own is NaN too)
+            // (three parts leave no registers: the backward of 1,000 x 5,003 x 384 takes 95 us with a product and sum here, 101 with a choice; in
+            // one part, 16,384 x 50,304 x 768: 3.27 and 3.15 ms.  p is finite unless own is NaN too)
             if (__any_sync(0xffffffffu, at < 32u)) {
 #pragma unroll
               for (int j = 0; j < 32; ++j)
