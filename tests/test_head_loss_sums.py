@@ -203,3 +203,47 @@ def test_compiled_callers_form_the_gradients_that_are_wanted(monkeypatch, frozen
     got = torch.autograd.grad(compiled(x, w, t), leaves)
     assert asked == [(frozen != "x", frozen != "weight")]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("dtype,n", [("bf16", 2000), ("fp16", 1300), ("fp32", 700), ("bf16", 60)])
+def test_replays_with_other_numbers_of_targets(dtype, n, reduction):
+    """How many rows have a target is known on the device only: a captured call follows it, across the borders of tiles and of parts."""
+    from machinelearning_b200 import head_loss
+    x, w, t = _inputs(dtype, n, 1200, 200)
+
+    def step():
+        loss = head_loss.linear_cross_entropy(x, w, t, reduction=reduction)
+        return loss.detach(), *torch.autograd.grad(loss.sum(), (x, w))
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    full = t.clone()
+    for keep in (n, 257, 256, 100, 1, 0, n):
+        t.copy_(full)
+        t[torch.randperm(n, device="cuda")[min(keep, n):]] = -1
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step()):
+            assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
+@pytest.mark.gpu
+def test_saved_tensors_that_are_moved_or_recomputed():
+    from torch.utils.checkpoint import checkpoint
+    from machinelearning_b200 import head_loss
+    x, w, t = _inputs("bf16", 300, 700, 64)
+    store = torch.zeros(700 * 64 + 1, device="cuda", dtype=torch.bfloat16)
+    store[1:] = w.detach().reshape(-1)
+    off = store[1:].view(700, 64).requires_grad_()               # 2 bytes off: copied to the tape; comes back aligned
+    loss = head_loss.linear_cross_entropy(x, w, t)
+    want = torch.autograd.grad(loss, (x, w), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (x, w)), want))
+    for weight in (w, off):
+        with torch.autograd.graph.save_on_cpu():
+            loss = head_loss.linear_cross_entropy(x, weight, t)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (x, weight)), want))
+    loss = checkpoint(lambda a, b: head_loss.linear_cross_entropy(a, b, t), x, w, use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (x, w)), want))
