@@ -375,6 +375,29 @@ size_t nlfa_clip_scratch_bytes(void);
 int nlfa_clip_grads(const nlfa_grad* grads, int count, float max_norm, int norm, int scale, float* total_norm, void* scratch,
                     size_t scratch_bytes, void* stream);
 
+/* Gated linear recurrence along the sequence, what a MinGRU mixer (nanolab/mixers.py) mixes with: for each of D channels of B sequences
+ *   h_t = (1 - s_t) h_{t-1} + s_t f(value_t),  s = sigmoid(gate),  t = 1 .. T,
+ * f the identity, or (NLFA_SCAN_POSITIVE) v + 1/2 from zero on and sigmoid(v) below.  gate and value are [B, T, D] of `dtype`
+ * with strides in elements for sequences and steps (channels lie side by side: they may be halves of one projection's output); h is
+ * contiguous.  h_0 is `state` [B, D] (NULL: zeros), `last` [B, D] the state behind the last step, both float32, as all sums are.
+ * `reset` [B, T] (NULL: none): where it is not 0, h_{t-1} counts as zero, whatever it holds.  `lengths` [B], int32 or int64
+ * (length_bytes; NULL: all T): steps from lengths[b] on (taken between 0 and T) leave the state as it is, their h is zero, and what gate and value hold there reaches nothing.
+ * `tape` (nlfa_gated_scan_tape_bytes; NULL when no backward follows) takes the states at the start of every 16 steps.
+ * An infinite state or value makes the states behind it infinite or NaN, up to the next reset.
+ * Bit-reproducible; may be captured; no scratch.  Any alignment of the element type; pairs of channels are faster. */
+#define NLFA_SCAN_NONE 0
+#define NLFA_SCAN_POSITIVE 1
+size_t nlfa_gated_scan_tape_bytes(int B, int T, int D);
+int nlfa_gated_scan_fwd(const void* gate, long long gate_b, long long gate_t, const void* value, long long value_b, long long value_t,
+                        int dtype, const float* state, const unsigned char* reset, const void* lengths, int length_bytes, int activation,
+                        int B, int T, int D, void* h, float* last, void* tape, size_t tape_bytes, void* stream);
+/* Its gradients: dgate and dvalue, contiguous [B, T, D] of `dtype` (zeros where a step does not count), dstate [B, D]; any may be NULL.
+ * dh is contiguous [B, T, D], dlast [B, D]; NULL stands for zeros.  The tape is the forward's. */
+int nlfa_gated_scan_bwd(const void* dh, const float* dlast, const void* gate, long long gate_b, long long gate_t, const void* value,
+                        long long value_b, long long value_t, int dtype, const unsigned char* reset, const void* lengths, int length_bytes,
+                        int activation, int B, int T, int D, const void* tape, size_t tape_bytes, void* dgate, void* dvalue, float* dstate,
+                        void* stream);
+
 /* Bytes of device workspace `nlfa_selftest` needs. */
 size_t nlfa_selftest_workspace_bytes(void);
 

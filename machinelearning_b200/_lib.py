@@ -15,6 +15,7 @@ LIB_PATH = PKG / "libnlfa.so"
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 PATH_AUTO, PATH_SIMT, PATH_TENSOR = 0, 1, 2
 PASS_DELTA, PASS_DKV, PASS_DQ, PASS_ALL, PASS_FUSED = 1, 2, 4, 7, 8
+SCAN_NONE, SCAN_POSITIVE = 0, 1
 REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
 OK = 0
 ERR_DEVICE_TIMEOUT = 10
@@ -82,6 +83,11 @@ SIGNATURES = {
                            + [_c_float, ctypes.c_longlong, _c_void_p, _c_size_t, _c_void_p]),
     "nlfa_clip_scratch_bytes": (_c_size_t, []),
     "nlfa_clip_grads": (_c_int, [_c_void_p, _c_int, _c_float, _c_int, _c_int, _c_void_p, _c_void_p, _c_size_t, _c_void_p]),
+    "nlfa_gated_scan_tape_bytes": (_c_size_t, [_c_int] * 3),
+    "nlfa_gated_scan_fwd": (_c_int, [_c_void_p, ctypes.c_longlong, ctypes.c_longlong] * 2 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 5
+                            + [_c_void_p] * 3 + [_c_size_t, _c_void_p]),
+    "nlfa_gated_scan_bwd": (_c_int, [_c_void_p] * 2 + [_c_void_p, ctypes.c_longlong, ctypes.c_longlong] * 2 + [_c_int] + [_c_void_p] * 2
+                            + [_c_int] * 5 + [_c_void_p, _c_size_t] + [_c_void_p] * 4),
     "nlfa_selftest_workspace_bytes": (_c_size_t, []),
     "nlfa_selftest": (_c_int, [_c_int, _c_int, _c_void_p, _c_size_t,
                                ctypes.POINTER(_c_float), _c_void_p]),

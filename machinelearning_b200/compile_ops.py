@@ -288,3 +288,60 @@ embedding_fwd.register_autograd(_te_backward, setup_context=_te_setup)
 def embedding(idx, weight, scale, padding):
     """``token_embedding.embedding`` through the registered operators."""
     return embedding_fwd(idx.contiguous(), weight.contiguous(), scale, padding)
+
+
+# ---------------------------------------------------------------- gated recurrence
+from . import gated_scan as _gs  # noqa: E402
+
+
+@torch.library.custom_op("nlfa::gated_scan_fwd", mutates_args=(), device_types="cuda")
+def gated_scan_fwd(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor | None, reset: torch.Tensor | None,
+                   lengths: torch.Tensor | None, activation: str, train: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _gs.fwd(_gs._rows(gate), _gs._rows(value), state, reset, lengths, activation, train)
+
+
+@gated_scan_fwd.register_fake
+def _(gate, value, state, reset, lengths, activation, train):
+    tape = torch.library.get_ctx().new_dynamic_size()
+    return (gate.new_empty(gate.shape), gate.new_empty((gate.shape[0], gate.shape[2]), dtype=torch.float32),
+            gate.new_empty((tape,), dtype=torch.uint8))
+
+
+@torch.library.custom_op("nlfa::gated_scan_bwd", mutates_args=(), device_types="cuda")
+def gated_scan_bwd(dh: torch.Tensor | None, dlast: torch.Tensor | None, gate: torch.Tensor, value: torch.Tensor,
+                   reset: torch.Tensor | None, lengths: torch.Tensor | None, tape: torch.Tensor, activation: str, want_gate: bool,
+                   want_value: bool, want_state: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """A gradient that is not wanted costs nothing and comes back without elements."""
+    dh = None if dh is None else dh.to(gate.dtype).contiguous()
+    dlast = None if dlast is None else dlast.to(torch.float32).contiguous()
+    grads = _gs.bwd(dh, dlast, _gs._rows(gate), _gs._rows(value), reset, lengths, tape, activation, (want_gate, want_value, want_state))
+    return tuple(gate.new_empty(0) if g is None else g for g in grads)
+
+
+@gated_scan_bwd.register_fake
+def _(dh, dlast, gate, value, reset, lengths, tape, activation, want_gate, want_value, want_state):
+    return (gate.new_empty(gate.shape if want_gate else 0), gate.new_empty(gate.shape if want_value else 0),
+            gate.new_empty((gate.shape[0], gate.shape[2]), dtype=torch.float32) if want_state else gate.new_empty(0))
+
+
+def _gs_setup(ctx, inputs, output):
+    gate, value, _, reset, lengths, activation, _ = inputs
+    ctx.save_for_backward(gate, value, reset, lengths, output[2])
+    ctx.activation = activation
+
+
+def _gs_backward(ctx, dh, dlast, gtape):
+    gate, value, reset, lengths, tape = ctx.saved_tensors
+    want = [bool(w) for w in ctx.needs_input_grad[:3]]
+    grads = gated_scan_bwd(dh, dlast, gate, value, reset, lengths, tape, ctx.activation, *want)
+    return *(g if w else None for g, w in zip(grads, want)), None, None, None, None
+
+
+gated_scan_fwd.register_autograd(_gs_backward, setup_context=_gs_setup)
+
+
+def gated_scan(gate, value, state, reset, lengths, activation):
+    """``gated_scan.gated_scan`` through the registered operators."""
+    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (gate, value, state))
+    h, last, _ = gated_scan_fwd(gate, value, state, reset, lengths, activation, train)
+    return h, last

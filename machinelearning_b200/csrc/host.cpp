@@ -443,6 +443,72 @@ struct TokenEmbeddingBackward : public Node {
   std::string name() const override { return "TokenEmbeddingBackward"; }
 };
 
+// ------------------------------------------------------------------------------------------- gated recurrence
+
+struct ScanCall {
+  int B, T, D, dtype, activation, length_bytes;
+  const unsigned char* reset;
+  const void* lengths;
+};
+ScanCall scan_call(const Tensor& gate, const Tensor& reset, const Tensor& lengths, int activation) {
+  return {static_cast<int>(gate.size(0)), static_cast<int>(gate.size(1)), static_cast<int>(gate.size(2)), dtype_code(gate.scalar_type()), activation,
+          lengths.defined() ? static_cast<int>(lengths.element_size()) : 0,
+          reset.defined() ? static_cast<const unsigned char*>(reset.data_ptr()) : nullptr, lengths.defined() ? lengths.data_ptr() : nullptr};
+}
+
+// (h, last, tape; no tape unless a backward follows)
+std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor& gate, const Tensor& value, const Tensor& state, const Tensor& reset,
+                                                const Tensor& lengths, int activation, bool train) {
+  const c10::cuda::CUDAGuard guard(gate.device());
+  const ScanCall c = scan_call(gate, reset, lengths, activation);
+  Tensor h = empty(gate.sizes(), gate.scalar_type(), gate), last = empty({c.B, c.D}, at::kFloat, gate), tape;
+  if (train) tape = empty({static_cast<int64_t>(nlfa_gated_scan_tape_bytes(c.B, c.T, c.D))}, at::kByte, gate);
+  check("nlfa_gated_scan_fwd",
+        nlfa_gated_scan_fwd(gate.data_ptr(), gate.stride(0), gate.stride(1), value.data_ptr(), value.stride(0), value.stride(1), c.dtype,
+                            state.defined() ? static_cast<const float*>(state.data_ptr()) : nullptr, c.reset, c.lengths, c.length_bytes,
+                            activation, c.B, c.T, c.D, h.data_ptr(), static_cast<float*>(last.data_ptr()), train ? tape.data_ptr() : nullptr,
+                            train ? static_cast<size_t>(tape.numel()) : 0, stream_of(gate)));
+  return {h, last, tape};
+}
+
+struct GatedScanBackward : public Node {
+  SavedVariable gate, value, reset, lengths, tape;
+  int activation;
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor()};
+    Tensor gate_ = gate.unpack(), value_ = value.unpack(), reset_ = reset.unpack(), lengths_ = lengths.unpack(), tape_ = tape.unpack();
+    const c10::cuda::CUDAGuard guard(gate_.device());
+    const ScanCall c = scan_call(gate_, reset_, lengths_, activation);
+    Tensor dh, dlast, out[3];
+    if (grads[0].defined()) dh = contiguous(cast(grads[0], gate_.scalar_type()));
+    if (grads[1].defined()) dlast = contiguous(cast(grads[1], at::kFloat));
+    for (int i = 0; i < 2; ++i)
+      if (task_should_compute_output(i)) out[i] = empty(gate_.sizes(), gate_.scalar_type(), gate_);
+    if (task_should_compute_output(2)) out[2] = empty({c.B, c.D}, at::kFloat, gate_);
+    auto at = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    check("nlfa_gated_scan_bwd",
+          nlfa_gated_scan_bwd(at(dh), static_cast<const float*>(at(dlast)), gate_.data_ptr(), gate_.stride(0), gate_.stride(1), value_.data_ptr(),
+                              value_.stride(0), value_.stride(1), c.dtype, c.reset, c.lengths, c.length_bytes, activation, c.B, c.T, c.D,
+                              tape_.data_ptr(), static_cast<size_t>(tape_.numel()), at(out[0]), at(out[1]), static_cast<float*>(at(out[2])),
+                              stream_of(gate_)));
+    variable_list list;
+    for (const Tensor& t : out)
+      if (t.defined()) list.push_back(t);
+    list = once(std::move(list), grads[0].defined() && grads[0].requires_grad() ? grads[0] : grads[1].defined() ? grads[1] : grads[0]);
+    size_t next = 0;
+    variable_list result(3);
+    for (int i = 0; i < 3; ++i)
+      if (out[i].defined()) result[i] = list[next++];
+    return result;
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&gate, &value, &reset, &lengths, &tape}) v->reset_data();
+  }
+  std::string name() const override { return "GatedScanBackward"; }
+};
+
 // ------------------------------------------------------------------------------------------- gradient clip
 
 struct Span {
@@ -927,6 +993,57 @@ PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// gated_scan(gate, value, state | None, reset | None, lengths | None, activation code) -> (h, last) | None
+PyObject* py_gated_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !is_tensor(a[0]) || !is_tensor(a[1]) || !tensor_or_none(a[2]) || !tensor_or_none(a[3]) || !tensor_or_none(a[4])) return decline();
+  Tensor gate = tensor(a[0]), value = tensor(a[1]), state = maybe(a[2]), reset = maybe(a[3]), lengths = maybe(a[4]);
+  constexpr int64_t kMost = int64_t(1) << 30;
+  if (!plain(gate) || !plain(value) || !watched(gate) || value.device() != gate.device() || gate.dim() != 3 || value.sizes() != gate.sizes() ||
+      dtype_code(gate.scalar_type()) < 0 || value.scalar_type() != gate.scalar_type() || gate.size(0) > kMost || gate.size(1) > kMost ||
+      gate.size(2) > kMost)
+    return decline();
+  const int64_t B = gate.size(0), T = gate.size(1), D = gate.size(2);
+  if (state.defined() && (!plain(state) || state.device() != gate.device() || state.scalar_type() != at::kFloat ||
+                          state.sizes() != at::IntArrayRef({B, D})))
+    return decline();
+  if (reset.defined() && (!plain(reset) || reset.device() != gate.device() || reset.scalar_type() != at::kBool ||
+                          reset.sizes() != at::IntArrayRef({B, T})))
+    return decline();
+  if (lengths.defined() && (!plain(lengths) || lengths.device() != gate.device() || lengths.sizes() != at::IntArrayRef({B}) ||
+                            (lengths.scalar_type() != at::kInt && lengths.scalar_type() != at::kLong)))
+    return decline();
+  const int activation = integer(a[5]);
+  Tensor h, last;
+  {
+    py::gil_scoped_release no_gil;
+    const c10::cuda::CUDAGuard guard(gate.device());
+    // (rows with strides of their own are read where they lie)
+    if (D > 1 && gate.stride(2) != 1) gate = gate.contiguous();
+    if (D > 1 && value.stride(2) != 1) value = value.contiguous();
+    for (Tensor* t : {&state, &reset, &lengths})
+      if (t->defined()) *t = contiguous(*t);
+    const bool train = recording({&gate, &value, &state});
+    Tensor tape;
+    std::tie(h, last, tape) = scan_forward(gate, value, state, reset, lengths, activation, train);
+    if (train) {
+      auto node = make_node<GatedScanBackward>();
+      node->set_next_edges(torch::autograd::collect_next_edges(gate, value, state));
+      node->gate = SavedVariable(gate, false);
+      node->value = SavedVariable(value, false);
+      node->reset = SavedVariable(reset, false);
+      node->lengths = SavedVariable(lengths, false);
+      node->tape = SavedVariable(tape, false);
+      node->activation = activation;
+      torch::autograd::set_history(h, node);
+      torch::autograd::set_history(last, node);
+    }
+  }
+  THPObjectPtr first(THPVariable_Wrap(h)), second(THPVariable_Wrap(last));
+  return first && second ? PyTuple_Pack(2, first.get(), second.get()) : nullptr;
+  END_HANDLE_TH_ERRORS
+}
+
 // clip_grads(list of tensors, list of tensors | None, max_norm, norm code, scale, of_parameters) -> norm | None
 // of_parameters: the tensors' gradients, where they have one (None: none has).
 PyObject* py_clip_grads(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -985,6 +1102,7 @@ PyObject* py_watch(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef g_methods[] = {NLFA_METHOD(attn),        NLFA_METHOD(attn_fwd),    NLFA_METHOD(attn_bwd),  NLFA_METHOD(attn_cached),
                            NLFA_METHOD(qk_prologue), NLFA_METHOD(value_blend), NLFA_METHOD(head_gate), NLFA_METHOD(linear_ce),
                            NLFA_METHOD(embedding),   NLFA_METHOD(clip_grads),  NLFA_METHOD(configure), NLFA_METHOD(watch),
+                           NLFA_METHOD(gated_scan),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", "torch-facing call path of libnlfa (host.cpp)", -1, g_methods};
 
