@@ -13,6 +13,7 @@
 #include <type_traits>
 
 #include "loss.cuh"
+#include "operands.cuh"
 #include "rowwise.cuh"
 
 namespace nlfa {
@@ -25,59 +26,14 @@ namespace {
 using rowwise::aligned16;
 using rowwise::dtype_ok;
 using rowwise::last_cta;
+using operands::box_map;
+using operands::column_map;
+using operands::copy_chunk;
+using operands::copy_rows;
+using operands::row_map;
 
 constexpr int kScanCtas = 8, kScanThreads = 1024;
-constexpr int kBlock = 256;
-
-// ------------------------------------------------------------------------------------------------ 16-bit operands
-
-template <typename T> __device__ __forceinline__ float load1(const T* p) { return static_cast<float>(*p); }
-
-// Eight columns (from c) of row `from` of src [*, d] (-1: zeros) to row r of dst [planes][d_pad / 64][n_rows][64]; planes = 3: dst = a + b + c,
-// each the nearest bf16 value to what is left (of infinity: NaN; and its products with the other operand's small parts would be NaN whatever was left).
-template <typename S, typename T>
-__device__ __forceinline__ void copy_chunk(const S* __restrict__ src, T* __restrict__ dst, int from, int r, int c, int n_rows, int d, int d_pad,
-                                           int planes, int vec) {
-  float v[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = 0.f;
-  if (from >= 0 && c < d) {
-    const S* s = src + static_cast<size_t>(from) * d + c;
-    if (vec) rowwise::Elem<S>::load(s, v);
-    else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (c + j < d) v[j] = load1(s + j);
-    }
-  }
-  T* o = dst + (static_cast<size_t>(c / 64) * n_rows + r) * 64 + c % 64;
-  for (int part = 0; part < planes; ++part) {
-    rowwise::Elem<T>::store(o, v);
-    o += static_cast<size_t>(n_rows) * d_pad;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] -= rowwise::Elem<T>::round(v[j]);
-  }
-}
-
-// Rows from row_of (or r itself), zeros behind the last one up to a whole tile and behind column d.
-template <typename S, typename T>
-__global__ void __launch_bounds__(kBlock)
-copy_rows_kernel(const S* __restrict__ src, T* __restrict__ dst, const Head* head, const int* __restrict__ row_of, int n_src,
-                 int n_rows, int d, int d_pad, int planes, int vec) {
-  grid_dep_wait();
-  grid_dep_release();
-  int end = n_src;
-  if (row_of != nullptr) {
-    const int all = head->count;
-    end = all < kRowTile ? kRowTile : (all + kRowTile - 1) / kRowTile * kRowTile;
-  }
-  const int chunks = d_pad / 8;
-  const long long total = static_cast<long long>(end) * chunks;
-  for (long long i = static_cast<long long>(blockIdx.x) * kBlock + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * kBlock) {
-    const int r = static_cast<int>(i / chunks), c = 8 * static_cast<int>(i - static_cast<long long>(r) * chunks);
-    copy_chunk(src, dst, row_of != nullptr ? row_of[r] : r, r, c, n_rows, d, d_pad, planes, vec);
-  }
-}
+constexpr int kBlock = operands::kBlock;
 
 // ------------------------------------------------------------------------------------------------ rows with a target
 
@@ -494,49 +450,9 @@ BwdLayout bwd_layout(const Call& c, const Layout& l) {
   return b;
 }
 
-// What lies in tape and scratch lies in blocks, [planes][blocks of 64 columns][rows][64], so that a box is contiguous; the caller's w is
-// [rows][cols].  Either as (64 columns, rows, blocks of 64 columns, planes), cols a multiple of 64.
-int box_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes, int box_rows, int box_blocks,
-            int box_planes, bool blocked) {
-  const unsigned long long pitch = static_cast<unsigned long long>(cols) * 2, r = static_cast<unsigned long long>(rows);
-  const unsigned long long dims[4] = {64ull, r, pitch / 128, static_cast<unsigned long long>(planes)};
-  const unsigned long long strides[3] = {blocked ? 128ull : pitch, blocked ? 128ull * r : 128ull, pitch * r};
-  const unsigned box[4] = {64u, static_cast<unsigned>(box_rows), static_cast<unsigned>(box_blocks), static_cast<unsigned>(box_planes)};
-  return make_map(map, base, dtype, dims, strides, box);
-}
-// One CTA's half of an operand, a stage of it, in all its parts: 128 rows, the summands along the columns ...
-int column_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes, bool blocked = true) {
-  return box_map(map, base, dtype, cols, rows, planes, 128, summands(planes) / 64, planes == 3 ? 3 : 1, blocked);
-}
-// ... or 128 columns, the summands along the rows.
-int row_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows, int planes, bool blocked = true) {
-  return box_map(map, base, dtype, cols, rows, planes, summands(planes), 2, planes == 3 ? 3 : 1, blocked);
-}
-
 int checked(cudaError_t e) {
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? NLFA_OK : NLFA_ERR_CUDA;
-}
-
-template <typename S, typename T>
-int copy_rows_typed(const void* src, void* dst, const Head* head, const int* row_of, int n_src, int n_rows, int d, int d_pad,
-                    int planes, cudaStream_t st) {
-  const int vec = d % 8 == 0 && aligned16(src) ? 1 : 0;
-  const long long work = static_cast<long long>(row_of != nullptr ? n_rows : n_src) * (d_pad / 8);
-  const long long most = 16ll * sm_count();
-  const long long need = (work + kBlock - 1) / kBlock;
-  return checked(launch_kernel(copy_rows_kernel<S, T>, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(kBlock), 0, st,
-                               overlap_launches(kOverlapRowwise), static_cast<const S*>(src), static_cast<T*>(dst), head, row_of,
-                               n_src, n_rows, d, d_pad, planes, vec));
-}
-int copy_rows(const void* src, int src_dtype, void* dst, int dtype, const Head* head, const int* row_of, int n_src, int n_rows,
-              int d, int d_pad, int planes, cudaStream_t st) {
-#define NLFA_TO(S) (dtype == NLFA_DTYPE_F16 ? copy_rows_typed<S, __half>(src, dst, head, row_of, n_src, n_rows, d, d_pad, planes, st) \
-                                            : copy_rows_typed<S, __nv_bfloat16>(src, dst, head, row_of, n_src, n_rows, d, d_pad, planes, st))
-  if (src_dtype == NLFA_DTYPE_F32) return NLFA_TO(float);
-  if (src_dtype == NLFA_DTYPE_F16) return NLFA_TO(__half);
-  return NLFA_TO(__nv_bfloat16);
-#undef NLFA_TO
 }
 
 struct Pointers {
@@ -617,7 +533,7 @@ int run_fwd(const Call& c, const void* x, const void* w, const void* targets, in
     rc = copy_rows(w, c.w_dtype, tape + l.w, dtype, nullptr, nullptr, c.V, c.V, c.d, l.d_pad, l.x_planes, st);
     if (rc != NLFA_OK) return rc;
   }
-  if (!few) rc = copy_rows(x, c.x_dtype, tape + l.x, dtype, t.head(), t.row_of(), c.n, l.n_rows, c.d, l.d_pad, l.x_planes, st);
+  if (!few) rc = copy_rows(x, c.x_dtype, tape + l.x, dtype, &t.head()->count, t.row_of(), c.n, l.n_rows, c.d, l.d_pad, l.x_planes, st);
   if (rc != NLFA_OK) return rc;
   CUtensorMap mx, mw;
   rc = few ? box_map(&mx, tape + l.x, dtype, l.d_pad, l.n_rows, l.x_planes, kFewRows / 2, summands(l.x_planes) / 64, l.x_planes, true)

@@ -2,14 +2,14 @@
 #pragma once
 
 #include "common.cuh"
+#include "operands.cuh"
 
 namespace nlfa {
 namespace loss {
 
-constexpr int kRowTile = 256;       // rows of a product's tile: two CTAs of 128
+using operands::kRowTile;
 constexpr int kColTile = 256;       // columns of a tile
-// Summands per stage of a product's pipeline: 128, or 64 of operands in three parts.
-__host__ __device__ constexpr int summands(int planes) { return planes == 3 ? 64 : 128; }
+using operands::summands;
 // dl is held in 16 bits.  Its roundings (half a step, 2^-8 in bf16) are independent and largely cancel in sums over many rows or words:
 // gradients of 513 rows are off by 2.2e-3 as a whole, 1.7e-3 of that by their own rounding.  A row's own target has most of its dl,
 // though, and in a sum of a few rows one such rounding shows (3.3e-3 for one row): up to a tile of rows with a target dl is held in two
