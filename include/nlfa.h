@@ -398,6 +398,32 @@ int nlfa_gated_scan_bwd(const void* dh, const float* dlast, const void* gate, lo
                         int activation, int B, int T, int D, const void* tape, size_t tape_bytes, void* dgate, void* dvalue, float* dstate,
                         void* stream);
 
+/* Gated feed-forward layer, what nanolab's SwiGLU does (nanolab/model.py:29-43): for x [n, d], w_gate and w_up [F, d], w_down [o, F]
+ *   y = (f(x w_gate^T) * (x w_up^T)) w_down^T,  f one of NLFA_FFN_*  (gelu: with erf).
+ * Every extent may be of any size; tensors are contiguous.  x is of x_dtype, the weights of w_dtype, y and its gradient of `dtype`, which is
+ * what the products run in (the autocast type, say): 16-bit types on the tensor cores, NLFA_DTYPE_F32 on the tensor cores as sums of three bf16
+ * parts (finite values below 3.39e38; an infinity makes what it enters NaN).  Sums are float32.  Between the products the hidden values are rounded once to `dtype`'s
+ * precision; in float16 they carry a power of two, so that they neither overflow nor lose digits below the type's normal range.
+ *
+ * `copies` (nlfa_gated_ffn_copies): which of x, w_gate, w_up, w_down (bits 0 to 3) the forward copies into the tape, because the products cannot read
+ * them as they lie: of another type, float32, rows not a multiple of 64 long, not 16-byte aligned.  The backward takes the same value; operands that
+ * were copied may be NULL there, the others have to be what they were.  `tape`: with `train` what the backward reads, without it workspace.
+ * dx (x_dtype), dw_gate, dw_up, dw_down (w_dtype): any may be NULL.  Bit-reproducible; may be captured.  Tape, scratch, y and the gradients are 16-byte
+ * aligned.  Needs compute capability 10.x. */
+#define NLFA_FFN_SILU 0
+#define NLFA_FFN_GELU 1
+#define NLFA_FFN_RELU 2
+int nlfa_gated_ffn_copies(const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype, int dtype, int d,
+                          int F);
+size_t nlfa_gated_ffn_tape_bytes(int n, int d, int F, int o, int dtype, int copies, int train);
+size_t nlfa_gated_ffn_scratch_bytes(int n, int d, int F, int o, int dtype, int copies, int backward);
+int nlfa_gated_ffn_fwd(const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype, int dtype,
+                       int activation, int n, int d, int F, int o, void* y, int copies, int train, void* tape, size_t tape_bytes, void* scratch,
+                       size_t scratch_bytes, void* stream);
+int nlfa_gated_ffn_bwd(const void* dy, const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype,
+                       int dtype, int activation, int n, int d, int F, int o, int copies, void* tape, size_t tape_bytes, void* dx,
+                       void* dw_gate, void* dw_up, void* dw_down, void* scratch, size_t scratch_bytes, void* stream);
+
 /* Bytes of device workspace `nlfa_selftest` needs. */
 size_t nlfa_selftest_workspace_bytes(void);
 

@@ -16,6 +16,7 @@ DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 PATH_AUTO, PATH_SIMT, PATH_TENSOR = 0, 1, 2
 PASS_DELTA, PASS_DKV, PASS_DQ, PASS_ALL, PASS_FUSED = 1, 2, 4, 7, 8
 SCAN_NONE, SCAN_POSITIVE = 0, 1
+FFN_SILU, FFN_GELU, FFN_RELU = 0, 1, 2
 REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
 OK = 0
 ERR_DEVICE_TIMEOUT = 10
@@ -88,6 +89,13 @@ SIGNATURES = {
                             + [_c_void_p] * 3 + [_c_size_t, _c_void_p]),
     "nlfa_gated_scan_bwd": (_c_int, [_c_void_p] * 2 + [_c_void_p, ctypes.c_longlong, ctypes.c_longlong] * 2 + [_c_int] + [_c_void_p] * 2
                             + [_c_int] * 5 + [_c_void_p, _c_size_t] + [_c_void_p] * 4),
+    "nlfa_gated_ffn_copies": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 3 + [_c_int] * 4),
+    "nlfa_gated_ffn_tape_bytes": (_c_size_t, [_c_int] * 7),
+    "nlfa_gated_ffn_scratch_bytes": (_c_size_t, [_c_int] * 7),
+    "nlfa_gated_ffn_fwd": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 3 + [_c_int] * 7 + [_c_void_p] + [_c_int] * 2
+                           + [_c_void_p, _c_size_t] * 2 + [_c_void_p]),
+    "nlfa_gated_ffn_bwd": (_c_int, [_c_void_p] * 2 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 8 + [_c_void_p, _c_size_t] + [_c_void_p] * 5
+                           + [_c_size_t, _c_void_p]),
     "nlfa_selftest_workspace_bytes": (_c_size_t, []),
     "nlfa_selftest": (_c_int, [_c_int, _c_int, _c_void_p, _c_size_t,
                                ctypes.POINTER(_c_float), _c_void_p]),

@@ -345,3 +345,62 @@ def gated_scan(gate, value, state, reset, lengths, activation):
     train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (gate, value, state))
     h, last, _ = gated_scan_fwd(gate, value, state, reset, lengths, activation, train)
     return h, last
+
+
+# ---------------------------------------------------------------- gated feed-forward layer
+from . import gated_ffn as _gf  # noqa: E402
+
+
+def _aligned(inputs):
+    """On 16-byte boundaries, so that which operands the tape has copies of follows from types and sizes alone."""
+    return [t if t.data_ptr() % 16 == 0 else t.clone() for t in inputs]
+
+
+@torch.library.custom_op("nlfa::gated_ffn_fwd", mutates_args=(), device_types="cuda")
+def gated_ffn_fwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str, dtype: torch.dtype,
+                  train: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    y, tape, _ = _gf.fwd(*_aligned((x, w_gate, w_up, w_down)), activation, dtype, train)
+    return y, tape if train else tape.new_empty(0)
+
+
+@gated_ffn_fwd.register_fake
+def _(x, w_gate, w_up, w_down, activation, dtype, train):
+    tape = torch.library.get_ctx().new_dynamic_size()
+    return x.new_empty((*x.shape[:-1], w_down.shape[0]), dtype=dtype), x.new_empty((tape,), dtype=torch.uint8)
+
+
+@torch.library.custom_op("nlfa::gated_ffn_bwd", mutates_args=(), device_types="cuda")
+def gated_ffn_bwd(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, tape: torch.Tensor,
+                  activation: str, dtype: torch.dtype, want: list[bool]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """A gradient that is not wanted costs nothing and comes back without elements."""
+    inputs = _aligned((x, w_gate, w_up, w_down))
+    grads = _gf.bwd(dy.to(dtype).contiguous(), *inputs, tape, _gf.copies_of(*inputs, dtype), [t.shape for t in inputs], x.dtype, w_gate.dtype,
+                    activation, want)
+    return tuple(t.new_empty(0) if g is None else g for t, g in zip(inputs, grads))
+
+
+@gated_ffn_bwd.register_fake
+def _(dy, x, w_gate, w_up, w_down, tape, activation, dtype, want):
+    return tuple(t.new_empty(t.shape if w else 0) for t, w in zip((x, w_gate, w_up, w_down), want))
+
+
+def _gf_setup(ctx, inputs, output):
+    *tensors, activation, dtype, _ = inputs
+    ctx.save_for_backward(*tensors, output[1])
+    ctx.args = (activation, dtype)
+
+
+def _gf_backward(ctx, dy, gtape):
+    want = [bool(w) for w in ctx.needs_input_grad[:4]]
+    grads = gated_ffn_bwd(dy, *ctx.saved_tensors, *ctx.args, want)
+    return *(g if w else None for g, w in zip(grads, want)), None, None, None
+
+
+gated_ffn_fwd.register_autograd(_gf_backward, setup_context=_gf_setup)
+
+
+def gated_ffn(x, w_gate, w_up, w_down, activation, dtype):
+    """``gated_ffn.gated_ffn`` through the registered operators."""
+    inputs = [t.contiguous() for t in (x, w_gate, w_up, w_down)]
+    train = torch.is_grad_enabled() and any(t.requires_grad for t in inputs)
+    return gated_ffn_fwd(*inputs, activation, dtype, train)[0]

@@ -1,0 +1,525 @@
+// Gated feed-forward layer, forward and backward:
+//
+//   g = x Wg^T,  u = x Wu^T,  h = f(g) u,  y = h Wd^T                              f: silu, gelu, relu
+//   dh = dy Wd,  du = dh f(g),  dg = dh u f'(g)
+//   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h
+//
+// Bound by the tensor cores: 2 N F (2 d + o) operations forward and twice that backward, in four launches of products (ffn_tc.cu).  g and u exist in
+// tensor memory, and in the tape for the backward; dh in tensor memory alone.  Between the products h, dg and du are operands: 16 bits (float32:
+// three bf16 parts), one rounding each beside that of the results.
+//
+// This file has what goes around the products: 16-bit copies of operands that TMA cannot read as they are, the list of tiles and
+// parts, and the powers of two that hold float16's h, dg and du inside their type's range.
+#include <cmath>
+
+#include "ffn.cuh"
+#include "rowwise.cuh"
+
+namespace nlfa {
+
+unsigned* status_block();      // api.cu
+
+namespace ffn {
+namespace {
+
+using operands::column_map;
+using operands::copy_rows;
+using operands::row_map;
+using rowwise::aligned16;
+using rowwise::dtype_ok;
+
+enum { kCopyX = 1, kCopyGate = 2, kCopyUp = 4, kCopyDown = 8 };
+
+struct Call {
+  int x_dtype, w_dtype, dtype;      // dtype: what the products run in
+  int n, d, F, o;
+  int copies;                       // operands that are converted or re-laid (otherwise the products read the caller's)
+  int train;
+};
+
+size_t up(size_t v) { return (v + 255) / 256 * 256; }
+int up64(int v) { return (v + 63) / 64 * 64; }
+int element_bytes(int dtype) { return dtype == NLFA_DTYPE_F32 ? 4 : 2; }
+bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+__host__ __device__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+constexpr int kMostRows = 1 << 30, kMostWidth = 1 << 24;
+int check_call(const Call& c) {
+  if (c.n < 0 || c.d < 1 || c.F < 1 || c.o < 1 || c.n > kMostRows || c.d > kMostWidth || c.F > kMostWidth || c.o > kMostWidth)
+    return NLFA_ERR_BAD_SHAPE;
+  if (!dtype_ok(c.x_dtype) || !dtype_ok(c.w_dtype) || !dtype_ok(c.dtype)) return NLFA_ERR_BAD_DTYPE;
+  return NLFA_OK;
+}
+
+bool must_copy(const void* p, int type, int dtype, int cols) { return dtype == NLFA_DTYPE_F32 || type != dtype || cols % 64 != 0 || !aligned16(p); }
+
+// What the forward leaves for the backward, and (inference) the forward's own workspace.
+struct Layout {
+  int planes, n_rows, d_pad, f_pad, o_pad;
+  int type;                         // of an operand
+  size_t limits, x, gate, up, down, h, kept, exponents, bytes;
+};
+Layout layout(const Call& c) {
+  Layout l{};
+  l.planes = c.dtype == NLFA_DTYPE_F32 ? 3 : 1;
+  l.type = c.dtype == NLFA_DTYPE_F32 ? NLFA_DTYPE_BF16 : c.dtype;
+  l.n_rows = (c.n + kRowTile - 1) / kRowTile * kRowTile;
+  l.d_pad = up64(c.d);
+  l.f_pad = up64(c.F);
+  l.o_pad = up64(c.o);
+  const size_t two = 2 * static_cast<size_t>(l.planes), hidden = static_cast<size_t>(l.n_rows) * l.f_pad;
+  size_t at = 0;
+  l.limits = at; at += 256;
+  l.x = at; if (c.copies & kCopyX) at = up(at + two * c.n * l.d_pad);
+  l.gate = at; if (c.copies & kCopyGate) at = up(at + two * c.F * l.d_pad);
+  l.up = at; if (c.copies & kCopyUp) at = up(at + two * c.F * l.d_pad);
+  l.down = at; if (c.copies & kCopyDown) at = up(at + two * c.o * l.f_pad);
+  l.h = at; at = up(at + two * hidden);
+  if (c.train) {
+    l.kept = at; at = up(at + 2 * hidden * (l.planes == 3 ? 4 : 2));
+    l.exponents = at; if (l.planes == 1) at = up(at + 2 * hidden / 32);
+  }
+  l.bytes = at;
+  return l;
+}
+
+// ------------------------------------------------------------------------------------------------ tiles
+
+// In how many parts the sums of `rest` tiles of k stages are formed: the fewest stages for the busiest pair of CTAs, with `share` more for every
+// share written and added.  The units are handed out in turn behind `ahead` units of `length` stages.
+int choose_parts(int rest, int k, int n_pairs, int share, int ahead, int length) {
+  if (rest == 0) return 1;
+  int best = 1;
+  long long least = -1;
+  for (int s = 1; s <= kPartsPerPair * n_pairs / rest && s <= k; ++s) {
+    const int end = ahead + rest * s, mine = (k + s - 1) / s + (s > 1 ? share : 0);
+    long long cost = 0;
+    for (int i = 0; i < 3; ++i) {                          // the first pair, and the first that gets one unit less of either kind
+      const int b = i == 0 ? 0 : (i == 1 ? ahead : end) % n_pairs;
+      const int first = (ahead + n_pairs - 1 - b) / n_pairs, both = (end + n_pairs - 1 - b) / n_pairs;
+      const long long c = static_cast<long long>(first) * length + static_cast<long long>(both - first) * mine;
+      cost = c > cost ? c : cost;
+    }
+    cost += s > 1 ? s : 0;
+    if (least < 0 || cost < least) { least = cost; best = s; }
+  }
+  return best;
+}
+
+// Adds a group of the segments [seg0, seg1), whose sums take k stages.
+void add_group(Params& p, int seg0, int seg1, int k, int planes) {
+  Group& g = p.group[p.groups];
+  g = Group{};
+  const int n_pairs = pairs(), share = planes == 3 ? 1 : 4;       // (a stage of three parts is three times as long)
+  int tiles = 0, ahead = 0, length = 0;
+  for (int i = seg0; i < seg1; ++i) tiles += p.seg[i].tiles;
+  if (p.groups > 0) {
+    const Group& b = p.group[p.groups - 1];
+    ahead = b.rest * b.parts;
+    length = ceil_div(b.k, b.parts) + (b.parts > 1 ? share : 0);
+    g.first = b.end;
+    g.slot = b.slot + (b.parts > 1 ? ahead : 0);
+  }
+  g.seg0 = seg0;
+  g.seg1 = seg1;
+  g.k = k;
+  g.whole = tiles / n_pairs * n_pairs;
+  g.rest = tiles - g.whole;
+  g.parts = choose_parts(g.rest, k, n_pairs, share, ahead, length);
+  g.end = g.first + g.whole + g.rest * g.parts;
+  p.units = g.end;
+  ++p.groups;
+}
+size_t share_bytes(const Params& p) {
+  size_t n = 0;
+  for (int i = 0; i < p.groups; ++i)
+    if (p.group[i].parts > 1) n += static_cast<size_t>(p.group[i].rest) * p.group[i].parts;
+  return n * kRowTile * kColTile * sizeof(float);
+}
+Segment segment(int a_map, int a_mn, int a_plane, int b_map, int b_mn, int k, int m, int n, void* to, int dtype, const float* inverse) {
+  Segment s{};
+  s.a_map = a_map; s.a_mn = a_mn; s.a_plane = s.a_plane2 = a_plane;
+  s.b_map = s.b_map2 = b_map; s.b_mn = b_mn;
+  s.k_half = k;
+  s.tiles_n = ceil_div(n, kColTile);
+  s.tiles = ceil_div(m, kRowTile) * s.tiles_n;
+  s.m_end = m; s.n_end = n; s.to = to; s.dtype = dtype; s.inverse = inverse;
+  return s;
+}
+
+// Stages per chain of the tensor core (ffn_tc.cu).  Operands of 16 bits leave their own roundings in a sum, 2^-9 (bf16; 2^-12 in fp16) of each summand and
+// independent: over 4,096 of one sign 2^-15, under which a chain of 4,096, low by 1.1e-5, hides; in fp16 one of 2,048.
+int chain(const Layout& l) { return l.planes == 3 ? 1 : l.type == NLFA_DTYPE_F16 ? 16 : 32; }
+
+enum { kMapY = 0, kMapDownColumns = 1 };                   // forward: h, Wd
+void plan_fwd(Params& p, const Call& c, const Layout& l, void* y, const float* inverse) {
+  const int k = ceil_div(c.F, summands(l.planes));
+  p.groups = p.units = 0;
+  p.seg[0] = segment(0, 0, 0, 1, 0, k, c.n, c.o, y, c.dtype, inverse);
+  add_group(p, 0, 1, k, l.planes);
+}
+// backward: maps
+enum { kHiddenRows = 0, kHiddenColumns, kX, kDy, kH, kGateRows, kUpRows };
+void plan_bwd(Params& p, const Call& c, const Layout& l, void* dx, void* dwg, void* dwu, void* dwd, const float* inv_h, const float* inv_d) {
+  const int s = summands(l.planes), kw = ceil_div(c.n, s), kf = ceil_div(c.F, s);
+  int n = 0;
+  p.groups = p.units = 0;
+  if (dwg) p.seg[n++] = segment(kHiddenRows, 1, 0, kX, 1, kw, c.F, c.d, dwg, c.w_dtype, inv_d);
+  if (dwu) p.seg[n++] = segment(kHiddenRows, 1, l.planes, kX, 1, kw, c.F, c.d, dwu, c.w_dtype, inv_d);
+  if (dwd) p.seg[n++] = segment(kDy, 1, 0, kH, 1, kw, c.o, c.F, dwd, c.w_dtype, inv_h);
+  if (n > 0) add_group(p, 0, n, kw, l.planes);
+  if (dx) {
+    p.seg[n] = segment(kHiddenColumns, 0, 0, kGateRows, 1, kf, c.n, c.d, dx, c.x_dtype, inv_d);
+    p.seg[n].a_plane2 = l.planes;
+    p.seg[n].b_map2 = kUpRows;
+    add_group(p, n, n + 1, 2 * kf, l.planes);
+  }
+}
+bool needs_chains(const Params& p, const Layout& l) {
+  for (int i = 0; i < p.groups; ++i)
+    if (p.group[i].k > chain(l)) return true;
+  return false;
+}
+
+// The backward's workspace.
+struct BwdLayout {
+  size_t limits, dy, hidden, shares, bytes;
+};
+BwdLayout bwd_layout(const Call& c, const Layout& l, bool copy_dy) {
+  BwdLayout b{};
+  const size_t two = 2 * static_cast<size_t>(l.planes);
+  size_t at = 256;
+  b.dy = at; if (copy_dy) at = up(at + two * c.n * l.o_pad);
+  b.hidden = at; at = up(at + 2 * two * l.n_rows * l.f_pad);
+  b.shares = at;
+  // enough for any choice of gradients
+  at += static_cast<size_t>(kMostGroups * kPartsPerPair * pairs()) * kRowTile * kColTile * sizeof(float);
+  b.bytes = at;
+  return b;
+}
+
+// ------------------------------------------------------------------------------------------------ float16's range
+
+// h, dg and du of float16 are operands of float16: of a size that nobody has seen to.  They carry one power of two per call that puts what they can be
+// at most, by Cauchy and Schwarz from the lengths of the rows, just below 2^15.  Typical values lie some 2^10 below that, and 2^18 above
+// the smallest normal number.  |f(g)| <= |g|, |f'| < 1.13.
+constexpr int kLimitCtas = 592;
+struct Limits {                     // squares of the largest row lengths; of Wd the largest element
+  float x, gate, up, down;
+  float scale, inverse;             // of h
+};
+struct BwdLimits {
+  float dy, unused;
+  float scale, inverse;             // of dg and du
+};
+struct Rows {
+  const void* src;
+  int dtype, rows, cols, element;   // element: the largest element instead of the largest row
+  float* to;
+};
+struct RowList {
+  Rows r[4];
+  int n;
+};
+
+__device__ __forceinline__ float element_of(const void* p, int dtype, size_t i) {
+  if (dtype == NLFA_DTYPE_F32) return static_cast<const float*>(p)[i];
+  if (dtype == NLFA_DTYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+// A warp per row; rows that are not finite in float16 are left out (their results are not, whatever the factor).
+__global__ void __launch_bounds__(256)
+limits_kernel(const RowList list) {
+  grid_dep_wait();
+  grid_dep_release();
+  const Rows s = list.r[blockIdx.y];
+  const int lane = threadIdx.x & 31;
+  float most = 0.f;
+  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < s.rows; r += gridDim.x * 8) {
+    const size_t row = static_cast<size_t>(r) * s.cols;
+    float sum = 0.f, top = 0.f;
+#pragma unroll 4
+    for (int i = lane; i < s.cols; i += 32) {
+      const float v = element_of(s.src, s.dtype, row + i);
+      sum = fmaf(v, v, sum);
+      top = fabsf(v) <= 65504.f ? fmaxf(top, fabsf(v)) : INFINITY;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    }
+    if (top < INFINITY) most = fmaxf(most, s.element ? top : sum);
+  }
+  // (of non-negative floats the order is that of their bits: no order of these matters)
+  if (lane == 0 && most > 0.f) atomicMax(reinterpret_cast<int*>(s.to), __float_as_int(most));
+}
+
+__device__ __forceinline__ void set_scale(float bound, float* scale, float* inverse) {
+  int e = 0;
+  if (bound > 0.f && bound < INFINITY) {
+    int b;
+    frexpf(bound, &b);                                      // bound < 2^b
+    e = min(max(14 - b, -100), 100);
+  }
+  *scale = ldexpf(1.f, e);
+  *inverse = ldexpf(1.f, -e);
+}
+__global__ void fwd_scale_kernel(Limits* l) {
+  grid_dep_wait();
+  grid_dep_release();
+  set_scale(l->x * sqrtf(l->gate) * sqrtf(l->up), &l->scale, &l->inverse);
+}
+__global__ void bwd_scale_kernel(const Limits* l, BwdLimits* b, float o) {
+  grid_dep_wait();
+  grid_dep_release();
+  const float dh = sqrtf(b->dy) * sqrtf(o) * l->down;
+  set_scale(dh * sqrtf(l->x) * fmaxf(sqrtf(l->gate), 1.13f * sqrtf(l->up)), &b->scale, &b->inverse);
+}
+
+int checked(cudaError_t e) {
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e == cudaSuccess ? NLFA_OK : NLFA_ERR_CUDA;
+}
+
+int find_limits(const RowList& list, void* to, size_t bytes, cudaStream_t st) {
+  const int rc = checked(cudaMemsetAsync(to, 0, bytes, st));
+  if (rc != NLFA_OK) return rc;
+  return checked(launch_kernel(limits_kernel, dim3(kLimitCtas, static_cast<unsigned>(list.n)), dim3(256), 0, st, false, list));
+}
+
+// ------------------------------------------------------------------------------------------------ calls
+
+struct Weights {
+  const void *x, *gate, *up, *down;
+};
+
+// A tensor as an operand: the caller's, or its copy.
+struct Operand {
+  const void* at;
+  long long cols, rows;
+  bool blocked;
+};
+Operand operand(const void* own, const void* copy, bool copied, int cols, int rows) { return {copied ? copy : own, up64(cols), rows, copied}; }
+int columns(CUtensorMap* m, const Operand& a, const Layout& l) { return column_map(m, a.at, l.type, a.cols, a.rows, l.planes, a.blocked); }
+int rows(CUtensorMap* m, const Operand& a, const Layout& l) { return row_map(m, a.at, l.type, a.cols, a.rows, l.planes, a.blocked); }
+
+struct Operands {
+  Operand x, gate, up, down, h;
+};
+Operands operands_of(const Call& c, const Layout& l, const Weights& w, const uint8_t* tape) {
+  return {operand(w.x, tape + l.x, c.copies & kCopyX, c.d, c.n), operand(w.gate, tape + l.gate, c.copies & kCopyGate, c.d, c.F),
+          operand(w.up, tape + l.up, c.copies & kCopyUp, c.d, c.F), operand(w.down, tape + l.down, c.copies & kCopyDown, c.F, c.o),
+          Operand{tape + l.h, l.f_pad, l.n_rows, true}};
+}
+
+Params params(const Call& c, const Layout& l, int activation, uint8_t* tape, unsigned* status) {
+  Params p{};
+  p.rows = c.n;
+  p.cols = c.F;
+  p.n_rows = l.n_rows;
+  p.f_pad = l.f_pad;
+  p.chunk = chain(l);
+  p.activation = activation;
+  p.kept = c.train ? tape + l.kept : nullptr;
+  p.exponents = reinterpret_cast<int8_t*>(tape + l.exponents);
+  p.h = tape + l.h;
+  p.status = status;
+  return p;
+}
+void fill(Maps& maps, int n) {
+  for (int i = n; i < kMostMaps; ++i) maps.m[i] = maps.m[0];
+}
+bool long_sum(int k, const Layout& l) { return ceil_div(k, summands(l.planes)) > chain(l); }
+
+int run_fwd(const Call& c, const Weights& w, int activation, void* y, uint8_t* tape, uint8_t* scratch, cudaStream_t st) {
+  const Layout l = layout(c);
+  unsigned* status = status_block();
+  if (!status) return NLFA_ERR_CUDA;
+  auto copy = [&](int flag, const void* src, int src_dtype, size_t to, int n, int cols) {
+    if (!(c.copies & flag)) return static_cast<int>(NLFA_OK);
+    return copy_rows(src, src_dtype, tape + to, l.type, nullptr, nullptr, n, n, cols, up64(cols), l.planes, st);
+  };
+  int rc = copy(kCopyX, w.x, c.x_dtype, l.x, c.n, c.d);
+  if (rc == NLFA_OK) rc = copy(kCopyGate, w.gate, c.w_dtype, l.gate, c.F, c.d);
+  if (rc == NLFA_OK) rc = copy(kCopyUp, w.up, c.w_dtype, l.up, c.F, c.d);
+  if (rc == NLFA_OK) rc = copy(kCopyDown, w.down, c.w_dtype, l.down, c.o, c.F);
+  Limits* limits = c.dtype == NLFA_DTYPE_F16 ? reinterpret_cast<Limits*>(tape + l.limits) : nullptr;
+  if (rc == NLFA_OK && limits != nullptr) {
+    RowList list{};
+    list.r[0] = {w.x, c.x_dtype, c.n, c.d, 0, &limits->x};
+    list.r[1] = {w.gate, c.w_dtype, c.F, c.d, 0, &limits->gate};
+    list.r[2] = {w.up, c.w_dtype, c.F, c.d, 0, &limits->up};
+    list.r[3] = {w.down, c.w_dtype, c.o, c.F, 1, &limits->down};
+    list.n = c.train ? 4 : 3;
+    rc = find_limits(list, limits, sizeof(Limits), st);
+    if (rc == NLFA_OK) rc = checked(launch_kernel(fwd_scale_kernel, dim3(1), dim3(1), 0, st, overlap_launches(kOverlapRowwise), limits));
+  }
+  if (rc != NLFA_OK) return rc;
+  const Operands a = operands_of(c, l, w, tape);
+  Maps maps;
+  rc = columns(&maps.m[0], a.x, l);
+  if (rc == NLFA_OK) rc = columns(&maps.m[1], a.gate, l);
+  if (rc == NLFA_OK) rc = columns(&maps.m[2], a.up, l);
+  if (rc == NLFA_OK) rc = operands::box_map(&maps.m[3], tape + l.h, l.type, l.f_pad, l.n_rows, l.planes, 32, 1, 1, true);
+  if (rc != NLFA_OK) return rc;
+  fill(maps, 4);
+  Params p = params(c, l, activation, tape, status);
+  p.k = c.d;
+  p.scale = limits != nullptr ? &limits->scale : nullptr;
+  rc = launch_product(kUp, l.type, l.planes, long_sum(c.d, l), p, maps, st);
+  if (rc != NLFA_OK) return rc;
+  rc = columns(&maps.m[0], a.h, l);
+  if (rc == NLFA_OK) rc = columns(&maps.m[1], a.down, l);
+  if (rc != NLFA_OK) return rc;
+  fill(maps, 2);
+  plan_fwd(p, c, l, y, limits != nullptr ? &limits->inverse : nullptr);
+  p.shares = reinterpret_cast<float*>(scratch);
+  return launch_product(kProducts, l.type, l.planes, needs_chains(p, l), p, maps, st);
+}
+
+int run_bwd(const Call& c, const void* dy, const Weights& w, int activation, uint8_t* tape, void* dx, void* dwg, void* dwu, void* dwd,
+            uint8_t* scratch, cudaStream_t st) {
+  const Layout l = layout(c);
+  const bool copy_dy = must_copy(dy, c.dtype, c.dtype, c.o);
+  const BwdLayout b = bwd_layout(c, l, copy_dy);
+  unsigned* status = status_block();
+  if (!status) return NLFA_ERR_CUDA;
+  int rc = NLFA_OK;
+  if (copy_dy) rc = copy_rows(dy, c.dtype, scratch + b.dy, l.type, nullptr, nullptr, c.n, c.n, c.o, l.o_pad, l.planes, st);
+  const Limits* limits = c.dtype == NLFA_DTYPE_F16 ? reinterpret_cast<const Limits*>(tape + l.limits) : nullptr;
+  BwdLimits* more = reinterpret_cast<BwdLimits*>(scratch + b.limits);
+  const bool through = dx || dwg || dwu;                   // whether dg and du are needed
+  if (rc == NLFA_OK && limits != nullptr && through) {
+    RowList list{};
+    list.r[0] = {dy, c.dtype, c.n, c.o, 0, &more->dy};
+    list.n = 1;
+    rc = find_limits(list, more, sizeof(BwdLimits), st);
+    if (rc == NLFA_OK)
+      rc = checked(launch_kernel(bwd_scale_kernel, dim3(1), dim3(1), 0, st, overlap_launches(kOverlapRowwise), limits, more, static_cast<float>(c.o)));
+  }
+  if (rc != NLFA_OK) return rc;
+  const Operands a = operands_of(c, l, w, tape);
+  const Operand up_grad = operand(dy, scratch + b.dy, copy_dy, c.o, c.n), hidden{scratch + b.hidden, l.f_pad, l.n_rows, true};
+  // dg in the first planes, du in the next
+  auto hidden_map = [&](CUtensorMap* m, int box_rows, int blocks, int planes) {
+    return operands::box_map(m, hidden.at, l.type, l.f_pad, l.n_rows, 2 * l.planes, box_rows, blocks, planes, true);
+  };
+  Params p = params(c, l, activation, tape, status);
+  p.dg = scratch + b.hidden;
+  p.du = scratch + b.hidden + static_cast<size_t>(2 * l.planes) * l.n_rows * l.f_pad;
+  Maps maps;
+  if (through) {
+    rc = columns(&maps.m[0], up_grad, l);
+    if (rc == NLFA_OK) rc = rows(&maps.m[1], a.down, l);
+    if (rc == NLFA_OK) rc = hidden_map(&maps.m[2], 32, 1, 1);
+    if (rc != NLFA_OK) return rc;
+    fill(maps, 3);
+    p.k = c.o;
+    p.scale = limits != nullptr ? &more->scale : nullptr;
+    rc = launch_product(kDh, l.type, l.planes, long_sum(c.o, l), p, maps, st);
+    if (rc != NLFA_OK) return rc;
+  }
+  rc = hidden_map(&maps.m[kHiddenRows], summands(l.planes), 2, l.planes);
+  if (rc == NLFA_OK) rc = hidden_map(&maps.m[kHiddenColumns], 128, summands(l.planes) / 64, l.planes);
+  if (rc == NLFA_OK) rc = rows(&maps.m[kX], a.x, l);
+  if (rc == NLFA_OK) rc = rows(&maps.m[kDy], up_grad, l);
+  if (rc == NLFA_OK) rc = rows(&maps.m[kH], a.h, l);
+  if (rc == NLFA_OK) rc = rows(&maps.m[kGateRows], a.gate, l);
+  if (rc == NLFA_OK) rc = rows(&maps.m[kUpRows], a.up, l);
+  if (rc != NLFA_OK) return rc;
+  fill(maps, kUpRows + 1);
+  plan_bwd(p, c, l, dx, dwg, dwu, dwd, limits != nullptr ? &limits->inverse : nullptr, limits != nullptr ? &more->inverse : nullptr);
+  p.shares = reinterpret_cast<float*>(scratch + b.shares);
+  return launch_product(kProducts, l.type, l.planes, needs_chains(p, l), p, maps, st);
+}
+
+}  // namespace
+}  // namespace ffn
+}  // namespace nlfa
+
+using namespace nlfa;
+using namespace nlfa::ffn;
+using rowwise::aligned16;
+
+extern "C" {
+
+int nlfa_gated_ffn_copies(const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype, int dtype, int d,
+                          int F) {
+  return (must_copy(x, x_dtype, dtype, d) ? kCopyX : 0) | (must_copy(w_gate, w_dtype, dtype, d) ? kCopyGate : 0) |
+         (must_copy(w_up, w_dtype, dtype, d) ? kCopyUp : 0) | (must_copy(w_down, w_dtype, dtype, F) ? kCopyDown : 0);
+}
+size_t nlfa_gated_ffn_tape_bytes(int n, int d, int F, int o, int dtype, int copies, int train) {
+  const Call c{dtype, dtype, dtype, n, d, F, o, copies, train};
+  return check_call(c) == NLFA_OK ? layout(c).bytes : 0;
+}
+size_t nlfa_gated_ffn_scratch_bytes(int n, int d, int F, int o, int dtype, int copies, int backward) {
+  const Call c{dtype, dtype, dtype, n, d, F, o, copies, 1};
+  if (check_call(c) != NLFA_OK) return 0;
+  const Layout l = layout(c);
+  // (the gradient of y is copied where it has to be: there is room)
+  if (backward) return bwd_layout(c, l, true).bytes;
+  Params p{};
+  plan_fwd(p, c, l, nullptr, nullptr);
+  return 256 + share_bytes(p);
+}
+
+int nlfa_gated_ffn_fwd(const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype, int dtype,
+                       int activation, int n, int d, int F, int o, void* y, int copies, int train, void* tape, size_t tape_bytes, void* scratch,
+                       size_t scratch_bytes, void* stream) {
+  const Call c{x_dtype, w_dtype, dtype, n, d, F, o, copies, train};
+  const int rc = check_call(c);
+  if (rc != NLFA_OK) return rc;
+  if (activation < NLFA_FFN_SILU || activation > NLFA_FFN_RELU) return NLFA_ERR_BAD_ARGUMENT;
+  if (!w_gate || !w_up || !w_down || !tape || !scratch || (n > 0 && (!x || !y))) return NLFA_ERR_NULL_POINTER;
+  if (n == 0) return NLFA_OK;
+  const int x_bytes = element_bytes(x_dtype), w_bytes = element_bytes(w_dtype);
+  if (!aligned16(tape) || !aligned16(scratch) || !aligned16(y) || !aligned_to(x, x_bytes) || !aligned_to(w_gate, w_bytes) ||
+      !aligned_to(w_up, w_bytes) || !aligned_to(w_down, w_bytes))
+    return NLFA_ERR_MISALIGNED;
+  if (nlfa_gated_ffn_copies(x, x_dtype, w_gate, w_up, w_down, w_dtype, dtype, d, F) & ~copies) return NLFA_ERR_MISALIGNED;
+  if (tape_bytes < layout(c).bytes || scratch_bytes < nlfa_gated_ffn_scratch_bytes(n, d, F, o, dtype, copies, 0)) return NLFA_ERR_SCRATCH_TOO_SMALL;
+  if (!nlfa_device_supported()) return NLFA_ERR_NOT_SM100;
+  if (nlfa_peek_status() != NLFA_OK) return NLFA_ERR_DEVICE_TIMEOUT;
+  return run_fwd(c, {x, w_gate, w_up, w_down}, activation, y, static_cast<uint8_t*>(tape), static_cast<uint8_t*>(scratch),
+                 static_cast<cudaStream_t>(stream));
+}
+
+int nlfa_gated_ffn_bwd(const void* dy, const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype,
+                       int dtype, int activation, int n, int d, int F, int o, int copies, void* tape, size_t tape_bytes, void* dx,
+                       void* dw_gate, void* dw_up, void* dw_down, void* scratch, size_t scratch_bytes, void* stream) {
+  const Call c{x_dtype, w_dtype, dtype, n, d, F, o, copies, 1};
+  const int rc = check_call(c);
+  if (rc != NLFA_OK) return rc;
+  if (activation < NLFA_FFN_SILU || activation > NLFA_FFN_RELU) return NLFA_ERR_BAD_ARGUMENT;
+  if (!dx && !dw_gate && !dw_up && !dw_down) return NLFA_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t w_bytes = element_bytes(w_dtype);
+  if (!aligned16(dx) || !aligned16(dw_gate) || !aligned16(dw_up) || !aligned16(dw_down)) return NLFA_ERR_MISALIGNED;
+  if (n == 0) {                                             // no token: gradients of zero
+    for (void* t : {dw_gate, dw_up, dw_down})
+      if (t != nullptr && cudaMemsetAsync(t, 0, static_cast<size_t>(F) * (t == dw_down ? o : d) * w_bytes, st) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return NLFA_ERR_CUDA;
+      }
+    return NLFA_OK;
+  }
+  // operands that were copied are not read again
+  const void* read[4] = {copies & kCopyX ? nullptr : x, copies & kCopyGate ? nullptr : w_gate, copies & kCopyUp ? nullptr : w_up,
+                         copies & kCopyDown ? nullptr : w_down};
+  if (!dy || !tape || !scratch) return NLFA_ERR_NULL_POINTER;
+  for (int i = 0; i < 4; ++i) {
+    if (!(copies >> i & 1) && !read[i]) return NLFA_ERR_NULL_POINTER;
+    if (!aligned16(read[i])) return NLFA_ERR_MISALIGNED;
+  }
+  if (!aligned16(tape) || !aligned16(scratch) || !aligned_to(dy, element_bytes(dtype))) return NLFA_ERR_MISALIGNED;
+  const Layout l = layout(c);
+  if (tape_bytes < l.bytes || scratch_bytes < bwd_layout(c, l, true).bytes) return NLFA_ERR_SCRATCH_TOO_SMALL;
+  if (!nlfa_device_supported()) return NLFA_ERR_NOT_SM100;
+  if (nlfa_peek_status() != NLFA_OK) return NLFA_ERR_DEVICE_TIMEOUT;
+  return run_bwd(c, dy, {read[0], read[1], read[2], read[3]}, activation, static_cast<uint8_t*>(tape), dx, dw_gate, dw_up, dw_down,
+                 static_cast<uint8_t*>(scratch), st);
+}
+
+}  // extern "C"

@@ -1,0 +1,64 @@
+// Gated feed-forward layer (ffn.cu: layouts, copies, the C ABI; ffn_tc.cu: the products): what the two share.
+#pragma once
+
+#include "common.cuh"
+#include "operands.cuh"
+
+namespace nlfa {
+namespace ffn {
+
+using operands::kRowTile;
+using operands::summands;
+constexpr int kColTile = 256;       // columns of a product's tile
+constexpr int kPartsPerPair = 2;    // shares of odd tiles there is room for, per pair of CTAs and group
+
+enum { kUp = 0, kDh = 1, kProducts = 2 };
+
+// One product of kProducts: to [m_end, n_end] = scale^-1 A B, the sum in `k` stages.
+struct Segment {
+  int a_map, b_map, b_map2;         // b_map2, a_plane2: from stage k_half on (dx = dg Wg + du Wu)
+  int a_plane, a_plane2;
+  int a_mn, b_mn;                   // the sum runs along the operand's rows
+  int k_half;
+  int tiles, tiles_n, m_end, n_end;
+  void* to;
+  int dtype;
+  const float* inverse;             // NULL: 1
+};
+// Segments whose sums have the same number of stages.  Units: whole tiles, as many as all pairs of CTAs get, then the rest, whose sums are cut
+// into parts so that every pair is busy; parts of one index stand together (they read the same summands).
+struct Group {
+  int seg0, seg1;
+  int k, whole, rest, parts;
+  int first, end;                   // units
+  int slot;                         // first share
+};
+constexpr int kMostSegments = 4, kMostGroups = 2, kMostMaps = 8;
+
+struct Maps {
+  CUtensorMap m[kMostMaps];
+};
+
+struct Params {
+  int rows, cols, k;                // kUp, kDh: tokens, hidden columns, length of the sums
+  int n_rows, f_pad;                // extents of h, dg, du
+  int chunk;                        // stages per chain of the tensor core
+  int activation;
+  // kept g and u: 16-bit values with a power of two per 32 values of a row, or float32 (ffn_tc.cu)
+  uint8_t *kept;
+  int8_t* exponents;
+  void *h, *dg, *du;                // float32: written without TMA
+  const float* scale;               // of h (kUp) or dg and du (kDh); NULL: 1
+  Segment seg[kMostSegments];
+  Group group[kMostGroups];
+  int groups, units;
+  float* shares;
+  unsigned* status;
+};
+
+int pairs();                        // of CTAs that run at once
+// Maps: kUp x, Wg, Wu, h to store; kDh dy, Wd, dg and du to store; kProducts as the segments say.
+int launch_product(int mode, int dtype, int planes, bool chains, const Params& p, const Maps& maps, cudaStream_t stream);
+
+}  // namespace ffn
+}  // namespace nlfa

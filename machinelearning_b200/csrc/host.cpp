@@ -509,6 +509,69 @@ struct GatedScanBackward : public Node {
   std::string name() const override { return "GatedScanBackward"; }
 };
 
+// ------------------------------------------------------------------------------------------- gated feed-forward
+
+struct FfnCall {
+  int n, d, F, o, x, w, dtype, activation, copies;
+};
+
+// (y, tape)
+std::pair<Tensor, Tensor> ffn_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, const FfnCall& c, at::ScalarType out,
+                                      bool train) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = c.o;
+  Tensor y = empty(shape, out, x);
+  Tensor tape = empty({static_cast<int64_t>(nlfa_gated_ffn_tape_bytes(c.n, c.d, c.F, c.o, c.dtype, c.copies, train))}, at::kByte, x);
+  Tensor scratch = empty({static_cast<int64_t>(nlfa_gated_ffn_scratch_bytes(c.n, c.d, c.F, c.o, c.dtype, c.copies, 0))}, at::kByte, x);
+  check("nlfa_gated_ffn_fwd",
+        nlfa_gated_ffn_fwd(x.data_ptr(), c.x, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), c.w, c.dtype, c.activation, c.n, c.d, c.F, c.o,
+                           y.data_ptr(), c.copies, train, tape.data_ptr(), static_cast<size_t>(tape.numel()), scratch.data_ptr(),
+                           static_cast<size_t>(scratch.numel()), stream_of(x)));
+  return {y, tape};
+}
+
+struct GatedFfnBackward : public Node {
+  SavedVariable in[4], tape;          // x and the weights, where the tape has no copy
+  std::vector<int64_t> x_shape;
+  at::ScalarType x_dtype, w_dtype, y_dtype;
+  FfnCall call;
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return variable_list(4);
+    Tensor tape_ = tape.unpack(), read[4], out[4];
+    for (int i = 0; i < 4; ++i)
+      if (!(call.copies >> i & 1)) read[i] = in[i].unpack();
+    const c10::cuda::CUDAGuard guard(tape_.device());
+    const FfnCall& c = call;
+    Tensor g = contiguous(cast(grads[0], y_dtype));
+    const std::vector<int64_t> shapes[4] = {x_shape, {c.F, c.d}, {c.F, c.d}, {c.o, c.F}};
+    for (int i = 0; i < 4; ++i)
+      if (task_should_compute_output(i)) out[i] = empty(shapes[i], i == 0 ? x_dtype : w_dtype, tape_);
+    auto at = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    Tensor scratch = empty({static_cast<int64_t>(nlfa_gated_ffn_scratch_bytes(c.n, c.d, c.F, c.o, c.dtype, c.copies, 1))}, at::kByte, tape_);
+    check("nlfa_gated_ffn_bwd",
+          nlfa_gated_ffn_bwd(g.data_ptr(), at(read[0]), c.x, at(read[1]), at(read[2]), at(read[3]), c.w, c.dtype, c.activation, c.n, c.d, c.F,
+                             c.o, c.copies, tape_.data_ptr(), static_cast<size_t>(tape_.numel()), at(out[0]), at(out[1]), at(out[2]), at(out[3]),
+                             scratch.data_ptr(), static_cast<size_t>(scratch.numel()), stream_of(tape_)));
+    variable_list list;
+    for (const Tensor& t : out)
+      if (t.defined()) list.push_back(t);
+    list = once(std::move(list), grads[0]);
+    size_t next = 0;
+    variable_list result(4);
+    for (int i = 0; i < 4; ++i)
+      if (out[i].defined()) result[i] = list[next++];
+    return result;
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable& v : in) v.reset_data();
+    tape.reset_data();
+  }
+  std::string name() const override { return "GatedFfnBackward"; }
+};
+
 // ------------------------------------------------------------------------------------------- gradient clip
 
 struct Span {
@@ -993,6 +1056,53 @@ PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// gated_ffn(x, w_gate, w_up, w_down, activation code) -> y | None
+PyObject* py_gated_ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || !is_tensor(a[0]) || !is_tensor(a[1]) || !is_tensor(a[2]) || !is_tensor(a[3])) return decline();
+  Tensor t[4] = {tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3])};
+  for (const Tensor& v : t)
+    if (!plain(v) || v.device() != t[0].device() || dtype_code(v.scalar_type()) < 0) return decline();
+  const Tensor &x = t[0], &wg = t[1], &wu = t[2], &wd = t[3];
+  if (!watched(x) || x.dim() < 1 || wg.dim() != 2 || wu.sizes() != wg.sizes() || wd.dim() != 2 || wd.size(1) != wg.size(0) ||
+      wg.size(1) != x.size(-1) || wu.scalar_type() != wg.scalar_type() || wd.scalar_type() != wg.scalar_type())
+    return decline();
+  const auto ac = autocast_dtype();
+  if (!ac && x.scalar_type() != wg.scalar_type()) return decline();
+  const at::ScalarType out = ac ? *ac : x.scalar_type();
+  constexpr int64_t kMostRows = int64_t(1) << 30, kMostWidth = int64_t(1) << 24;
+  const int64_t d = wg.size(1), F = wg.size(0), o = wd.size(0);
+  if (dtype_code(out) < 0 || d < 1 || F < 1 || o < 1 || d > kMostWidth || F > kMostWidth || o > kMostWidth || x.numel() / d > kMostRows)
+    return decline();
+  FfnCall c{static_cast<int>(x.numel() / d), static_cast<int>(d), static_cast<int>(F), static_cast<int>(o), dtype_code(x.scalar_type()),
+            dtype_code(wg.scalar_type()), dtype_code(out), integer(a[4]), 0};
+  Tensor y;
+  {
+    py::gil_scoped_release no_gil;
+    const c10::cuda::CUDAGuard guard(x.device());
+    for (Tensor& v : t) v = contiguous(v);
+    c.copies = nlfa_gated_ffn_copies(x.data_ptr(), c.x, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), c.w, c.dtype, c.d, c.F);
+    const bool train = recording({&t[0], &t[1], &t[2], &t[3]});
+    Tensor tape;
+    std::tie(y, tape) = ffn_forward(x, wg, wu, wd, c, out, train);
+    if (train) {
+      auto node = make_node<GatedFfnBackward>();
+      node->set_next_edges(torch::autograd::collect_next_edges(x, wg, wu, wd));
+      for (int i = 0; i < 4; ++i)
+        if (!(c.copies >> i & 1)) node->in[i] = SavedVariable(t[i], false);
+      node->tape = SavedVariable(tape, false);
+      node->x_shape = x.sizes().vec();
+      node->x_dtype = x.scalar_type();
+      node->w_dtype = wg.scalar_type();
+      node->y_dtype = out;
+      node->call = c;
+      torch::autograd::set_history(y, node);
+    }
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 // gated_scan(gate, value, state | None, reset | None, lengths | None, activation code) -> (h, last) | None
 PyObject* py_gated_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -1102,7 +1212,7 @@ PyObject* py_watch(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef g_methods[] = {NLFA_METHOD(attn),        NLFA_METHOD(attn_fwd),    NLFA_METHOD(attn_bwd),  NLFA_METHOD(attn_cached),
                            NLFA_METHOD(qk_prologue), NLFA_METHOD(value_blend), NLFA_METHOD(head_gate), NLFA_METHOD(linear_ce),
                            NLFA_METHOD(embedding),   NLFA_METHOD(clip_grads),  NLFA_METHOD(configure), NLFA_METHOD(watch),
-                           NLFA_METHOD(gated_scan),
+                           NLFA_METHOD(gated_ffn),   NLFA_METHOD(gated_scan),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", "torch-facing call path of libnlfa (host.cpp)", -1, g_methods};
 

@@ -67,3 +67,33 @@ def activation(g, kind):
         p = 0.5 * (1 + _erf(g / math.sqrt(2)))
         return g * p, p + g * np.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
     return np.maximum(g, 0), (g > 0).astype(np.float64)
+
+
+def gated_ffn(x, w_gate, w_up, w_down, kind="silu", dy=None, step=0.0):
+    """dict of ``y`` and, for an upstream ``dy``, ``dx``, ``dw_gate``, ``dw_up``, ``dw_down``; ``noise_*``: the standard deviation that these have when h, dg
+    and du are rounded independently, each by a standard deviation of ``step`` of its value, and ``size_*``: the sums of their summands' magnitudes."""
+    x, wg, wu, wd = (np.asarray(t, np.float64) for t in (x, w_gate, w_up, w_down))
+    g, u = x @ wg.T, x @ wu.T
+    a, da = activation(g, kind)
+    h = a * u
+    out = {"y": h @ wd.T, "noise_y": step * np.sqrt((h * h) @ (wd * wd).T), "g": g, "u": u, "h": h}
+    # what an error of g or u in proportion to their own summands does to h, dg and du
+    size_g, size_u = np.abs(x) @ np.abs(wg).T, np.abs(x) @ np.abs(wu).T
+    size_h = np.abs(h) + 1.2 * size_g * np.abs(u) + np.abs(a) * size_u
+    out["size_y"] = size_h @ np.abs(wd).T
+    if dy is None:
+        return out
+    dy = np.asarray(dy, np.float64)
+    dh = dy @ wd
+    du, dg = dh * a, dh * u * da
+    size_dh = np.abs(dy) @ np.abs(wd)
+    size_du = size_dh * (np.abs(a) + 1.2 * size_g)
+    size_dg = size_dh * (np.abs(u * da) + 1.2 * size_u + 1.2 * np.abs(u) * size_g)      # |f'| < 1.2, |f''| < 1.2
+    out.update(dx=dg @ wg + du @ wu, dw_gate=dg.T @ x, dw_up=du.T @ x, dw_down=dy.T @ h, dg=dg, du=du)
+    out["size_dx"] = size_dg @ np.abs(wg) + size_du @ np.abs(wu)
+    out["size_dw_gate"], out["size_dw_up"], out["size_dw_down"] = size_dg.T @ np.abs(x), size_du.T @ np.abs(x), np.abs(dy).T @ size_h
+    sq = np.square
+    out["noise_dx"] = step * np.sqrt(sq(dg) @ sq(wg) + sq(du) @ sq(wu))
+    out["noise_dw_gate"], out["noise_dw_up"] = step * np.sqrt(sq(dg).T @ sq(x)), step * np.sqrt(sq(du).T @ sq(x))
+    out["noise_dw_down"] = step * np.sqrt(sq(dy).T @ sq(h))
+    return out
