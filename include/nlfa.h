@@ -382,21 +382,24 @@ int nlfa_clip_grads(const nlfa_grad* grads, int count, float max_norm, int norm,
  * contiguous.  h_0 is `state` [B, D] (NULL: zeros), `last` [B, D] the state behind the last step, both float32, as all sums are.
  * `reset` [B, T] (NULL: none): where it is not 0, h_{t-1} counts as zero, whatever it holds.  `lengths` [B], int32 or int64
  * (length_bytes; NULL: all T): steps from lengths[b] on (taken between 0 and T) leave the state as it is, their h is zero, and what gate and value hold there reaches nothing.
- * `tape` (nlfa_gated_scan_tape_bytes; NULL when no backward follows) takes the states at the start of every 16 steps.
+ * `tape` (nlfa_gated_scan_tape_bytes; NULL when no backward follows) takes the states at the start of every 16 steps (float32: 8).
+ * `scratch`, 16-byte aligned (nlfa_gated_scan_scratch_bytes; 0: none): maps of segments, into which long sequences of few channels are cut.
  * An infinite state or value makes the states behind it infinite or NaN, up to the next reset.
- * Bit-reproducible; may be captured; no scratch.  Any alignment of the element type; pairs of channels are faster. */
+ * Bit-reproducible; may be captured.  Any alignment of the element type; rows on 16 bytes are faster. */
 #define NLFA_SCAN_NONE 0
 #define NLFA_SCAN_POSITIVE 1
-size_t nlfa_gated_scan_tape_bytes(int B, int T, int D);
+size_t nlfa_gated_scan_tape_bytes(int B, int T, int D, int dtype);
+size_t nlfa_gated_scan_scratch_bytes(int B, int T, int D, int dtype);
 int nlfa_gated_scan_fwd(const void* gate, long long gate_b, long long gate_t, const void* value, long long value_b, long long value_t,
                         int dtype, const float* state, const unsigned char* reset, const void* lengths, int length_bytes, int activation,
-                        int B, int T, int D, void* h, float* last, void* tape, size_t tape_bytes, void* stream);
+                        int B, int T, int D, void* h, float* last, void* tape, size_t tape_bytes, void* scratch, size_t scratch_bytes,
+                        void* stream);
 /* Its gradients: dgate and dvalue, contiguous [B, T, D] of `dtype` (zeros where a step does not count), dstate [B, D]; any may be NULL.
  * dh is contiguous [B, T, D], dlast [B, D]; NULL stands for zeros.  The tape is the forward's. */
 int nlfa_gated_scan_bwd(const void* dh, const float* dlast, const void* gate, long long gate_b, long long gate_t, const void* value,
                         long long value_b, long long value_t, int dtype, const unsigned char* reset, const void* lengths, int length_bytes,
                         int activation, int B, int T, int D, const void* tape, size_t tape_bytes, void* dgate, void* dvalue, float* dstate,
-                        void* stream);
+                        void* scratch, size_t scratch_bytes, void* stream);
 
 /* Gated feed-forward layer, what nanolab's SwiGLU does (nanolab/model.py:29-43): for x [n, d], w_gate and w_up [F, d], w_down [o, F]
  *   y = (f(x w_gate^T) * (x w_up^T)) w_down^T,  f one of NLFA_FFN_*  (gelu: with erf).

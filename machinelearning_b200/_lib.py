@@ -84,11 +84,12 @@ SIGNATURES = {
                            + [_c_float, ctypes.c_longlong, _c_void_p, _c_size_t, _c_void_p]),
     "nlfa_clip_scratch_bytes": (_c_size_t, []),
     "nlfa_clip_grads": (_c_int, [_c_void_p, _c_int, _c_float, _c_int, _c_int, _c_void_p, _c_void_p, _c_size_t, _c_void_p]),
-    "nlfa_gated_scan_tape_bytes": (_c_size_t, [_c_int] * 3),
+    "nlfa_gated_scan_tape_bytes": (_c_size_t, [_c_int] * 4),
+    "nlfa_gated_scan_scratch_bytes": (_c_size_t, [_c_int] * 4),
     "nlfa_gated_scan_fwd": (_c_int, [_c_void_p, ctypes.c_longlong, ctypes.c_longlong] * 2 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 5
-                            + [_c_void_p] * 3 + [_c_size_t, _c_void_p]),
+                            + [_c_void_p] * 3 + [_c_size_t, _c_void_p, _c_size_t, _c_void_p]),
     "nlfa_gated_scan_bwd": (_c_int, [_c_void_p] * 2 + [_c_void_p, ctypes.c_longlong, ctypes.c_longlong] * 2 + [_c_int] + [_c_void_p] * 2
-                            + [_c_int] * 5 + [_c_void_p, _c_size_t] + [_c_void_p] * 4),
+                            + [_c_int] * 5 + [_c_void_p, _c_size_t] + [_c_void_p] * 4 + [_c_size_t, _c_void_p]),
     "nlfa_gated_ffn_copies": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 3 + [_c_int] * 4),
     "nlfa_gated_ffn_tape_bytes": (_c_size_t, [_c_int] * 7),
     "nlfa_gated_ffn_scratch_bytes": (_c_size_t, [_c_int] * 7),

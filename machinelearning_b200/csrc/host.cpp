@@ -456,18 +456,25 @@ ScanCall scan_call(const Tensor& gate, const Tensor& reset, const Tensor& length
           reset.defined() ? static_cast<const unsigned char*>(reset.data_ptr()) : nullptr, lengths.defined() ? lengths.data_ptr() : nullptr};
 }
 
+Tensor scan_scratch(const ScanCall& c, const Tensor& like) {
+  const size_t bytes = nlfa_gated_scan_scratch_bytes(c.B, c.T, c.D, c.dtype);
+  return bytes > 0 ? empty({static_cast<int64_t>(bytes)}, at::kByte, like) : Tensor();
+}
+
 // (h, last, tape; no tape unless a backward follows)
 std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor& gate, const Tensor& value, const Tensor& state, const Tensor& reset,
                                                 const Tensor& lengths, int activation, bool train) {
   const c10::cuda::CUDAGuard guard(gate.device());
   const ScanCall c = scan_call(gate, reset, lengths, activation);
   Tensor h = empty(gate.sizes(), gate.scalar_type(), gate), last = empty({c.B, c.D}, at::kFloat, gate), tape;
-  if (train) tape = empty({static_cast<int64_t>(nlfa_gated_scan_tape_bytes(c.B, c.T, c.D))}, at::kByte, gate);
+  if (train) tape = empty({static_cast<int64_t>(nlfa_gated_scan_tape_bytes(c.B, c.T, c.D, c.dtype))}, at::kByte, gate);
+  Tensor scratch = scan_scratch(c, gate);
   check("nlfa_gated_scan_fwd",
         nlfa_gated_scan_fwd(gate.data_ptr(), gate.stride(0), gate.stride(1), value.data_ptr(), value.stride(0), value.stride(1), c.dtype,
                             state.defined() ? static_cast<const float*>(state.data_ptr()) : nullptr, c.reset, c.lengths, c.length_bytes,
                             activation, c.B, c.T, c.D, h.data_ptr(), static_cast<float*>(last.data_ptr()), train ? tape.data_ptr() : nullptr,
-                            train ? static_cast<size_t>(tape.numel()) : 0, stream_of(gate)));
+                            train ? static_cast<size_t>(tape.numel()) : 0, scratch.defined() ? scratch.data_ptr() : nullptr,
+                            scratch.defined() ? static_cast<size_t>(scratch.numel()) : 0, stream_of(gate)));
   return {h, last, tape};
 }
 
@@ -487,11 +494,12 @@ struct GatedScanBackward : public Node {
       if (task_should_compute_output(i)) out[i] = empty(gate_.sizes(), gate_.scalar_type(), gate_);
     if (task_should_compute_output(2)) out[2] = empty({c.B, c.D}, at::kFloat, gate_);
     auto at = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    Tensor scratch = scan_scratch(c, gate_);
     check("nlfa_gated_scan_bwd",
           nlfa_gated_scan_bwd(at(dh), static_cast<const float*>(at(dlast)), gate_.data_ptr(), gate_.stride(0), gate_.stride(1), value_.data_ptr(),
                               value_.stride(0), value_.stride(1), c.dtype, c.reset, c.lengths, c.length_bytes, activation, c.B, c.T, c.D,
-                              tape_.data_ptr(), static_cast<size_t>(tape_.numel()), at(out[0]), at(out[1]), static_cast<float*>(at(out[2])),
-                              stream_of(gate_)));
+                              tape_.data_ptr(), static_cast<size_t>(tape_.numel()), at(out[0]), at(out[1]), static_cast<float*>(at(out[2])), at(scratch),
+                              scratch.defined() ? static_cast<size_t>(scratch.numel()) : 0, stream_of(gate_)));
     variable_list list;
     for (const Tensor& t : out)
       if (t.defined()) list.push_back(t);

@@ -2,7 +2,7 @@
 
 ``gated_scan(gate, value, state)`` walks ``h_t = (1 - s_t) h_{t-1} + s_t f(value_t)``, ``s = sigmoid(gate)``, for every channel: in one pass
 over the data (``csrc/scan.cu``), where torch would join runs of 1, 2, 4, ... steps in some 2 log2(T) passes, and with gradients that
-need no more than the states at every 16th step.
+need no more than the states at every 16th step (float32: every 8th).
 
 An ``autograd`` node over the C entry points.  No CPU path: ``supports`` says whether a call can run; the function raises otherwise.
 """
@@ -43,6 +43,10 @@ def _rows(t):
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+def _scratch(lib, gate):
+    return torch.empty(lib.nlfa_gated_scan_scratch_bytes(*gate.shape, _DTYPE_CODE[gate.dtype]), dtype=torch.uint8, device=gate.device)
+
+
 def fwd(gate, value, state, reset, lengths, activation: str, train: bool):
     """(h, last float32, tape) through the C ABI; no elements in ``tape`` unless ``train``."""
     lib = _lib_or_raise()
@@ -51,11 +55,13 @@ def fwd(gate, value, state, reset, lengths, activation: str, train: bool):
     B, T, D = gate.shape
     h = torch.empty((B, T, D), dtype=gate.dtype, device=gate.device)
     last = torch.empty((B, D), dtype=torch.float32, device=gate.device)
-    tape = torch.empty(lib.nlfa_gated_scan_tape_bytes(B, T, D) if train else 0, dtype=torch.uint8, device=gate.device)
+    tape = torch.empty(lib.nlfa_gated_scan_tape_bytes(B, T, D, _DTYPE_CODE[gate.dtype]) if train else 0, dtype=torch.uint8, device=gate.device)
     with flash_cuda._on_device(gate.device.index):
+        scratch = _scratch(lib, gate)
         st = lib.nlfa_gated_scan_fwd(gate.data_ptr(), gate.stride(0), gate.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
                                      _DTYPE_CODE[gate.dtype], _ptr(state), *_mask_args(reset, lengths), ACTIVATIONS[activation], B, T, D,
-                                     h.data_ptr(), last.data_ptr(), tape.data_ptr() if train else None, tape.numel(), _stream(gate))
+                                     h.data_ptr(), last.data_ptr(), tape.data_ptr() if train else None, tape.numel(), scratch.data_ptr(),
+                                     scratch.numel(), _stream(gate))
     _lib.check("nlfa_gated_scan_fwd", st)
     return h, last, tape
 
@@ -67,9 +73,11 @@ def bwd(dh, dlast, gate, value, reset, lengths, tape, activation: str, want=(Tru
     dgate, dvalue = (torch.empty((B, T, D), dtype=gate.dtype, device=gate.device) if w else None for w in want[:2])
     dstate = torch.empty((B, D), dtype=torch.float32, device=gate.device) if want[2] else None
     with flash_cuda._on_device(gate.device.index):
+        scratch = _scratch(lib, gate)
         st = lib.nlfa_gated_scan_bwd(_ptr(dh), _ptr(dlast), gate.data_ptr(), gate.stride(0), gate.stride(1), value.data_ptr(), value.stride(0),
                                      value.stride(1), _DTYPE_CODE[gate.dtype], *_mask_args(reset, lengths), ACTIVATIONS[activation], B, T, D,
-                                     tape.data_ptr(), tape.numel(), _ptr(dgate), _ptr(dvalue), _ptr(dstate), _stream(gate))
+                                     tape.data_ptr(), tape.numel(), _ptr(dgate), _ptr(dvalue), _ptr(dstate), scratch.data_ptr(),
+                                     scratch.numel(), _stream(gate))
     _lib.check("nlfa_gated_scan_bwd", st)
     return dgate, dvalue, dstate
 

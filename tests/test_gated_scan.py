@@ -54,19 +54,23 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
     _build.build()
     lib = _lib.load()
 
-    def fwd(z=256, v=256, dt=2, state=None, reset=None, lengths=None, lb=0, act=0, B=2, T=40, D=8, h=256, last=256, tape=256, tb=None):
-        need = lib.nlfa_gated_scan_tape_bytes(2, 40, 8)
-        return lib.nlfa_gated_scan_fwd(z, T * D, D, v, T * D, D, dt, state, reset, lengths, lb, act, B, T, D, h, last, tape, need if tb is None else tb, None)
-    assert lib.nlfa_gated_scan_tape_bytes(2, 40, 8) == 2 * 3 * 8 * 4 and lib.nlfa_gated_scan_tape_bytes(2, -1, 8) == 0
+    def fwd(z=256, v=256, dt=2, state=None, reset=None, lengths=None, lb=0, act=0, B=2, T=40, D=8, h=256, last=256, tape=256, tb=None,
+            s=256, sb=1 << 20):
+        need = lib.nlfa_gated_scan_tape_bytes(2, 40, 8, 2)
+        return lib.nlfa_gated_scan_fwd(z, T * D, D, v, T * D, D, dt, state, reset, lengths, lb, act, B, T, D, h, last, tape, need if tb is None else tb,
+                                       s, sb, None)
+    assert lib.nlfa_gated_scan_tape_bytes(2, 40, 8, 2) == 2 * 3 * 8 * 4 and lib.nlfa_gated_scan_tape_bytes(2, 40, 8, 0) == 2 * 5 * 8 * 4
+    assert lib.nlfa_gated_scan_tape_bytes(2, -1, 8, 2) == 0 and lib.nlfa_gated_scan_scratch_bytes(2, 40, 8, 9) == 0
     assert fwd(B=-1) == 2 and fwd(T=-1) == 2 and fwd(D=-1) == 2 and fwd(T=(1 << 30) + 1) == 2
     assert fwd(dt=3) == 3 and fwd(act=2) == 14 and fwd(lengths=256, lb=2) == 14
     assert fwd(z=None) == 1 and fwd(v=None) == 1 and fwd(h=None) == 1 and fwd(last=None) == 1
     assert fwd(z=257) == 6 and fwd(v=257) == 6 and fwd(h=258, dt=0) == 6 and fwd(state=258) == 6 and fwd(last=258) == 6 and fwd(lengths=260, lb=8) == 6
-    assert fwd(tb=191) == 11
+    assert fwd(tb=191) == 11 and fwd(s=264) == 6
     assert fwd(B=0, z=None, v=None, h=None, last=None) == 0 and fwd(D=0) == 0
 
-    def bwd(z=256, v=256, dt=2, dh=256, dlast=256, lengths=None, lb=0, act=0, B=2, T=40, D=8, tape=256, tb=192, dz=256, dv=256, ds=256):
-        return lib.nlfa_gated_scan_bwd(dh, dlast, z, T * D, D, v, T * D, D, dt, None, lengths, lb, act, B, T, D, tape, tb, dz, dv, ds, None)
+    def bwd(z=256, v=256, dt=2, dh=256, dlast=256, lengths=None, lb=0, act=0, B=2, T=40, D=8, tape=256, tb=192, dz=256, dv=256, ds=256,
+            s=256, sb=1 << 20):
+        return lib.nlfa_gated_scan_bwd(dh, dlast, z, T * D, D, v, T * D, D, dt, None, lengths, lb, act, B, T, D, tape, tb, dz, dv, ds, s, sb, None)
     assert bwd(B=-1) == 2 and bwd(dt=7) == 3 and bwd(act=-1) == 14 and bwd(lengths=256, lb=3) == 14
     assert bwd(z=None) == 1 and bwd(v=None) == 1 and bwd(tape=None) == 1
     assert bwd(dh=257) == 6 and bwd(dz=257) == 6 and bwd(dv=257) == 6 and bwd(dlast=258) == 6 and bwd(ds=258) == 6 and bwd(tape=258) == 6
@@ -113,7 +117,7 @@ def _check(got, want, dtype, T, what=("h", "last", "dgate", "dvalue", "dstate"))
 
 
 SIZES = [(1, 1, 1), (2, 1, 64), (5, 2, 7), (3, 15, 33), (2, 16, 64), (1, 17, 2), (2, 63, 66), (2, 64, 65), (1, 65, 130), (2, 129, 30), (2, 513, 34),
-         (1, 1100, 70), (1, 2500, 3)]
+         (1, 1100, 70), (1, 2500, 3), (1, 1300, 136), (40, 70, 520)]
 
 
 @pytest.mark.gpu
