@@ -409,15 +409,15 @@ int nlfa_gated_scan_bwd(const void* dh, const float* dlast, const void* gate, lo
  * precision; in float16 they carry a power of two, so that they neither overflow nor lose digits below the type's normal range.
  *
  * `copies` (nlfa_gated_ffn_copies): which of x, w_gate, w_up, w_down (bits 0 to 3) the forward copies into the tape, because the products cannot read
- * them as they lie: of another type, float32, rows not a multiple of 64 long, not 16-byte aligned.  The backward takes the same value; operands that
+ * them as they lie: of another type, float32, rows not a multiple of 64 long, not 16-byte aligned (without `train` up to 32 tokens take most as they lie).  The backward takes the same value; operands that
  * were copied may be NULL there, the others have to be what they were.  `tape`: with `train` what the backward reads, without it workspace.
  * dx (x_dtype), dw_gate, dw_up, dw_down (w_dtype): any may be NULL.  Bit-reproducible; may be captured.  Tape, scratch, y and the gradients are 16-byte
  * aligned.  Needs compute capability 10.x. */
 #define NLFA_FFN_SILU 0
 #define NLFA_FFN_GELU 1
 #define NLFA_FFN_RELU 2
-int nlfa_gated_ffn_copies(const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype, int dtype, int d,
-                          int F);
+int nlfa_gated_ffn_copies(const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype, int dtype, int n, int d,
+                          int F, int train);
 size_t nlfa_gated_ffn_tape_bytes(int n, int d, int F, int o, int dtype, int copies, int train);
 size_t nlfa_gated_ffn_scratch_bytes(int n, int d, int F, int o, int dtype, int copies, int backward);
 int nlfa_gated_ffn_fwd(const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype, int dtype,

@@ -374,7 +374,7 @@ def gated_ffn_bwd(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up:
                   activation: str, dtype: torch.dtype, want: list[bool]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """A gradient that is not wanted costs nothing and comes back without elements."""
     inputs = _aligned((x, w_gate, w_up, w_down))
-    grads = _gf.bwd(dy.to(dtype).contiguous(), *inputs, tape, _gf.copies_of(*inputs, dtype), [t.shape for t in inputs], x.dtype, w_gate.dtype,
+    grads = _gf.bwd(dy.to(dtype).contiguous(), *inputs, tape, _gf.copies_of(*inputs, dtype, True), [t.shape for t in inputs], x.dtype, w_gate.dtype,
                     activation, want)
     return tuple(t.new_empty(0) if g is None else g for t, g in zip(inputs, grads))
 

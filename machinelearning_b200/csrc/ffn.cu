@@ -4,13 +4,14 @@
 //   dh = dy Wd,  du = dh f(g),  dg = dh u f'(g)
 //   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h
 //
-// Bound by the tensor cores: 2 N F (2 d + o) operations forward and twice that backward, in four launches of products (ffn_tc.cu).  g and u exist in
-// tensor memory, and in the tape for the backward; dh in tensor memory alone.  Between the products h, dg and du are operands: 16 bits (float32:
+// Bound by the tensor cores: 2 N F (2 d + o) operations forward and twice that backward, in four launches of products (ffn_tc.cu).  g, u and dh exist in
+// tensor memory alone; the tape keeps f(g) and u f'(g) for the backward.  Between the products h, dg and du are operands: 16 bits (float32:
 // three bf16 parts), one rounding each beside that of the results.
 //
 // This file has what goes around the products: 16-bit copies of operands that TMA cannot read as they are, the list of tiles and
 // parts, and the powers of two that hold float16's h, dg and du inside their type's range.
 #include <cmath>
+#include <cstdlib>
 
 #include "ffn.cuh"
 #include "rowwise.cuh"
@@ -53,6 +54,11 @@ int check_call(const Call& c) {
 
 bool must_copy(const void* p, int type, int dtype, int cols) { return dtype == NLFA_DTYPE_F32 || type != dtype || cols % 64 != 0 || !aligned16(p); }
 
+bool is_few(const void* x, const void* gate, const void* up, const void* down, int w_dtype, int dtype, int n, int d, int F, int train) {
+  static const char* env = getenv("FFN_FEW");
+  return !train && n <= (env ? atoi(env) : kFewTokens) && few_types(w_dtype, dtype) && d % 8 == 0 && F % 8 == 0 && aligned16(x) && aligned16(gate) && aligned16(up) && aligned16(down);
+}
+
 // What the forward leaves for the backward, and (inference) the forward's own workspace.
 struct Layout {
   int planes, n_rows, d_pad, f_pad, o_pad;
@@ -74,10 +80,11 @@ Layout layout(const Call& c) {
   l.gate = at; if (c.copies & kCopyGate) at = up(at + two * c.F * l.d_pad);
   l.up = at; if (c.copies & kCopyUp) at = up(at + two * c.F * l.d_pad);
   l.down = at; if (c.copies & kCopyDown) at = up(at + two * c.o * l.f_pad);
-  l.h = at; at = up(at + two * hidden);
+  l.h = at; at = up(at + two * hidden);                   // (a few tokens: float32, which takes less than a tile of 256 in 16 bits)
   if (c.train) {
-    l.kept = at; at = up(at + 2 * hidden * (l.planes == 3 ? 4 : 2));
-    l.exponents = at; if (l.planes == 1) at = up(at + 2 * hidden / 32);
+    const bool wide = c.dtype != NLFA_DTYPE_BF16;
+    l.kept = at; at = up(at + 2 * hidden * (wide ? 4 : 2));
+    l.exponents = at; if (!wide) at = up(at + 2 * hidden / 32);
   }
   l.bytes = at;
   return l;
@@ -216,34 +223,38 @@ struct Rows {
   const void* src;
   int dtype, rows, cols, element;   // element: the largest element instead of the largest row
   float* to;
+  int vec;
 };
 struct RowList {
   Rows r[4];
   int n;
 };
 
-__device__ __forceinline__ float element_of(const void* p, int dtype, size_t i) {
-  if (dtype == NLFA_DTYPE_F32) return static_cast<const float*>(p)[i];
-  if (dtype == NLFA_DTYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-
-// A warp per row; rows that are not finite in float16 are left out (their results are not, whatever the factor).
-__global__ void __launch_bounds__(256)
-limits_kernel(const RowList list) {
-  grid_dep_wait();
-  grid_dep_release();
-  const Rows s = list.r[blockIdx.y];
+// A warp per row; rows that are not finite in float16 are left out (their results are not, whatever the factor).  Eight elements a load where rows lie on
+// 16 bytes (element by element 65,536 x 768 takes 42 us).
+template <typename S>
+__device__ __forceinline__ void largest_row(const Rows& s) {
+  const S* src = static_cast<const S*>(s.src);
   const int lane = threadIdx.x & 31;
   float most = 0.f;
   for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < s.rows; r += gridDim.x * 8) {
-    const size_t row = static_cast<size_t>(r) * s.cols;
+    const S* row = src + static_cast<size_t>(r) * s.cols;
     float sum = 0.f, top = 0.f;
-#pragma unroll 4
-    for (int i = lane; i < s.cols; i += 32) {
-      const float v = element_of(s.src, s.dtype, row + i);
+    auto add = [&](float v) {
       sum = fmaf(v, v, sum);
       top = fabsf(v) <= 65504.f ? fmaxf(top, fabsf(v)) : INFINITY;
+    };
+    if (s.vec) {
+#pragma unroll 4
+      for (int i = 8 * lane; i < s.cols; i += 256) {
+        float v[8];
+        rowwise::Elem<S>::load(row + i, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) add(v[j]);
+      }
+    } else {
+#pragma unroll 4
+      for (int i = lane; i < s.cols; i += 32) add(static_cast<float>(row[i]));
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
@@ -254,6 +265,15 @@ limits_kernel(const RowList list) {
   }
   // (of non-negative floats the order is that of their bits: no order of these matters)
   if (lane == 0 && most > 0.f) atomicMax(reinterpret_cast<int*>(s.to), __float_as_int(most));
+}
+__global__ void __launch_bounds__(256)
+limits_kernel(const RowList list) {
+  grid_dep_wait();
+  grid_dep_release();
+  const Rows s = list.r[blockIdx.y];
+  if (s.dtype == NLFA_DTYPE_F32) largest_row<float>(s);
+  else if (s.dtype == NLFA_DTYPE_F16) largest_row<__half>(s);
+  else largest_row<__nv_bfloat16>(s);
 }
 
 __device__ __forceinline__ void set_scale(float bound, float* scale, float* inverse) {
@@ -283,7 +303,8 @@ int checked(cudaError_t e) {
   return e == cudaSuccess ? NLFA_OK : NLFA_ERR_CUDA;
 }
 
-int find_limits(const RowList& list, void* to, size_t bytes, cudaStream_t st) {
+int find_limits(RowList list, void* to, size_t bytes, cudaStream_t st) {
+  for (Rows& r : list.r) r.vec = r.cols % 8 == 0 && aligned16(r.src);
   const int rc = checked(cudaMemsetAsync(to, 0, bytes, st));
   if (rc != NLFA_OK) return rc;
   return checked(launch_kernel(limits_kernel, dim3(kLimitCtas, static_cast<unsigned>(list.n)), dim3(256), 0, st, false, list));
@@ -445,8 +466,9 @@ using rowwise::aligned16;
 
 extern "C" {
 
-int nlfa_gated_ffn_copies(const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype, int dtype, int d,
-                          int F) {
+int nlfa_gated_ffn_copies(const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype, int dtype, int n, int d,
+                          int F, int train) {
+  if (is_few(x, w_gate, w_up, w_down, w_dtype, dtype, n, d, F, train)) return 0;
   return (must_copy(x, x_dtype, dtype, d) ? kCopyX : 0) | (must_copy(w_gate, w_dtype, dtype, d) ? kCopyGate : 0) |
          (must_copy(w_up, w_dtype, dtype, d) ? kCopyUp : 0) | (must_copy(w_down, w_dtype, dtype, F) ? kCopyDown : 0);
 }
@@ -478,10 +500,13 @@ int nlfa_gated_ffn_fwd(const void* x, int x_dtype, const void* w_gate, const voi
   if (!aligned16(tape) || !aligned16(scratch) || !aligned16(y) || !aligned_to(x, x_bytes) || !aligned_to(w_gate, w_bytes) ||
       !aligned_to(w_up, w_bytes) || !aligned_to(w_down, w_bytes))
     return NLFA_ERR_MISALIGNED;
-  if (nlfa_gated_ffn_copies(x, x_dtype, w_gate, w_up, w_down, w_dtype, dtype, d, F) & ~copies) return NLFA_ERR_MISALIGNED;
+  if (nlfa_gated_ffn_copies(x, x_dtype, w_gate, w_up, w_down, w_dtype, dtype, n, d, F, train) & ~copies) return NLFA_ERR_MISALIGNED;
   if (tape_bytes < layout(c).bytes || scratch_bytes < nlfa_gated_ffn_scratch_bytes(n, d, F, o, dtype, copies, 0)) return NLFA_ERR_SCRATCH_TOO_SMALL;
   if (!nlfa_device_supported()) return NLFA_ERR_NOT_SM100;
   if (nlfa_peek_status() != NLFA_OK) return NLFA_ERR_DEVICE_TIMEOUT;
+  if (is_few(x, w_gate, w_up, w_down, w_dtype, dtype, n, d, F, train))
+    return launch_few_tokens(x, x_dtype, w_gate, w_up, w_down, w_dtype, dtype, activation, n, d, F, o,
+                             reinterpret_cast<float*>(static_cast<uint8_t*>(tape) + layout(c).h), y, static_cast<cudaStream_t>(stream));
   return run_fwd(c, {x, w_gate, w_up, w_down}, activation, y, static_cast<uint8_t*>(tape), static_cast<uint8_t*>(scratch),
                  static_cast<cudaStream_t>(stream));
 }

@@ -44,7 +44,7 @@ struct Params {
   int n_rows, f_pad;                // extents of h, dg, du
   int chunk;                        // stages per chain of the tensor core
   int activation;
-  // kept g and u: 16-bit values with a power of two per 32 values of a row, or float32 (ffn_tc.cu)
+  // kept f(g) and u f'(g): 16-bit values with a power of two per 32 values of a row, or float32 (ffn_tc.cu)
   uint8_t *kept;
   int8_t* exponents;
   void *h, *dg, *du;                // float32: written without TMA
@@ -59,6 +59,12 @@ struct Params {
 int pairs();                        // of CTAs that run at once
 // Maps: kUp x, Wg, Wu, h to store; kDh dy, Wd, dg and du to store; kProducts as the segments say.
 int launch_product(int mode, int dtype, int planes, bool chains, const Params& p, const Maps& maps, cudaStream_t stream);
+
+// A few tokens, no backward (ffn_few.cu): operands as they lie, d and F multiples of 8, on 16 bytes.  h: n x F.
+constexpr int kFewTokens = 32;
+bool few_types(int w_dtype, int dtype);
+int launch_few_tokens(const void* x, int x_dtype, const void* gate, const void* up, const void* down, int w_dtype, int dtype, int activation, int n,
+                      int d, int F, int o, float* h, void* y, cudaStream_t st);
 
 }  // namespace ffn
 }  // namespace nlfa

@@ -1,5 +1,5 @@
 // The products of the gated feed-forward layer (ffn.cu) on the tensor cores:
-//   kUp        g = x Wg^T and u = x Wu^T of the same tile, h = f(g) u (and g, u kept for the backward);
+//   kUp        g = x Wg^T and u = x Wu^T of the same tile, h = f(g) u (and f(g), u f'(g) kept for the backward);
 //   kDh        dh = dy Wd, of which only du = dh f(g) and dg = dh u f'(g) leave the SM;
 //   kProducts  plain products: y = h Wd^T; or dWg = dg^T x, dWu = du^T x, dWd = dy^T h and dx = dg Wg + du Wu in one launch.
 //
@@ -11,10 +11,11 @@
 // The tensor core adds by truncation (loss_tc.cu), so where a sum is long its chain is cut (LONG): formed chunk by chunk, the chunks' sums
 // added in registers.
 //
-// What the backward needs of g and u: u f'(g) and f(g), which enter dg and du.  Kept in bf16 they would bring two more roundings of 2^-9 to
-// results that have one in dg and one in their own type (2.4e-3 of dx, 3.0e-3 with them); so they are kept with 2^-12: as fp16 times a power
-// of two per 32 values of a row, which puts the largest of them just below fp16's limit.  They lie as the lanes write and read
-// them, [32 rows][32 columns][g, u][8 columns][lane], 512 bytes an instruction.
+// What the backward needs of g and u are a = f(g) and b = u f'(g): du = dh a, dg = dh b.  They are formed where g and u are, under products that
+// take twice as long per hidden value as those under which dh is used (65,536 x 768 x 2,048: with g and u kept the dh kernel took 324 us).  Kept in
+// bf16 they would bring one more rounding of 2^-9 to results that have one in dg and one in their own type (2.4e-3 of dx, 2.9e-3 with it); so
+// they are kept with 2^-12: as fp16 times a power of two per 32 values of a row, which puts the largest of them just below fp16's limit;
+// beside float16's own 2^-12, and float32's, as float32.  They lie as the lanes write and read them, [32 rows][32 columns][a, b][16 bytes of each lane].
 //
 // Warps: 0 producer, 1 MMA issuer (even CTA) and TMEM owner, 2-9 epilogue: two warps per quarter of the rows.  Every wait is bounded (ptx.cuh);
 // no multicast loads.
@@ -174,8 +175,13 @@ fold_kernel(const __grid_constant__ Params p) {
 
 // ---- the activation: f(g), and f'(g).  EXACT (float32): no approximate exponential or quotient
 
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 template <bool EXACT> __device__ __forceinline__ float logistic(float g) {
-  return EXACT ? 1.f / (1.f + expf(-g)) : __fdividef(1.f, 1.f + fast_exp2(-kLog2e * g));
+  return EXACT ? 1.f / (1.f + expf(-g)) : reciprocal(1.f + fast_exp2(-kLog2e * g));
 }
 template <int ACT, bool EXACT> __device__ __forceinline__ void activate(float g, float& a, float& da) {
   if (ACT == NLFA_FFN_SILU) {
@@ -193,12 +199,12 @@ template <int ACT, bool EXACT> __device__ __forceinline__ void activate(float g,
   }
 }
 
-// ---- kept g and u: this thread's 32 values of one of them
+// ---- kept a and b: this thread's 32 values of one of them (WIDE: float32)
 
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 
-template <int PARTS> __device__ __forceinline__ void keep(uint8_t* at, int8_t* exponent, const float (&v)[32]) {
-  if constexpr (PARTS == 3) {
+template <bool WIDE> __device__ __forceinline__ void keep(uint8_t* at, int8_t* exponent, const float (&v)[32]) {
+  if constexpr (WIDE) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(at + 512 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   } else {
@@ -226,19 +232,19 @@ template <int PARTS> __device__ __forceinline__ void keep(uint8_t* at, int8_t* e
     }
   }
 }
-// Eight of them: the ones at 8 i.
-template <int PARTS> __device__ __forceinline__ void kept(const uint8_t* at, int i, float f, float (&v)[8]) {
-  if constexpr (PARTS == 3) {
-    const float4 a = *reinterpret_cast<const float4*>(at + 1024 * i), b = *reinterpret_cast<const float4*>(at + 1024 * i + 512);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// Eight of them, those at 8 i, each times v's.
+template <bool WIDE> __device__ __forceinline__ void times_kept(const uint8_t* at, int i, const float (&v)[8], float f, float (&out)[8]) {
+  if constexpr (WIDE) {
+    const float4 x = *reinterpret_cast<const float4*>(at + 1024 * i), y = *reinterpret_cast<const float4*>(at + 1024 * i + 512);
+    out[0] = v[0] * x.x; out[1] = v[1] * x.y; out[2] = v[2] * x.z; out[3] = v[3] * x.w;
+    out[4] = v[4] * y.x; out[5] = v[5] * y.y; out[6] = v[6] * y.z; out[7] = v[7] * y.w;
   } else {
     const uint4 w = *reinterpret_cast<const uint4*>(at + 512 * i);
     const __half2* h = reinterpret_cast<const __half2*>(&w);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 x = __half22float2(h[j]);
-      v[2 * j] = x.x * f;
-      v[2 * j + 1] = x.y * f;
+      unpack_f2(fmul2(fmul2(pack_f2(v[2 * j], v[2 * j + 1]), pack_f2(f, f)), pack_f2(x.x, x.y)), out[2 * j], out[2 * j + 1]);
     }
   }
 }
@@ -478,8 +484,9 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
       }
       if (!ok) break;
       const int c0 = t.n0 + kOwn * half;
-      // kept g and u: of 32 rows and 32 columns g, then u
-      constexpr int kKeptBytes = PARTS == 3 ? 4096 : 2048;
+      // kept a and b: of 32 rows and 32 columns a, then b
+      constexpr bool kWide = PARTS == 3 || !kBf16;
+      constexpr int kKeptBytes = kWide ? 4096 : 2048;
       auto kept_at = [&](int col) -> size_t { return (static_cast<size_t>(row0 / 32) * (p.f_pad / 32) + col / 32) * 2; };
 
       if constexpr (MODE == kUp) {
@@ -492,14 +499,27 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
             l.get(2 + c, u);
             if (p.kept != nullptr) {
               const size_t at = kept_at(c0 + 32 * c);
-              keep<PARTS>(p.kept + at * kKeptBytes + 16 * lane, p.exponents + 32 * at + lane, g);
-              keep<PARTS>(p.kept + (at + 1) * kKeptBytes + 16 * lane, p.exponents + 32 * (at + 1) + lane, u);
-            }
+              float f[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              float a, da;
-              activate<ACT, PARTS == 3>(g[j], a, da);
-              g[j] = a * u[j] * scale;
+              for (int j = 0; j < 32; ++j) {
+                float slope;
+                activate<ACT, PARTS == 3>(g[j], f[j], slope);
+                g[j] = f[j] * u[j];
+                u[j] *= slope;
+              }
+              keep<kWide>(p.kept + at * kKeptBytes + 16 * lane, p.exponents + 32 * at + lane, f);
+              keep<kWide>(p.kept + (at + 1) * kKeptBytes + 16 * lane, p.exponents + 32 * (at + 1) + lane, u);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                float f, slope;
+                activate<ACT, PARTS == 3>(g[j], f, slope);
+                g[j] = f * u[j];
+              }
+            }
+            if (!kBf16) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) g[j] *= scale;
             }
             if (PARTS == 3) {
               store_parts(p.h, plane, p.n_rows, row, c0 + 32 * c, g);
@@ -523,36 +543,35 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const size_t at = kept_at(col0 + 32 * c);
-            const uint8_t* gs = p.kept + at * kKeptBytes + 16 * lane;
-            const uint8_t* us = gs + kKeptBytes;
-            float fg = 1.f, fu = 1.f;
-            if (PARTS == 1) {
-              fg = power_of_two(p.exponents[32 * at + lane]);
-              fu = power_of_two(p.exponents[32 * (at + 1) + lane]);
+            const uint8_t* as = p.kept + at * kKeptBytes + 16 * lane;
+            const uint8_t* bs = as + kKeptBytes;
+            float fa = 1.f, fb = 1.f;
+            if (!kWide) {
+              fa = power_of_two(p.exponents[32 * at + lane]);
+              fb = power_of_two(p.exponents[32 * (at + 1) + lane]);
             }
-            float d[32], e[32];
+            float d[32], e[PARTS == 3 ? 32 : 1];
             l.get(2 * c2 + c, d);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              float g[8], u[8];
-              kept<PARTS>(gs, i, fg, g);
-              kept<PARTS>(us, i, fu, u);
+              float v[8], dg[8], du[8];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                float a, da;
-                activate<ACT, PARTS == 3>(g[j], a, da);
-                const float dh = d[8 * i + j] * scale;
-                e[8 * i + j] = dh * a;
-                d[8 * i + j] = dh * (u[j] * da);
-              }
-              if (PARTS == 1) {
-                const float v[8] = {d[8 * i], d[8 * i + 1], d[8 * i + 2], d[8 * i + 3], d[8 * i + 4], d[8 * i + 5], d[8 * i + 6], d[8 * i + 7]};
-                stage(4 * c + i, v);
+              for (int j = 0; j < 8; ++j) v[j] = kBf16 ? d[8 * i + j] : d[8 * i + j] * scale;
+              times_kept<kWide>(as, i, v, fa, du);
+              times_kept<kWide>(bs, i, v, fb, dg);
+              if constexpr (PARTS == 1) {
+                stage(4 * c + i, dg);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) held[PARTS == 1 ? 16 * c + 4 * i + j : 0] = Pack2<T>::pack(e[8 * i + 2 * j], e[8 * i + 2 * j + 1]);
+                for (int j = 0; j < 4; ++j) held[16 * c + 4 * i + j] = Pack2<T>::pack(du[2 * j], du[2 * j + 1]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  d[8 * i + j] = dg[j];
+                  e[8 * i + j] = du[j];
+                }
               }
             }
-            if (PARTS == 3) {
+            if constexpr (PARTS == 3) {
               store_parts(p.dg, plane, p.n_rows, row, col0 + 32 * c, d);
               store_parts(p.du, plane, p.n_rows, row, col0 + 32 * c, e);
             }

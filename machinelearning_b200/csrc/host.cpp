@@ -1089,8 +1089,8 @@ PyObject* py_gated_ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     py::gil_scoped_release no_gil;
     const c10::cuda::CUDAGuard guard(x.device());
     for (Tensor& v : t) v = contiguous(v);
-    c.copies = nlfa_gated_ffn_copies(x.data_ptr(), c.x, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), c.w, c.dtype, c.d, c.F);
     const bool train = recording({&t[0], &t[1], &t[2], &t[3]});
+    c.copies = nlfa_gated_ffn_copies(x.data_ptr(), c.x, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), c.w, c.dtype, c.n, c.d, c.F, train);
     Tensor tape;
     std::tie(y, tape) = ffn_forward(x, wg, wu, wd, c, out, train);
     if (train) {

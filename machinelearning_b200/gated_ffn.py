@@ -41,10 +41,11 @@ def _sizes(x_shape, w_gate_shape, o):
     return n, w_gate_shape[1], w_gate_shape[0], o
 
 
-def copies_of(x, w_gate, w_up, w_down, dtype: torch.dtype) -> int:
+def copies_of(x, w_gate, w_up, w_down, dtype: torch.dtype, train: bool) -> int:
     """Which of the four (bits 0 to 3) the tape gets copies of: where the products cannot read them as they lie."""
     return _lib_or_raise().nlfa_gated_ffn_copies(x.data_ptr(), _DTYPE_CODE[x.dtype], w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
-                                                 _DTYPE_CODE[w_gate.dtype], _DTYPE_CODE[dtype], w_gate.shape[1], w_gate.shape[0])
+                                                 _DTYPE_CODE[w_gate.dtype], _DTYPE_CODE[dtype], x.numel() // x.shape[-1],
+                                                 w_gate.shape[1], w_gate.shape[0], train)
 
 
 def fwd(x, w_gate, w_up, w_down, activation: str, dtype: torch.dtype, train: bool):
@@ -57,7 +58,7 @@ def fwd(x, w_gate, w_up, w_down, activation: str, dtype: torch.dtype, train: boo
     weights = (w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr())
     y = torch.empty((*x.shape[:-1], w_down.shape[0]), dtype=dtype, device=x.device)
     with flash_cuda._on_device(x.device.index):
-        copies = copies_of(x, w_gate, w_up, w_down, dtype)
+        copies = copies_of(x, w_gate, w_up, w_down, dtype, train)
         tape = torch.empty(lib.nlfa_gated_ffn_tape_bytes(*sizes, dc, copies, train), dtype=torch.uint8, device=x.device)
         scratch = torch.empty(lib.nlfa_gated_ffn_scratch_bytes(*sizes, dc, copies, 0), dtype=torch.uint8, device=x.device)
         st = lib.nlfa_gated_ffn_fwd(x.data_ptr(), xc, *weights, wc, dc, ACTIVATIONS[activation], *sizes, y.data_ptr(), copies, train,

@@ -40,9 +40,10 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
     from machinelearning_b200 import _build, _lib
     _build.build()
     lib = _lib.load()
-    copies = lambda x=256, xd=2, wg=256, wu=256, wd=256, w=2, dt=2, d=64, F=128: lib.nlfa_gated_ffn_copies(x, xd, wg, wu, wd, w, dt, d, F)
+    copies = lambda x=256, xd=2, wg=256, wu=256, wd=256, w=2, dt=2, n=10, d=64, F=128, tr=1: lib.nlfa_gated_ffn_copies(x, xd, wg, wu, wd, w, dt, n, d, F, tr)
     assert copies() == 0 and copies(x=264) == 1 and copies(wu=258) == 4 and copies(F=96) == 8 and copies(d=40) == 7
     assert copies(xd=0) == 1 and copies(w=0) == 14 and copies(xd=0, w=0, dt=0) == 15
+    assert copies(xd=0, w=0, tr=0) == 0 and copies(d=40, tr=0) == 0 and copies(d=40, tr=0, n=100) == 7 and copies(d=44, tr=0) == 7
     tape = lambda n=10, d=64, F=128, o=64, dt=2, cp=0, train=1: lib.nlfa_gated_ffn_tape_bytes(n, d, F, o, dt, cp, train)
     scratch = lambda n=10, d=64, F=128, o=64, dt=2, cp=0, b=0: lib.nlfa_gated_ffn_scratch_bytes(n, d, F, o, dt, cp, b)
     assert 0 < tape(train=0) < tape() < tape(cp=15) and tape(F=0) == 0 and tape(n=-1) == 0 and tape(dt=4) == 0
@@ -150,6 +151,31 @@ def test_many_tiles_and_chains(dtype):
         most = 2.0**-20 if dtype == torch.float32 else 1.2 * HALF_STEP[dtype]
         for got, want in zip((y, *grads), (ref, *wants)):
             assert float((got.double() - want).norm() / want.norm()) <= most
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=_id)
+@pytest.mark.parametrize("n", [1, 7, 8, 9, 16, 31, 32, 33])
+def test_a_few_tokens_without_a_backward(dtype, n):
+    """The kernels of decoding steps: h is not rounded to 16 bits (its parts keep 2^-17), so the bound has no such term; and types that only autocast gives."""
+    from machinelearning_b200 import gated_ffn
+    for d, F, o in ((768, 2048, 768), (8, 8, 3), (64, 40, 300), (200, 1000, 17), (1032, 136, 65)):
+        leaves, _ = _inputs(dtype, n, d, F, o, seed=5)
+        with torch.no_grad():
+            for kind in ("silu", "gelu", "relu"):
+                y = gated_ffn.gated_ffn(*leaves, activation=kind)
+                want = block_f64.gated_ffn(*(_np(t) for t in leaves), kind, step=0.0 if n <= 32 else HALF_STEP[dtype] / 3**0.5)
+                assert (np.abs(_np(y) - want["y"]) <= _bounds(want, "y", dtype, dtype)).all()
+                assert torch.equal(y, gated_ffn.gated_ffn(*leaves, activation=kind))
+    if dtype == torch.float32:
+        return
+    for x_dtype in (torch.float32, torch.bfloat16, torch.float16):
+        leaves, _ = _inputs(x_dtype, n, 128, 256, 64, w_dtype=torch.float32)
+        with torch.no_grad(), torch.autocast("cuda", dtype=dtype):
+            y = gated_ffn.gated_ffn(*leaves)
+        assert y.dtype == dtype
+        want = block_f64.gated_ffn(*(_np(t.detach().to(dtype)) for t in leaves), step=HALF_STEP[dtype] / 3**0.5)
+        assert (np.abs(_np(y) - want["y"]) <= _bounds(want, "y", dtype, dtype)).all()
 
 
 @pytest.mark.gpu
