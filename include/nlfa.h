@@ -409,7 +409,7 @@ int nlfa_gated_scan_bwd(const void* dh, const float* dlast, const void* gate, lo
  * precision; in float16 they carry a power of two, so that they neither overflow nor lose digits below the type's normal range.
  *
  * `copies` (nlfa_gated_ffn_copies): which of x, w_gate, w_up, w_down (bits 0 to 3) the forward copies into the tape, because the products cannot read
- * them as they lie: of another type, float32, rows not a multiple of 64 long, not 16-byte aligned (without `train` up to 32 tokens take most as they lie).  The backward takes the same value; operands that
+ * them as they lie: of another type, float32, rows not a multiple of 64 long, not 16-byte aligned (without `train` up to 64 tokens take most as they lie).  The backward takes the same value; operands that
  * were copied may be NULL there, the others have to be what they were.  `tape`: with `train` what the backward reads, without it workspace.
  * dx (x_dtype), dw_gate, dw_up, dw_down (w_dtype): any may be NULL.  Bit-reproducible; may be captured.  Tape, scratch, y and the gradients are 16-byte
  * aligned.  Needs compute capability 10.x. */

@@ -11,7 +11,6 @@
 // This file has what goes around the products: 16-bit copies of operands that TMA cannot read as they are, the list of tiles and
 // parts, and the powers of two that hold float16's h, dg and du inside their type's range.
 #include <cmath>
-#include <cstdlib>
 
 #include "ffn.cuh"
 #include "rowwise.cuh"
@@ -55,8 +54,9 @@ int check_call(const Call& c) {
 bool must_copy(const void* p, int type, int dtype, int cols) { return dtype == NLFA_DTYPE_F32 || type != dtype || cols % 64 != 0 || !aligned16(p); }
 
 bool is_few(const void* x, const void* gate, const void* up, const void* down, int w_dtype, int dtype, int n, int d, int F, int train) {
-  static const char* env = getenv("FFN_FEW");
-  return !train && n <= (env ? atoi(env) : kFewTokens) && few_types(w_dtype, dtype) && d % 8 == 0 && F % 8 == 0 && aligned16(x) && aligned16(gate) && aligned16(up) && aligned16(down);
+  if (n > kFewTokens || (n > kVeryFewTokens && static_cast<long long>(n) * d * F > kFewProducts)) return false;
+  return !train && few_types(w_dtype, dtype) && d % 8 == 0 && F % 8 == 0 && aligned16(x) && aligned16(gate) && aligned16(up) &&
+         aligned16(down);
 }
 
 // What the forward leaves for the backward, and (inference) the forward's own workspace.

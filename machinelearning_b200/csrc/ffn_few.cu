@@ -103,23 +103,38 @@ __device__ __forceinline__ void ask(Ahead<S>& a, int i, const S* lo, const S* hi
 template <typename S, typename X, typename CW, typename CX, int WP, int XP, int NT>
 __device__ __forceinline__ void run(float (&acc)[NT][2][4], Ahead<S>& ahead, const S* lo, const S* hi, const X* x, int n, int s0, int s1, int k) {
   const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+  // the tokens of a step, one step ahead (of 32 tokens there are no registers for that: 64 of them 13.7 us so, 11.8 without)
+  constexpr bool kAhead = NT < 4;
+  Eight<X> xs[NT];
+  auto tokens = [&](int step) {
+    const int at = 32 * step + 8 * t;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) load(xs[j], x + static_cast<size_t>(8 * j + g) * k + at, step < s1 && 8 * j + g < n && at < k);
+  };
+  if (kAhead) tokens(s0);
   for (int s = s0; s < s1; s += kDeep) {
 #pragma unroll
     for (int i = 0; i < kDeep; ++i) {
       if (s + i >= s1) break;
-      Eight<X> xs[NT];
-      const int at = 32 * (s + i) + 8 * t;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) load(xs[j], x + static_cast<size_t>(8 * j + g) * k + at, 8 * j + g < n && at < k);
+      if (!kAhead) tokens(s + i);
       uint32_t wl[WP][4], wh[WP][4];
       split<S, CW, WP>(ahead.lo[i], wl);
       split<S, CW, WP>(ahead.hi[i], wh);
       ask(ahead, i, lo, hi, s + i + kDeep, s1, k);
+      if constexpr (kAhead) {
+        uint32_t xp[NT][XP][4];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        uint32_t xp[XP][4];
-        split<X, CX, XP>(xs[j], xp);
-        product<WP, XP>(acc[j], wl, wh, xp);
+        for (int j = 0; j < NT; ++j) split<X, CX, XP>(xs[j], xp[j]);
+        tokens(s + i + 1);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) product<WP, XP>(acc[j], wl, wh, xp[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          uint32_t xp[XP][4];
+          split<X, CX, XP>(xs[j], xp);
+          product<WP, XP>(acc[j], wl, wh, xp);
+        }
       }
     }
   }
@@ -141,6 +156,16 @@ struct FewParams {
   float* h;
   void* y;
   int n, d, F, o, x_dtype, activation, out_dtype;
+  int turns;
+  // This CTA's rows of the weights (the CTAs that read the same ones stand side by side), and its tokens, up to `most`.
+  __device__ __forceinline__ int turn(int most) {
+    const int tile = blockIdx.x / turns, first = most * (blockIdx.x - tile * turns);
+    x = static_cast<const uint8_t*>(x) + static_cast<size_t>(first) * d * (x_dtype == NLFA_DTYPE_F32 ? 4 : 2);
+    h += static_cast<size_t>(first) * F;
+    y = static_cast<uint8_t*>(y) + static_cast<size_t>(first) * o * (out_dtype == NLFA_DTYPE_F32 ? 4 : 2);
+    n = min(n - first, most);
+    return tile * kRows;
+  }
 };
 
 __device__ __forceinline__ float activated(float g, int activation) {
@@ -151,10 +176,11 @@ __device__ __forceinline__ float activated(float g, int activation) {
 
 template <typename S, typename C, int NT>
 __global__ void __launch_bounds__(32 * kUpWarps)
-few_up_kernel(const FewParams p) {
+few_up_kernel(FewParams p) {
+  const int row0 = p.turn(8 * NT);
   __shared__ float sums[kUpWarps * 8 * NT * kPitch];
   constexpr int kHalf = kUpWarps / 2, WP = Parts<C>::kCount;
-  const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2, row0 = blockIdx.x * kRows;
+  const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2;
   const int steps = (p.d + 31) / 32, q = warp % kHalf, s0 = steps * q / kHalf, s1 = steps * (q + 1) / kHalf;
   const S* w = static_cast<const S*>(warp < kHalf ? p.gate : p.up);
   // (rows behind the last one: the last one again, and nothing is written)
@@ -186,9 +212,10 @@ few_up_kernel(const FewParams p) {
 
 template <typename S, typename C, int NT>
 __global__ void __launch_bounds__(32 * kDownWarps)
-few_down_kernel(const FewParams p) {
+few_down_kernel(FewParams p) {
+  const int row0 = p.turn(8 * NT);
   __shared__ float sums[kDownWarps * 8 * NT * kPitch];
-  const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2, row0 = blockIdx.x * kRows;
+  const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2;
   const int steps = (p.F + 31) / 32, s0 = steps * warp / kDownWarps, s1 = steps * (warp + 1) / kDownWarps;
   const S* lo = static_cast<const S*>(p.down) + static_cast<size_t>(min(row0 + g, p.o - 1)) * p.F;
   const S* hi = static_cast<const S*>(p.down) + static_cast<size_t>(min(row0 + g + 8, p.o - 1)) * p.F;
@@ -216,18 +243,21 @@ few_down_kernel(const FewParams p) {
 }
 
 template <typename S, typename C, int NT>
-int launch_few(const FewParams& p, cudaStream_t st) {
+int launch_few(FewParams p, cudaStream_t st) {
   const bool overlap = overlap_launches(kOverlapRowwise);
-  cudaError_t e = launch_kernel(few_up_kernel<S, C, NT>, dim3(static_cast<unsigned>((p.F + kRows - 1) / kRows)), dim3(32 * kUpWarps), 0, st, overlap, p);
+  p.turns = (p.n + 8 * NT - 1) / (8 * NT);
+  auto tiles = [&](int rows) { return dim3(static_cast<unsigned>((rows + kRows - 1) / kRows * p.turns)); };
+  cudaError_t e = launch_kernel(few_up_kernel<S, C, NT>, tiles(p.F), dim3(32 * kUpWarps), 0, st, overlap, p);
   if (e == cudaSuccess)
-    e = launch_kernel(few_down_kernel<S, C, NT>, dim3(static_cast<unsigned>((p.o + kRows - 1) / kRows)), dim3(32 * kDownWarps), 0, st, overlap, p);
+    e = launch_kernel(few_down_kernel<S, C, NT>, tiles(p.o), dim3(32 * kDownWarps), 0, st, overlap, p);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? NLFA_OK : NLFA_ERR_CUDA;
 }
 template <typename S, typename C>
 int launch_tokens(const FewParams& p, cudaStream_t st) {
   if (p.n <= 8) return launch_few<S, C, 1>(p, st);
-  return p.n <= 16 ? launch_few<S, C, 2>(p, st) : launch_few<S, C, 4>(p, st);
+  // (two turns of 16 for 32 tokens 8.3 us, one of 32 10.9; two of 32 for 64 11.1, four of 16 15.2)
+  return p.n <= 32 ? launch_few<S, C, 2>(p, st) : launch_few<S, C, 4>(p, st);
 }
 
 }  // namespace
@@ -237,7 +267,7 @@ bool few_types(int w_dtype, int dtype) { return w_dtype == dtype || w_dtype == N
 
 int launch_few_tokens(const void* x, int x_dtype, const void* gate, const void* up, const void* down, int w_dtype, int dtype, int activation, int n,
                       int d, int F, int o, float* h, void* y, cudaStream_t st) {
-  const FewParams p{x, gate, up, down, h, y, n, d, F, o, x_dtype, activation, dtype};
+  const FewParams p{x, gate, up, down, h, y, n, d, F, o, x_dtype, activation, dtype, 1};
   if (dtype == NLFA_DTYPE_F32) return launch_tokens<float, float>(p, st);
   if (dtype == NLFA_DTYPE_F16) return w_dtype == dtype ? launch_tokens<__half, __half>(p, st) : launch_tokens<float, __half>(p, st);
   return w_dtype == dtype ? launch_tokens<__nv_bfloat16, __nv_bfloat16>(p, st) : launch_tokens<float, __nv_bfloat16>(p, st);

@@ -11,6 +11,9 @@ into it, and ``tests/golden/whole_model_tiny.npz`` (written by
 ``tests/golden/make_whole_model_golden.py`` from nanolab itself) pins its loss and
 gradients to nanolab's.
 
+``ModelShape(mixer="mingru")`` is the same model with nanolab's recurrent mixer (``nanolab/mixers.py``, ``MinGRU``) in attention's place: no cache
+of keys and values, a state of ``d_model`` floats per layer, and ``GPT.forward_states`` to decode from it.
+
 The attention core goes through ``mixer_glue.attention_core`` -- the routing of
 ``Attention._flash_cuda_attn`` (``nanolab/mixers.py:347-370``) -- and falls back
 to SDPA exactly where nanolab's mixer does (CPU tensors, flag off).
@@ -32,7 +35,7 @@ import torch.distributed as dist
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import flash_cuda, grad_clip, head_loss, mixer_glue, qk_prologue, token_embedding, value_gate
+from . import flash_cuda, gated_ffn, gated_scan, grad_clip, head_loss, mixer_glue, qk_prologue, token_embedding, value_gate
 
 
 @dataclasses.dataclass
@@ -63,12 +66,17 @@ class ModelShape:
     fused_epilogue: bool = True  # with flash_cuda on: value blend and head gate in one kernel each (value_gate)
     fused_loss: bool = False     # head and cross entropy without the logits (head_loss); a training step then returns none
     fused_embedding: bool = False  # rows of the table and their gradient by sorted tokens (token_embedding)
+    mixer: str = "attention"     # or "mingru": the gated recurrence along the sequence
+    fused_ffn: bool = False      # the feed-forward layer's projections with activation and product (gated_ffn)
+    fused_scan: bool = False     # mingru: the recurrence in one pass (gated_scan)
 
     def __post_init__(self):
         if self.n_kv_head == 0:
             self.n_kv_head = self.n_head
         if self.n_head % self.n_kv_head:
             raise ValueError("n_head must be a multiple of n_kv_head")
+        if self.mixer not in ("attention", "mingru"):
+            raise ValueError(f"mixer must be 'attention' or 'mingru', got {self.mixer!r}")
 
     @property
     def ffn_hidden(self) -> int:
@@ -180,16 +188,68 @@ class Attention(nn.Module):
         return self.o_proj(y.reshape(B, T, self.H * self.D)), raw_v
 
 
+def plain_scan(gate, value, state=None, reset=None, lengths=None):
+    """``gated_scan.gated_scan(..., activation="positive")`` in tensor operations: runs of 1, 2, 4, ... steps joined."""
+    z, v = gate.float(), value.float()
+    a, b = torch.sigmoid(-z), torch.sigmoid(z) * torch.where(v < 0, torch.sigmoid(v), v + 0.5)
+    if reset is not None:
+        a = a.masked_fill(reset[..., None], 0.0)
+    h0 = z.new_zeros(z.shape[0], z.shape[2]) if state is None else state.float()
+    if z.shape[1] == 0:
+        return gate, h0
+    live = None
+    if lengths is not None:
+        live = (torch.arange(z.shape[1], device=z.device) < lengths[:, None])[..., None]
+        a, b = torch.where(live, a, 1.0), torch.where(live, b, 0.0)
+    k = 1
+    while k < z.shape[1]:
+        b = torch.cat((b[:, :k], b[:, k:] + a[:, k:] * b[:, :-k]), 1)
+        a = torch.cat((a[:, :k], a[:, k:] * a[:, :-k]), 1)
+        k *= 2
+    h = a * h0[:, None] + b
+    return (h if live is None else torch.where(live, h, 0.0)).to(gate.dtype), h[:, -1]
+
+
+class MinGRU(nn.Module):
+    """Gates and candidates from the input, a recurrence without products of states (``nanolab/mixers.py``, ``MinGRU``), a projection."""
+
+    gate = None                  # no gate on the mixer's output
+
+    def __init__(self, s: ModelShape):
+        super().__init__()
+        self.z_proj = nn.Linear(s.d_model, s.d_model, bias=False)
+        self.h_proj = nn.Linear(s.d_model, s.d_model, bias=False)
+        self.o_proj = nn.Linear(s.d_model, s.d_model, bias=False)
+        self.fused = bool(s.fused_scan)
+        self._flash_declined = False
+
+    def forward_state(self, x, state=None, reset=None, lengths=None):
+        """(output, state behind the last step); ``reset`` and ``lengths`` as in ``gated_scan``."""
+        gate, value = self.z_proj(x), self.h_proj(x)
+        if self.fused and gated_scan.supports(gate, value, state, reset, lengths) and flash_cuda.is_available():
+            h, last = gated_scan.gated_scan(gate, value, state, activation="positive", reset=reset, lengths=lengths)
+        else:
+            h, last = plain_scan(gate, value, state, reset, lengths)
+        return self.o_proj(h), last
+
+    def forward(self, x, cos, sin, v0):
+        return self.forward_state(x)[0], None
+
+
 class SwiGLU(nn.Module):
     """``down(silu(gate(x)) * up(x))`` (``nanolab/model.py:29-43``)."""
 
     def __init__(self, s: ModelShape):
         super().__init__()
+        self.fused = bool(s.fused_ffn)
         self.gate = nn.Linear(s.d_model, s.ffn_hidden, bias=False)
         self.up = nn.Linear(s.d_model, s.ffn_hidden, bias=False)
         self.down = nn.Linear(s.ffn_hidden, s.d_model, bias=False)
 
     def forward(self, x):
+        weights = (self.gate.weight, self.up.weight, self.down.weight)
+        if self.fused and gated_ffn.supports(x, *weights) and flash_cuda.is_available():
+            return gated_ffn.gated_ffn(x, *weights)
         return self.down(F.silu(self.gate(x)) * self.up(x))
 
 
@@ -198,7 +258,7 @@ class Block(nn.Module):
 
     def __init__(self, s: ModelShape):
         super().__init__()
-        self.norm1, self.mixer = RMSNorm(s.d_model), Attention(s)
+        self.norm1, self.mixer = RMSNorm(s.d_model), Attention(s) if s.mixer == "attention" else MinGRU(s)
         self.norm2, self.ffn = RMSNorm(s.d_model), SwiGLU(s)
 
     def forward(self, x, cos, sin, v0):
@@ -239,14 +299,33 @@ class GPT(nn.Module):
         """nanolab's estimate, 6·N + 12·L·H·D·T (``model.py:461-490``)."""
         s = self.shape
         span = min(s.swa_window, s.block_size) if s.swa_window else s.block_size
+        if s.mixer != "attention":
+            span = 0
         return 6.0 * self.n_params() + 12.0 * s.n_layer * s.n_head * s.head_dim * span
+
+    def _embed(self, idx):
+        if self.shape.fused_embedding and token_embedding.supports(idx, self.tok_emb.weight) and flash_cuda.is_available():
+            return token_embedding.embedding(idx, self.tok_emb.weight)
+        return self.tok_emb(idx)
+
+    @torch.no_grad()
+    def forward_states(self, idx, states=None, lengths=None):
+        """A chunk of tokens ``[B, T]`` of a recurrent model behind ``states`` (one per layer; ``None``: the beginning): logits ``[B, V]`` behind each
+        sequence's last token, and the states for the next chunk.  ``lengths [B]``, each at least 1: tokens from there on are padding."""
+        if self.shape.mixer != "mingru":
+            raise ValueError("forward_states needs a recurrent mixer")
+        x, behind = self._embed(idx), []
+        for i, blk in enumerate(self.blocks):
+            mixed, last = blk.mixer.forward_state(blk.norm1(x), None if states is None else states[i], None, lengths)
+            behind.append(last)
+            x = x + mixed
+            x = x + blk.ffn(blk.norm2(x))
+        at = x[:, -1] if lengths is None else x[torch.arange(len(x), device=x.device), lengths - 1]
+        return self.lm_head(self.norm_f(at)), behind
 
     def forward(self, idx, targets=None):
         s = self.shape
-        if s.fused_embedding and token_embedding.supports(idx, self.tok_emb.weight) and flash_cuda.is_available():
-            x = token_embedding.embedding(idx, self.tok_emb.weight)
-        else:
-            x = self.tok_emb(idx)
+        x = self._embed(idx)
         key = (idx.shape[1], x.device, x.dtype)
         if key not in self._rope:
             self._rope[key] = rope_tables(idx.shape[1], s.head_dim, s.rope_base, x.device, x.dtype)
@@ -474,6 +553,8 @@ def main(argv=None) -> int:
 
         python -m machinelearning_b200.whole_model --flash_cuda true [--batch_size 16 --iters 10 --swa_window 0]
         ... --fused_loss true --fused_embedding true --fused_clip true     # the step's ends through their kernels as well
+        ... --fused_ffn true                                               # and the feed-forward layers
+        ... --mixer mingru --fused_scan true                               # the recurrent model
 
     Prints tokens/s, ms per step, the model-FLOPs estimate nanolab uses and the loss, for one GPU.
     """
@@ -486,6 +567,9 @@ def main(argv=None) -> int:
     ap.add_argument("--fused_loss", type=_flag, default=False)
     ap.add_argument("--fused_embedding", type=_flag, default=False)
     ap.add_argument("--fused_clip", type=_flag, default=False)
+    ap.add_argument("--fused_ffn", type=_flag, default=False)
+    ap.add_argument("--mixer", choices=("attention", "mingru"), default="attention")
+    ap.add_argument("--fused_scan", type=_flag, default=False)
     ap.add_argument("--batch_size", type=int, default=16)
     ap.add_argument("--swa_window", type=int, default=0)
     ap.add_argument("--swa_sinks", type=int, default=0)
@@ -496,7 +580,8 @@ def main(argv=None) -> int:
         raise SystemExit("no CUDA device")
     torch.manual_seed(0)
     shape = ModelShape(flash_cuda=a.flash_cuda, fused_prologue=a.fused_prologue, swa_window=a.swa_window,
-                       swa_sinks=a.swa_sinks, fused_loss=a.fused_loss, fused_embedding=a.fused_embedding)
+                       swa_sinks=a.swa_sinks, fused_loss=a.fused_loss, fused_embedding=a.fused_embedding, mixer=a.mixer,
+                       fused_ffn=a.fused_ffn, fused_scan=a.fused_scan)
     model = GPT(shape).cuda()
     step = DataParallelStep(model, fused_clip=a.fused_clip)
     x, y = (t.cuda() for t in synthetic_tokens(shape.vocab_size, a.batch_size, shape.block_size))
@@ -511,6 +596,7 @@ def main(argv=None) -> int:
     tokens = a.batch_size * shape.block_size
     print(json.dumps({"flash_cuda": a.flash_cuda, "fused_prologue": a.fused_prologue and a.flash_cuda,
                       "fused_loss": a.fused_loss, "fused_embedding": a.fused_embedding, "fused_clip": a.fused_clip,
+                      "mixer": a.mixer, "fused_ffn": a.fused_ffn, "fused_scan": a.fused_scan,
                       "tok_s": tokens / sec, "ms_per_step": sec * 1e3, "loss": loss.item(),
                       "params_m": model.n_params() / 1e6, "flops_per_tok": model.flops_per_token(),
                       "model_tflops": model.flops_per_token() * tokens / sec / 1e12,
