@@ -419,7 +419,7 @@ int nlfa_gated_scan_bwd(const void* dh, const float* dlast, const void* gate, lo
 int nlfa_gated_ffn_copies(const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype, int dtype, int n, int d,
                           int F, int train);
 size_t nlfa_gated_ffn_tape_bytes(int n, int d, int F, int o, int dtype, int copies, int train);
-size_t nlfa_gated_ffn_scratch_bytes(int n, int d, int F, int o, int dtype, int copies, int backward);
+size_t nlfa_gated_ffn_scratch_bytes(int n, int d, int F, int o, int dtype, int copies, int train, int backward);
 int nlfa_gated_ffn_fwd(const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype, int dtype,
                        int activation, int n, int d, int F, int o, void* y, int copies, int train, void* tape, size_t tape_bytes, void* scratch,
                        size_t scratch_bytes, void* stream);

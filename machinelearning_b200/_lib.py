@@ -92,7 +92,7 @@ SIGNATURES = {
                             + [_c_int] * 5 + [_c_void_p, _c_size_t] + [_c_void_p] * 4 + [_c_size_t, _c_void_p]),
     "nlfa_gated_ffn_copies": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 3 + [_c_int] * 6),
     "nlfa_gated_ffn_tape_bytes": (_c_size_t, [_c_int] * 7),
-    "nlfa_gated_ffn_scratch_bytes": (_c_size_t, [_c_int] * 7),
+    "nlfa_gated_ffn_scratch_bytes": (_c_size_t, [_c_int] * 8),
     "nlfa_gated_ffn_fwd": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 3 + [_c_int] * 7 + [_c_void_p] + [_c_int] * 2
                            + [_c_void_p, _c_size_t] * 2 + [_c_void_p]),
     "nlfa_gated_ffn_bwd": (_c_int, [_c_void_p] * 2 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 8 + [_c_void_p, _c_size_t] + [_c_void_p] * 5

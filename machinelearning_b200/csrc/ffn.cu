@@ -22,9 +22,6 @@ unsigned* status_block();      // api.cu
 namespace ffn {
 namespace {
 
-using operands::column_map;
-using operands::copy_rows;
-using operands::row_map;
 using rowwise::aligned16;
 using rowwise::dtype_ok;
 
@@ -62,6 +59,7 @@ bool is_few(const void* x, const void* gate, const void* up, const void* down, i
 // What the forward leaves for the backward, and (inference) the forward's own workspace.
 struct Layout {
   int planes, n_rows, d_pad, f_pad, o_pad;
+  int parts;                        // in how many h, dg and du are held (of `planes` planes where planes is 3)
   int type;                         // of an operand
   size_t limits, x, gate, up, down, h, kept, exponents, bytes;
 };
@@ -69,6 +67,9 @@ Layout layout(const Call& c) {
   Layout l{};
   l.planes = c.dtype == NLFA_DTYPE_F32 ? 3 : 1;
   l.type = c.dtype == NLFA_DTYPE_F32 ? NLFA_DTYPE_BF16 : c.dtype;
+  // The roundings of h, dg and du are independent and largely cancel in sums, but results of a few tokens are few: beside their own rounding
+  // the others leave 1.4 times its error on average, and up to 1.6 for 15 tokens.  A tile of rows is held in two parts: its products are short.
+  l.parts = l.planes == 3 ? 3 : c.train && c.n <= kRowTile ? 2 : 1;
   l.n_rows = (c.n + kRowTile - 1) / kRowTile * kRowTile;
   l.d_pad = up64(c.d);
   l.f_pad = up64(c.F);
@@ -80,7 +81,7 @@ Layout layout(const Call& c) {
   l.gate = at; if (c.copies & kCopyGate) at = up(at + two * c.F * l.d_pad);
   l.up = at; if (c.copies & kCopyUp) at = up(at + two * c.F * l.d_pad);
   l.down = at; if (c.copies & kCopyDown) at = up(at + two * c.o * l.f_pad);
-  l.h = at; at = up(at + two * hidden);                   // (a few tokens: float32, which takes less than a tile of 256 in 16 bits)
+  l.h = at; at = up(at + 2 * l.parts * hidden);                   // (a few tokens: float32, which takes less than a tile of 256 in 16 bits)
   if (c.train) {
     const bool wide = c.dtype != NLFA_DTYPE_BF16;
     l.kept = at; at = up(at + 2 * hidden * (wide ? 4 : 2));
@@ -93,7 +94,8 @@ Layout layout(const Call& c) {
 // ------------------------------------------------------------------------------------------------ tiles
 
 // In how many parts the sums of `rest` tiles of k stages are formed: the fewest stages for the busiest pair of CTAs, with `share` more for every
-// share written and added.  The units are handed out in turn behind `ahead` units of `length` stages.
+// share written and added, and some for the launch that adds them.  The units are handed out in turn behind `ahead` units of `length` stages.
+constexpr int kFoldStages = 1;
 int choose_parts(int rest, int k, int n_pairs, int share, int ahead, int length) {
   if (rest == 0) return 1;
   int best = 1;
@@ -107,7 +109,7 @@ int choose_parts(int rest, int k, int n_pairs, int share, int ahead, int length)
       const long long c = static_cast<long long>(first) * length + static_cast<long long>(both - first) * mine;
       cost = c > cost ? c : cost;
     }
-    cost += s > 1 ? s : 0;
+    cost += s > 1 ? s + kFoldStages : 0;
     if (least < 0 || cost < least) { least = cost; best = s; }
   }
   return best;
@@ -143,43 +145,76 @@ size_t share_bytes(const Params& p) {
     if (p.group[i].parts > 1) n += static_cast<size_t>(p.group[i].rest) * p.group[i].parts;
   return n * kRowTile * kColTile * sizeof(float);
 }
-Segment segment(int a_map, int a_mn, int a_plane, int b_map, int b_mn, int k, int m, int n, void* to, int dtype, const float* inverse) {
+// A product of one sum; add() gives it more.
+Segment segment(int a_map, int a_mn, int a_plane, int b_map, int b_mn, int b_plane, int k, int m, int n, void* to, int dtype, const float* inverse) {
   Segment s{};
-  s.a_map = a_map; s.a_mn = a_mn; s.a_plane = s.a_plane2 = a_plane;
-  s.b_map = s.b_map2 = b_map; s.b_mn = b_mn;
-  s.k_half = k;
+  s.a_map = a_map; s.a_mn = a_mn; s.b_mn = b_mn;
+  s.subs = 1; s.k_sub = k;
+  s.a_plane[0] = a_plane; s.b_map[0] = b_map; s.b_plane[0] = b_plane;
   s.tiles_n = ceil_div(n, kColTile);
   s.tiles = ceil_div(m, kRowTile) * s.tiles_n;
   s.m_end = m; s.n_end = n; s.to = to; s.dtype = dtype; s.inverse = inverse;
   return s;
+}
+void add(Segment& s, int a_plane, int b_map, int b_plane) {
+  s.a_plane[s.subs] = a_plane; s.b_map[s.subs] = b_map; s.b_plane[s.subs++] = b_plane;
 }
 
 // Stages per chain of the tensor core (ffn_tc.cu).  Operands of 16 bits leave their own roundings in a sum, 2^-9 (bf16; 2^-12 in fp16) of each summand and
 // independent: over 4,096 of one sign 2^-15, under which a chain of 4,096, low by 1.1e-5, hides; in fp16 one of 2,048.
 int chain(const Layout& l) { return l.planes == 3 ? 1 : l.type == NLFA_DTYPE_F16 ? 16 : 32; }
 
-enum { kMapY = 0, kMapDownColumns = 1 };                   // forward: h, Wd
+// Whether g and u, or dh, are formed apart from what is done with them: where there are so few tiles that most pairs of CTAs would watch, and their sums
+// are so long that three more launches are less (80 tokens x 3,903 x 32 in float32, forward and backward 270 us with one tile's sums of 61 stages); and for parts.
+bool apart(const Layout& l, int cols, int k) {
+  if (l.parts == 2) return true;
+  return 2 * (l.n_rows / kRowTile) * ceil_div(cols, kColTile) <= pairs() && ceil_div(k, summands(l.planes)) > (l.planes == 3 ? 12 : 36);
+}
+
+// Forward, g and u apart: maps x, Wg, Wu.
+void plan_up(Params& p, const Call& c, const Layout& l, float* g, float* u) {
+  const int k = ceil_div(c.d, summands(l.planes));
+  p.groups = p.units = 0;
+  p.seg[0] = segment(0, 0, 0, 1, 0, 0, k, c.n, c.F, g, NLFA_DTYPE_F32, nullptr);
+  p.seg[1] = segment(0, 0, 0, 2, 0, 0, k, c.n, c.F, u, NLFA_DTYPE_F32, nullptr);
+  add_group(p, 0, 2, k, l.planes);
+}
+// y: maps h, Wd.
 void plan_fwd(Params& p, const Call& c, const Layout& l, void* y, const float* inverse) {
   const int k = ceil_div(c.F, summands(l.planes));
   p.groups = p.units = 0;
-  p.seg[0] = segment(0, 0, 0, 1, 0, k, c.n, c.o, y, c.dtype, inverse);
+  p.seg[0] = segment(0, 0, 0, 1, 0, 0, k, c.n, c.o, y, c.dtype, inverse);
+  if (l.parts == 2) add(p.seg[0], 1, 1, 0);
+  add_group(p, 0, 1, p.seg[0].subs * k, l.planes);
+}
+// Backward, dh apart: maps dy, Wd.
+void plan_dh(Params& p, const Call& c, const Layout& l, float* dh) {
+  const int k = ceil_div(c.o, summands(l.planes));
+  p.groups = p.units = 0;
+  p.seg[0] = segment(0, 0, 0, 1, 1, 0, k, c.n, c.F, dh, NLFA_DTYPE_F32, nullptr);
   add_group(p, 0, 1, k, l.planes);
 }
-// backward: maps
+// The gradients; du's planes are behind dg's.
 enum { kHiddenRows = 0, kHiddenColumns, kX, kDy, kH, kGateRows, kUpRows };
 void plan_bwd(Params& p, const Call& c, const Layout& l, void* dx, void* dwg, void* dwu, void* dwd, const float* inv_h, const float* inv_d) {
   const int s = summands(l.planes), kw = ceil_div(c.n, s), kf = ceil_div(c.F, s);
   int n = 0;
   p.groups = p.units = 0;
-  if (dwg) p.seg[n++] = segment(kHiddenRows, 1, 0, kX, 1, kw, c.F, c.d, dwg, c.w_dtype, inv_d);
-  if (dwu) p.seg[n++] = segment(kHiddenRows, 1, l.planes, kX, 1, kw, c.F, c.d, dwu, c.w_dtype, inv_d);
-  if (dwd) p.seg[n++] = segment(kDy, 1, 0, kH, 1, kw, c.o, c.F, dwd, c.w_dtype, inv_h);
-  if (n > 0) add_group(p, 0, n, kw, l.planes);
+  if (dwg) p.seg[n++] = segment(kHiddenRows, 1, 0, kX, 1, 0, kw, c.F, c.d, dwg, c.w_dtype, inv_d);
+  if (dwu) p.seg[n++] = segment(kHiddenRows, 1, l.parts, kX, 1, 0, kw, c.F, c.d, dwu, c.w_dtype, inv_d);
+  if (dwd) p.seg[n++] = segment(kDy, 1, 0, kH, 1, 0, kw, c.o, c.F, dwd, c.w_dtype, inv_h);
+  if (l.parts == 2)
+    for (int i = 0; i < n; ++i) {
+      if (p.seg[i].a_map == kDy) add(p.seg[i], 0, kH, 1);
+      else add(p.seg[i], p.seg[i].a_plane[0] + 1, kX, 0);
+    }
+  if (n > 0) add_group(p, 0, n, p.seg[0].subs * kw, l.planes);
   if (dx) {
-    p.seg[n] = segment(kHiddenColumns, 0, 0, kGateRows, 1, kf, c.n, c.d, dx, c.x_dtype, inv_d);
-    p.seg[n].a_plane2 = l.planes;
-    p.seg[n].b_map2 = kUpRows;
-    add_group(p, n, n + 1, 2 * kf, l.planes);
+    Segment& g = p.seg[n] = segment(kHiddenColumns, 0, 0, kGateRows, 1, 0, kf, c.n, c.d, dx, c.x_dtype, inv_d);
+    if (l.parts == 2) add(g, 1, kGateRows, 0);
+    add(g, l.parts, kUpRows, 0);
+    if (l.parts == 2) add(g, l.parts + 1, kUpRows, 0);
+    add_group(p, n, n + 1, g.subs * kf, l.planes);
   }
 }
 bool needs_chains(const Params& p, const Layout& l) {
@@ -190,19 +225,41 @@ bool needs_chains(const Params& p, const Layout& l) {
 
 // The backward's workspace.
 struct BwdLayout {
-  size_t limits, dy, hidden, shares, bytes;
+  size_t limits, dy, hidden, dh, shares, bytes;
 };
 BwdLayout bwd_layout(const Call& c, const Layout& l, bool copy_dy) {
   BwdLayout b{};
   const size_t two = 2 * static_cast<size_t>(l.planes);
   size_t at = 256;
   b.dy = at; if (copy_dy) at = up(at + two * c.n * l.o_pad);
-  b.hidden = at; at = up(at + 2 * two * l.n_rows * l.f_pad);
+  b.hidden = at; at = up(at + 4 * static_cast<size_t>(l.parts) * l.n_rows * l.f_pad);
+  b.dh = at; if (apart(l, c.F, c.o)) at = up(at + static_cast<size_t>(c.n) * c.F * 4);
   b.shares = at;
   // enough for any choice of gradients
   at += static_cast<size_t>(kMostGroups * kPartsPerPair * pairs()) * kRowTile * kColTile * sizeof(float);
   b.bytes = at;
   return b;
+}
+
+// The forward's.
+struct FwdLayout {
+  size_t g, u, shares, bytes;
+};
+FwdLayout fwd_layout(const Call& c, const Layout& l) {
+  FwdLayout f{};
+  size_t at = 0, most = 0;
+  Params p{};
+  plan_fwd(p, c, l, nullptr, nullptr);
+  most = share_bytes(p);
+  if (apart(l, c.F, c.d)) {
+    f.g = at; at = up(at + static_cast<size_t>(c.n) * c.F * 4);
+    f.u = at; at = up(at + static_cast<size_t>(c.n) * c.F * 4);
+    plan_up(p, c, l, nullptr, nullptr);
+    if (share_bytes(p) > most) most = share_bytes(p);
+  }
+  f.shares = at;
+  f.bytes = at + most + 256;
+  return f;
 }
 
 // ------------------------------------------------------------------------------------------------ float16's range
@@ -312,6 +369,45 @@ int find_limits(RowList list, void* to, size_t bytes, cudaStream_t st) {
 
 // ------------------------------------------------------------------------------------------------ calls
 
+// Copies of operands, up to four in one launch (blockIdx.y): [planes][cols padded / 64][rows][64]
+struct Copy {
+  const void* src;
+  void* dst;
+  int dtype, rows, cols, pad, vec;
+};
+struct CopyList {
+  Copy c[4];
+  int n;
+};
+template <typename T>
+__global__ void __launch_bounds__(operands::kBlock)
+copies_kernel(const CopyList list, int planes) {
+  grid_dep_wait();
+  grid_dep_release();
+  const Copy c = list.c[blockIdx.y];
+  const int chunks = c.pad / 8;
+  const long long total = static_cast<long long>(c.rows) * chunks;
+  T* dst = static_cast<T*>(c.dst);
+  for (long long i = static_cast<long long>(blockIdx.x) * operands::kBlock + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * operands::kBlock) {
+    const int r = static_cast<int>(i / chunks), col = 8 * static_cast<int>(i - static_cast<long long>(r) * chunks);
+    if (c.dtype == NLFA_DTYPE_F32) operands::copy_chunk(static_cast<const float*>(c.src), dst, r, r, col, c.rows, c.cols, c.pad, planes, c.vec);
+    else if (c.dtype == NLFA_DTYPE_F16) operands::copy_chunk(static_cast<const __half*>(c.src), dst, r, r, col, c.rows, c.cols, c.pad, planes, c.vec);
+    else operands::copy_chunk(static_cast<const __nv_bfloat16*>(c.src), dst, r, r, col, c.rows, c.cols, c.pad, planes, c.vec);
+  }
+}
+int make_copies(const CopyList& list, const Layout& l, cudaStream_t st) {
+  if (list.n == 0) return NLFA_OK;
+  long long most = 1;
+  for (int i = 0; i < list.n; ++i) {
+    const long long ctas = (static_cast<long long>(list.c[i].rows) * (list.c[i].pad / 8) + operands::kBlock - 1) / operands::kBlock;
+    most = ctas > most ? ctas : most;
+  }
+  const long long limit = 16ll * sm_count();
+  const dim3 grid(static_cast<unsigned>(most < limit ? most : limit), static_cast<unsigned>(list.n));
+  auto* kernel = l.type == NLFA_DTYPE_F16 ? copies_kernel<__half> : copies_kernel<__nv_bfloat16>;
+  return checked(launch_kernel(kernel, grid, dim3(operands::kBlock), 0, st, overlap_launches(kOverlapRowwise), list, l.planes));
+}
+
 struct Weights {
   const void *x, *gate, *up, *down;
 };
@@ -321,10 +417,16 @@ struct Operand {
   const void* at;
   long long cols, rows;
   bool blocked;
+  int planes;                       // 0: as every operand's
 };
-Operand operand(const void* own, const void* copy, bool copied, int cols, int rows) { return {copied ? copy : own, up64(cols), rows, copied}; }
-int columns(CUtensorMap* m, const Operand& a, const Layout& l) { return column_map(m, a.at, l.type, a.cols, a.rows, l.planes, a.blocked); }
-int rows(CUtensorMap* m, const Operand& a, const Layout& l) { return row_map(m, a.at, l.type, a.cols, a.rows, l.planes, a.blocked); }
+Operand operand(const void* own, const void* copy, bool copied, int cols, int rows) { return {copied ? copy : own, up64(cols), rows, copied, 0}; }
+// A stage of one CTA's half of it: 128 rows, the summands along the columns; or 128 columns, the summands along the rows.
+int columns(CUtensorMap* m, const Operand& a, const Layout& l) {
+  return operands::box_map(m, a.at, l.type, a.cols, a.rows, a.planes > 0 ? a.planes : l.planes, 128, summands(l.planes) / 64, l.planes, a.blocked);
+}
+int rows(CUtensorMap* m, const Operand& a, const Layout& l) {
+  return operands::box_map(m, a.at, l.type, a.cols, a.rows, a.planes > 0 ? a.planes : l.planes, summands(l.planes), 2, l.planes, a.blocked);
+}
 
 struct Operands {
   Operand x, gate, up, down, h;
@@ -332,7 +434,7 @@ struct Operands {
 Operands operands_of(const Call& c, const Layout& l, const Weights& w, const uint8_t* tape) {
   return {operand(w.x, tape + l.x, c.copies & kCopyX, c.d, c.n), operand(w.gate, tape + l.gate, c.copies & kCopyGate, c.d, c.F),
           operand(w.up, tape + l.up, c.copies & kCopyUp, c.d, c.F), operand(w.down, tape + l.down, c.copies & kCopyDown, c.F, c.o),
-          Operand{tape + l.h, l.f_pad, l.n_rows, true}};
+          Operand{tape + l.h, l.f_pad, l.n_rows, true, l.parts}};
 }
 
 Params params(const Call& c, const Layout& l, int activation, uint8_t* tape, unsigned* status) {
@@ -358,14 +460,15 @@ int run_fwd(const Call& c, const Weights& w, int activation, void* y, uint8_t* t
   const Layout l = layout(c);
   unsigned* status = status_block();
   if (!status) return NLFA_ERR_CUDA;
+  CopyList copies{};
   auto copy = [&](int flag, const void* src, int src_dtype, size_t to, int n, int cols) {
-    if (!(c.copies & flag)) return static_cast<int>(NLFA_OK);
-    return copy_rows(src, src_dtype, tape + to, l.type, nullptr, nullptr, n, n, cols, up64(cols), l.planes, st);
+    if (c.copies & flag) copies.c[copies.n++] = {src, tape + to, src_dtype, n, cols, up64(cols), cols % 8 == 0 && aligned16(src)};
   };
-  int rc = copy(kCopyX, w.x, c.x_dtype, l.x, c.n, c.d);
-  if (rc == NLFA_OK) rc = copy(kCopyGate, w.gate, c.w_dtype, l.gate, c.F, c.d);
-  if (rc == NLFA_OK) rc = copy(kCopyUp, w.up, c.w_dtype, l.up, c.F, c.d);
-  if (rc == NLFA_OK) rc = copy(kCopyDown, w.down, c.w_dtype, l.down, c.o, c.F);
+  copy(kCopyX, w.x, c.x_dtype, l.x, c.n, c.d);
+  copy(kCopyGate, w.gate, c.w_dtype, l.gate, c.F, c.d);
+  copy(kCopyUp, w.up, c.w_dtype, l.up, c.F, c.d);
+  copy(kCopyDown, w.down, c.w_dtype, l.down, c.o, c.F);
+  int rc = make_copies(copies, l, st);
   Limits* limits = c.dtype == NLFA_DTYPE_F16 ? reinterpret_cast<Limits*>(tape + l.limits) : nullptr;
   if (rc == NLFA_OK && limits != nullptr) {
     RowList list{};
@@ -379,24 +482,32 @@ int run_fwd(const Call& c, const Weights& w, int activation, void* y, uint8_t* t
   }
   if (rc != NLFA_OK) return rc;
   const Operands a = operands_of(c, l, w, tape);
+  const FwdLayout f = fwd_layout(c, l);
   Maps maps;
   rc = columns(&maps.m[0], a.x, l);
   if (rc == NLFA_OK) rc = columns(&maps.m[1], a.gate, l);
   if (rc == NLFA_OK) rc = columns(&maps.m[2], a.up, l);
-  if (rc == NLFA_OK) rc = operands::box_map(&maps.m[3], tape + l.h, l.type, l.f_pad, l.n_rows, l.planes, 32, 1, 1, true);
+  if (rc == NLFA_OK) rc = operands::box_map(&maps.m[3], tape + l.h, l.type, l.f_pad, l.n_rows, l.parts, 32, 1, 1, true);
   if (rc != NLFA_OK) return rc;
   fill(maps, 4);
   Params p = params(c, l, activation, tape, status);
   p.k = c.d;
   p.scale = limits != nullptr ? &limits->scale : nullptr;
-  rc = launch_product(kUp, l.type, l.planes, long_sum(c.d, l), p, maps, st);
+  p.shares = reinterpret_cast<float*>(scratch + f.shares);
+  if (apart(l, c.F, c.d)) {
+    float *g = reinterpret_cast<float*>(scratch + f.g), *u = reinterpret_cast<float*>(scratch + f.u);
+    plan_up(p, c, l, g, u);
+    rc = launch_product(kProducts, l.type, l.planes, needs_chains(p, l), p, maps, st);
+    if (rc == NLFA_OK) rc = launch_hidden(l.type, l.planes, l.parts, p, g, u, st);
+  } else {
+    rc = launch_product(kUp, l.type, l.planes, long_sum(c.d, l), p, maps, st);
+  }
   if (rc != NLFA_OK) return rc;
   rc = columns(&maps.m[0], a.h, l);
   if (rc == NLFA_OK) rc = columns(&maps.m[1], a.down, l);
   if (rc != NLFA_OK) return rc;
   fill(maps, 2);
   plan_fwd(p, c, l, y, limits != nullptr ? &limits->inverse : nullptr);
-  p.shares = reinterpret_cast<float*>(scratch);
   return launch_product(kProducts, l.type, l.planes, needs_chains(p, l), p, maps, st);
 }
 
@@ -408,7 +519,11 @@ int run_bwd(const Call& c, const void* dy, const Weights& w, int activation, uin
   unsigned* status = status_block();
   if (!status) return NLFA_ERR_CUDA;
   int rc = NLFA_OK;
-  if (copy_dy) rc = copy_rows(dy, c.dtype, scratch + b.dy, l.type, nullptr, nullptr, c.n, c.n, c.o, l.o_pad, l.planes, st);
+  if (copy_dy) {
+    CopyList copies{};
+    copies.c[copies.n++] = {dy, scratch + b.dy, c.dtype, c.n, c.o, l.o_pad, c.o % 8 == 0 && aligned16(dy)};
+    rc = make_copies(copies, l, st);
+  }
   const Limits* limits = c.dtype == NLFA_DTYPE_F16 ? reinterpret_cast<const Limits*>(tape + l.limits) : nullptr;
   BwdLimits* more = reinterpret_cast<BwdLimits*>(scratch + b.limits);
   const bool through = dx || dwg || dwu;                   // whether dg and du are needed
@@ -422,28 +537,32 @@ int run_bwd(const Call& c, const void* dy, const Weights& w, int activation, uin
   }
   if (rc != NLFA_OK) return rc;
   const Operands a = operands_of(c, l, w, tape);
-  const Operand up_grad = operand(dy, scratch + b.dy, copy_dy, c.o, c.n), hidden{scratch + b.hidden, l.f_pad, l.n_rows, true};
-  // dg in the first planes, du in the next
-  auto hidden_map = [&](CUtensorMap* m, int box_rows, int blocks, int planes) {
-    return operands::box_map(m, hidden.at, l.type, l.f_pad, l.n_rows, 2 * l.planes, box_rows, blocks, planes, true);
-  };
+  const Operand up_grad = operand(dy, scratch + b.dy, copy_dy, c.o, c.n), hidden{scratch + b.hidden, l.f_pad, l.n_rows, true, 2 * l.parts};
   Params p = params(c, l, activation, tape, status);
   p.dg = scratch + b.hidden;
-  p.du = scratch + b.hidden + static_cast<size_t>(2 * l.planes) * l.n_rows * l.f_pad;
+  p.du = scratch + b.hidden + static_cast<size_t>(2 * l.parts) * l.n_rows * l.f_pad;
+  p.shares = reinterpret_cast<float*>(scratch + b.shares);
   Maps maps;
   if (through) {
     rc = columns(&maps.m[0], up_grad, l);
     if (rc == NLFA_OK) rc = rows(&maps.m[1], a.down, l);
-    if (rc == NLFA_OK) rc = hidden_map(&maps.m[2], 32, 1, 1);
+    if (rc == NLFA_OK) rc = operands::box_map(&maps.m[2], hidden.at, l.type, l.f_pad, l.n_rows, 2 * l.parts, 32, 1, 1, true);
     if (rc != NLFA_OK) return rc;
     fill(maps, 3);
     p.k = c.o;
     p.scale = limits != nullptr ? &more->scale : nullptr;
-    rc = launch_product(kDh, l.type, l.planes, long_sum(c.o, l), p, maps, st);
+    if (apart(l, c.F, c.o)) {
+      float* dh = reinterpret_cast<float*>(scratch + b.dh);
+      plan_dh(p, c, l, dh);
+      rc = launch_product(kProducts, l.type, l.planes, needs_chains(p, l), p, maps, st);
+      if (rc == NLFA_OK) rc = launch_grads(l.type, l.planes, l.parts, p, dh, st);
+    } else {
+      rc = launch_product(kDh, l.type, l.planes, long_sum(c.o, l), p, maps, st);
+    }
     if (rc != NLFA_OK) return rc;
   }
-  rc = hidden_map(&maps.m[kHiddenRows], summands(l.planes), 2, l.planes);
-  if (rc == NLFA_OK) rc = hidden_map(&maps.m[kHiddenColumns], 128, summands(l.planes) / 64, l.planes);
+  rc = rows(&maps.m[kHiddenRows], hidden, l);
+  if (rc == NLFA_OK) rc = columns(&maps.m[kHiddenColumns], hidden, l);
   if (rc == NLFA_OK) rc = rows(&maps.m[kX], a.x, l);
   if (rc == NLFA_OK) rc = rows(&maps.m[kDy], up_grad, l);
   if (rc == NLFA_OK) rc = rows(&maps.m[kH], a.h, l);
@@ -452,7 +571,6 @@ int run_bwd(const Call& c, const void* dy, const Weights& w, int activation, uin
   if (rc != NLFA_OK) return rc;
   fill(maps, kUpRows + 1);
   plan_bwd(p, c, l, dx, dwg, dwu, dwd, limits != nullptr ? &limits->inverse : nullptr, limits != nullptr ? &more->inverse : nullptr);
-  p.shares = reinterpret_cast<float*>(scratch + b.shares);
   return launch_product(kProducts, l.type, l.planes, needs_chains(p, l), p, maps, st);
 }
 
@@ -476,15 +594,13 @@ size_t nlfa_gated_ffn_tape_bytes(int n, int d, int F, int o, int dtype, int copi
   const Call c{dtype, dtype, dtype, n, d, F, o, copies, train};
   return check_call(c) == NLFA_OK ? layout(c).bytes : 0;
 }
-size_t nlfa_gated_ffn_scratch_bytes(int n, int d, int F, int o, int dtype, int copies, int backward) {
-  const Call c{dtype, dtype, dtype, n, d, F, o, copies, 1};
+size_t nlfa_gated_ffn_scratch_bytes(int n, int d, int F, int o, int dtype, int copies, int train, int backward) {
+  const Call c{dtype, dtype, dtype, n, d, F, o, copies, train};
   if (check_call(c) != NLFA_OK) return 0;
   const Layout l = layout(c);
   // (the gradient of y is copied where it has to be: there is room)
   if (backward) return bwd_layout(c, l, true).bytes;
-  Params p{};
-  plan_fwd(p, c, l, nullptr, nullptr);
-  return 256 + share_bytes(p);
+  return fwd_layout(c, l).bytes;
 }
 
 int nlfa_gated_ffn_fwd(const void* x, int x_dtype, const void* w_gate, const void* w_up, const void* w_down, int w_dtype, int dtype,
@@ -501,7 +617,7 @@ int nlfa_gated_ffn_fwd(const void* x, int x_dtype, const void* w_gate, const voi
       !aligned_to(w_up, w_bytes) || !aligned_to(w_down, w_bytes))
     return NLFA_ERR_MISALIGNED;
   if (nlfa_gated_ffn_copies(x, x_dtype, w_gate, w_up, w_down, w_dtype, dtype, n, d, F, train) & ~copies) return NLFA_ERR_MISALIGNED;
-  if (tape_bytes < layout(c).bytes || scratch_bytes < nlfa_gated_ffn_scratch_bytes(n, d, F, o, dtype, copies, 0)) return NLFA_ERR_SCRATCH_TOO_SMALL;
+  if (tape_bytes < layout(c).bytes || scratch_bytes < nlfa_gated_ffn_scratch_bytes(n, d, F, o, dtype, copies, train, 0)) return NLFA_ERR_SCRATCH_TOO_SMALL;
   if (!nlfa_device_supported()) return NLFA_ERR_NOT_SM100;
   if (nlfa_peek_status() != NLFA_OK) return NLFA_ERR_DEVICE_TIMEOUT;
   if (is_few(x, w_gate, w_up, w_down, w_dtype, dtype, n, d, F, train))

@@ -14,12 +14,13 @@ constexpr int kPartsPerPair = 2;    // shares of odd tiles there is room for, pe
 
 enum { kUp = 0, kDh = 1, kProducts = 2 };
 
-// One product of kProducts: to [m_end, n_end] = scale^-1 A B, the sum in `k` stages.
+// One product of kProducts: to [m_end, n_end] = scale^-1 (A_0 B_0 + A_1 B_1 + ...), `subs` sums of `k_sub` stages that differ in maps and planes (dx = dg Wg + du Wu;
+// hidden values in two parts).
+constexpr int kMostSubs = 4;
 struct Segment {
-  int a_map, b_map, b_map2;         // b_map2, a_plane2: from stage k_half on (dx = dg Wg + du Wu)
-  int a_plane, a_plane2;
-  int a_mn, b_mn;                   // the sum runs along the operand's rows
-  int k_half;
+  int a_map, a_mn, b_mn;            // _mn: the sum runs along the operand's rows
+  int subs, k_sub;
+  int a_plane[kMostSubs], b_map[kMostSubs], b_plane[kMostSubs];
   int tiles, tiles_n, m_end, n_end;
   void* to;
   int dtype;
@@ -47,7 +48,7 @@ struct Params {
   // kept f(g) and u f'(g): 16-bit values with a power of two per 32 values of a row, or float32 (ffn_tc.cu)
   uint8_t *kept;
   int8_t* exponents;
-  void *h, *dg, *du;                // float32: written without TMA
+  void *h, *dg, *du;                // (written without TMA in float32 and by launch_hidden, launch_grads)
   const float* scale;               // of h (kUp) or dg and du (kDh); NULL: 1
   Segment seg[kMostSegments];
   Group group[kMostGroups];
@@ -59,6 +60,10 @@ struct Params {
 int pairs();                        // of CTAs that run at once
 // Maps: kUp x, Wg, Wu, h to store; kDh dy, Wd, dg and du to store; kProducts as the segments say.
 int launch_product(int mode, int dtype, int planes, bool chains, const Params& p, const Maps& maps, cudaStream_t stream);
+
+// What kUp and kDh do behind their products, from products in float32 [rows, cols]: h in `parts` parts and what is kept; dg and du in as many.
+int launch_hidden(int dtype, int planes, int parts, const Params& p, const float* g, const float* u, cudaStream_t stream);
+int launch_grads(int dtype, int planes, int parts, const Params& p, const float* dh, cudaStream_t stream);
 
 // A few tokens, no backward (ffn_few.cu): operands as they lie, d and F multiples of 8, on 16 bytes.  h: n x F.
 // Up to 16 tokens, and up to 64 where tokens times weights are few: the products here are not tcgen05's.  768 x 2,048, 64 tokens: 11 us in bf16, 18 in fp16, 33 in float32,

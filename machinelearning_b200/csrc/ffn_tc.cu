@@ -20,6 +20,7 @@
 // Warps: 0 producer, 1 MMA issuer (even CTA) and TMEM owner, 2-9 epilogue: two warps per quarter of the rows.  Every wait is bounded (ptx.cuh);
 // no multicast loads.
 #include <cfloat>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -249,16 +250,20 @@ template <bool WIDE> __device__ __forceinline__ void times_kept(const uint8_t* a
   }
 }
 
-// float32: 32 columns of a row in three parts, [part][64 columns][rows][64]
-__device__ __forceinline__ void store_parts(void* to, size_t plane, int n_rows, int row, int col, float (&v)[32]) {
-  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(to) + (static_cast<size_t>(col / 64) * n_rows + row) * 64 + col % 64;
-  for (int part = 0; part < 3; ++part, o += plane) {
+// 32 columns of a row in parts, each the nearest value to what is left: [part][64 columns][rows][64]
+template <typename T> __device__ __forceinline__ float round_to(float x);
+template <> __device__ __forceinline__ float round_to<__nv_bfloat16>(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
+template <> __device__ __forceinline__ float round_to<__half>(float x) { return __half2float(__float2half_rn(x)); }
+template <typename T>
+__device__ __forceinline__ void store_parts(void* to, size_t plane, int n_rows, int row, int col, float (&v)[32], int parts = 3) {
+  T* o = static_cast<T*>(to) + (static_cast<size_t>(col / 64) * n_rows + row) * 64 + col % 64;
+  for (int part = 0; part < parts; ++part, o += plane) {
 #pragma unroll
     for (int j = 0; j < 32; j += 8)
-      *reinterpret_cast<uint4*>(o + j) = make_uint4(Pack2<__nv_bfloat16>::pack(v[j], v[j + 1]), Pack2<__nv_bfloat16>::pack(v[j + 2], v[j + 3]),
-                                                    Pack2<__nv_bfloat16>::pack(v[j + 4], v[j + 5]), Pack2<__nv_bfloat16>::pack(v[j + 6], v[j + 7]));
+      *reinterpret_cast<uint4*>(o + j) = make_uint4(Pack2<T>::pack(v[j], v[j + 1]), Pack2<T>::pack(v[j + 2], v[j + 3]),
+                                                    Pack2<T>::pack(v[j + 4], v[j + 5]), Pack2<T>::pack(v[j + 6], v[j + 7]));
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
+    for (int j = 0; j < 32; ++j) v[j] -= round_to<T>(v[j]);
   }
 }
 
@@ -365,10 +370,9 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
             load(st, &maps.m[0], false, a0, k, 0);
             load(st + R::kOperandBytes, &maps.m[1], true, b0, k, 0);
           } else {
-            const bool second = kb >= seg->k_half;
-            const int k = (kb - (second ? seg->k_half : 0)) * R::kSummands;
-            load(st, &maps.m[seg->a_map], seg->a_mn, a0, k, second ? seg->a_plane2 : seg->a_plane);
-            load(st + R::kOperandBytes, &maps.m[second ? seg->b_map2 : seg->b_map], seg->b_mn, b0, k, 0);
+            const int sub = kb / seg->k_sub, k = (kb - sub * seg->k_sub) * R::kSummands;
+            load(st, &maps.m[seg->a_map], seg->a_mn, a0, k, seg->a_plane[sub]);
+            load(st + R::kOperandBytes, &maps.m[seg->b_map[sub]], seg->b_mn, b0, k, seg->b_plane[sub]);
           }
         }
       }
@@ -522,7 +526,7 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
               for (int j = 0; j < 32; ++j) g[j] *= scale;
             }
             if (PARTS == 3) {
-              store_parts(p.h, plane, p.n_rows, row, c0 + 32 * c, g);
+              store_parts<T>(p.h, plane, p.n_rows, row, c0 + 32 * c, g);
             } else {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -572,8 +576,8 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
               }
             }
             if constexpr (PARTS == 3) {
-              store_parts(p.dg, plane, p.n_rows, row, col0 + 32 * c, d);
-              store_parts(p.du, plane, p.n_rows, row, col0 + 32 * c, e);
+              store_parts<T>(p.dg, plane, p.n_rows, row, col0 + 32 * c, d);
+              store_parts<T>(p.du, plane, p.n_rows, row, col0 + 32 * c, e);
             }
           }
           if constexpr (PARTS == 1) {
@@ -629,6 +633,111 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
+// ---- few tiles: the products in float32 first, formed in parts by all pairs of CTAs (ffn.cu: apart), then this; a warp has 32 rows of 32 columns
+constexpr int kApartThreads = 256;
+struct Block {
+  int row, col;                     // this thread's row, the block's first column
+  size_t kept;                      // the block's place among what is kept
+  __device__ bool next(const Params& p, int& i) {
+    const int cols = p.f_pad / 32;
+    if (i >= p.n_rows / 32 * cols) return false;
+    row = i / cols * 32 + (threadIdx.x & 31);
+    col = i % cols * 32;
+    kept = static_cast<size_t>(i) * 2;
+    i += gridDim.x * (kApartThreads / 32);
+    return true;
+  }
+  __device__ void load(const Params& p, const float* from, float (&v)[32]) const {
+    const float* s = from + static_cast<size_t>(row) * p.cols + col;
+    if (row < p.rows && p.cols % 4 == 0 && col + 32 <= p.cols) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(s + j);
+        v[j] = x.x; v[j + 1] = x.y; v[j + 2] = x.z; v[j + 3] = x.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = row < p.rows && col + j < p.cols ? s[j] : 0.f;
+    }
+  }
+};
+
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(kApartThreads)
+hidden_kernel(const __grid_constant__ Params p, int parts, const float* __restrict__ gs, const float* __restrict__ us) {
+  constexpr bool kWide = PLANES == 3 || !Pack2<T>::kIsBf16;
+  constexpr int kKeptBytes = kWide ? 4096 : 2048;
+  grid_dep_wait();
+  grid_dep_release();
+  const float scale = p.scale != nullptr ? *p.scale : 1.f;
+  const int lane = threadIdx.x & 31;
+  int i = blockIdx.x * (kApartThreads / 32) + (threadIdx.x >> 5);
+  Block b;
+  while (b.next(p, i)) {
+    float g[32], u[32], f[32];
+    b.load(p, gs, g);
+    b.load(p, us, u);
+    auto walk = [&](auto act) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        float slope;
+        activate<decltype(act)::value, PLANES == 3>(g[j], f[j], slope);
+        g[j] = f[j] * u[j];
+        u[j] *= slope;
+      }
+    };
+    if (p.activation == NLFA_FFN_SILU) walk(std::integral_constant<int, NLFA_FFN_SILU>{});
+    else if (p.activation == NLFA_FFN_GELU) walk(std::integral_constant<int, NLFA_FFN_GELU>{});
+    else walk(std::integral_constant<int, NLFA_FFN_RELU>{});
+    if (p.kept != nullptr) {
+      keep<kWide>(p.kept + b.kept * kKeptBytes + 16 * lane, p.exponents + 32 * b.kept + lane, f);
+      keep<kWide>(p.kept + (b.kept + 1) * kKeptBytes + 16 * lane, p.exponents + 32 * (b.kept + 1) + lane, u);
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) g[j] *= scale;
+    store_parts<T>(p.h, static_cast<size_t>(p.n_rows) * p.f_pad, p.n_rows, b.row, b.col, g, parts);
+  }
+}
+
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(kApartThreads)
+grads_kernel(const __grid_constant__ Params p, int parts, const float* __restrict__ dh) {
+  constexpr bool kWide = PLANES == 3 || !Pack2<T>::kIsBf16;
+  constexpr int kKeptBytes = kWide ? 4096 : 2048;
+  grid_dep_wait();
+  grid_dep_release();
+  const float scale = p.scale != nullptr ? *p.scale : 1.f;
+  const int lane = threadIdx.x & 31;
+  int i = blockIdx.x * (kApartThreads / 32) + (threadIdx.x >> 5);
+  Block b;
+  while (b.next(p, i)) {
+    float d[32], e[32];
+    b.load(p, dh, d);
+    const uint8_t* as = p.kept + b.kept * kKeptBytes + 16 * lane;
+    float fa = 1.f, fb = 1.f;
+    if (!kWide) {
+      fa = power_of_two(p.exponents[32 * b.kept + lane]);
+      fb = power_of_two(p.exponents[32 * (b.kept + 1) + lane]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float v[8], dg[8], du[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = d[8 * k + j] * scale;
+      times_kept<kWide>(as, k, v, fa, du);
+      times_kept<kWide>(as + kKeptBytes, k, v, fb, dg);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        d[8 * k + j] = dg[j];
+        e[8 * k + j] = du[j];
+      }
+    }
+    const size_t plane = static_cast<size_t>(p.n_rows) * p.f_pad;
+    store_parts<T>(p.dg, plane, p.n_rows, b.row, b.col, d, parts);
+    store_parts<T>(p.du, plane, p.n_rows, b.row, b.col, e, parts);
+  }
+}
+
 int checked(cudaError_t e) {
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? NLFA_OK : NLFA_ERR_CUDA;
@@ -682,7 +791,27 @@ int launch_mode(int mode, bool chains, const Params& p, const Maps& maps, cudaSt
   return act(std::integral_constant<int, NLFA_FFN_RELU>{});
 }
 
+unsigned apart_ctas(const Params& p) {
+  const int need = ceil_div(p.n_rows / 32 * (p.f_pad / 32), kApartThreads / 32), most = 4 * sm_count();
+  return static_cast<unsigned>(need < most ? need : most);
+}
+
 }  // namespace
+
+int launch_hidden(int dtype, int planes, int parts, const Params& p, const float* g, const float* u, cudaStream_t stream) {
+  auto go = [&](auto* kernel) {
+    return checked(launch_kernel(kernel, dim3(apart_ctas(p)), dim3(kApartThreads), 0, stream, overlap_launches(kOverlapRowwise), p, parts, g, u));
+  };
+  if (planes == 3) return go(hidden_kernel<__nv_bfloat16, 3>);
+  return dtype == NLFA_DTYPE_F16 ? go(hidden_kernel<__half, 1>) : go(hidden_kernel<__nv_bfloat16, 1>);
+}
+int launch_grads(int dtype, int planes, int parts, const Params& p, const float* dh, cudaStream_t stream) {
+  auto go = [&](auto* kernel) {
+    return checked(launch_kernel(kernel, dim3(apart_ctas(p)), dim3(kApartThreads), 0, stream, overlap_launches(kOverlapRowwise), p, parts, dh));
+  };
+  if (planes == 3) return go(grads_kernel<__nv_bfloat16, 3>);
+  return dtype == NLFA_DTYPE_F16 ? go(grads_kernel<__half, 1>) : go(grads_kernel<__nv_bfloat16, 1>);
+}
 
 int pairs() { return sm_count() > 1 ? sm_count() / 2 : 1; }     // (without a device: sizes are still asked for)
 

@@ -531,7 +531,7 @@ std::pair<Tensor, Tensor> ffn_forward(const Tensor& x, const Tensor& wg, const T
   shape.back() = c.o;
   Tensor y = empty(shape, out, x);
   Tensor tape = empty({static_cast<int64_t>(nlfa_gated_ffn_tape_bytes(c.n, c.d, c.F, c.o, c.dtype, c.copies, train))}, at::kByte, x);
-  Tensor scratch = empty({static_cast<int64_t>(nlfa_gated_ffn_scratch_bytes(c.n, c.d, c.F, c.o, c.dtype, c.copies, 0))}, at::kByte, x);
+  Tensor scratch = empty({static_cast<int64_t>(nlfa_gated_ffn_scratch_bytes(c.n, c.d, c.F, c.o, c.dtype, c.copies, train, 0))}, at::kByte, x);
   check("nlfa_gated_ffn_fwd",
         nlfa_gated_ffn_fwd(x.data_ptr(), c.x, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), c.w, c.dtype, c.activation, c.n, c.d, c.F, c.o,
                            y.data_ptr(), c.copies, train, tape.data_ptr(), static_cast<size_t>(tape.numel()), scratch.data_ptr(),
@@ -557,7 +557,7 @@ struct GatedFfnBackward : public Node {
     for (int i = 0; i < 4; ++i)
       if (task_should_compute_output(i)) out[i] = empty(shapes[i], i == 0 ? x_dtype : w_dtype, tape_);
     auto at = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
-    Tensor scratch = empty({static_cast<int64_t>(nlfa_gated_ffn_scratch_bytes(c.n, c.d, c.F, c.o, c.dtype, c.copies, 1))}, at::kByte, tape_);
+    Tensor scratch = empty({static_cast<int64_t>(nlfa_gated_ffn_scratch_bytes(c.n, c.d, c.F, c.o, c.dtype, c.copies, 1, 1))}, at::kByte, tape_);
     check("nlfa_gated_ffn_bwd",
           nlfa_gated_ffn_bwd(g.data_ptr(), at(read[0]), c.x, at(read[1]), at(read[2]), at(read[3]), c.w, c.dtype, c.activation, c.n, c.d, c.F,
                              c.o, c.copies, tape_.data_ptr(), static_cast<size_t>(tape_.numel()), at(out[0]), at(out[1]), at(out[2]), at(out[3]),

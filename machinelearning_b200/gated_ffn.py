@@ -60,7 +60,7 @@ def fwd(x, w_gate, w_up, w_down, activation: str, dtype: torch.dtype, train: boo
     with flash_cuda._on_device(x.device.index):
         copies = copies_of(x, w_gate, w_up, w_down, dtype, train)
         tape = torch.empty(lib.nlfa_gated_ffn_tape_bytes(*sizes, dc, copies, train), dtype=torch.uint8, device=x.device)
-        scratch = torch.empty(lib.nlfa_gated_ffn_scratch_bytes(*sizes, dc, copies, 0), dtype=torch.uint8, device=x.device)
+        scratch = torch.empty(lib.nlfa_gated_ffn_scratch_bytes(*sizes, dc, copies, train, 0), dtype=torch.uint8, device=x.device)
         st = lib.nlfa_gated_ffn_fwd(x.data_ptr(), xc, *weights, wc, dc, ACTIVATIONS[activation], *sizes, y.data_ptr(), copies, train,
                                     tape.data_ptr(), tape.numel(), scratch.data_ptr(), scratch.numel(), _stream(x))
     _lib.check("nlfa_gated_ffn_fwd", st)
@@ -75,7 +75,7 @@ def bwd(dy, x, w_gate, w_up, w_down, tape, copies: int, shapes, x_dtype, w_dtype
     dc = _DTYPE_CODE[dy.dtype]
     out = [torch.empty(s, dtype=x_dtype if i == 0 else w_dtype, device=dy.device) if want[i] else None for i, s in enumerate(shapes)]
     with flash_cuda._on_device(dy.device.index):
-        scratch = torch.empty(lib.nlfa_gated_ffn_scratch_bytes(*sizes, dc, copies, 1), dtype=torch.uint8, device=dy.device)
+        scratch = torch.empty(lib.nlfa_gated_ffn_scratch_bytes(*sizes, dc, copies, True, 1), dtype=torch.uint8, device=dy.device)
         st = lib.nlfa_gated_ffn_bwd(dy.data_ptr(), _ptr(x), _DTYPE_CODE[x_dtype], _ptr(w_gate), _ptr(w_up), _ptr(w_down), _DTYPE_CODE[w_dtype],
                                     dc, ACTIVATIONS[activation], *sizes, copies, tape.data_ptr(), tape.numel(), *(_ptr(t) for t in out),
                                     scratch.data_ptr(), scratch.numel(), _stream(dy))

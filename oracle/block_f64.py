@@ -71,7 +71,7 @@ def activation(g, kind):
 
 def gated_ffn(x, w_gate, w_up, w_down, kind="silu", dy=None, step=0.0):
     """dict of ``y`` and, for an upstream ``dy``, ``dx``, ``dw_gate``, ``dw_up``, ``dw_down``; ``noise_*``: the standard deviation that these have when h, dg
-    and du are rounded independently, each by a standard deviation of ``step`` of its value, and ``size_*``: the sums of their summands' magnitudes."""
+    and du are rounded independently, each by a standard deviation of ``step`` of its value (so with 1 it is to be scaled), and ``size_*``: the sums of their summands' magnitudes."""
     x, wg, wu, wd = (np.asarray(t, np.float64) for t in (x, w_gate, w_up, w_down))
     g, u = x @ wg.T, x @ wu.T
     a, da = activation(g, kind)
