@@ -106,3 +106,70 @@ def test_captured_step_and_decoding_beside_it():
         losses.append(seen)
         step.close()
     assert losses[0] == losses[1]
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_and_a_backward_that_runs_twice():
+    """Workspaces are each call's own: calls that overlap, and a graph that is kept, give the bits of calls alone."""
+    from machinelearning_b200 import gated_ffn, gated_scan
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    x, wg, wu, wd = (t.bfloat16().requires_grad_() for t in (rand(900, 128), rand(320, 128) * 0.1, rand(320, 128) * 0.1, rand(128, 320) * 0.1))
+    z, v, s = (t.requires_grad_() for t in (rand(2, 3000, 40), rand(2, 3000, 40), rand(2, 40)))
+
+    def both():
+        y = gated_ffn.gated_ffn(x, wg, wu, wd)
+        h, last = gated_scan.gated_scan(z, v, s)
+        return y, h, last
+
+    def grads(out, keep=False):
+        y, h, last = out
+        return (*torch.autograd.grad(y, (x, wg, wu, wd), torch.ones_like(y), retain_graph=keep),
+                *torch.autograd.grad((h, last), (z, v, s), (torch.ones_like(h), torch.ones_like(last)), retain_graph=keep))
+    out = both()
+    want = (*out, *grads(out, keep=True))
+    assert all(torch.equal(a, b) for a, b in zip(grads(out), want[3:]))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for st in streams:
+        with torch.cuda.stream(st):
+            out = both()
+            got.append((*out, *grads(out)))
+    torch.cuda.synchronize()
+    for one in got:
+        assert all(torch.equal(a, b) for a, b in zip(one, want))
+
+
+@pytest.mark.gpu
+def test_outputs_have_no_more_than_their_own_memory():
+    """Results between guard values: nothing behind the last row or column is written."""
+    from machinelearning_b200 import _lib, flash_cuda, gated_scan
+    lib = flash_cuda._load()
+    g = torch.Generator(device="cuda").manual_seed(6)
+    for B, T, D in ((2, 37, 24), (1, 1030, 7), (3, 20, 72)):
+        z, v = torch.randn(B, T, D, device="cuda", generator=g), torch.randn(B, T, D, device="cuda", generator=g)
+        guarded = torch.full((B * T * D + 128,), 777.0, device="cuda")
+        last = torch.full((B * D + 64,), 777.0, device="cuda")
+        scratch = gated_scan._scratch(lib, z)
+        st = lib.nlfa_gated_scan_fwd(z.data_ptr(), T * D, D, v.data_ptr(), T * D, D, 0, None, None, None, 0, 0, B, T, D, guarded[64:].data_ptr(),
+                                     last[32:].data_ptr(), None, 0, scratch.data_ptr(), scratch.numel(), torch.cuda.current_stream().cuda_stream)
+        assert st == _lib.OK
+        want = gated_scan.gated_scan(z, v)
+        assert torch.equal(guarded[64:-64].view(B, T, D), want[0]) and torch.equal(last[32:-32].view(B, D), want[1])
+        assert bool((guarded[:64] == 777).all()) and bool((guarded[-64:] == 777).all()) and bool((last[:32] == 777).all()) and bool((last[-32:] == 777).all())
+    for n, d, F, o in ((70, 64, 128, 72), (9, 24, 40, 19), (300, 100, 70, 130)):
+        x, wg, wu, wd = (torch.randn(*s, device="cuda", generator=g) for s in ((n, d), (F, d), (F, d), (o, F)))
+        y = torch.full((n * o + 128,), 777.0, device="cuda")
+        copies = lib.nlfa_gated_ffn_copies(x.data_ptr(), 0, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), 0, 0, n, d, F, 1)
+        tape = torch.empty(lib.nlfa_gated_ffn_tape_bytes(n, d, F, o, 0, copies, 1), dtype=torch.uint8, device="cuda")
+        scratch = torch.empty(lib.nlfa_gated_ffn_scratch_bytes(n, d, F, o, 0, copies, 1, 0), dtype=torch.uint8, device="cuda")
+        at = torch.cuda.current_stream().cuda_stream
+        assert lib.nlfa_gated_ffn_fwd(x.data_ptr(), 0, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), 0, 0, 0, n, d, F, o, y[64:].data_ptr(), copies, 1,
+                                      tape.data_ptr(), tape.numel(), scratch.data_ptr(), scratch.numel(), at) == _lib.OK
+        out = [torch.full((a * b + 128,), 777.0, device="cuda") for a, b in ((n, d), (F, d), (F, d), (o, F))]
+        back = torch.empty(lib.nlfa_gated_ffn_scratch_bytes(n, d, F, o, 0, copies, 1, 1), dtype=torch.uint8, device="cuda")
+        dy = torch.randn(n, o, device="cuda", generator=g)
+        assert lib.nlfa_gated_ffn_bwd(dy.data_ptr(), None, 0, None, None, None, 0, 0, 0, n, d, F, o, copies, tape.data_ptr(), tape.numel(),
+                                      *(t[64:].data_ptr() for t in out), back.data_ptr(), back.numel(), at) == _lib.OK
+        for t in (y, *out):
+            assert bool((t[:64] == 777).all()) and bool((t[-64:] == 777).all()) and not bool((t[64:-64] == 777).any())
