@@ -68,8 +68,9 @@ Layout layout(const Call& c) {
   l.planes = c.dtype == NLFA_DTYPE_F32 ? 3 : 1;
   l.type = c.dtype == NLFA_DTYPE_F32 ? NLFA_DTYPE_BF16 : c.dtype;
   // The roundings of h, dg and du are independent and largely cancel in sums, but results of a few tokens are few: beside their own rounding
-  // the others leave 1.4 times its error on average, and up to 1.6 for 15 tokens.  A tile of rows is held in two parts: its products are short.
-  l.parts = l.planes == 3 ? 3 : c.train && c.n <= kRowTile ? 2 : 1;
+  // the others leave 1.4 times its error on average, and up to 1.7 for a few.  A tile of rows with a backward, and as many as the kernels for a few tokens
+  // would take without one, are held in two parts: their products are short.
+  l.parts = l.planes == 3 ? 3 : c.n <= (c.train ? kRowTile : kFewTokens) ? 2 : 1;
   l.n_rows = (c.n + kRowTile - 1) / kRowTile * kRowTile;
   l.d_pad = up64(c.d);
   l.f_pad = up64(c.F);

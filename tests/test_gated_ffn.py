@@ -2,7 +2,7 @@
 oracle, types and autocast, ranges of float16, graphs and streams.
 
 Bounds.  16 bits: h, dg and du are rounded once, each by at most half a step u (bf16 2^-8, fp16 2^-11) of its value -- up to 256 tokens with a backward they are held in two parts, and
-the half step is u u; up to 64 without one it is 2^-17.  The roundings are independent, u / sqrt(3) of a value in the worst place of a binade (its standard deviation), so a sum of them has the
+the half step is u u; up to 64 without one it is 2^-16 or less.  The roundings are independent, u / sqrt(3) of a value in the worst place of a binade (its standard deviation), so a sum of them has the
 deviation u / sqrt(3) `noise` (block_f64), and 6 of these bound every element of 10^5.  In bf16 what is kept of g and u for the backward has fp16's half step, 2^-11.  Where a sum has few summands it is bounded by u of their magnitudes instead.  Beside that: the result's own half
 step, and float32 sums on the tensor cores, 2^-17 of the summands' magnitudes for chains of up to 4,096 (loss_tc.cu: 1.1e-5 for positive ones).
 float32: three parts are exact to 2^-24, chains of 64 summands low by under 2^-22, up to 8 chains of which are added here, and products of parts
@@ -136,7 +136,7 @@ def test_result_and_gradients(dtype, n, d, F, o):
         assert torch.equal(again, y) and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(again, leaves, dy), grads))
         with torch.no_grad():
             alone = gated_ffn.gated_ffn(*leaves, activation=kind)
-        _check((alone,), leaves, None, kind, dtype, hidden=2.0**-17 if n <= 64 and d % 8 == 0 and F % 8 == 0 else None)
+        _check((alone,), leaves, None, kind, dtype, hidden=2.0**-16 if n <= 64 else None)
 
 
 @pytest.mark.gpu
