@@ -167,10 +167,13 @@ int chain(const Layout& l) { return l.planes == 3 ? 1 : l.type == NLFA_DTYPE_F16
 
 // Whether g and u, or dh, are formed apart from what is done with them: where there are so few tiles that most pairs of CTAs would watch, and their sums
 // are so long that three more launches are less (80 tokens x 3,903 x 32 in float32, forward and backward 270 us with one tile's sums of 61 stages); and for parts.
-bool apart(const Layout& l, int cols, int k) {
+// `most`: stages that are not worth it (float32's dh, whose epilogue writes six planes, 1,000 x 384 x 1,024: 43 us, apart 29 with the launches; its g and u 26, apart 37).
+bool apart(const Layout& l, int cols, int k, int most) {
   if (l.parts == 2) return true;
-  return 2 * (l.n_rows / kRowTile) * ceil_div(cols, kColTile) <= pairs() && ceil_div(k, summands(l.planes)) > (l.planes == 3 ? 12 : 36);
+  return 2 * (l.n_rows / kRowTile) * ceil_div(cols, kColTile) <= pairs() && ceil_div(k, summands(l.planes)) > most;
 }
+bool apart_up(const Call& c, const Layout& l) { return apart(l, c.F, c.d, l.planes == 3 ? 12 : 36); }
+bool apart_dh(const Call& c, const Layout& l) { return apart(l, c.F, c.o, l.planes == 3 ? 4 : 36); }
 
 // Forward, g and u apart: maps x, Wg, Wu.
 void plan_up(Params& p, const Call& c, const Layout& l, float* g, float* u) {
@@ -234,7 +237,7 @@ BwdLayout bwd_layout(const Call& c, const Layout& l, bool copy_dy) {
   size_t at = 256;
   b.dy = at; if (copy_dy) at = up(at + two * c.n * l.o_pad);
   b.hidden = at; at = up(at + 4 * static_cast<size_t>(l.parts) * l.n_rows * l.f_pad);
-  b.dh = at; if (apart(l, c.F, c.o)) at = up(at + static_cast<size_t>(c.n) * c.F * 4);
+  b.dh = at; if (apart_dh(c, l)) at = up(at + static_cast<size_t>(c.n) * c.F * 4);
   b.shares = at;
   // enough for any choice of gradients
   at += static_cast<size_t>(kMostGroups * kPartsPerPair * pairs()) * kRowTile * kColTile * sizeof(float);
@@ -252,7 +255,7 @@ FwdLayout fwd_layout(const Call& c, const Layout& l) {
   Params p{};
   plan_fwd(p, c, l, nullptr, nullptr);
   most = share_bytes(p);
-  if (apart(l, c.F, c.d)) {
+  if (apart_up(c, l)) {
     f.g = at; at = up(at + static_cast<size_t>(c.n) * c.F * 4);
     f.u = at; at = up(at + static_cast<size_t>(c.n) * c.F * 4);
     plan_up(p, c, l, nullptr, nullptr);
@@ -495,7 +498,7 @@ int run_fwd(const Call& c, const Weights& w, int activation, void* y, uint8_t* t
   p.k = c.d;
   p.scale = limits != nullptr ? &limits->scale : nullptr;
   p.shares = reinterpret_cast<float*>(scratch + f.shares);
-  if (apart(l, c.F, c.d)) {
+  if (apart_up(c, l)) {
     float *g = reinterpret_cast<float*>(scratch + f.g), *u = reinterpret_cast<float*>(scratch + f.u);
     plan_up(p, c, l, g, u);
     rc = launch_product(kProducts, l.type, l.planes, needs_chains(p, l), p, maps, st);
@@ -552,7 +555,7 @@ int run_bwd(const Call& c, const void* dy, const Weights& w, int activation, uin
     fill(maps, 3);
     p.k = c.o;
     p.scale = limits != nullptr ? &more->scale : nullptr;
-    if (apart(l, c.F, c.o)) {
+    if (apart_dh(c, l)) {
       float* dh = reinterpret_cast<float*>(scratch + b.dh);
       plan_dh(p, c, l, dh);
       rc = launch_product(kProducts, l.type, l.planes, needs_chains(p, l), p, maps, st);
