@@ -67,7 +67,7 @@ int launch_grads(int dtype, int planes, int parts, const Params& p, const float*
 
 // A few tokens, no backward (ffn_few.cu): operands as they lie, d and F multiples of 8, on 16 bytes.  h: n x F.
 // Up to 16 tokens, and up to 64 where tokens times weights are few: the products here are not tcgen05's.  768 x 2,048, 64 tokens: 11 us in bf16, 18 in fp16, 33 in float32,
-// by tiles of 256 rows 20, 30, 69; 4,096 x 8,192: 150, 284, 533 and 60, 89, 400, 16 tokens 66, 102, 244 and 60, 89, 405.
+// by tiles of 256 rows 20, 30, 69; 4,096 x 8,192: 150, 284, 533 and 60, 89, 400, 16 tokens 72, 88, 185 and 60, 89, 405.
 constexpr int kFewTokens = 64, kVeryFewTokens = 16;
 constexpr long long kFewProducts = 1ll << 28;               // n d F
 bool few_types(int w_dtype, int dtype);

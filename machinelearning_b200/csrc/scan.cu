@@ -29,7 +29,7 @@ namespace scan {
 namespace {
 
 // Steps in a thread's registers; states at their starts are the backward's tape.  (float32 with 16: 96 KB of shared memory a CTA, backward of
-// 32 x 1,024 x 768 168 us; with 8 117.  bf16, 64 x 1,024 x 768, with 8: 70 and 128 us, with 16 67 and 118.)
+// 32 x 1,024 x 768 168 us; with 8 100.  bf16, 64 x 1,024 x 768, with 8: 70 and 128 us, with 16 67 and 118 then, 65 and 105 now.)
 template <typename T> constexpr int kRunOf = sizeof(T) == 4 ? 8 : 16;
 constexpr int kWarps = 4;           // runs side by side in a CTA (or twice as many)
 constexpr int kMostExtent = 1 << 30;
@@ -581,7 +581,7 @@ int run_of(int dtype) { return dtype == NLFA_DTYPE_F32 ? kRunOf<float> : kRunOf<
 
 // Into how many segments the sequences are cut, and how many runs a CTA walks side by side: by the columns (of 64 channels of a sequence) there are.
 //   up to an eighth of what runs at once: segments, twice as many CTAs as run at once.  1 x 131,072 x 1,024 (16 columns) forward and backward
-//     281 + 397 us, uncut with 8 warps 1,500 + 2,600; 8 x 4,096 x 512 (64) 36 + 54, uncut 50 + 86; but 8 x 2,048 x 768 (96) 28 + 41, uncut 26 + 45:
+//     274 + 410 us, uncut with 4 warps 1,854 + 3,128; 8 x 4,096 x 512 (64) 36 + 54, uncut 50 + 86; but 8 x 2,048 x 768 (96) 28 + 41, uncut 26 + 45:
 //     the maps read the inputs once more.
 //   up to two per SM: 8 warps.  16 x 1,024 x 768 (192) 23 + 38 us, with 4 warps 28 + 38; 16 x 2,048 x 512 (128) 26 + 45, with 4 34 + 53.
 //   else 4: 64 x 1,024 x 768 (768) 64 + 105 us, with 8 62 + 108.

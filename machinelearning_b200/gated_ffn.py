@@ -2,8 +2,8 @@
 
 ``gated_ffn(x, w_gate, w_up, w_down)`` is nanolab's ``SwiGLU`` (``nanolab/model.py:29-43``; ``f`` may be another one).  Both projections, the
 activation and the product are one kernel, the projection down another; the backward is two more (``csrc/ffn.cu``, ``csrc/ffn_tc.cu``).
-Kept for the backward: the hidden values, and what the activation was applied to, 6 bytes for each of the ``F`` hidden values of a token
-in 16-bit types -- torch's own graph of the same layer keeps 8.
+Kept for the backward: the hidden values and what turns their gradient into the projections', 6 bytes for each of the ``F`` hidden values of a token in
+bfloat16 (float16 10, float32 14; torch's own graph of the same layer keeps 8, in float32 16).
 
 An ``autograd`` node over the C entry points.  No CPU path: ``supports`` says whether a call can run; the function raises otherwise.
 """
