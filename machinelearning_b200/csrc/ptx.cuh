@@ -187,11 +187,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-// `bytes` contiguous bytes (a multiple of 16, on a 16-byte boundary) into L2 alone
-__device__ __forceinline__ void bulk_prefetch(const void* src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
-}
-
 // 4-D tiled store from shared memory (same box and swizzle as the loads).  Rows that fall
 // outside the tensor are clipped by the hardware.
 __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1,
