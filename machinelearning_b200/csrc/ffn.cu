@@ -5,8 +5,8 @@
 //   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h
 //
 // Bound by the tensor cores: 2 N F (2 d + o) operations forward and twice that backward, in four launches of products (ffn_tc.cu).  g, u and dh exist in
-// tensor memory alone; the tape keeps f(g) and u f'(g) for the backward.  Between the products h, dg and du are operands: 16 bits (float32:
-// three bf16 parts), one rounding each beside that of the results.
+// tensor memory alone (where few tiles have long sums, in float32 beside the products: apart() below); the tape keeps f(g) and u f'(g) for the
+// backward.  Between the products h, dg and du are operands: 16 bits (float32: three bf16 parts), one rounding each beside that of the results.
 //
 // This file has what goes around the products: 16-bit copies of operands that TMA cannot read as they are, the list of tiles and
 // parts, and the powers of two that hold float16's h, dg and du inside their type's range.
@@ -101,7 +101,8 @@ int choose_parts(int rest, int k, int n_pairs, int share, int ahead, int length)
   if (rest == 0) return 1;
   int best = 1;
   long long least = -1;
-  for (int s = 1; s <= kPartsPerPair * n_pairs / rest && s <= k; ++s) {
+  const int most = kPartsPerPair * n_pairs / rest < k ? kPartsPerPair * n_pairs / rest : k;
+  for (int s = 1; s <= most;) {
     const int end = ahead + rest * s, mine = (k + s - 1) / s + (s > 1 ? share : 0);
     long long cost = 0;
     for (int i = 0; i < 3; ++i) {                          // the first pair, and the first that gets one unit less of either kind
@@ -112,6 +113,10 @@ int choose_parts(int rest, int k, int n_pairs, int share, int ahead, int length)
     }
     cost += s > 1 ? s + kFoldStages : 0;
     if (least < 0 || cost < least) { least = cost; best = s; }
+    // on to the next number of parts that makes the longest one shorter (a call is planned on the host, each time)
+    const int longest = (k + s - 1) / s;
+    if (longest == 1) break;
+    s = (k + longest - 2) / (longest - 1);
   }
   return best;
 }
@@ -140,11 +145,10 @@ void add_group(Params& p, int seg0, int seg1, int k, int planes) {
   p.units = g.end;
   ++p.groups;
 }
-size_t share_bytes(const Params& p) {
-  size_t n = 0;
-  for (int i = 0; i < p.groups; ++i)
-    if (p.group[i].parts > 1) n += static_cast<size_t>(p.group[i].rest) * p.group[i].parts;
-  return n * kRowTile * kColTile * sizeof(float);
+// Room for the shares of a group, however it is cut.
+size_t share_room(int tiles, int k) {
+  const long long odd = static_cast<long long>(tiles % pairs()) * k, most = static_cast<long long>(kPartsPerPair) * pairs();
+  return static_cast<size_t>(odd < most ? odd : most) * kRowTile * kColTile * sizeof(float);
 }
 // A product of one sum; add() gives it more.
 Segment segment(int a_map, int a_mn, int a_plane, int b_map, int b_mn, int b_plane, int k, int m, int n, void* to, int dtype, const float* inverse) {
@@ -251,15 +255,13 @@ struct FwdLayout {
 };
 FwdLayout fwd_layout(const Call& c, const Layout& l) {
   FwdLayout f{};
-  size_t at = 0, most = 0;
-  Params p{};
-  plan_fwd(p, c, l, nullptr, nullptr);
-  most = share_bytes(p);
+  const int row_tiles = l.n_rows / kRowTile, stage = summands(l.planes);
+  size_t at = 0, most = share_room(row_tiles * ceil_div(c.o, kColTile), (l.parts == 2 ? 2 : 1) * ceil_div(c.F, stage));
   if (apart_up(c, l)) {
     f.g = at; at = up(at + static_cast<size_t>(c.n) * c.F * 4);
     f.u = at; at = up(at + static_cast<size_t>(c.n) * c.F * 4);
-    plan_up(p, c, l, nullptr, nullptr);
-    if (share_bytes(p) > most) most = share_bytes(p);
+    const size_t more = share_room(2 * row_tiles * ceil_div(c.F, kColTile), ceil_div(c.d, stage));
+    most = more > most ? more : most;
   }
   f.shares = at;
   f.bytes = at + most + 256;
