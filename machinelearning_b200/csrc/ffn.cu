@@ -305,7 +305,7 @@ __device__ __forceinline__ void largest_row(const Rows& s) {
     float sum = 0.f, top = 0.f;
     auto add = [&](float v) {
       sum = fmaf(v, v, sum);
-      top = fabsf(v) <= 65504.f ? fmaxf(top, fabsf(v)) : INFINITY;
+      top = fabsf(v) < 65520.f ? fmaxf(top, fabsf(v)) : INFINITY;      // (what is below is rounded to at most 65,504)
     };
     if (s.vec) {
 #pragma unroll 4

@@ -247,6 +247,32 @@ def test_float16_hidden_values_outside_the_types_range(x_size, w_size, up):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("where", ["x", "w_down"])
+def test_float32_values_that_round_to_the_largest_float16(where):
+    """65,512 is above float16's largest value, 65,504, and is rounded to it: finite, and part of what bounds h, dg and du."""
+    from machinelearning_b200 import gated_ffn
+    leaves, dy = _inputs(torch.float32, 5, 64, 64, 32)
+    dy = dy.half()
+    with torch.no_grad():
+        if where == "x":                                           # every g and u some 512, h up to 2^20; y some 2^10
+            leaves[0][:, 0] = 65512.0
+            for w in leaves[1:3]:
+                w[:, 0] = w[:, 0].sign() * 2.0**-7
+            leaves[3] *= 2.0**-8
+        else:                                                      # dg of one hidden value up to 2^18; y there is outside float16
+            leaves[3][7, 11] = 65512.0
+    with torch.autocast("cuda", dtype=torch.float16):
+        y = gated_ffn.gated_ffn(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy)
+    # (what h, dg and du lose below float16's normal range is 2^-25 of 2^15 / the largest: below 2^-17 of the sums' magnitudes, which hold the largest, or
+    # of one rounding's 2^-11 of the others, which are above 2^-14 of it there)
+    if where == "x":
+        _check((y, *grads), leaves, dy, "silu", torch.float16)
+    else:
+        _check(grads, leaves, dy, "silu", torch.float16, NAMES)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=_id)
 def test_a_row_that_is_not_finite_stays_alone(dtype):
     """Its own y and dx, and the weights' gradients it enters; other rows' bits are what they were (in 16 bits; and in float32, where an infinity gives NaN)."""
