@@ -173,3 +173,46 @@ def test_outputs_have_no_more_than_their_own_memory():
                                       *(t[64:].data_ptr() for t in out), back.data_ptr(), back.numel(), at) == _lib.OK
         for t in (y, *out):
             assert bool((t[:64] == 777).all()) and bool((t[-64:] == 777).all()) and not bool((t[64:-64] == 777).any())
+
+
+@pytest.mark.gpu
+def test_rows_behind_two_to_the_31_elements():
+    """What stands at the end of tensors of more than 2^31 elements is what a short call of the same rows gives, up to where sums are cut.
+
+    Two float32 sums of one value round to neighbours in bfloat16 at most: 2^-7 of it, beside the sums' own difference.  Recurrence: states and gradients
+    below 16, 2^-22 of which a walk is off by: 2^-18.  Layer: 2^-17 of the summands' magnitudes for each of the two calls (tests of the layer), which are below 64
+    for y (2,048 of some 0.4 x 0.018) and below 512 for dx (twice 2,048 of some 0.5 x 0.1)."""
+    from machinelearning_b200 import gated_ffn, gated_scan
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of free device memory")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rand = lambda *s, std=1.0: (torch.randn(*s, device="cuda", dtype=torch.bfloat16, generator=g) * std).requires_grad_()
+
+    def close(got, want, beside):
+        want = want.float()
+        assert bool(((got.float() - want).abs() <= 2.0**-7 * want.abs() + beside).all())
+
+    for width in (1032, 1031):
+        gate, value, dh = (rand(2, 1 << 20, width) for _ in range(3))
+        h, last = gated_scan.gated_scan(gate, value)
+        grads = torch.autograd.grad(h, (gate, value), dh)
+        short = [t.detach()[1:, -4096:].clone().requires_grad_() for t in (gate, value)]
+        end, end_last = gated_scan.gated_scan(*short)
+        want = torch.autograd.grad(end, short, dh.detach()[1:, -4096:])
+        # (behind 1,000 steps nothing of the state in front of them is left)
+        for a, b in zip((h, *grads), (end, *want)):
+            close(a.detach()[1:, -3096:], b.detach()[:, 1000:], 2.0**-18)
+        close(last.detach()[1:], end_last.detach(), 2.0**-18)
+        del gate, value, dh, h, last, grads, short, end, want
+        torch.cuda.empty_cache()
+    n = 1_100_000
+    x, wg, wu, wd, dy = rand(n, 64), rand(2048, 64, std=0.125), rand(2048, 64, std=0.125), rand(64, 2048, std=2048**-0.5), rand(n, 64)
+    y = gated_ffn.gated_ffn(x, wg, wu, wd)
+    dx = torch.autograd.grad(y, x, dy)[0]
+    for at in (n // 2, n - 700):
+        some = x.detach()[at:at + 700].clone().requires_grad_()
+        part = gated_ffn.gated_ffn(some, wg, wu, wd)
+        close(y.detach()[at:at + 700], part.detach(), 2.0**-16 * 64)
+        close(dx[at:at + 700], torch.autograd.grad(part, some, dy.detach()[at:at + 700])[0], 2.0**-16 * 512)
+    del x, y, dy, dx
+    torch.cuda.empty_cache()
