@@ -150,25 +150,33 @@ template <int V> __device__ __forceinline__ float2 step(float2 y, float2 f, floa
 // (1 - s) q
 template <int V> __device__ __forceinline__ float2 kept(float2 y, float2 q) { return fma_<V>(y, q, choose(y, q, both(0.f))); }
 
-// Two channels' maps h -> a h + b of some steps, (a, b, a, b).  With resets, a == 0: nothing of h is left, whatever it holds.
-__device__ __forceinline__ float2 apply(const float4& m, float2 h, bool select = true) {
-  if (!select) return make_float2(fmaf(m.x, h.x, m.y), fmaf(m.z, h.y, m.w));
-  return make_float2(m.x == 0.f ? m.y : fmaf(m.x, h.x, m.y), m.z == 0.f ? m.w : fmaf(m.z, h.y, m.w));
+// Two channels' maps h -> a h + b of some steps, (a, b, a, b).  Behind a reset nothing of h is left, whatever it holds: a is -0.  Factors are not
+// negative otherwise, and one that underflows is +0: what is not finite goes through it as NaN.
+constexpr float kNothing = -0.f;
+__device__ __forceinline__ bool is_nothing(float a) { return __float_as_int(a) == __float_as_int(kNothing); }
+template <bool RESET> __device__ __forceinline__ float2 apply(const float4& m, float2 h) {
+  const float2 r = make_float2(fmaf(m.x, h.x, m.y), fmaf(m.z, h.y, m.w));
+  return RESET ? make_float2(is_nothing(m.x) ? m.y : r.x, is_nothing(m.z) ? m.w : r.y) : r;
 }
 // m, then n
-__device__ __forceinline__ float4 then(const float4& m, const float4& n) {
-  const float2 b = apply(n, make_float2(m.y, m.w));
-  return make_float4(m.x * n.x, b.x, m.z * n.z, b.y);
+template <bool RESET> __device__ __forceinline__ float4 then(const float4& m, const float4& n) {
+  const float2 b = apply<RESET>(n, make_float2(m.y, m.w));
+  auto factor = [](float a, float c) { return RESET && (is_nothing(a) || is_nothing(c)) ? kNothing : a * c; };
+  return make_float4(factor(m.x, n.x), b.x, factor(m.z, n.z), b.y);
+}
+// The map of some steps, of which `resets` begin anew (the same ones for all channels of a sequence).
+template <bool RESET> __device__ __forceinline__ float4 map_of(float2 a, float2 b, bool resets) {
+  return RESET && resets ? make_float4(kNothing, b.x, kNothing, b.y) : make_float4(a.x, b.x, a.y, b.y);
 }
 
 // The state in front of this thread's run, given its run's map, and the state behind the CTA's runs in `carry`.  `maps`: in shared memory, [2][WARPS][lane];
 // `order`: this warp's place in its CTA, in the order in which the runs are walked.
 template <int WARPS> __host__ __device__ constexpr int exchange_bytes() { return WARPS > 1 ? 2 * WARPS * 32 * 16 : 0; }
-template <int WARPS>
+template <int WARPS, bool RESET>
 __device__ __forceinline__ float2 enter(float4* maps, int buf, int order, float4 own, float2& carry) {
   if (WARPS == 1) {
     const float2 in = carry;
-    carry = apply(own, in);
+    carry = apply<RESET>(own, in);
     return in;
   }
   float4* mine = maps + buf * WARPS * 32 + (threadIdx.x & 31);
@@ -178,7 +186,7 @@ __device__ __forceinline__ float2 enter(float4* maps, int buf, int order, float4
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) {
     if (w == order) in = carry;
-    carry = apply(mine[32 * w], carry);
+    carry = apply<RESET>(mine[32 * w], carry);
   }
   return in;
 }
@@ -346,7 +354,7 @@ scan_fwd_kernel(const Params p) {
   settle(0);
   float2 carry = load_state<V>(p.state + row, w.live && p.state != nullptr);
 #pragma unroll 4
-  for (int s = 0; s < w.segment; ++s) carry = apply(*w.map(p, s), carry);
+  for (int s = 0; s < w.segment; ++s) carry = apply<RESET>(*w.map(p, s), carry);
   int buf = 0;
   for (int from = w.t0; from < w.t1; from += kStretch, buf ^= 1) {
     const int t0 = from + first, n = live - t0;                // (steps of this run that count: n, if it is between 0 and kRun)
@@ -372,17 +380,16 @@ scan_fwd_kernel(const Params p) {
     };
     if (n >= kRun) walk(std::true_type{});
     else walk(std::false_type{});
-    const float4 map = make_float4(a.x, b.x, a.y, b.y);
-    const float2 in = enter<WARPS>(maps, buf, w.warp, map, carry);
+    const float4 map = map_of<RESET>(a, b, resets != 0u);
+    const float2 in = enter<WARPS, RESET>(maps, buf, w.warp, map, carry);
     if (t0 < p.T) {
       if (p.tape != nullptr && w.live) store_state<V>(p.tape + (static_cast<long long>(w.b) * runs + t0 / kRun) * p.D + w.c, in);
       auto put = [&](auto whole) {
 #pragma unroll
         for (int i = 0; i < kRun; ++i) {
           if (!decltype(whole)::value && t0 + i >= p.T) break;
-          float2 v;
-          if (RESET) v = apply(make_float4(left[i].x, h[i].x, left[i].y, h[i].y), in);
-          else v = fma_<V>(left[i], in, h[i]);
+          float2 v = h[i];
+          if (!RESET || !(resets & ((2u << i) - 1u))) v = fma_<V>(left[i], in, h[i]);
           if (!decltype(whole)::value && i >= n) v = both(0.f);
           out.put(zs, buf, t0, i, v);
         }
@@ -391,7 +398,7 @@ scan_fwd_kernel(const Params p) {
       else put(std::false_type{});
       __syncwarp();
       out.write(zs, buf, t0, p.T - t0);
-      if (p.T - t0 <= kRun && w.live) store_state<V>(p.last + row, RESET ? apply(map, in) : fma_<V>(a, in, b));
+      if (p.T - t0 <= kRun && w.live) store_state<V>(p.last + row, apply<RESET>(map, in));
     }
     settle(buf ^ 1);
   }
@@ -436,7 +443,7 @@ scan_bwd_kernel(const Params p) {
   settle(0);
   float2 next = state_at(last + first), carry = load_state<V>(p.dlast + row, w.live && p.dlast != nullptr);
 #pragma unroll 4
-  for (int s = p.segments - 1; s > w.segment; --s) carry = apply(*w.map(p, s), carry);
+  for (int s = p.segments - 1; s > w.segment; --s) carry = apply<RESET>(*w.map(p, s), carry);
   int buf = 0;
   for (int from = last; from >= w.t0 && p.T > 0; from -= kStretch, buf ^= 1) {
     const int t0 = from + first, n = live - t0;
@@ -475,7 +482,7 @@ scan_bwd_kernel(const Params p) {
     };
     if (n >= kRun) walk(std::true_type{});
     else walk(std::false_type{});
-    float2 q = enter<WARPS>(maps, buf, WARPS - 1 - w.warp, make_float4(a.x, b.x, a.y, b.y), carry);
+    float2 q = enter<WARPS, RESET>(maps, buf, WARPS - 1 - w.warp, map_of<RESET>(a, b, resets != 0u), carry);
     if (t0 < p.T) {
       auto put = [&](auto whole) {
 #pragma unroll
@@ -541,9 +548,11 @@ scan_maps_kernel(const Params p) {
   if (runs > 0) ask(0, at(0));
   settle(0);
   float2 a = both(1.f), b = both(0.f);
+  bool any = false;                                            // resets so far
   for (int r = 0, buf = 0; r < runs; ++r, buf ^= 1) {
     const int t0 = at(r), n = live - t0;
     const unsigned resets = RESET ? reset_bits(kRun, p, w.b, t0, n) : 0u;
+    any = any || resets != 0u;
     async_wait();
     __syncwarp();
     if (r + 1 < runs) ask(buf ^ 1, at(r + 1));
@@ -565,12 +574,12 @@ scan_maps_kernel(const Params p) {
     settle(buf ^ 1);
   }
   const int lane = threadIdx.x & 31;
-  maps[32 * w.warp + lane] = make_float4(a.x, b.x, a.y, b.y);
+  maps[32 * w.warp + lane] = map_of<RESET>(a, b, any);
   __syncthreads();
   if (w.warp != 0) return;
   float4 all = maps[32 * (BACKWARD ? kWarps - 1 : 0) + lane];
 #pragma unroll
-  for (int i = 1; i < kWarps; ++i) all = then(all, maps[32 * (BACKWARD ? kWarps - 1 - i : i) + lane]);
+  for (int i = 1; i < kWarps; ++i) all = then<RESET>(all, maps[32 * (BACKWARD ? kWarps - 1 - i : i) + lane]);
   *w.map(p, w.segment) = all;
 }
 
