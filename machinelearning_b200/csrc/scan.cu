@@ -13,8 +13,10 @@
 // each CTA of the second starts from the maps in front of its segment.  Nothing waits on another CTA; the order of all sums is fixed.
 //
 // Digits: the smaller of s and 1 - s, e / (1 + e) with e = exp(-|z|), is exact to a few units of 2^-24, the larger is not further than that from 1.  With
-// it the step is h + s (f - h) or f + (1 - s) (h - f), whichever it belongs to: where s is 1e-6 a state that is multiplied with a rounded 1 - s
-// would be off by 3% after the million steps that it lasts.
+// it the step is h + s (f - h) or f + (1 - s) (h - f), whichever it belongs to: 1 - s itself is rounded by up to 2^-25, always the same way, which
+// is 3% after the million steps that a state lasts where s is 1e-6.  A map's factor has the same two forms (Map below), or it would bring that rounding back with
+// every run (2.4% measured at z = -14.1 after 2^20 steps; so 1e-5 to 1e-4): what is left out of a state is summed beside the factor, one multiply-add a step, and
+// the states of a run are formed from the state in front of it, step by step (64 x 1,024 x 768 bf16: 65 us forward as before; 16 x 1,024 x 768: 23 -> 26).
 #include <type_traits>
 
 #include <cuda_bf16.h>
@@ -150,24 +152,43 @@ template <int V> __device__ __forceinline__ float2 step(float2 y, float2 f, floa
 // (1 - s) q
 template <int V> __device__ __forceinline__ float2 kept(float2 y, float2 q) { return fma_<V>(y, q, choose(y, q, both(0.f))); }
 
-// Two channels' maps h -> a h + b of some steps, (a, b, a, b).  Behind a reset nothing of h is left, whatever it holds: a is -0.  Factors are not
-// negative otherwise, and one that underflows is +0: what is not finite goes through it as NaN.
-constexpr float kNothing = -0.f;
-__device__ __forceinline__ bool is_nothing(float a) { return __float_as_int(a) == __float_as_int(kNothing); }
+// Two channels' maps h -> a h + b of some steps, (y, b, y, b).  Like a step's y: a where it is at most 1/2, else minus 1 - a, so that a state of which
+// little is left out keeps its digits; minus zero: all of it is left, whatever it holds.  Behind a reset nothing is, whatever it held: y is -1, which 1 - a
+// (at most 1/2) is not otherwise.  A factor that underflows is +0: what is not finite goes through it as NaN.
+constexpr float kNothing = -1.f;
+__device__ __forceinline__ bool is_identity(float y) { return __float_as_int(y) == static_cast<int>(0x80000000u); }
+template <bool RESET> __device__ __forceinline__ float apply_one(float y, float b, float h) {
+  const float r = (is_identity(y) ? b : fmaf(y, h, b)) + (is_minus(y) ? h : 0.f);
+  return RESET && y == kNothing ? b : r;
+}
 template <bool RESET> __device__ __forceinline__ float2 apply(const float4& m, float2 h) {
-  const float2 r = make_float2(fmaf(m.x, h.x, m.y), fmaf(m.z, h.y, m.w));
-  return RESET ? make_float2(is_nothing(m.x) ? m.y : r.x, is_nothing(m.z) ? m.w : r.y) : r;
+  return make_float2(apply_one<RESET>(m.x, m.y, h.x), apply_one<RESET>(m.z, m.w, h.y));
 }
 // m, then n
+template <bool RESET> __device__ __forceinline__ float both_left(float m, float n) {
+  const float a = is_minus(m) ? 1.f + m : m, c = a * (is_minus(n) ? 1.f + n : n), out = fmaf(n, a, m);
+  const float y = is_minus(m) && is_minus(n) && out >= -0.5f ? out : c;
+  return RESET && (m == kNothing || n == kNothing) ? kNothing : y;
+}
 template <bool RESET> __device__ __forceinline__ float4 then(const float4& m, const float4& n) {
   const float2 b = apply<RESET>(n, make_float2(m.y, m.w));
-  auto factor = [](float a, float c) { return RESET && (is_nothing(a) || is_nothing(c)) ? kNothing : a * c; };
-  return make_float4(factor(m.x, n.x), b.x, factor(m.z, n.z), b.y);
+  return make_float4(both_left<RESET>(m.x, n.x), b.x, both_left<RESET>(m.z, n.z), b.y);
 }
-// The map of some steps, of which `resets` begin anew (the same ones for all channels of a sequence).
-template <bool RESET> __device__ __forceinline__ float4 map_of(float2 a, float2 b, bool resets) {
-  return RESET && resets ? make_float4(kNothing, b.x, kNothing, b.y) : make_float4(a.x, b.x, a.y, b.y);
-}
+__device__ __forceinline__ float4 identity() { return make_float4(-0.f, 0.f, -0.f, 0.f); }
+// The map of a run's steps, formed one by one.  What is left out is only looked at where every step leaves more than half.
+template <int V> struct Map {
+  float2 a, out, b;                                            // what is left of the state, minus what is left out, what is added
+  __device__ __forceinline__ Map() : a(both(1.f)), out(both(-0.f)), b(both(0.f)) {}
+  __device__ __forceinline__ void leave(float2 y) {            // y of lesser()
+    out = fma_<V>(y, a, out);
+    a = kept<V>(y, a);
+  }
+  // (resets: the same ones for all channels of a sequence)
+  template <bool RESET> __device__ __forceinline__ float4 pack(bool resets) const {
+    if (RESET && resets) return make_float4(kNothing, b.x, kNothing, b.y);
+    return make_float4(a.x > 0.5f ? out.x : a.x, b.x, a.y > 0.5f ? out.y : a.y, b.y);
+  }
+};
 
 // The state in front of this thread's run, given its run's map, and the state behind the CTA's runs in `carry`.  `maps`: in shared memory, [2][WARPS][lane];
 // `order`: this warp's place in its CTA, in the order in which the runs are walked.
@@ -362,43 +383,43 @@ scan_fwd_kernel(const Params p) {
     async_wait();
     __syncwarp();
     if (from + kStretch < w.t1) ask(buf ^ 1, t0 + kStretch);
-    // h from nothing, and what is left of the state in front of the run, behind every step
-    float2 h[kRun], left[kRun];
-    float2 a = both(1.f), b = both(0.f);
+    // the run's map: h from nothing, and what is left of the state in front
+    float2 y[kRun], f[kRun];
+    Map<V> m;
     auto walk = [&](auto whole) {
 #pragma unroll
       for (int i = 0; i < kRun; ++i) {
         if (decltype(whole)::value || i < n) {                 // (a step that does not count leaves h as it is)
-          if (RESET && (resets >> i & 1u)) a = b = both(0.f);
-          const float2 y = lesser<T, V>(zs.get(buf, i));
-          a = kept<V>(y, a);
-          b = step<V>(y, mapped<T, POSITIVE>(vs.get(buf, i)), b);
+          if (RESET && (resets >> i & 1u)) m.b = both(0.f);
+          y[i] = lesser<T, V>(zs.get(buf, i));
+          f[i] = mapped<T, POSITIVE>(vs.get(buf, i));
+          m.leave(y[i]);
+          m.b = step<V>(y[i], f[i], m.b);
         }
-        h[i] = b;
-        left[i] = a;
       }
     };
     if (n >= kRun) walk(std::true_type{});
     else walk(std::false_type{});
-    const float4 map = map_of<RESET>(a, b, resets != 0u);
-    const float2 in = enter<WARPS, RESET>(maps, buf, w.warp, map, carry);
+    float2 h = enter<WARPS, RESET>(maps, buf, w.warp, m.template pack<RESET>(resets != 0u), carry);
     if (t0 < p.T) {
-      if (p.tape != nullptr && w.live) store_state<V>(p.tape + (static_cast<long long>(w.b) * runs + t0 / kRun) * p.D + w.c, in);
+      if (p.tape != nullptr && w.live) store_state<V>(p.tape + (static_cast<long long>(w.b) * runs + t0 / kRun) * p.D + w.c, h);
       auto put = [&](auto whole) {
 #pragma unroll
         for (int i = 0; i < kRun; ++i) {
           if (!decltype(whole)::value && t0 + i >= p.T) break;
-          float2 v = h[i];
-          if (!RESET || !(resets & ((2u << i) - 1u))) v = fma_<V>(left[i], in, h[i]);
-          if (!decltype(whole)::value && i >= n) v = both(0.f);
-          out.put(zs, buf, t0, i, v);
+          const bool counts = decltype(whole)::value || i < n;
+          if (counts) {
+            if (RESET && (resets >> i & 1u)) h = both(0.f);
+            h = step<V>(y[i], f[i], h);
+          }
+          out.put(zs, buf, t0, i, counts ? h : both(0.f));
         }
       };
       if (n >= kRun) put(std::true_type{});
       else put(std::false_type{});
       __syncwarp();
       out.write(zs, buf, t0, p.T - t0);
-      if (p.T - t0 <= kRun && w.live) store_state<V>(p.last + row, apply<RESET>(map, in));
+      if (p.T - t0 <= kRun && w.live) store_state<V>(p.last + row, h);
     }
     settle(buf ^ 1);
   }
@@ -457,7 +478,7 @@ scan_bwd_kernel(const Params p) {
     }
     // forward through the run: y of lesser(), and h of the step before less f; and back: the map of what comes from behind the run
     float2 y[kRun], rest[kRun];
-    float2 a = both(1.f), b = both(0.f);
+    Map<V> m;
     auto grad = [&](int i) { return gs.get(buf, i); };         // (without dh: zeros)
     auto walk = [&](auto whole) {
 #pragma unroll
@@ -474,15 +495,15 @@ scan_bwd_kernel(const Params p) {
 #pragma unroll
       for (int i = kRun - 1; i >= 0; --i) {
         if (decltype(whole)::value || i < n) {
-          a = kept<V>(y[i], a);
-          b = kept<V>(y[i], add_<V>(b, grad(i)));
-          if (RESET && (resets >> i & 1u)) a = b = both(0.f);
+          m.leave(y[i]);
+          m.b = kept<V>(y[i], add_<V>(m.b, grad(i)));
+          if (RESET && (resets >> i & 1u)) m.b = both(0.f);
         }
       }
     };
     if (n >= kRun) walk(std::true_type{});
     else walk(std::false_type{});
-    float2 q = enter<WARPS, RESET>(maps, buf, WARPS - 1 - w.warp, map_of<RESET>(a, b, resets != 0u), carry);
+    float2 q = enter<WARPS, RESET>(maps, buf, WARPS - 1 - w.warp, m.template pack<RESET>(resets != 0u), carry);
     if (t0 < p.T) {
       auto put = [&](auto whole) {
 #pragma unroll
@@ -547,37 +568,37 @@ scan_maps_kernel(const Params p) {
   };
   if (runs > 0) ask(0, at(0));
   settle(0);
-  float2 a = both(1.f), b = both(0.f);
-  bool any = false;                                            // resets so far
+  float4 all = identity();
   for (int r = 0, buf = 0; r < runs; ++r, buf ^= 1) {
     const int t0 = at(r), n = live - t0;
     const unsigned resets = RESET ? reset_bits(kRun, p, w.b, t0, n) : 0u;
-    any = any || resets != 0u;
     async_wait();
     __syncwarp();
     if (r + 1 < runs) ask(buf ^ 1, at(r + 1));
+    Map<V> m;
     auto walk = [&](auto whole) {
 #pragma unroll
       for (int j = 0; j < kRun; ++j) {
         const int i = BACKWARD ? kRun - 1 - j : j;
         if (decltype(whole)::value || i < n) {
-          if (!BACKWARD && RESET && (resets >> i & 1u)) a = b = both(0.f);
+          if (!BACKWARD && RESET && (resets >> i & 1u)) m.b = both(0.f);
           const float2 y = lesser<T, V>(zs.get(buf, i)), v = with ? vs.get(buf, i) : both(0.f);
-          a = kept<V>(y, a);
-          b = BACKWARD ? kept<V>(y, add_<V>(b, v)) : step<V>(y, mapped<T, POSITIVE>(v), b);
-          if (BACKWARD && RESET && (resets >> i & 1u)) a = b = both(0.f);
+          m.leave(y);
+          m.b = BACKWARD ? kept<V>(y, add_<V>(m.b, v)) : step<V>(y, mapped<T, POSITIVE>(v), m.b);
+          if (BACKWARD && RESET && (resets >> i & 1u)) m.b = both(0.f);
         }
       }
     };
     if (n >= kRun) walk(std::true_type{});
     else walk(std::false_type{});
+    all = then<RESET>(all, m.template pack<RESET>(resets != 0u));
     settle(buf ^ 1);
   }
   const int lane = threadIdx.x & 31;
-  maps[32 * w.warp + lane] = map_of<RESET>(a, b, any);
+  maps[32 * w.warp + lane] = all;
   __syncthreads();
   if (w.warp != 0) return;
-  float4 all = maps[32 * (BACKWARD ? kWarps - 1 : 0) + lane];
+  all = maps[32 * (BACKWARD ? kWarps - 1 : 0) + lane];
 #pragma unroll
   for (int i = 1; i < kWarps; ++i) all = then<RESET>(all, maps[32 * (BACKWARD ? kWarps - 1 - i : i) + lane]);
   *w.map(p, w.segment) = all;
