@@ -406,7 +406,8 @@ int nlfa_gated_scan_bwd(const void* dh, const float* dlast, const void* gate, lo
  * Every extent may be of any size; tensors are contiguous.  x is of x_dtype, the weights of w_dtype, y and its gradient of `dtype`, which is
  * what the products run in (the autocast type, say): 16-bit types on the tensor cores, NLFA_DTYPE_F32 on the tensor cores as sums of three bf16
  * parts (finite values below 3.39e38; an infinity makes what it enters NaN).  Sums are float32.  Between the products the hidden values are rounded once to `dtype`'s
- * precision; in float16 they carry a power of two, so that they neither overflow nor lose digits below the type's normal range.
+ * precision; in float16 those of a token carry a power of two, from the lengths of its x and dy and of the weights' rows, so that a token's y and dx neither overflow nor lose digits
+ * between them, whatever the other tokens are; to the weights' gradients a token's share is exact to 2^-11 of itself or 2^-30 of the largest token's.
  *
  * `copies` (nlfa_gated_ffn_copies): which of x, w_gate, w_up, w_down (bits 0 to 3) the forward copies into the tape, because the products cannot read
  * them as they lie: of another type, float32, rows not a multiple of 64 long, not 16-byte aligned (without `train` up to 64 tokens take most as they lie).  The backward takes the same value; operands that

@@ -9,8 +9,9 @@
 // backward.  Between the products h, dg and du are operands: 16 bits (float32: three bf16 parts), one rounding each beside that of the results.
 //
 // This file has what goes around the products: 16-bit copies of operands that TMA cannot read as they are, the list of tiles and
-// parts, and the powers of two that hold float16's h, dg and du inside their type's range.
+// parts, and the powers of two that hold float16's h, dg and du inside their type's range, token by token.
 #include <cmath>
+#include <type_traits>
 
 #include "ffn.cuh"
 #include "rowwise.cuh"
@@ -56,6 +57,8 @@ bool is_few(const void* x, const void* gate, const void* up, const void* down, i
          aligned16(down);
 }
 
+constexpr size_t kHeaderBytes = 256;          // Limits, BwdLimits
+
 // What the forward leaves for the backward, and (inference) the forward's own workspace.
 struct Layout {
   int planes, n_rows, d_pad, f_pad, o_pad;
@@ -77,7 +80,7 @@ Layout layout(const Call& c) {
   l.o_pad = up64(c.o);
   const size_t two = 2 * static_cast<size_t>(l.planes), hidden = static_cast<size_t>(l.n_rows) * l.f_pad;
   size_t at = 0;
-  l.limits = at; at += 256;
+  l.limits = at; at = up(at + kHeaderBytes + (c.dtype == NLFA_DTYPE_F16 ? 2 * sizeof(float) * c.n : 0));
   l.x = at; if (c.copies & kCopyX) at = up(at + two * c.n * l.d_pad);
   l.gate = at; if (c.copies & kCopyGate) at = up(at + two * c.F * l.d_pad);
   l.up = at; if (c.copies & kCopyUp) at = up(at + two * c.F * l.d_pad);
@@ -151,14 +154,15 @@ size_t share_room(int tiles, int k) {
   return static_cast<size_t>(odd < most ? odd : most) * kRowTile * kColTile * sizeof(float);
 }
 // A product of one sum; add() gives it more.
-Segment segment(int a_map, int a_mn, int a_plane, int b_map, int b_mn, int b_plane, int k, int m, int n, void* to, int dtype, const float* inverse) {
+Segment segment(int a_map, int a_mn, int a_plane, int b_map, int b_mn, int b_plane, int k, int m, int n, void* to, int dtype, const float* scale,
+                int by_row) {
   Segment s{};
   s.a_map = a_map; s.a_mn = a_mn; s.b_mn = b_mn;
   s.subs = 1; s.k_sub = k;
   s.a_plane[0] = a_plane; s.b_map[0] = b_map; s.b_plane[0] = b_plane;
   s.tiles_n = ceil_div(n, kColTile);
   s.tiles = ceil_div(m, kRowTile) * s.tiles_n;
-  s.m_end = m; s.n_end = n; s.to = to; s.dtype = dtype; s.inverse = inverse;
+  s.m_end = m; s.n_end = n; s.to = to; s.dtype = dtype; s.scale = scale; s.by_row = by_row;
   return s;
 }
 void add(Segment& s, int a_plane, int b_map, int b_plane) {
@@ -183,15 +187,15 @@ bool apart_dh(const Call& c, const Layout& l) { return apart(l, c.F, c.o, l.plan
 void plan_up(Params& p, const Call& c, const Layout& l, float* g, float* u) {
   const int k = ceil_div(c.d, summands(l.planes));
   p.groups = p.units = 0;
-  p.seg[0] = segment(0, 0, 0, 1, 0, 0, k, c.n, c.F, g, NLFA_DTYPE_F32, nullptr);
-  p.seg[1] = segment(0, 0, 0, 2, 0, 0, k, c.n, c.F, u, NLFA_DTYPE_F32, nullptr);
+  p.seg[0] = segment(0, 0, 0, 1, 0, 0, k, c.n, c.F, g, NLFA_DTYPE_F32, nullptr, 0);
+  p.seg[1] = segment(0, 0, 0, 2, 0, 0, k, c.n, c.F, u, NLFA_DTYPE_F32, nullptr, 0);
   add_group(p, 0, 2, k, l.planes);
 }
 // y: maps h, Wd.
-void plan_fwd(Params& p, const Call& c, const Layout& l, void* y, const float* inverse) {
+void plan_fwd(Params& p, const Call& c, const Layout& l, void* y, const float* scale) {
   const int k = ceil_div(c.F, summands(l.planes));
   p.groups = p.units = 0;
-  p.seg[0] = segment(0, 0, 0, 1, 0, 0, k, c.n, c.o, y, c.dtype, inverse);
+  p.seg[0] = segment(0, 0, 0, 1, 0, 0, k, c.n, c.o, y, c.dtype, scale, 1);
   if (l.parts == 2) add(p.seg[0], 1, 1, 0);
   add_group(p, 0, 1, p.seg[0].subs * k, l.planes);
 }
@@ -199,18 +203,19 @@ void plan_fwd(Params& p, const Call& c, const Layout& l, void* y, const float* i
 void plan_dh(Params& p, const Call& c, const Layout& l, float* dh) {
   const int k = ceil_div(c.o, summands(l.planes));
   p.groups = p.units = 0;
-  p.seg[0] = segment(0, 0, 0, 1, 1, 0, k, c.n, c.F, dh, NLFA_DTYPE_F32, nullptr);
+  p.seg[0] = segment(0, 0, 0, 1, 1, 0, k, c.n, c.F, dh, NLFA_DTYPE_F32, nullptr, 0);
   add_group(p, 0, 1, k, l.planes);
 }
 // The gradients; du's planes are behind dg's.
 enum { kHiddenRows = 0, kHiddenColumns, kX, kDy, kH, kGateRows, kUpRows };
-void plan_bwd(Params& p, const Call& c, const Layout& l, void* dx, void* dwg, void* dwu, void* dwd, const float* inv_h, const float* inv_d) {
+// `scale`: of dx's rows; of_x, of_dy: of the weights' gradients.
+void plan_bwd(Params& p, const Call& c, const Layout& l, void* dx, void* dwg, void* dwu, void* dwd, const float* scale, const float* of_x, const float* of_dy) {
   const int s = summands(l.planes), kw = ceil_div(c.n, s), kf = ceil_div(c.F, s);
   int n = 0;
   p.groups = p.units = 0;
-  if (dwg) p.seg[n++] = segment(kHiddenRows, 1, 0, kX, 1, 0, kw, c.F, c.d, dwg, c.w_dtype, inv_d);
-  if (dwu) p.seg[n++] = segment(kHiddenRows, 1, l.parts, kX, 1, 0, kw, c.F, c.d, dwu, c.w_dtype, inv_d);
-  if (dwd) p.seg[n++] = segment(kDy, 1, 0, kH, 1, 0, kw, c.o, c.F, dwd, c.w_dtype, inv_h);
+  if (dwg) p.seg[n++] = segment(kHiddenRows, 1, 0, kX, 1, 0, kw, c.F, c.d, dwg, c.w_dtype, of_x, 0);
+  if (dwu) p.seg[n++] = segment(kHiddenRows, 1, l.parts, kX, 1, 0, kw, c.F, c.d, dwu, c.w_dtype, of_x, 0);
+  if (dwd) p.seg[n++] = segment(kDy, 1, 0, kH, 1, 0, kw, c.o, c.F, dwd, c.w_dtype, of_dy, 0);
   if (l.parts == 2)
     for (int i = 0; i < n; ++i) {
       if (p.seg[i].a_map == kDy) add(p.seg[i], 0, kH, 1);
@@ -218,7 +223,7 @@ void plan_bwd(Params& p, const Call& c, const Layout& l, void* dx, void* dwg, vo
     }
   if (n > 0) add_group(p, 0, n, p.seg[0].subs * kw, l.planes);
   if (dx) {
-    Segment& g = p.seg[n] = segment(kHiddenColumns, 0, 0, kGateRows, 1, 0, kf, c.n, c.d, dx, c.x_dtype, inv_d);
+    Segment& g = p.seg[n] = segment(kHiddenColumns, 0, 0, kGateRows, 1, 0, kf, c.n, c.d, dx, c.x_dtype, scale, 1);
     if (l.parts == 2) add(g, 1, kGateRows, 0);
     add(g, l.parts, kUpRows, 0);
     if (l.parts == 2) add(g, l.parts + 1, kUpRows, 0);
@@ -233,13 +238,17 @@ bool needs_chains(const Params& p, const Layout& l) {
 
 // The backward's workspace.
 struct BwdLayout {
-  size_t limits, dy, hidden, dh, shares, bytes;
+  size_t limits, dy, level_x, level_dy, hidden, dh, shares, bytes;
 };
 BwdLayout bwd_layout(const Call& c, const Layout& l, bool copy_dy) {
   BwdLayout b{};
   const size_t two = 2 * static_cast<size_t>(l.planes);
-  size_t at = 256;
+  const bool half = c.dtype == NLFA_DTYPE_F16;
+  size_t at = 0;
+  b.limits = at; at = up(at + kHeaderBytes + (half ? 2 * sizeof(float) * c.n : 0));
   b.dy = at; if (copy_dy) at = up(at + two * c.n * l.o_pad);
+  b.level_x = at; if (half) at = up(at + two * c.n * l.d_pad);
+  b.level_dy = at; if (half) at = up(at + two * c.n * l.o_pad);
   b.hidden = at; at = up(at + 4 * static_cast<size_t>(l.parts) * l.n_rows * l.f_pad);
   b.dh = at; if (apart_dh(c, l)) at = up(at + static_cast<size_t>(c.n) * c.F * 4);
   b.shares = at;
@@ -270,21 +279,33 @@ FwdLayout fwd_layout(const Call& c, const Layout& l) {
 
 // ------------------------------------------------------------------------------------------------ float16's range
 
-// h, dg and du of float16 are operands of float16: of a size that nobody has seen to.  They carry one power of two per call that puts what they can be
-// at most, by Cauchy and Schwarz from the lengths of the rows, just below 2^15.  Typical values lie some 2^10 below that, and 2^18 above
-// the smallest normal number.  |f(g)| <= |g|, |f'| < 1.13.
+// h, dg and du of float16 are operands of float16: of a size that nobody has seen to.  Those of a token carry a power of two that puts what they can be at
+// most, by Cauchy and Schwarz from the lengths of the token's x and dy and of the weights' rows, just below 2^15.  Typical values lie some 2^10 below that, and
+// 2^18 above the smallest normal number.  |f(g)| <= |g|, |f'| < 1.13.  y and dx are divided by it row by row.  (One power of two per call would take the digits
+// of all other tokens' h where one x is 1,000 times as long.)
+//
+// A weight's gradient is a sum over tokens, so there the other operand, x or dy, carries what makes the powers alike: 2^(level - e) beside 2^e, the level being
+// such that the longest row of that operand is just below 2^15 too.  What is lost is 2^-30 and less of the largest share of a token.
 constexpr int kLimitCtas = 592;
 struct Limits {                     // squares of the largest row lengths; of Wd the largest element
-  float x, gate, up, down;
-  float scale, inverse;             // of h
+  float gate, up, down;
 };
 struct BwdLimits {
-  float dy, unused;
-  float scale, inverse;             // of dg and du
+  int top_x, top_dy;                // the largest exponent of a row of x, of dy, less the row's own of dg and du, of h, and 1,024 (0: no row has one)
+  float of_x, of_dy;                // 2^level
 };
+// Behind either, a float per token: the square of its row's length (x; dy), its power of two (h; dg and du).
+struct Tokens {
+  float *square, *scale;
+};
+Tokens tokens_of(void* limits, int n) {
+  float* at = reinterpret_cast<float*>(static_cast<uint8_t*>(limits) + kHeaderBytes);
+  return {at, at + n};
+}
+enum { kLongestRow = 0, kLargestElement, kEveryRow };
 struct Rows {
   const void* src;
-  int dtype, rows, cols, element;   // element: the largest element instead of the largest row
+  int dtype, rows, cols, what;
   float* to;
   int vec;
 };
@@ -293,10 +314,10 @@ struct RowList {
   int n;
 };
 
-// A warp per row; rows that are not finite in float16 are left out (their results are not, whatever the factor).  Eight elements a load where rows lie on
-// 16 bytes (element by element 65,536 x 768 takes 42 us).
+// A warp per row, of values as float16 has them; what is not finite there is left out (its results are not finite, whatever the factor).  Eight elements a load where
+// rows lie on 16 bytes (element by element 65,536 x 768 takes 42 us).
 template <typename S>
-__device__ __forceinline__ void largest_row(const Rows& s) {
+__device__ __forceinline__ void row_lengths(const Rows& s) {
   const S* src = static_cast<const S*>(s.src);
   const int lane = threadIdx.x & 31;
   float most = 0.f;
@@ -304,8 +325,10 @@ __device__ __forceinline__ void largest_row(const Rows& s) {
     const S* row = src + static_cast<size_t>(r) * s.cols;
     float sum = 0.f, top = 0.f;
     auto add = [&](float v) {
+      if constexpr (!std::is_same_v<S, __half>) v = __half2float(__float2half_rn(v));
+      v = fabsf(v) < INFINITY ? v : 0.f;
       sum = fmaf(v, v, sum);
-      top = fabsf(v) < 65520.f ? fmaxf(top, fabsf(v)) : INFINITY;      // (what is below is rounded to at most 65,504)
+      top = fmaxf(top, fabsf(v));
     };
     if (s.vec) {
 #pragma unroll 4
@@ -324,41 +347,58 @@ __device__ __forceinline__ void largest_row(const Rows& s) {
       sum += __shfl_xor_sync(0xffffffffu, sum, off);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
     }
-    if (top < INFINITY) most = fmaxf(most, s.element ? top : sum);
+    if (s.what == kEveryRow && lane == 0) s.to[r] = sum;
+    most = fmaxf(most, s.what == kLargestElement ? top : sum);
   }
   // (of non-negative floats the order is that of their bits: no order of these matters)
-  if (lane == 0 && most > 0.f) atomicMax(reinterpret_cast<int*>(s.to), __float_as_int(most));
+  if (s.what != kEveryRow && lane == 0 && most > 0.f) atomicMax(reinterpret_cast<int*>(s.to), __float_as_int(most));
 }
 __global__ void __launch_bounds__(256)
 limits_kernel(const RowList list) {
   grid_dep_wait();
   grid_dep_release();
   const Rows s = list.r[blockIdx.y];
-  if (s.dtype == NLFA_DTYPE_F32) largest_row<float>(s);
-  else if (s.dtype == NLFA_DTYPE_F16) largest_row<__half>(s);
-  else largest_row<__nv_bfloat16>(s);
+  if (s.dtype == NLFA_DTYPE_F32) row_lengths<float>(s);
+  else if (s.dtype == NLFA_DTYPE_F16) row_lengths<__half>(s);
+  else row_lengths<__nv_bfloat16>(s);
 }
 
-__device__ __forceinline__ void set_scale(float bound, float* scale, float* inverse) {
-  int e = 0;
-  if (bound > 0.f && bound < INFINITY) {
-    int b;
-    frexpf(bound, &b);                                      // bound < 2^b
-    e = min(max(14 - b, -100), 100);
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }    // -127 < e < 128
+// v < 2^exponent(v)
+__device__ __forceinline__ int exponent(float v) {
+  int b;
+  frexpf(v, &b);
+  return b;
+}
+// The exponent that a token's values carry whose largest is `bound`.  (Bounds of float16 values: below 2^113.)
+__device__ __forceinline__ int carried(float bound) { return bound > 0.f && bound < INFINITY ? min(max(14 - exponent(bound), -100), 100) : 0; }
+
+__global__ void __launch_bounds__(256)
+fwd_scale_kernel(const Limits* l, Tokens x, int n) {
+  grid_dep_wait();
+  grid_dep_release();
+  const float weights = sqrtf(l->gate) * sqrtf(l->up);
+  for (int r = blockIdx.x * 256 + threadIdx.x; r < n; r += gridDim.x * 256) x.scale[r] = power_of_two(carried(x.square[r] * weights));
+}
+__global__ void __launch_bounds__(256)
+bwd_scale_kernel(const Limits* l, Tokens x, BwdLimits* b, Tokens dy, int n, float o) {
+  grid_dep_wait();
+  grid_dep_release();
+  const float weights = sqrtf(o) * l->down * fmaxf(sqrtf(l->gate), 1.13f * sqrtf(l->up));
+  int top_x = 0, top_dy = 0;
+  for (int r = blockIdx.x * 256 + threadIdx.x; r < n; r += gridDim.x * 256) {
+    const float xs = sqrtf(x.square[r]), ys = sqrtf(dy.square[r]), bound = ys * weights * xs;
+    const int e = carried(bound);
+    dy.scale[r] = power_of_two(e);
+    if (bound > 0.f) top_x = max(top_x, exponent(xs) - e + 1024);
+    if (xs > 0.f && ys > 0.f) top_dy = max(top_dy, exponent(ys) - (exponent(x.scale[r]) - 1) + 1024);
   }
-  *scale = ldexpf(1.f, e);
-  *inverse = ldexpf(1.f, -e);
-}
-__global__ void fwd_scale_kernel(Limits* l) {
-  grid_dep_wait();
-  grid_dep_release();
-  set_scale(l->x * sqrtf(l->gate) * sqrtf(l->up), &l->scale, &l->inverse);
-}
-__global__ void bwd_scale_kernel(const Limits* l, BwdLimits* b, float o) {
-  grid_dep_wait();
-  grid_dep_release();
-  const float dh = sqrtf(b->dy) * sqrtf(o) * l->down;
-  set_scale(dh * sqrtf(l->x) * fmaxf(sqrtf(l->gate), 1.13f * sqrtf(l->up)), &b->scale, &b->inverse);
+  top_x = __reduce_max_sync(0xffffffffu, top_x);
+  top_dy = __reduce_max_sync(0xffffffffu, top_dy);
+  if ((threadIdx.x & 31) == 0) {
+    if (top_x > 0) atomicMax(&b->top_x, top_x);
+    if (top_dy > 0) atomicMax(&b->top_dy, top_dy);
+  }
 }
 
 int checked(cudaError_t e) {
@@ -372,6 +412,7 @@ int find_limits(RowList list, void* to, size_t bytes, cudaStream_t st) {
   if (rc != NLFA_OK) return rc;
   return checked(launch_kernel(limits_kernel, dim3(kLimitCtas, static_cast<unsigned>(list.n)), dim3(256), 0, st, false, list));
 }
+unsigned token_ctas(int n) { return static_cast<unsigned>((n < 256 * kLimitCtas ? n + 255 : 256 * kLimitCtas) / 256); }
 
 // ------------------------------------------------------------------------------------------------ calls
 
@@ -434,6 +475,52 @@ int rows(CUtensorMap* m, const Operand& a, const Layout& l) {
   return operands::box_map(m, a.at, l.type, a.cols, a.rows, a.planes > 0 ? a.planes : l.planes, summands(l.planes), 2, l.planes, a.blocked);
 }
 
+// x beside dg and du, dy beside h, brought to one level (float16; above): a copy in blocks, a warp per row.  A token without a gradient, or with an x of zeros, gives zeros: its own
+// level would be any.
+struct Level {
+  const __half* src;
+  __half* dst;
+  int pad, blocked;                 // columns; whether src lies in blocks too
+  const float *other, *scale;       // squares of the other's row lengths; powers of two of what stands beside
+  const int* top;
+  float* of;
+};
+struct LevelList {
+  Level c[2];
+  int n;
+};
+__global__ void __launch_bounds__(operands::kBlock)
+level_kernel(const LevelList list, int rows) {
+  grid_dep_wait();
+  grid_dep_release();
+  const Level c = list.c[blockIdx.y];
+  const int top = *c.top, level = top > 0 ? min(max(14 - (top - 1024), -120), 120) : 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *c.of = power_of_two(level);
+  constexpr int kWarps = operands::kBlock / 32;
+  for (int r = blockIdx.x * kWarps + (threadIdx.x >> 5); r < rows; r += gridDim.x * kWarps) {
+    // (level - e may be outside float32's exponents: two factors)
+    const int k = level - (exponent(c.scale[r]) - 1), k0 = k / 2;
+    const float f0 = c.other[r] > 0.f ? power_of_two(k0) : 0.f, f1 = power_of_two(k - k0);
+#pragma unroll 4
+    for (int col = 8 * (threadIdx.x & 31); col < c.pad; col += 256) {
+      const size_t block = (static_cast<size_t>(col / 64) * rows + r) * 64 + col % 64;
+      float v[8];
+      rowwise::Elem<__half>::load(c.src + (c.blocked ? block : static_cast<size_t>(r) * c.pad + col), v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = v[j] * f0 * f1;
+      rowwise::Elem<__half>::store(c.dst + block, v);
+    }
+  }
+}
+Level level_of(const Operand& a, void* dst, const float* other, const float* scale, const int* top, float* of) {
+  return {static_cast<const __half*>(a.at), static_cast<__half*>(dst), static_cast<int>(a.cols), a.blocked, other, scale, top, of};
+}
+int make_levels(const LevelList& list, int rows, cudaStream_t st) {
+  const int need = ceil_div(rows, operands::kBlock / 32), most = 16 * sm_count();
+  return checked(launch_kernel(level_kernel, dim3(static_cast<unsigned>(need < most ? need : most), static_cast<unsigned>(list.n)), dim3(operands::kBlock), 0, st,
+                               overlap_launches(kOverlapRowwise), list, rows));
+}
+
 struct Operands {
   Operand x, gate, up, down, h;
 };
@@ -476,15 +563,17 @@ int run_fwd(const Call& c, const Weights& w, int activation, void* y, uint8_t* t
   copy(kCopyDown, w.down, c.w_dtype, l.down, c.o, c.F);
   int rc = make_copies(copies, l, st);
   Limits* limits = c.dtype == NLFA_DTYPE_F16 ? reinterpret_cast<Limits*>(tape + l.limits) : nullptr;
+  const Tokens tokens = tokens_of(tape + l.limits, c.n);
   if (rc == NLFA_OK && limits != nullptr) {
     RowList list{};
-    list.r[0] = {w.x, c.x_dtype, c.n, c.d, 0, &limits->x};
-    list.r[1] = {w.gate, c.w_dtype, c.F, c.d, 0, &limits->gate};
-    list.r[2] = {w.up, c.w_dtype, c.F, c.d, 0, &limits->up};
-    list.r[3] = {w.down, c.w_dtype, c.o, c.F, 1, &limits->down};
+    list.r[0] = {w.x, c.x_dtype, c.n, c.d, kEveryRow, tokens.square};
+    list.r[1] = {w.gate, c.w_dtype, c.F, c.d, kLongestRow, &limits->gate};
+    list.r[2] = {w.up, c.w_dtype, c.F, c.d, kLongestRow, &limits->up};
+    list.r[3] = {w.down, c.w_dtype, c.o, c.F, kLargestElement, &limits->down};
     list.n = c.train ? 4 : 3;
     rc = find_limits(list, limits, sizeof(Limits), st);
-    if (rc == NLFA_OK) rc = checked(launch_kernel(fwd_scale_kernel, dim3(1), dim3(1), 0, st, overlap_launches(kOverlapRowwise), limits));
+    if (rc == NLFA_OK)
+      rc = checked(launch_kernel(fwd_scale_kernel, dim3(token_ctas(c.n)), dim3(256), 0, st, overlap_launches(kOverlapRowwise), limits, tokens, c.n));
   }
   if (rc != NLFA_OK) return rc;
   const Operands a = operands_of(c, l, w, tape);
@@ -498,7 +587,7 @@ int run_fwd(const Call& c, const Weights& w, int activation, void* y, uint8_t* t
   fill(maps, 4);
   Params p = params(c, l, activation, tape, status);
   p.k = c.d;
-  p.scale = limits != nullptr ? &limits->scale : nullptr;
+  p.scale = limits != nullptr ? tokens.scale : nullptr;
   p.shares = reinterpret_cast<float*>(scratch + f.shares);
   if (apart_up(c, l)) {
     float *g = reinterpret_cast<float*>(scratch + f.g), *u = reinterpret_cast<float*>(scratch + f.u);
@@ -513,7 +602,7 @@ int run_fwd(const Call& c, const Weights& w, int activation, void* y, uint8_t* t
   if (rc == NLFA_OK) rc = columns(&maps.m[1], a.down, l);
   if (rc != NLFA_OK) return rc;
   fill(maps, 2);
-  plan_fwd(p, c, l, y, limits != nullptr ? &limits->inverse : nullptr);
+  plan_fwd(p, c, l, y, limits != nullptr ? tokens.scale : nullptr);
   return launch_product(kProducts, l.type, l.planes, needs_chains(p, l), p, maps, st);
 }
 
@@ -532,14 +621,16 @@ int run_bwd(const Call& c, const void* dy, const Weights& w, int activation, uin
   }
   const Limits* limits = c.dtype == NLFA_DTYPE_F16 ? reinterpret_cast<const Limits*>(tape + l.limits) : nullptr;
   BwdLimits* more = reinterpret_cast<BwdLimits*>(scratch + b.limits);
+  const Tokens x_tokens = tokens_of(tape + l.limits, c.n), dy_tokens = tokens_of(scratch + b.limits, c.n);
   const bool through = dx || dwg || dwu;                   // whether dg and du are needed
-  if (rc == NLFA_OK && limits != nullptr && through) {
+  if (rc == NLFA_OK && limits != nullptr) {
     RowList list{};
-    list.r[0] = {dy, c.dtype, c.n, c.o, 0, &more->dy};
+    list.r[0] = {dy, c.dtype, c.n, c.o, kEveryRow, dy_tokens.square};
     list.n = 1;
     rc = find_limits(list, more, sizeof(BwdLimits), st);
     if (rc == NLFA_OK)
-      rc = checked(launch_kernel(bwd_scale_kernel, dim3(1), dim3(1), 0, st, overlap_launches(kOverlapRowwise), limits, more, static_cast<float>(c.o)));
+      rc = checked(launch_kernel(bwd_scale_kernel, dim3(token_ctas(c.n)), dim3(256), 0, st, overlap_launches(kOverlapRowwise), limits, x_tokens, more,
+                                 dy_tokens, c.n, static_cast<float>(c.o)));
   }
   if (rc != NLFA_OK) return rc;
   const Operands a = operands_of(c, l, w, tape);
@@ -556,7 +647,7 @@ int run_bwd(const Call& c, const void* dy, const Weights& w, int activation, uin
     if (rc != NLFA_OK) return rc;
     fill(maps, 3);
     p.k = c.o;
-    p.scale = limits != nullptr ? &more->scale : nullptr;
+    p.scale = limits != nullptr ? dy_tokens.scale : nullptr;
     if (apart_dh(c, l)) {
       float* dh = reinterpret_cast<float*>(scratch + b.dh);
       plan_dh(p, c, l, dh);
@@ -567,16 +658,32 @@ int run_bwd(const Call& c, const void* dy, const Weights& w, int activation, uin
     }
     if (rc != NLFA_OK) return rc;
   }
+  // x and dy as the weights' gradients read them
+  Operand x_rows = a.x, dy_rows = up_grad;
+  if (limits != nullptr) {
+    LevelList list{};
+    if (dwg || dwu) {
+      list.c[list.n++] = level_of(a.x, scratch + b.level_x, dy_tokens.square, dy_tokens.scale, &more->top_x, &more->of_x);
+      x_rows = operand(nullptr, scratch + b.level_x, true, c.d, c.n);
+    }
+    if (dwd) {
+      list.c[list.n++] = level_of(up_grad, scratch + b.level_dy, x_tokens.square, x_tokens.scale, &more->top_dy, &more->of_dy);
+      dy_rows = operand(nullptr, scratch + b.level_dy, true, c.o, c.n);
+    }
+    if (list.n > 0) rc = make_levels(list, c.n, st);
+    if (rc != NLFA_OK) return rc;
+  }
   rc = rows(&maps.m[kHiddenRows], hidden, l);
   if (rc == NLFA_OK) rc = columns(&maps.m[kHiddenColumns], hidden, l);
-  if (rc == NLFA_OK) rc = rows(&maps.m[kX], a.x, l);
-  if (rc == NLFA_OK) rc = rows(&maps.m[kDy], up_grad, l);
+  if (rc == NLFA_OK) rc = rows(&maps.m[kX], x_rows, l);
+  if (rc == NLFA_OK) rc = rows(&maps.m[kDy], dy_rows, l);
   if (rc == NLFA_OK) rc = rows(&maps.m[kH], a.h, l);
   if (rc == NLFA_OK) rc = rows(&maps.m[kGateRows], a.gate, l);
   if (rc == NLFA_OK) rc = rows(&maps.m[kUpRows], a.up, l);
   if (rc != NLFA_OK) return rc;
   fill(maps, kUpRows + 1);
-  plan_bwd(p, c, l, dx, dwg, dwu, dwd, limits != nullptr ? &limits->inverse : nullptr, limits != nullptr ? &more->inverse : nullptr);
+  if (limits != nullptr) plan_bwd(p, c, l, dx, dwg, dwu, dwd, dy_tokens.scale, &more->of_x, &more->of_dy);
+  else plan_bwd(p, c, l, dx, dwg, dwu, dwd, nullptr, nullptr, nullptr);
   return launch_product(kProducts, l.type, l.planes, needs_chains(p, l), p, maps, st);
 }
 

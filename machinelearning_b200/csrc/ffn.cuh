@@ -14,7 +14,7 @@ constexpr int kPartsPerPair = 2;    // shares of odd tiles there is room for, pe
 
 enum { kUp = 0, kDh = 1, kProducts = 2 };
 
-// One product of kProducts: to [m_end, n_end] = scale^-1 (A_0 B_0 + A_1 B_1 + ...), `subs` sums of `k_sub` stages that differ in maps and planes (dx = dg Wg + du Wu;
+// One product of kProducts: to [m_end, n_end] = (A_0 B_0 + A_1 B_1 + ...) / scale, `subs` sums of `k_sub` stages that differ in maps and planes (dx = dg Wg + du Wu;
 // hidden values in two parts).
 constexpr int kMostSubs = 4;
 struct Segment {
@@ -24,7 +24,8 @@ struct Segment {
   int tiles, tiles_n, m_end, n_end;
   void* to;
   int dtype;
-  const float* inverse;             // NULL: 1
+  const float* scale;               // powers of two, one or (by_row) each row's; NULL: 1
+  int by_row;
 };
 // Segments whose sums have the same number of stages.  Units: whole tiles, as many as all pairs of CTAs get, then the rest, whose sums are cut
 // into parts so that every pair is busy; parts of one index stand together (they read the same summands).
@@ -49,7 +50,7 @@ struct Params {
   uint8_t *kept;
   int8_t* exponents;
   void *h, *dg, *du;                // (written without TMA in float32 and by launch_hidden, launch_grads)
-  const float* scale;               // of h (kUp) or dg and du (kDh); NULL: 1
+  const float* scale;               // powers of two of h's rows (kUp) or dg's and du's (kDh), float16 only; NULL: 1
   Segment seg[kMostSegments];
   Group group[kMostGroups];
   int groups, units;

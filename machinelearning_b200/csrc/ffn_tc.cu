@@ -126,14 +126,17 @@ struct Walk {
   }
 };
 
+// What row m of a segment's sums is multiplied with: 1 / f of a power of two.
+__device__ __forceinline__ float factor_of(const Segment& s, int m) {
+  return s.scale != nullptr && m < s.m_end ? __int_as_float(0x7f000000 - __float_as_int(s.scale[s.by_row ? m : 0])) : 1.f;
+}
+
 // Four values of row m, columns n .. of a segment's result
-__device__ __forceinline__ void put(const Segment& s, float alpha, int m, int n, float (&v)[4]) {
+__device__ __forceinline__ void put(const Segment& s, int m, int n, float (&v)[4]) {
   if (m >= s.m_end || n >= s.n_end) return;
   const bool vec = s.n_end % 4 == 0;
   const int count = s.n_end - n < 4 ? s.n_end - n : 4;
   const size_t at = static_cast<size_t>(m) * s.n_end + n;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] *= alpha;
   if (s.dtype == NLFA_DTYPE_F32) {
     float* o = static_cast<float*>(s.to) + at;
     if (vec) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
@@ -171,7 +174,10 @@ fold_kernel(const __grid_constant__ Params p) {
     const float4 x = *reinterpret_cast<const float4*>(shares + (static_cast<size_t>(part) * g.rest * kRowTile + r) * kColTile);
     v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
   }
-  put(s, s.inverse != nullptr ? *s.inverse : 1.f, t.m0 + r, t.n0 + c, v);
+  const float factor = factor_of(s, t.m0 + r);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] *= factor;
+  put(s, t.m0 + r, t.n0 + c, v);
 }
 
 // ---- the activation: f(g), and f'(g).  EXACT (float32): no approximate exponential or quotient
@@ -432,7 +438,6 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
     Tile t;
     int sums = 0;
     bool ok = true;
-    const float scale = p.scale != nullptr ? *p.scale : 1.f;
     const size_t plane = static_cast<size_t>(p.n_rows) * p.f_pad;
     Sums<MODE, LONG> l;
     auto release = [&](int buf) {                              // this warp has read its part of the buffer
@@ -463,6 +468,7 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
     auto kept_at = [&](int row, int col) -> size_t { return (static_cast<size_t>(row / 32) * (p.f_pad / 32) + col / 32) * 2; };
     while (walk.next(t)) {
       const int row0 = t.m0 + 128 * rank + 32 * q, row = row0 + lane;
+      const float scale = !kBf16 && MODE != kProducts && row < p.rows ? p.scale[row] : 1.f;
       int buf = 0;
       if constexpr (LONG) {
 #pragma unroll
@@ -596,8 +602,8 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
       } else {
         // 32 x 32 values through shared memory, so that a row's columns leave side by side
         const Segment& seg = p.seg[t.seg];
-        const float alpha = seg.inverse != nullptr ? *seg.inverse : 1.f;
         const int local = 128 * rank + 32 * q;
+        const float factor = kBf16 || t.slot >= 0 ? 1.f : factor_of(seg, row);
         float* share = t.slot < 0 ? nullptr : p.shares + (static_cast<size_t>(t.slot) * kRowTile + local) * kColTile;
 #pragma unroll (LONG ? 4 : 1)
         for (int c = 0; c < 4; ++c) {
@@ -605,6 +611,10 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
           if (col >= seg.n_end) break;
           float r[32];
           l.get(c, r);
+          if (!kBf16) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] *= factor;
+          }
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
@@ -619,7 +629,7 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
             ld_shared_v4(staging + lr * 128 + (((lane & 7) ^ (lr & 7)) * 16), w0, w1, w2, w3);
             float v[4] = {__uint_as_float(w0), __uint_as_float(w1), __uint_as_float(w2), __uint_as_float(w3)};
             if (share != nullptr) *reinterpret_cast<float4*>(share + static_cast<size_t>(lr) * kColTile + (cc - t.n0)) = make_float4(v[0], v[1], v[2], v[3]);
-            else put(seg, alpha, t.m0 + local + lr, cc, v);
+            else put(seg, t.m0 + local + lr, cc, v);
           }
           __syncwarp();
         }
@@ -651,6 +661,7 @@ struct Block {
     i += gridDim.x * (kApartThreads / 32);
     return true;
   }
+  __device__ float scale(const Params& p) const { return p.scale != nullptr && row < p.rows ? p.scale[row] : 1.f; }
   __device__ void load(const Params& p, const float* from, float (&v)[32]) const {
     const float* s = from + static_cast<size_t>(row) * p.cols + col;
     if (row < p.rows && p.cols % 4 == 0 && col + 32 <= p.cols) {
@@ -673,7 +684,6 @@ hidden_kernel(const __grid_constant__ Params p, int parts, const float* __restri
   constexpr int kKeptBytes = kWide ? 4096 : 2048;
   grid_dep_wait();
   grid_dep_release();
-  const float scale = p.scale != nullptr ? *p.scale : 1.f;
   const int lane = threadIdx.x & 31;
   int i = blockIdx.x * (kApartThreads / 32) + (threadIdx.x >> 5);
   Block b;
@@ -681,6 +691,7 @@ hidden_kernel(const __grid_constant__ Params p, int parts, const float* __restri
     float g[32], u[32], f[32];
     b.load(p, gs, g);
     b.load(p, us, u);
+    const float scale = b.scale(p);
     auto walk = [&](auto act) {
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
@@ -710,13 +721,13 @@ grads_kernel(const __grid_constant__ Params p, int parts, const float* __restric
   constexpr int kKeptBytes = kWide ? 4096 : 2048;
   grid_dep_wait();
   grid_dep_release();
-  const float scale = p.scale != nullptr ? *p.scale : 1.f;
   const int lane = threadIdx.x & 31;
   int i = blockIdx.x * (kApartThreads / 32) + (threadIdx.x >> 5);
   Block b;
   while (b.next(p, i)) {
     float d[32], e[32];
     b.load(p, dh, d);
+    const float scale = b.scale(p);
     const uint8_t* as = p.kept + b.kept * kKeptBytes + 16 * lane;
     float fa = 1.f, fb = 1.f;
     if (!kWide) {
