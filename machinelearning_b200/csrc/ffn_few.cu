@@ -7,8 +7,8 @@
 // All loads of a run are in flight at once; the second launch has its weights on the way before the first one's h is there.
 //
 // Types: every operand is a sum of bf16 parts, split in registers: bf16 one, float16 two (exact), float32 three (to 2^-24), h two (2^-17), beside float32 three; the products
-// of parts down to the type's own rounding.  The leading parts' product has a chain of its own: the tensor core truncates, and
-// a chain of one run is short.  So h is not rounded to 16 bits, nor kept to float16's range.
+// of parts down to the type's own rounding, the leading parts' last.  The tensor core truncates what it adds to, so a long chain of one sign comes out low: chains end
+// after 32 summands in float32, 128 in 16 bits, and their sums are added in registers.  So h is not rounded to 16 bits, nor kept to float16's range.
 #include <type_traits>
 
 #include <cuda_bf16.h>
@@ -72,9 +72,9 @@ template <typename S, typename C, int PARTS> __device__ __forceinline__ void spl
   }
 }
 
-// acc[0] += the leading parts' product, acc[1] += the others that count
+// acc += the parts' products that count, smallest first
 template <int WP, int XP>
-__device__ __forceinline__ void product(float (&acc)[2][4], const uint32_t (&lo)[WP][4], const uint32_t (&hi)[WP][4], const uint32_t (&x)[XP][4]) {
+__device__ __forceinline__ void product(float (&acc)[4], const uint32_t (&lo)[WP][4], const uint32_t (&hi)[WP][4], const uint32_t (&x)[XP][4]) {
 #pragma unroll
   for (int i = WP - 1; i >= 0; --i)
 #pragma unroll
@@ -83,12 +83,12 @@ __device__ __forceinline__ void product(float (&acc)[2][4], const uint32_t (&lo)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint32_t a[4] = {lo[i][2 * h], hi[i][2 * h], lo[i][2 * h + 1], hi[i][2 * h + 1]};
-        mma(acc[i + j > 0 ? 1 : 0], a, x[j][2 * h], x[j][2 * h + 1]);
+        mma(acc, a, x[j][2 * h], x[j][2 * h + 1]);
       }
     }
 }
 
-// Rows [row, row + 16) of w [rows, k] times the tokens, steps [s0, s1) of 32 summands: each lane's acc.  X: as the tokens lie.
+// Rows [row, row + 16) of w [rows, k] times the tokens, steps [s0, s1) of 32 summands: each lane's sums.  X: as the tokens lie.
 template <typename S> struct Ahead {
   Eight<S> lo[kDeep], hi[kDeep];
 };
@@ -101,7 +101,7 @@ __device__ __forceinline__ void ask(Ahead<S>& a, int i, const S* lo, const S* hi
 }
 // CW, CX: the types that weights and tokens are rounded to.
 template <typename S, typename X, typename CW, typename CX, int WP, int XP, int NT>
-__device__ __forceinline__ void run(float (&acc)[NT][2][4], Ahead<S>& ahead, const S* lo, const S* hi, const X* x, int n, int s0, int s1, int k) {
+__device__ __forceinline__ void run(float (&sum)[NT][4], Ahead<S>& ahead, const S* lo, const S* hi, const X* x, int n, int s0, int s1, int k) {
   const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
   // the tokens of a step, one step ahead (of 32 tokens there are no registers for that: 64 of them 13.7 us so, 11.8 without)
   constexpr bool kAhead = NT < 4;
@@ -110,6 +110,16 @@ __device__ __forceinline__ void run(float (&acc)[NT][2][4], Ahead<S>& ahead, con
     const int at = 32 * step + 8 * t;
 #pragma unroll
     for (int j = 0; j < NT; ++j) load(xs[j], x + static_cast<size_t>(8 * j + g) * k + at, step < s1 && 8 * j + g < n && at < k);
+  };
+  float acc[NT][4] = {};
+  auto cut = [&]() {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sum[j][i] += acc[j][i];
+        acc[j][i] = 0.f;
+      }
   };
   if (kAhead) tokens(s0);
   for (int s = s0; s < s1; s += kDeep) {
@@ -136,19 +146,21 @@ __device__ __forceinline__ void run(float (&acc)[NT][2][4], Ahead<S>& ahead, con
           product<WP, XP>(acc[j], wl, wh, xp);
         }
       }
+      if (WP == 3) cut();
     }
+    if (WP != 3) cut();
   }
 }
 
 // The sums of a tile's runs, [warp][token][16 rows], with a row's padding against bank conflicts
 constexpr int kPitch = kRows + 1;
-template <int NT> __device__ __forceinline__ void leave(float* sums, const float (&acc)[NT][2][4]) {
+template <int NT> __device__ __forceinline__ void leave(float* sums, const float (&sum)[NT][4]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      sums[(warp * 8 * NT + 8 * j + 2 * (lane & 3) + (i & 1)) * kPitch + (lane >> 2) + 8 * (i >> 1)] = acc[j][0][i] + acc[j][1][i];
+      sums[(warp * 8 * NT + 8 * j + 2 * (lane & 3) + (i & 1)) * kPitch + (lane >> 2) + 8 * (i >> 1)] = sum[j][i];
 }
 
 struct FewParams {
@@ -191,11 +203,11 @@ few_up_kernel(FewParams p) {
   Ahead<S> ahead;
 #pragma unroll
   for (int i = 0; i < kDeep; ++i) ask(ahead, i, lo, hi, s0 + i, s1, p.d);
-  float acc[NT][2][4] = {};
-  if (p.x_dtype == NLFA_DTYPE_F32) run<S, float, C, C, WP, WP, NT>(acc, ahead, lo, hi, static_cast<const float*>(p.x), p.n, s0, s1, p.d);
-  else if (p.x_dtype == NLFA_DTYPE_F16) run<S, __half, C, C, WP, WP, NT>(acc, ahead, lo, hi, static_cast<const __half*>(p.x), p.n, s0, s1, p.d);
-  else run<S, __nv_bfloat16, C, C, WP, WP, NT>(acc, ahead, lo, hi, static_cast<const __nv_bfloat16*>(p.x), p.n, s0, s1, p.d);
-  leave<NT>(sums, acc);
+  float sum[NT][4] = {};
+  if (p.x_dtype == NLFA_DTYPE_F32) run<S, float, C, C, WP, WP, NT>(sum, ahead, lo, hi, static_cast<const float*>(p.x), p.n, s0, s1, p.d);
+  else if (p.x_dtype == NLFA_DTYPE_F16) run<S, __half, C, C, WP, WP, NT>(sum, ahead, lo, hi, static_cast<const __half*>(p.x), p.n, s0, s1, p.d);
+  else run<S, __nv_bfloat16, C, C, WP, WP, NT>(sum, ahead, lo, hi, static_cast<const __nv_bfloat16*>(p.x), p.n, s0, s1, p.d);
+  leave<NT>(sums, sum);
   __syncthreads();
   for (int i = threadIdx.x; i < kRows * p.n; i += 32 * kUpWarps) {
     const int token = i / kRows, r = i % kRows;
@@ -225,9 +237,9 @@ few_down_kernel(FewParams p) {
   for (int i = 0; i < kDeep; ++i) ask(ahead, i, lo, hi, s0 + i, s1, p.F);
   grid_dep_wait();
   grid_dep_release();
-  float acc[NT][2][4] = {};
-  run<S, float, C, float, Parts<C>::kCount, Parts<C>::kHidden, NT>(acc, ahead, lo, hi, p.h, p.n, s0, s1, p.F);
-  leave<NT>(sums, acc);
+  float sum[NT][4] = {};
+  run<S, float, C, float, Parts<C>::kCount, Parts<C>::kHidden, NT>(sum, ahead, lo, hi, p.h, p.n, s0, s1, p.F);
+  leave<NT>(sums, sum);
   __syncthreads();
   for (int i = threadIdx.x; i < kRows * p.n; i += 32 * kDownWarps) {
     const int token = i / kRows, r = i % kRows;
