@@ -351,6 +351,13 @@ def prepare(q, k, v, scale, use_mma, window, sinks, block=0):
     return q, k, v, scale, use_mma
 
 
+def refuse_tangents(name: str, *tensors) -> None:
+    """Raise ``ValueError`` where a tensor carries a forward-mode derivative: no operator here has a rule for one, and the result would come without."""
+    for t in tensors:
+        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name}: forward-mode derivatives are not supported")
+
+
 def flash_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                scale: float | None = None, use_mma: bool | None = None, *,
                window: int = 0, sinks: int = 0, block: int = 0) -> torch.Tensor:
@@ -368,6 +375,8 @@ def flash_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         y = _host.attn(q, k, v, scale, use_mma, window, sinks, block)
         if y is not None:
             return y
+    if not torch.compiler.is_compiling():
+        refuse_tangents("flash_attn", q, k, v)
     q, k, v, scale, use_mma = prepare(q, k, v, scale, use_mma, window, sinks, block)
     if torch.compiler.is_compiling():
         from . import compile_ops              # registered operators: one graph node instead of a graph break
@@ -400,6 +409,7 @@ def flash_attn_cached(q: torch.Tensor, k_full: torch.Tensor, v_full: torch.Tenso
         if out is not None:
             return out
     # what the call above declined: say why
+    refuse_tangents("flash_attn_cached", q, k_full, v_full)
     ok = (q.dim() == 4 and k_full.dim() == 4 and v_full.dim() == 4 and q.is_cuda and k_full.is_cuda and v_full.is_cuda
           and q.dtype == k_full.dtype == v_full.dtype and q.dtype in SUPPORTED_DTYPES
           and q.shape[-1] in SUPPORTED_HEAD_DIMS and k_full.shape == v_full.shape

@@ -115,6 +115,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         y = flash_cuda._host.gated_ffn(x, w_gate, w_up, w_down, code)
         if y is not None:
             return y
+        flash_cuda.refuse_tangents("gated_ffn", x, w_gate, w_up, w_down)
     if not supports(x, w_gate, w_up, w_down):
         said = ", ".join(f"{n}={tuple(t.shape)}/{t.dtype} on {t.device}"
                          for n, t in (("x", x), ("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)))

@@ -120,6 +120,7 @@ def gated_scan(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor | No
         out = flash_cuda._host.gated_scan(gate, value, state, reset, lengths, code)
         if out is not None:
             return out
+        flash_cuda.refuse_tangents("gated_scan", gate, value, state)
     if not supports(gate, value, state, reset, lengths):
         def said(t):
             return None if t is None else f"{tuple(t.shape)}/{t.dtype} on {t.device}"

@@ -108,6 +108,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
         loss = flash_cuda._host.linear_ce(x, weight, targets, ignore_index, REDUCTIONS[reduction])
         if loss is not None:
             return loss
+        flash_cuda.refuse_tangents("linear_cross_entropy", x, weight)
     if not supports(x, weight, targets):
         raise ValueError(f"linear_cross_entropy: unsupported inputs (x={tuple(x.shape)}/{x.dtype} on {x.device}, "
                          f"weight={tuple(weight.shape)}/{weight.dtype}, targets={tuple(targets.shape)}/{targets.dtype})")

@@ -121,6 +121,7 @@ def qk_prologue(x: torch.Tensor, weight=None, cos=None, sin=None, eps: float = E
         y = flash_cuda._host.qk_prologue(x, weight, cos, sin, eps, out_dtype)
         if y is not None:
             return y
+        flash_cuda.refuse_tangents("qk_prologue", x, weight, cos, sin)
     if not supports(x, weight, cos, sin):
         raise ValueError(f"qk_prologue: unsupported inputs {tuple(x.shape)} {x.dtype} on {x.device}")
     if out_dtype is None:

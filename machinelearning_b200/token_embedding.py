@@ -81,6 +81,7 @@ def embedding(idx: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, pa
         out = flash_cuda._host.embedding(idx, weight, scale, padding)
         if out is not None:
             return out
+        flash_cuda.refuse_tangents("embedding", weight)
     if not supports(idx, weight):
         raise ValueError(f"embedding: unsupported inputs (idx={tuple(idx.shape)}/{idx.dtype} on {idx.device}, "
                          f"weight={tuple(weight.shape)}/{weight.dtype} on {weight.device})")

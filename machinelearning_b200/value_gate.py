@@ -129,6 +129,7 @@ def value_blend(v: torch.Tensor, v0: torch.Tensor, lam: torch.Tensor, out_dtype=
         out = flash_cuda._host.value_blend(v, v0, lam, out_dtype)
         if out is not None:
             return out
+        flash_cuda.refuse_tangents("value_blend", v, v0, lam)
     if not supports_blend(v, v0, lam):
         raise ValueError(f"value_blend: unsupported inputs {tuple(v.shape)} {v.dtype} / {v0.dtype} on {v.device}")
     if out_dtype is None:
@@ -149,6 +150,7 @@ def head_gate(y: torch.Tensor, gate: torch.Tensor) -> torch.Tensor:
         out = flash_cuda._host.head_gate(y, gate)
         if out is not None:
             return out
+        flash_cuda.refuse_tangents("head_gate", y, gate)
     if not supports_gate(y, gate):
         raise ValueError(f"head_gate: unsupported inputs {tuple(y.shape)} {y.dtype}, gate {tuple(gate.shape)} "
                          f"{gate.dtype} on {y.device}")
