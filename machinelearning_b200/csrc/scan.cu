@@ -8,15 +8,14 @@
 //
 // Both directions are bound by memory: three streams of B T D elements forward, five backward.  A step is an affine map h -> a h + b, and maps
 // compose, so the steps are walked in runs that start side by side: a warp has one run of 32 V channels in registers, forms its map, learns the
-// maps of its CTA's runs in front of it through shared memory, and walks the run again from the right state.  The data are read once.  Where there are too few
+// maps of its CTA's runs in front of it through shared memory, and adds to every step what is left there of the state in front of the run.  The data are read once.  Where there are too few
 // channels to fill the GPU, sequences are cut into segments: a first launch forms the segments' maps (which reads the inputs once more), and
 // each CTA of the second starts from the maps in front of its segment.  Nothing waits on another CTA; the order of all sums is fixed.
 //
 // Digits: the smaller of s and 1 - s, e / (1 + e) with e = exp(-|z|), is exact to a few units of 2^-24, the larger is not further than that from 1.  With
 // it the step is h + s (f - h) or f + (1 - s) (h - f), whichever it belongs to: 1 - s itself is rounded by up to 2^-25, always the same way, which
 // is 3% after the million steps that a state lasts where s is 1e-6.  A map's factor has the same two forms (Map below), or it would bring that rounding back with
-// every run (2.4% measured at z = -14.1 after 2^20 steps; so 1e-5 to 1e-4): what is left out of a state is summed beside the factor, one multiply-add a step, and
-// the states of a run are formed from the state in front of it, step by step (64 x 1,024 x 768 bf16: 65 us forward as before; 16 x 1,024 x 768: 23 -> 26).
+// every run (2.4% measured at z = -14.1 after 2^20 steps, 1e-6 so): what is left out of a state is summed beside the factor, one multiply-add a step.
 #include <type_traits>
 
 #include <cuda_bf16.h>
@@ -383,43 +382,48 @@ scan_fwd_kernel(const Params p) {
     async_wait();
     __syncwarp();
     if (from + kStretch < w.t1) ask(buf ^ 1, t0 + kStretch);
-    // the run's map: h from nothing, and what is left of the state in front
-    float2 y[kRun], f[kRun];
+    // h from nothing, and what is left of the state in front of the run, behind every step
+    float2 h[kRun], left[kRun];
     Map<V> m;
     auto walk = [&](auto whole) {
 #pragma unroll
       for (int i = 0; i < kRun; ++i) {
         if (decltype(whole)::value || i < n) {                 // (a step that does not count leaves h as it is)
           if (RESET && (resets >> i & 1u)) m.b = both(0.f);
-          y[i] = lesser<T, V>(zs.get(buf, i));
-          f[i] = mapped<T, POSITIVE>(vs.get(buf, i));
-          m.leave(y[i]);
-          m.b = step<V>(y[i], f[i], m.b);
+          const float2 y = lesser<T, V>(zs.get(buf, i));
+          m.leave(y);
+          m.b = step<V>(y, mapped<T, POSITIVE>(vs.get(buf, i)), m.b);
         }
+        h[i] = m.b;
+        left[i] = m.a;
       }
     };
     if (n >= kRun) walk(std::true_type{});
     else walk(std::false_type{});
-    float2 h = enter<WARPS, RESET>(maps, buf, w.warp, m.template pack<RESET>(resets != 0u), carry);
+    const float4 map = m.template pack<RESET>(resets != 0u);
+    const float2 in = enter<WARPS, RESET>(maps, buf, w.warp, map, carry);
     if (t0 < p.T) {
-      if (p.tape != nullptr && w.live) store_state<V>(p.tape + (static_cast<long long>(w.b) * runs + t0 / kRun) * p.D + w.c, h);
+      if (p.tape != nullptr && w.live) store_state<V>(p.tape + (static_cast<long long>(w.b) * runs + t0 / kRun) * p.D + w.c, in);
+      // (a factor of a run's steps is rounded 16 times at most: 2^-21, forgotten at the end of the run)
       auto put = [&](auto whole) {
 #pragma unroll
         for (int i = 0; i < kRun; ++i) {
           if (!decltype(whole)::value && t0 + i >= p.T) break;
-          const bool counts = decltype(whole)::value || i < n;
-          if (counts) {
-            if (RESET && (resets >> i & 1u)) h = both(0.f);
-            h = step<V>(y[i], f[i], h);
-          }
-          out.put(zs, buf, t0, i, counts ? h : both(0.f));
+          float2 v = h[i];
+          if (!RESET || !(resets & ((2u << i) - 1u))) v = fma_<V>(left[i], in, h[i]);
+          if (!decltype(whole)::value && i >= n) v = both(0.f);
+          out.put(zs, buf, t0, i, v);
         }
       };
       if (n >= kRun) put(std::true_type{});
       else put(std::false_type{});
+      if (p.T - t0 <= kRun) {                                  // the state behind the last step, for the next call: as the next run would get it
+        const float2 state = apply<RESET>(map, in);
+        if (w.live) store_state<V>(p.last + row, state);
+        if (n >= p.T - t0) out.put(zs, buf, t0, p.T - 1 - t0, state);
+      }
       __syncwarp();
       out.write(zs, buf, t0, p.T - t0);
-      if (p.T - t0 <= kRun && w.live) store_state<V>(p.last + row, h);
     }
     settle(buf ^ 1);
   }
