@@ -175,13 +175,15 @@ int chain(const Layout& l) { return l.planes == 3 ? 1 : l.type == NLFA_DTYPE_F16
 
 // Whether g and u, or dh, are formed apart from what is done with them: where there are so few tiles that most pairs of CTAs would watch, and their sums
 // are so long that three more launches are less (80 tokens x 3,903 x 32 in float32, forward and backward 270 us with one tile's sums of 61 stages); and for parts.
-// `most`: stages that are not worth it (float32's dh, whose epilogue writes six planes, 1,000 x 384 x 1,024: 43 us, apart 29 with the launches; its g and u 26, apart 37).
+// `most`: stages that are not worth it.  float32, forward: 6 stages (1,000 x 384 x 1,024) 50 us, apart 57, 12 (500 x 768 x 2,048) 69 and 73, 16 (1,000 x 1,024 x 384) 68 and 56; backward, where the
+// epilogue of dh writes six planes: 1 (2,000 x 64 x 512) 60 and 55, 4 (2,000 x 256 x 512) 68 and 61, 12 (300 x 768 x 2,048) 102 and 87.  bf16, forward and backward: 24 (300 x 3,000 x 256) 35 + 35 and 34 + 33,
+// 38 (300 x 4,800 x 64) 38 + 47 and 28 + 35.
 bool apart(const Layout& l, int cols, int k, int most) {
   if (l.parts == 2) return true;
   return 2 * (l.n_rows / kRowTile) * ceil_div(cols, kColTile) <= pairs() && ceil_div(k, summands(l.planes)) > most;
 }
 bool apart_up(const Call& c, const Layout& l) { return apart(l, c.F, c.d, l.planes == 3 ? 12 : 36); }
-bool apart_dh(const Call& c, const Layout& l) { return apart(l, c.F, c.o, l.planes == 3 ? 4 : 36); }
+bool apart_dh(const Call& c, const Layout& l) { return apart(l, c.F, c.o, l.planes == 3 ? 0 : 36); }
 
 // Forward, g and u apart: maps x, Wg, Wu.
 void plan_up(Params& p, const Call& c, const Layout& l, float* g, float* u) {

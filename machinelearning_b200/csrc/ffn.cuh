@@ -67,8 +67,9 @@ int launch_hidden(int dtype, int planes, int parts, const Params& p, const float
 int launch_grads(int dtype, int planes, int parts, const Params& p, const float* dh, cudaStream_t stream);
 
 // A few tokens, no backward (ffn_few.cu): operands as they lie, d and F multiples of 8, on 16 bytes.  h: n x F.
-// Up to 16 tokens, and up to 64 where tokens times weights are few: the products here are not tcgen05's.  768 x 2,048, 64 tokens: 11 us in bf16, 18 in fp16, 33 in float32,
-// by tiles of 256 rows 20, 30, 69; 4,096 x 8,192: 150, 284, 533 and 60, 89, 400, 16 tokens 72, 88, 185 and 60, 89, 405.
+// Up to 16 tokens, and up to 64 where tokens times weights are few: the products here are not tcgen05's.  768 x 2,048, 64 tokens: 11 us in bf16, 20 in fp16, 30 in float32,
+// by tiles of 256 rows 34, 45, 65; 2,048 x 4,096, 32 tokens: 29, 40, 92 and 44, 59, 129, 64 tokens 38, 80, 137 and 47, 62, 130; 4,096 x 8,192, 16 tokens: 71, 90, 182 and 81, 110, 395,
+// 32 tokens 124, 160, 318 and 84, 116, 397.
 constexpr int kFewTokens = 64, kVeryFewTokens = 16;
 constexpr long long kFewProducts = 1ll << 28;               // n d F
 bool few_types(int w_dtype, int dtype);

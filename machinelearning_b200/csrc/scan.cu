@@ -614,11 +614,11 @@ int element_bytes(int dtype) { return dtype == NLFA_DTYPE_F32 ? 4 : 2; }
 int run_of(int dtype) { return dtype == NLFA_DTYPE_F32 ? kRunOf<float> : kRunOf<__half>; }
 
 // Into how many segments the sequences are cut, and how many runs a CTA walks side by side: by the columns (of 64 channels of a sequence) there are.
-//   up to an eighth of what runs at once: segments, twice as many CTAs as run at once.  1 x 131,072 x 1,024 (16 columns) forward and backward
-//     274 + 410 us, uncut with 4 warps 1,854 + 3,128; 8 x 4,096 x 512 (64) 36 + 54, uncut 50 + 86; but 8 x 2,048 x 768 (96) 28 + 41, uncut 26 + 45:
-//     the maps read the inputs once more.
-//   up to two per SM: 8 warps.  16 x 1,024 x 768 (192) 23 + 38 us, with 4 warps 28 + 38; 16 x 2,048 x 512 (128) 26 + 45, with 4 34 + 53.
-//   else 4: 64 x 1,024 x 768 (768) 64 + 105 us, with 8 62 + 108.
+//   up to a sixth of what runs at once: segments, twice as many CTAs as run at once.  1 x 131,072 x 1,024 bf16 (16 columns), forward and backward,
+//     272 + 417 us, uncut with 8 warps 1,627 + 2,720; 2,048 steps of 64 columns 21 + 28, uncut 27 + 45; of 96 29 + 41, uncut 27 + 46 (float32 55 + 70, uncut 62 + 80); 16,384 of 96 197 + 283,
+//     uncut 208 + 346; but 2,048 of 128 36 + 50, uncut 28 + 46: the maps read the inputs once more.
+//   up to what runs at once: 8 warps.  1,024 steps of 192 23 + 39, with 4 warps 24 + 38 (float32 44 + 59, 55 + 75); of 384 36 + 60, with 4 39 + 64.
+//   else 4: of 768 60 + 97, with 8 65 + 110 (float32 117 + 182, 114 + 175).
 constexpr int kCtasPerSm = 4;
 struct Cut {
   int segments, segment, warps;
@@ -626,11 +626,11 @@ struct Cut {
 Cut cut(int B, int T, int D, int dtype) {
   const long long columns = static_cast<long long>(B) * ((D + 63) / 64), stretch = kWarps * run_of(dtype);
   const long long at_once = static_cast<long long>(kCtasPerSm) * sm_count();
-  if (columns > 0 && 8 * columns <= at_once && T >= 16 * stretch) {
+  if (columns > 0 && 6 * columns <= at_once && T >= 16 * stretch) {
     const long long parts = 2 * at_once / columns, length = (T + parts * stretch - 1) / (parts * stretch) * stretch;
     return {static_cast<int>((T + length - 1) / length), static_cast<int>(length), kWarps};
   }
-  return {1, T > 0 ? T : 1, 2 * columns <= at_once ? 2 * kWarps : kWarps};
+  return {1, T > 0 ? T : 1, columns <= at_once ? 2 * kWarps : kWarps};
 }
 size_t maps_bytes(int B, int T, int D, int dtype) {
   const Cut c = cut(B, T, D, dtype);

@@ -15,7 +15,7 @@ import torch
 HALF_STEP = {torch.float32: 2.0**-24, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}
 GATES = [-14.125, -13.875, -13.8125, -12.3125, -11.0, -9.0, -6.5, -2.0]      # (all exact in bfloat16)
 # B, T, D, and how many runs and segments a state is rounded at
-PLANS = [(1, 1 << 20, 8, 1400), (1, 1 << 18, 7, 1400), (80, 1 << 15, 64, None)]
+PLANS = [(1, 1 << 20, 8, 1400), (1, 1 << 18, 7, 1400), (80, 1 << 15, 64, None), (100, 1 << 15, 64, None)]
 _id = lambda d: str(d).split(".")[-1]
 _np = lambda t: t.detach().double().cpu().numpy()
 
