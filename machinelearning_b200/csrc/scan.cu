@@ -76,7 +76,7 @@ struct Params {
   const void* lengths;                              // [B]
   int length_bytes;
   int B, T, D, blocks;                              // blocks: of 32 V channels
-  int segments, segment, warps;                     // parts of a sequence, their steps; runs side by side in a CTA
+  int segments, segment;                            // parts of a sequence, their steps
   float4* maps;                                     // of the segments but the last walked: [B][segments][blocks][lane]
   void* h;
   float *last, *tape;
@@ -617,20 +617,20 @@ int run_of(int dtype) { return dtype == NLFA_DTYPE_F32 ? kRunOf<float> : kRunOf<
 //   up to a sixth of what runs at once: segments, twice as many CTAs as run at once.  1 x 131,072 x 1,024 bf16 (16 columns), forward and backward,
 //     272 + 417 us, uncut with 8 warps 1,627 + 2,720; 2,048 steps of 64 columns 21 + 28, uncut 27 + 45; of 96 29 + 41, uncut 27 + 46 (float32 55 + 70, uncut 62 + 80); 16,384 of 96 197 + 283,
 //     uncut 208 + 346; but 2,048 of 128 36 + 50, uncut 28 + 46: the maps read the inputs once more.
-//   up to what runs at once: 8 warps.  1,024 steps of 192 23 + 39, with 4 warps 24 + 38 (float32 44 + 59, 55 + 75); of 384 36 + 60, with 4 39 + 64.
+//   up to what runs at once (channels by themselves: of 32): 8 warps.  1,024 steps of 192 23 + 39, with 4 warps 24 + 38 (float32 44 + 59, 55 + 75); of 384 36 + 60, with 4 39 + 64.
 //   else 4: of 768 60 + 97, with 8 65 + 110 (float32 117 + 182, 114 + 175).
 constexpr int kCtasPerSm = 4;
 struct Cut {
-  int segments, segment, warps;
+  int segments, segment;
 };
 Cut cut(int B, int T, int D, int dtype) {
   const long long columns = static_cast<long long>(B) * ((D + 63) / 64), stretch = kWarps * run_of(dtype);
   const long long at_once = static_cast<long long>(kCtasPerSm) * sm_count();
   if (columns > 0 && 6 * columns <= at_once && T >= 16 * stretch) {
     const long long parts = 2 * at_once / columns, length = (T + parts * stretch - 1) / (parts * stretch) * stretch;
-    return {static_cast<int>((T + length - 1) / length), static_cast<int>(length), kWarps};
+    return {static_cast<int>((T + length - 1) / length), static_cast<int>(length)};
   }
-  return {1, T > 0 ? T : 1, columns <= at_once ? 2 * kWarps : kWarps};
+  return {1, T > 0 ? T : 1};
 }
 size_t maps_bytes(int B, int T, int D, int dtype) {
   const Cut c = cut(B, T, D, dtype);
@@ -666,7 +666,8 @@ int run_reset(Params p, bool backward, cudaStream_t st) {
                             : launch(scan_maps_kernel<T, V, POSITIVE, RESET, false>, kWarps, smem, p, st);
     if (rc != NLFA_OK) return rc;
   }
-  return p.warps > kWarps ? run_warps<T, V, 2 * kWarps, POSITIVE, RESET>(p, backward, st) : run_warps<T, V, kWarps, POSITIVE, RESET>(p, backward, st);
+  const bool more = p.segments == 1 && static_cast<long long>(p.B) * p.blocks <= static_cast<long long>(kCtasPerSm) * sm_count();
+  return more ? run_warps<T, V, 2 * kWarps, POSITIVE, RESET>(p, backward, st) : run_warps<T, V, kWarps, POSITIVE, RESET>(p, backward, st);
 }
 template <typename T, int V, bool POSITIVE>
 int run_positive(const Params& p, bool backward, cudaStream_t st) {
@@ -710,7 +711,6 @@ void set_cut(Params& p, int dtype, void* scratch) {
   const Cut c = cut(p.B, p.T, p.D, dtype);
   p.segments = c.segments;
   p.segment = c.segment;
-  p.warps = c.warps;
   p.maps = static_cast<float4*>(scratch);
 }
 
