@@ -384,7 +384,7 @@ int nlfa_clip_grads(const nlfa_grad* grads, int count, float max_norm, int norm,
  * (length_bytes; NULL: all T): steps from lengths[b] on (taken between 0 and T) leave the state as it is, their h is zero, and what gate and value hold there reaches nothing.
  * `tape` (nlfa_gated_scan_tape_bytes; NULL when no backward follows) takes the states at the start of every 16 steps (float32: 8).
  * `scratch`, 16-byte aligned (nlfa_gated_scan_scratch_bytes; 0: none): maps of segments, into which long sequences of few channels are cut.
- * An infinite state or value makes the states behind it infinite or NaN, up to the next reset.
+ * An infinite state or value makes the states behind it infinite or NaN, up to the next reset; so does a difference of a state and a value that float32 does not hold.
  * Bit-reproducible; may be captured.  Any alignment of the element type; rows on 16 bytes are faster. */
 #define NLFA_SCAN_NONE 0
 #define NLFA_SCAN_POSITIVE 1
@@ -406,8 +406,9 @@ int nlfa_gated_scan_bwd(const void* dh, const float* dlast, const void* gate, lo
  * Every extent may be of any size; tensors are contiguous.  x is of x_dtype, the weights of w_dtype, y and its gradient of `dtype`, which is
  * what the products run in (the autocast type, say): 16-bit types on the tensor cores, NLFA_DTYPE_F32 on the tensor cores as sums of three bf16
  * parts (finite values below 3.39e38; an infinity makes what it enters NaN).  Sums are float32.  Between the products the hidden values are rounded once to `dtype`'s
- * precision; in float16 those of a token carry a power of two, from the lengths of its x and dy and of the weights' rows, so that a token's y and dx neither overflow nor lose digits
- * between them, whatever the other tokens are; to the weights' gradients a token's share is exact to 2^-11 of itself or 2^-30 of the largest token's.
+ * precision; in float16 those of a token carry a power of two, from the lengths of its x and dy and of the weights' longest rows, so that between the products nothing overflows, and nothing
+ * loses digits above 2^-28 of what these lengths allow (typical values are some 2^-10 of it), whatever the other tokens are; to the weights' gradients a token's share is exact to 2^-11 of itself or some
+ * 2^-30 of the largest token's.  What an infinity enters is infinite or NaN.
  *
  * `copies` (nlfa_gated_ffn_copies): which of x, w_gate, w_up, w_down (bits 0 to 3) the forward copies into the tape, because the products cannot read
  * them as they lie: of another type, float32, rows not a multiple of 64 long, not 16-byte aligned (without `train` up to 64 tokens take most as they lie).  The backward takes the same value; operands that

@@ -3,7 +3,7 @@
 // Two launches: h = f(x Wg^T) (x Wu^T) in float32, then y = h Wd^T.  A warp has 16 rows of a weight and a run of the sum: each lane loads 16 bytes (8 summands) of
 // two rows at a time straight into the operand registers of mma.sync m16n8k16 -- the order of the summands is free, so a lane's 8 consecutive ones
 // serve as its places of two products, for weight and tokens alike.  A tensor-memory kernel's set-up and tiles of 256 rows cost more than
-// the whole sum here (8 x 768 x 2,048: 19.5 us in the kernels of ffn_tc.cu, 6.5 here).  The runs of a tile's sum are added through shared memory, in order.
+// the whole sum here (8 x 768 x 2,048: 30 us in the kernels of ffn_tc.cu, 6.7 here).  The runs of a tile's sum are added through shared memory, in order.
 // All loads of a run are in flight at once; the second launch has its weights on the way before the first one's h is there.
 //
 // Types: every operand is a sum of bf16 parts, split in registers: bf16 one, float16 two (exact), float32 three (to 2^-24), h two (2^-17), beside float32 three; the products
@@ -268,7 +268,7 @@ int launch_few(FewParams p, cudaStream_t st) {
 template <typename S, typename C>
 int launch_tokens(const FewParams& p, cudaStream_t st) {
   if (p.n <= 8) return launch_few<S, C, 1>(p, st);
-  // (two turns of 16 for 32 tokens 8.3 us, one of 32 10.9; two of 32 for 64 11.1, four of 16 15.2)
+  // (bf16, 768 x 2,048: two turns of 16 for 32 tokens 8.3 us, one of 32 10.9; two of 32 for 64 11.1, four of 16 15.2)
   return p.n <= 32 ? launch_few<S, C, 2>(p, st) : launch_few<S, C, 4>(p, st);
 }
 

@@ -30,7 +30,7 @@ namespace scan {
 namespace {
 
 // Steps in a thread's registers; states at their starts are the backward's tape.  (float32 with 16: 96 KB of shared memory a CTA, backward of
-// 32 x 1,024 x 768 168 us; with 8 100.  bf16, 64 x 1,024 x 768, with 8: 70 and 128 us, with 16 67 and 118 then, 65 and 105 now.)
+// 32 x 1,024 x 768 168 us; with 8 100.  bf16, 64 x 1,024 x 768, with 8: 70 and 128 us, with 16 67 and 118 then, 60 and 98 now.)
 template <typename T> constexpr int kRunOf = sizeof(T) == 4 ? 8 : 16;
 constexpr int kWarps = 4;           // runs side by side in a CTA (or twice as many)
 constexpr int kMostExtent = 1 << 30;

@@ -1,7 +1,8 @@
 """The gated feed-forward layer: ``down(f(gate(x)) * up(x))`` and its gradients.
 
-``gated_ffn(x, w_gate, w_up, w_down)`` is nanolab's ``SwiGLU`` (``nanolab/model.py:29-43``; ``f`` may be another one).  Both projections, the
-activation and the product are one kernel, the projection down another; the backward is two more (``csrc/ffn.cu``, ``csrc/ffn_tc.cu``).
+``gated_ffn(x, w_gate, w_up, w_down)`` is nanolab's ``SwiGLU`` (``nanolab/model.py:29-43``; ``f`` may be another one).  Where there are many tokens both projections,
+the activation and the product are one kernel, the projection down another; the backward is two more.  Up to 256 tokens with gradients, 64 without, and where few tiles have long sums, the products
+are formed in parts by the whole GPU and ``f`` is a kernel of its own; a few tokens without gradients have kernels of their own (``csrc/ffn.cu``, ``csrc/ffn_tc.cu``, ``csrc/ffn_few.cu``).
 Kept for the backward: the hidden values and what turns their gradient into the projections', 6 bytes for each of the ``F`` hidden values of a token in
 bfloat16 (float16 10, float32 14; torch's own graph of the same layer keeps 8, in float32 16).
 
